@@ -309,6 +309,78 @@ int dflash_attention_mixer(const dflash_attention* a, const float* hidden, int64
                            size_t workspace_bytes, void* stream);
 
 /*
+ * A paged KV cache of many sequences: a pool of pages of page_size rows per layer, and per sequence a table of the
+ * pages that hold its rows in order.  Replaces, for a batch, the growing cache of FusedOps.cache_update and
+ * attention (model/qwen35_moe_dflash/fused/ops.py:25-123), which serve one sequence.
+ * Element (page, head, row, d) of the keys lies at page * key_page_stride + head * key_head_stride +
+ * row * key_row_stride + d, all in elements, every stride a multiple of 8 and >= 0; the values likewise.
+ * Row r of sequence b is row r % page_size of page table[b * table_stride + r / page_size].
+ * lengths[b] counts the rows of sequence b, those of the block that a call appends or attends with included.
+ * table and lengths are read on the device when the call runs: a captured call follows their later values.  Table
+ * entries behind a sequence's last row are not read.  An entry outside [0, pages) within it is never followed out of
+ * the pool: attention reads the nearest page instead, append leaves such rows out.  Lengths are taken as at most
+ * table_width * page_size.
+ * Constraints: head_dim 128 or 256, dtype BF16 or F16, page_size % 16 == 0 or table_width == 1,
+ * page_size <= 2^30, table_width * page_size <= 2^30.
+ */
+typedef struct dflash_paged_kv {
+  void* keys;
+  void* values;
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t sequences, table_width, table_stride, pages, page_size, kv_heads, head_dim;
+  int64_t key_page_stride, key_head_stride, key_row_stride;
+  int64_t value_page_stride, value_head_stride, value_row_stride;
+  int32_t dtype; /* enum dflash_dtype */
+} dflash_paged_kv;
+
+/*
+ * A block of new tokens of a batch: rows data[token * token_stride + head * head_stride + d], 16 bits a value,
+ * strides multiples of 8.
+ */
+typedef struct dflash_rows {
+  const void* data;
+  int64_t token_stride, head_stride;
+} dflash_rows;
+
+/*
+ * Append a block's K and V rows to their sequences' pages, with the Q/K norm and the position rotation on the way
+ * (model/qwen35_moe_dflash/fused/model.py:265-294).  Tokens [starts[b], starts[b + 1]) of the block are the last ones of
+ * sequence b: token i of them goes to row lengths[b] - (starts[b + 1] - starts[b]) + i.  starts: int32 [sequences + 1] on
+ * the device, ascending from 0 to at most `tokens`; tokens past starts[sequences] are left out, as are rows before 0.
+ *   n = x / sqrt(mean(x^2) + eps) * (norm + 1)       (q_norm, k_norm: fp32 [head_dim] or NULL: n = x)
+ *   y_i = n_i cos(a_i) - n_{i+h} sin(a_i), y_{i+h} = n_{i+h} cos(a_i) + n_i sin(a_i)  for i < h = rotary_dim / 2,
+ *   a_i = position * inv_freq_i (inv_freq fp32 [h]; NULL: y = n); position: positions[token] (int32 [tokens]) or, NULL, the
+ *   token's row in its sequence.
+ * in fp32 with one rounding; angles are exact to fp32 at any position.  K rows are y, V rows the value as it is, and
+ * query_out [tokens][heads][head_dim] the queries' y (query NULL, heads 0: none).  No two sequences may hold the
+ * same page where a block's rows go.  Constraints: rotary_dim % 16 == 0, <= head_dim; tokens * (heads + 2 kv_heads) <= 2^24.
+ */
+int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, const dflash_rows* value,
+                        const int32_t* starts, int64_t tokens, const dflash_rows* query, int64_t heads,
+                        const float* q_norm, const float* k_norm, const float* inv_freq, int64_t rotary_dim,
+                        const int32_t* positions, float eps, void* query_out, void* stream);
+
+/*
+ * Attention of a batch of blocks over a paged cache (the math of FusedOps.attention,
+ * model/qwen35_moe_dflash/fused/ops.py:25-123, per sequence): out[token][head] = sum_j softmax_j(scale q.k_j) v_j.
+ * Tokens [starts[b], starts[b + 1]) are the last of sequence b's lengths[b] rows; causal: token i of them sees the rows up to
+ * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums, weights
+ * rounded to 16 bits for their product with V.  A row that sees no key gives zeros; rows of tokens in no sequence are not
+ * written.  Masked keys and values count for nothing, NaN and infinities among them.
+ * prefix (NULL: none): a cache of one sequence that every sequence of the batch continues.  Its rows are visible to all
+ * tokens, before the sequence's own, and are read once for the whole batch.  Same kv_heads, head_dim and dtype; pages of
+ * its own kind, of the same pool or another.
+ * out [tokens][heads][head_dim], the query's dtype.  Constraints: heads <= 1024, heads % kv_heads == 0, tokens * heads <=
+ * 2^22, sequences <= 2^20, scale > 0 and finite.  The workspace depends on the sizes alone, not on the lengths.
+ */
+size_t dflash_paged_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t sequences, int has_prefix);
+int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* prefix, const dflash_rows* query,
+                           const int32_t* starts, int64_t tokens, int64_t heads, float scale, int causal, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Measurement mode (no counterpart in the reference; for benchmarks and
  * profilers that time one kernel of the layer on its own): while a stage is
  * set, dflash_moe_w4a16 and dflash_moe_experts_w4a16 validate their arguments

@@ -95,6 +95,39 @@ class AttentionDesc(ctypes.Structure):
     ]
 
 
+class PagedDesc(ctypes.Structure):
+    """``struct dflash_paged_kv``."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("sequences", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("key_page_stride", ctypes.c_int64),
+        ("key_head_stride", ctypes.c_int64),
+        ("key_row_stride", ctypes.c_int64),
+        ("value_page_stride", ctypes.c_int64),
+        ("value_head_stride", ctypes.c_int64),
+        ("value_row_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class RowsDesc(ctypes.Structure):
+    """``struct dflash_rows``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+_PAGEDP = ctypes.POINTER(PagedDesc)
+_ROWSP = ctypes.POINTER(RowsDesc)
 _GDNP = ctypes.POINTER(GdnDesc)
 _ATTNP = ctypes.POINTER(AttentionDesc)
 
@@ -125,6 +158,11 @@ SIGNATURES = {
     "dflash_gdn_commit": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _P]),
     "dflash_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
     "dflash_attention_mixer": (ctypes.c_int, [_ATTNP, _P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
+    "dflash_paged_append": (ctypes.c_int, [_PAGEDP, _ROWSP, _ROWSP, _P, _I64, _ROWSP, _I64, _P, _P, _P, _I64, _P,
+                                           ctypes.c_float, _P, _P]),
+    "dflash_paged_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, ctypes.c_int]),
+    "dflash_paged_attention": (ctypes.c_int, [_PAGEDP, _PAGEDP, _ROWSP, _P, _I64, _I64, ctypes.c_float, ctypes.c_int, _P,
+                                              _P, _SZ, _P]),
     "dflash_set_split_down": (ctypes.c_int, [ctypes.c_int]),
     "dflash_set_tile_pieces": (ctypes.c_int, [ctypes.c_int]),
     "dflash_moe_split_down": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int32,

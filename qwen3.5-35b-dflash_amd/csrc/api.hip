@@ -1086,6 +1086,210 @@ int dflash_attention_mixer(const dflash_attention* a, const float* hidden, int64
   }
 }
 
+namespace {
+constexpr int64_t kPagedRows = int64_t(1) << 30;  // rows a sequence can have: key indices stay in 31 bits
+
+int check_paged(const dflash_paged_kv* c, const char* name) {
+  const auto bad = [&](const char* what) { return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
+  if (!c) return bad("descriptor is NULL");
+  if (c->head_dim != 128 && c->head_dim != 256)
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": head_dim must be 128 or 256");
+  if (c->dtype != DFLASH_DTYPE_BF16 && c->dtype != DFLASH_DTYPE_F16)
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": dtype must be BF16 or F16");
+  if (c->sequences < 0 || c->sequences > (1 << 20) || c->kv_heads < 1 || c->kv_heads > 1024 || c->pages < 1 ||
+      c->pages > INT32_MAX || c->table_width < 1 || c->page_size < 1 || c->table_stride < 0)
+    return bad("sequences, kv_heads, pages, page_size, table_width or table_stride out of range");
+  if (c->page_size > kPagedRows || c->table_width > kPagedRows / c->page_size)
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": table_width * page_size must be at most 2^30");
+  if (c->page_size % 16 && c->table_width != 1)
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": page_size must be a multiple of 16 where a sequence has more than one page");
+  for (int64_t s : {c->key_page_stride, c->key_head_stride, c->key_row_stride, c->value_page_stride, c->value_head_stride,
+                    c->value_row_stride})
+    if (s < 0 || s % 8) return bad("strides must be multiples of 8, not negative");
+  if (c->sequences == 0) return DFLASH_OK;  // an empty table and lengths have no address
+  if (!c->keys || !c->values || !c->table || !c->lengths) return bad("NULL pointer");
+  if (!aligned16(c->keys) || !aligned16(c->values)) return bad("keys and values must be 16-byte aligned");
+  return DFLASH_OK;
+}
+
+int check_rows(const dflash_rows* r, const char* name) {
+  if (!r || !r->data || !aligned16(r->data) || r->token_stride < 0 || r->head_stride < 0 || r->token_stride % 8 || r->head_stride % 8)
+    return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string(name) + ": NULL or misaligned data, or strides that are no multiples of 8");
+  return DFLASH_OK;
+}
+
+dflash::PagedSide paged_side(const dflash_paged_kv* c) {
+  dflash::PagedSide s{};
+  s.keys = static_cast<const uint16_t*>(c->keys);
+  s.values = static_cast<const uint16_t*>(c->values);
+  s.table = c->table;
+  s.lengths = c->lengths;
+  s.table_stride = c->table_stride;
+  s.key_page = c->key_page_stride;
+  s.key_head = c->key_head_stride;
+  s.key_row = c->key_row_stride;
+  s.value_page = c->value_page_stride;
+  s.value_head = c->value_head_stride;
+  s.value_row = c->value_row_stride;
+  s.pages = static_cast<int>(c->pages);
+  s.capacity = static_cast<int>(c->table_width * c->page_size);
+  s.page_groups = static_cast<int>((c->page_size + 15) / 16);
+  s.groups_per_page = dflash::fast_div(static_cast<uint32_t>(s.page_groups));
+  return s;
+}
+
+struct PagedLayout {
+  size_t part[2], ml[2], info[2], total;
+  int64_t rows[2];  // partial rows of the own-keys and the prefix stage
+  int slots[2];
+};
+bool paged_shape_ok(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B) {
+  return T >= 0 && heads > 0 && heads <= 1024 && kv > 0 && heads % kv == 0 && (D == 128 || D == 256) && B >= 0 &&
+         B <= (1 << 20) && T <= (1 << 22) && T * heads <= (1 << 22);
+}
+PagedLayout paged_layout(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B, bool prefix) {
+  PagedLayout L{};
+  Carver c;
+  for (int g = 0; g < (prefix ? 2 : 1); ++g) {
+    const int64_t tile = dflash::paged_tile_rows();
+    L.slots[g] = 2 * cu_count();
+    const int64_t tiles = g ? dflash::ceil_div(T * (heads / kv), tile) : dflash::max_tiles(T, B, heads / kv, tile);
+    L.rows[g] = dflash::max_partial_tiles(tiles, kv, L.slots[g], prefix) * tile;
+    L.part[g] = c.take(4 * static_cast<size_t>(L.rows[g]) * D);
+    L.ml[g] = c.take(8 * static_cast<size_t>(L.rows[g]));
+    L.info[g] = c.take(8 * static_cast<size_t>(T) * heads);
+  }
+  L.total = c.off;
+  return L;
+}
+}  // namespace
+
+int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, const dflash_rows* value,
+                        const int32_t* starts, int64_t tokens, const dflash_rows* query, int64_t heads,
+                        const float* q_norm, const float* k_norm, const float* inv_freq, int64_t rotary_dim,
+                        const int32_t* positions, float eps, void* query_out, void* stream) {
+  try {
+    if (int r = check_paged(cache, "paged append cache")) return r;
+    const bool with_query = query != nullptr;
+    if (heads < 0 || heads > 1024 || (heads > 0) != with_query)
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: heads must be in [1, 1024] with a query, 0 without");
+    if (tokens < 0 || tokens > (1 << 24) || tokens * (heads + 2 * cache->kv_heads) > (1 << 24))
+      return fail(DFLASH_ERR_UNSUPPORTED, "paged append: tokens * (heads + 2 kv_heads) must be at most 2^24");
+    if (inv_freq ? rotary_dim < 16 || rotary_dim % 16 || rotary_dim > cache->head_dim : rotary_dim != 0)
+      return fail(DFLASH_ERR_UNSUPPORTED, "paged append: rotary_dim must be a multiple of 16, at most head_dim, 0 without inv_freq");
+    if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: eps must be finite and not negative");
+    if (tokens == 0 || cache->sequences == 0) return DFLASH_OK;
+    if (!starts) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: starts is NULL");
+    if (int r = check_rows(key, "paged append key")) return r;
+    if (int r = check_rows(value, "paged append value")) return r;
+    if (with_query) {
+      if (int r = check_rows(query, "paged append query")) return r;
+      if (!query_out || !aligned16(query_out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: query_out is NULL or misaligned");
+    }
+    dflash::AppendParams p{};
+    p.side = paged_side(cache);
+    p.keys = static_cast<uint16_t*>(cache->keys);
+    p.values = static_cast<uint16_t*>(cache->values);
+    p.starts = starts;
+    p.B = static_cast<int>(cache->sequences);
+    p.T = static_cast<int>(tokens);
+    p.heads = static_cast<int>(heads);
+    p.kv = static_cast<int>(cache->kv_heads);
+    p.key = static_cast<const uint16_t*>(key->data);
+    p.value = static_cast<const uint16_t*>(value->data);
+    p.key_token = key->token_stride;
+    p.key_head = key->head_stride;
+    p.value_token = value->token_stride;
+    p.value_head = value->head_stride;
+    if (with_query) {
+      p.query = static_cast<const uint16_t*>(query->data);
+      p.query_token = query->token_stride;
+      p.query_head = query->head_stride;
+    }
+    p.q_norm = q_norm;
+    p.k_norm = k_norm;
+    p.inv_freq = inv_freq;
+    p.positions = positions;
+    p.half = static_cast<int>(rotary_dim / 2);
+    p.eps = eps;
+    p.query_out = static_cast<uint16_t*>(query_out);
+    dflash::launch_paged_append(static_cast<int>(cache->head_dim), cache->dtype == DFLASH_DTYPE_BF16, p,
+                                static_cast<hipStream_t>(stream));
+    return launch_status("paged append");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
+size_t dflash_paged_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t sequences, int has_prefix) {
+  if (!paged_shape_ok(tokens, heads, kv_heads, head_dim, sequences)) return 0;
+  return paged_layout(tokens, heads, kv_heads, head_dim, sequences, has_prefix != 0).total;
+}
+
+int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* prefix, const dflash_rows* query,
+                           const int32_t* starts, int64_t tokens, int64_t heads, float scale, int causal, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    if (int r = check_paged(cache, "paged attention cache")) return r;
+    const int64_t T = tokens, kv = cache->kv_heads, D = cache->head_dim, B = cache->sequences;
+    if (!paged_shape_ok(T, heads, kv, D, B))
+      return fail(DFLASH_ERR_UNSUPPORTED, "paged attention: heads must be a multiple of kv_heads, at most 1024, tokens * heads at most 2^22");
+    if (prefix) {
+      if (int r = check_paged(prefix, "paged attention prefix")) return r;
+      if (prefix->sequences != 1 || prefix->kv_heads != kv || prefix->head_dim != D || prefix->dtype != cache->dtype)
+        return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: the prefix is one sequence with the cache's kv_heads, head_dim and dtype");
+    }
+    if (!(scale > 0.0f) || scale > 3.0e38f)
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: scale must be positive and finite");
+    if (T == 0 || B == 0) return DFLASH_OK;
+    if (int r = check_rows(query, "paged attention query")) return r;
+    if (!starts || !out || !aligned16(out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: NULL starts, or NULL or misaligned out");
+    const PagedLayout L = paged_layout(T, heads, kv, D, B, prefix != nullptr);
+    if (!workspace || workspace_bytes < L.total || !aligned16(workspace))
+      return fail(DFLASH_ERR_WORKSPACE, "paged attention workspace needs " + std::to_string(L.total) + " bytes");
+    dflash::PagedParams p{};
+    p.own = paged_side(cache);
+    if (prefix) p.prefix = paged_side(prefix);
+    p.starts = starts;
+    p.B = static_cast<int>(B);
+    p.T = static_cast<int>(T);
+    p.heads = static_cast<int>(heads);
+    p.kv = static_cast<int>(kv);
+    p.group = static_cast<int>(heads / kv);
+    p.causal = causal != 0;
+    p.merge_prefix = prefix != nullptr;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.query = static_cast<const uint16_t*>(query->data);
+    p.query_token = query->token_stride;
+    p.query_head = query->head_stride;
+    p.out = static_cast<uint16_t*>(out);
+    p.own_tile_rows = p.prefix_tile_rows = dflash::paged_tile_rows();
+    const auto stage = [&](int g) {
+      p.slots = L.slots[g];
+      p.part = at<float>(workspace, L.part[g]);
+      p.ml = at<float2>(workspace, L.ml[g]);
+      p.info = at<int2>(workspace, L.info[g]);
+    };
+    p.part_rows[0] = L.rows[0];
+    p.part_rows[1] = L.rows[1];
+    dflash::PagedParams before = p;
+    if (prefix) {
+      stage(1);
+      before = p;
+      p.prefix_part = p.part;
+      p.prefix_ml = p.ml;
+      p.prefix_info = p.info;
+    }
+    stage(0);
+    dflash::launch_paged_attention(static_cast<int>(D), cache->dtype == DFLASH_DTYPE_BF16, p, before,
+                                   static_cast<hipStream_t>(stream));
+    return launch_status("paged attention");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
 int dflash_router_logits(const void* hidden, int64_t tokens, int64_t hidden_size, const void* router_weight,
                          int64_t experts, float* logits, void* stream) {
   try {

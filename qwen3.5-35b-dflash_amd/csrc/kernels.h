@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.h"
+#include "paged_index.h"
 
 namespace dflash {
 
@@ -356,5 +357,55 @@ struct AttnParams {
 int attn_splits(int rows, int kv, int keys, int cus);
 int64_t attn_partial_rows(int rows, int kv, int cus);  // bound on splits * kv * rows over any number of keys
 void launch_attention(int head_dim, const AttnParams& p, hipStream_t stream);
+
+// Paged caches (paged.hip): head dims 128 and 256, bf16 or fp16.  Strides in elements.
+struct PagedSide {
+  const uint16_t *keys, *values;  // [pages][kv][page rows][head_dim] by the strides below, head_dim contiguous
+  const int32_t* table;           // [sequences][table_stride]
+  const int32_t* lengths;         // [sequences]
+  int64_t table_stride;
+  int64_t key_page, key_head, key_row, value_page, value_head, value_row;
+  int pages, capacity;            // pages of the pool; rows a sequence can have (table width * page rows)
+  int page_groups;                // groups of 16 rows a page
+  FastDiv groups_per_page;        // the same, as a divisor
+};
+struct AppendParams {
+  PagedSide side;
+  uint16_t *keys, *values;        // side's, to write
+  const int32_t* starts;          // [B + 1]
+  int B, T, heads, kv;
+  const uint16_t *key, *value, *query;  // query may be null (heads 0)
+  int64_t key_token, key_head, value_token, value_head, query_token, query_head;
+  const float *q_norm, *k_norm, *inv_freq;
+  const int32_t* positions;       // [T] or null: the row in the sequence
+  int half;                       // rotary_dim / 2, a multiple of 8, or 0
+  float eps;
+  uint16_t* query_out;            // [T][heads][head_dim]
+};
+struct PagedParams {
+  PagedSide own, prefix;
+  const int32_t* starts;          // [B + 1]
+  int B, T, heads, kv, group, causal, merge_prefix;
+  int slots;                      // workgroups that the work is cut for
+  float scale_log2;               // scale * log2(e)
+  const uint16_t* query;
+  int64_t query_token, query_head;
+  uint16_t* out;                  // [T][heads][head_dim]
+  // partial results of this stage: rows of unnormalised sums, their maximum and sum, and per (token, head) the first
+  // row and how many (partial tiles of tile_rows rows, tile_rows * kv rows apart)
+  float* part;
+  float2* ml;
+  int2* info;
+  // the prefix stage's, for the merge
+  const float* prefix_part;
+  const float2* prefix_ml;
+  const int2* prefix_info;
+  int own_tile_rows, prefix_tile_rows;
+  int64_t part_rows[2];           // rows that part and prefix_part hold
+};
+int paged_tile_rows();
+void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStream_t stream);
+// `before`: the prefix stage's parameters (read where p.merge_prefix)
+void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, const PagedParams& before, hipStream_t stream);
 
 }  // namespace dflash

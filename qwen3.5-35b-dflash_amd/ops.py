@@ -332,6 +332,193 @@ def attention_mixer(hidden: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     return mid, normed
 
 
+class PagedKV(NamedTuple):
+    """A paged KV cache of ``B`` sequences (``dflash_paged_kv`` in ``include/dflash_hip.h``): row ``r`` of sequence ``b``
+    is row ``r % S`` of page ``table[b, r // S]``.  ``table`` and ``lengths`` are read on the device when a call runs, so a
+    captured call follows their later values."""
+
+    keys: torch.Tensor       # bf16 or fp16 [pages, kv heads, S, head dim], the head dim contiguous, other strides free
+    values: torch.Tensor     # the same shape and dtype
+    table: torch.Tensor      # int32 [B, pages a sequence can have]
+    lengths: torch.Tensor    # int32 [B]: rows of each sequence, the block's included
+
+
+_PAGED_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether 16-byte loads take the rows of ``t`` as they lie."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+
+
+def _int32(t, shape: tuple, name: str, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{name} must be int32 {list(shape)} on {device}")
+    return t.contiguous()
+
+
+def _paged(cache: PagedKV, name: str) -> tuple:
+    """The descriptor of a valid paged cache, and what has to outlive the call."""
+    if not isinstance(cache, PagedKV):
+        raise ValueError(f"{name} must be a PagedKV (keys, values, table, lengths)")
+    keys, values, table, lengths = cache
+    device = _require_device(*cache)
+    if keys.ndim != 4 or keys.dtype not in _PAGED_DTYPES or values.shape != keys.shape or values.dtype != keys.dtype:
+        raise ValueError(f"{name} needs keys and values of one dtype, bfloat16 or float16 [pages, kv heads, rows, head dim]")
+    if not _aligned(keys) or not _aligned(values):
+        raise ValueError(f"{name} needs pages with a contiguous head dim, 16-byte aligned rows")
+    if table.ndim != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+        raise ValueError(f"{name} needs an int32 table [sequences, pages of a sequence] with contiguous rows")
+    lengths = _int32(lengths, (table.shape[0],), f"{name} lengths", device)
+    pages, kv, size, dim = keys.shape
+    desc = _lib.PagedDesc(keys.data_ptr(), values.data_ptr(), table.data_ptr(), lengths.data_ptr(), table.shape[0],
+                          table.shape[1], table.stride(0), pages, size, kv, dim, *keys.stride()[:3], *values.stride()[:3],
+                          _PAGED_DTYPES[keys.dtype])
+    return desc, device, lengths
+
+
+def _token_rows(t, heads: int, cache: PagedKV, name: str, tokens: Optional[int] = None) -> torch.Tensor:
+    """``t`` as rows ``[tokens, heads, head dim]`` that the kernels read: as it lies, or a contiguous copy."""
+    dim, dtype = cache.keys.shape[3], cache.keys.dtype
+    if (not isinstance(t, torch.Tensor) or t.ndim != 3 or t.dtype != dtype or t.device != cache.keys.device
+            or t.shape[2] != dim or (heads and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens)):
+        raise ValueError(f"{name} must be {dtype} [{'tokens' if tokens is None else tokens}, {heads or 'heads'}, {dim}] "
+                         f"on {cache.keys.device}")
+    return t if _aligned(t) else t.contiguous()
+
+
+def _rows_desc(t: Optional[torch.Tensor]):
+    return None if t is None else ctypes.byref(_lib.RowsDesc(t.data_ptr(), t.stride(0), t.stride(1)))
+
+
+def _untracked(name: str, *tensors) -> None:
+    if _tracked(*(t for t in tensors if t is not None)):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
+def _disjoint(t: torch.Tensor) -> bool:
+    """Whether no two elements of ``t`` share memory, as far as its strides show it."""
+    span = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < span:
+            return False
+        span = stride * (size - 1) + span
+    return True
+
+
+def paged_append(cache: PagedKV, key: torch.Tensor, value: torch.Tensor, starts: torch.Tensor, *,
+                 query: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
+    """Write a block's ``key`` and ``value`` rows ``[tokens, kv heads, head dim]`` into their sequences' pages.
+
+    Tokens ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) are the last of sequence ``b``'s ``lengths[b]`` rows;
+    tokens past ``starts[B]`` are left out.  On the way ``key`` (and ``query`` ``[tokens, heads, head dim]``, whose result is
+    returned) gets its RMS norm (``q_norm``, ``k_norm`` fp32 ``[head dim]``, applied as weight + 1) and the rotation of its
+    first ``2 * len(inv_freq)`` features (half-split pairs) at ``positions`` (int32 ``[tokens]``; None: the row in the
+    sequence).  fp32 inside, one rounding.  ``key``, ``value`` and ``query`` may be views of one projection's rows.  No two
+    sequences may hold the same page where rows of the block go.  A table entry that is no page leaves its rows out.
+    """
+    desc, device, lengths = _paged(cache, "paged_append cache")
+    kv = cache.keys.shape[1]
+    if not _disjoint(cache.keys) or not _disjoint(cache.values):
+        raise ValueError("paged_append needs pages that do not overlap")
+    key = _token_rows(key, kv, cache, "key")
+    tokens = key.shape[0]
+    value = _token_rows(value, kv, cache, "value", tokens)
+    dim = cache.keys.shape[3]
+    if query is not None:
+        query = _token_rows(query, 0, cache, "query", tokens)
+        if query.shape[1] < 1:
+            raise ValueError("query must have at least one head")
+    starts = _int32(starts, (cache.table.shape[0] + 1,), "starts", device)
+    if positions is not None:
+        positions = _int32(positions, (tokens,), "positions", device)
+        if inv_freq is None:
+            raise ValueError("positions are those of a rotation: inv_freq is missing")
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != (dim,)
+                              or t.device != device):
+            raise ValueError(f"{name} must be float32 [{dim}] on {device}")
+    if q_norm is not None and query is None:
+        raise ValueError("q_norm needs a query")
+    if inv_freq is not None and (not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32
+                                 or inv_freq.ndim != 1 or inv_freq.device != device):
+        raise ValueError(f"inv_freq must be float32 [rotary dim / 2] on {device}")
+    _untracked("paged_append", cache.keys, cache.values, key, value, query, inv_freq, q_norm, k_norm)
+    q_norm, k_norm, inv_freq = (None if t is None else t.contiguous() for t in (q_norm, k_norm, inv_freq))
+    heads = 0 if query is None else query.shape[1]
+    out = None if query is None else torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    with torch.cuda.device(device):
+        _lib.call("dflash_paged_append", ctypes.byref(desc), _rows_desc(key), _rows_desc(value), _ptr(starts), tokens,
+                  _rows_desc(query), heads, _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+                  0 if inv_freq is None else 2 * inv_freq.shape[0], _ptr(positions), eps, _ptr(out), _stream(device))
+    return out
+
+
+def _paged_attention(name: str, query, prefix: Optional[PagedKV], cache: PagedKV, starts, scale, causal, out, workspace):
+    desc, device, lengths = _paged(cache, f"{name} cache")
+    before = None
+    if prefix is not None:
+        front, where, prefix_length = _paged(prefix, f"{name} prefix")
+        if (where != device or prefix.table.shape[0] != 1 or prefix.keys.dtype != cache.keys.dtype
+                or (prefix.keys.shape[1], prefix.keys.shape[3]) != (cache.keys.shape[1], cache.keys.shape[3])):
+            raise ValueError("the prefix must be a PagedKV of one sequence with the cache's kv heads, head dim and dtype")
+        before = ctypes.byref(front)
+    query = _token_rows(query, 0, cache, "query")
+    tokens, heads, dim = query.shape
+    kv = cache.keys.shape[1]
+    if heads < 1 or heads % kv:
+        raise ValueError("query heads must be a multiple of the cache's kv heads")
+    starts = _int32(starts, (cache.table.shape[0] + 1,), "starts", device)
+    if type(causal) is not bool or not isinstance(scale, (int, float)) or isinstance(scale, bool):
+        raise ValueError("scale must be a number and causal a bool")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    elif not _as(out, query.dtype, (tokens, heads, dim), device):
+        raise ValueError(f"out must be a contiguous {query.dtype} [{tokens}, {heads}, {dim}] tensor on {device}")
+    _untracked(name, query, cache.keys, cache.values, out, *(() if prefix is None else (prefix.keys, prefix.values)))
+    with torch.cuda.device(device):
+        need = _lib.load().dflash_paged_attention_workspace_bytes(tokens, heads, kv, dim, cache.table.shape[0],
+                                                                  int(prefix is not None))
+        ws = _workspace(need, device, workspace)
+        _lib.call("dflash_paged_attention", ctypes.byref(desc), before, _rows_desc(query), _ptr(starts), tokens, heads,
+                  scale, int(causal), _ptr(out), _ptr(ws), ws.numel(), _stream(device))
+    return out
+
+
+def paged_attention(query: torch.Tensor, cache: PagedKV, starts: torch.Tensor, *, scale: float, causal: bool = True,
+                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Grouped-query attention of a batch of blocks over a paged cache: ``query`` and result ``[tokens, heads, head dim]``.
+
+    Tokens ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) are the last of sequence ``b``'s ``lengths[b]`` rows
+    (``paged_append`` wrote theirs); ``causal``: each sees the rows up to its own, else all of its sequence.  fp32 scores
+    and sums.  A token that sees no row gives zeros; tokens past ``starts[B]`` are not written (``out``: a tensor to write
+    into, whose other rows stay as they are).
+    """
+    return _paged_attention("paged_attention", query, None, cache, starts, scale, causal, out, workspace)
+
+
+def shared_prefix_attention(query: torch.Tensor, prefix: PagedKV, cache: PagedKV, starts: torch.Tensor, *, scale: float,
+                            causal: bool = True, out: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_attention` where every sequence continues the rows of ``prefix`` (a ``PagedKV`` of one sequence).
+
+    All tokens see the whole prefix, before the rows of their own sequence in ``cache``; the prefix's keys and values are
+    read once for the stacked rows of the batch and the two parts merged.  The prefix may lie in the cache's pool or in
+    another tensor, a session's contiguous cache ``[1, kv heads, capacity, head dim]`` (one page) among them.
+    """
+    if prefix is None:
+        raise ValueError("shared_prefix_attention needs a prefix")
+    return _paged_attention("shared_prefix_attention", query, prefix, cache, starts, scale, causal, out, workspace)
+
+
+def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, sequences: int,
+                                    has_prefix: bool) -> int:
+    return int(_lib.load().dflash_paged_attention_workspace_bytes(tokens, heads, kv_heads, head_dim, sequences,
+                                                                  int(has_prefix)))
+
+
 def router_logits(hidden: torch.Tensor, router_weight: torch.Tensor) -> torch.Tensor:
     """fp32 ``[T, E]`` logits from bf16 ``hidden [..., H]`` and bf16 ``router_weight [E, H]``."""
     device = _require_device(hidden, router_weight)
