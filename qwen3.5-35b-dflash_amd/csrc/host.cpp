@@ -4,9 +4,9 @@
 // A decoded token's projection is 3.5 us of device time and was 17 us of Python (validation, descriptors, ctypes, two
 // allocations); a 16-token GDN layer 89 us of device time behind 156 us of it.  Every function here takes the arguments
 // of its namesake in ops.py, does what that does when they are plain (exact torch.Tensor and bank types, contiguous, on
-// one ROCm device, no dispatch or function mode active) and returns None otherwise, before anything is launched; ops.py
-// then takes its own path, which decides and reports as it always did.  A call that its entry refuses raises what ops.py
-// would (_lib.check).  No state but the entry points' addresses, the two bank types and that function, set once by
+// one ROCm device, no dispatch or function mode active; the paged-cache calls take strided rows, on the current device)
+// and returns None otherwise, before anything is launched; ops.py then takes its own path, which decides and reports as
+// it always did.  A call that its entry refuses raises what ops.py would (_lib.check).  No state but the entry points' addresses, the bank and cache types and that function, set once by
 // bind().  The GIL is released while an entry enqueues.
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -16,12 +16,16 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <array>
+
 #include "../../include/dflash_hip.h"
 
 namespace {
 
 PyTypeObject* g_packed_type = nullptr;
 PyTypeObject* g_shared_type = nullptr;
+PyTypeObject* g_paged_type = nullptr;
 PyObject* g_check = nullptr;
 
 struct Entries {
@@ -37,6 +41,9 @@ struct Entries {
   decltype(&dflash_rms_norm) rms_norm;
   decltype(&dflash_attention_workspace_bytes) attention_workspace_bytes;
   decltype(&dflash_attention_mixer) attention;
+  decltype(&dflash_paged_append) paged_append;
+  decltype(&dflash_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
+  decltype(&dflash_paged_attention) paged_attention;
 } g_entry;
 
 // _lib.check of a nonzero status: raises DflashError with the library's message
@@ -417,10 +424,171 @@ PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(PackedW4, SharedExpert, _lib.check, address of an entry by name)
+// 16-byte loads take its rows as they lie (ops._aligned).
+bool rows_aligned(const at::Tensor& t) {
+  const auto strides = t.strides();
+  if (strides.back() != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  return std::all_of(strides.begin(), strides.end() - 1, [](int64_t s) { return s % 8 == 0; });
+}
+
+// ops._disjoint
+bool disjoint(const at::Tensor& t) {
+  std::array<std::pair<int64_t, int64_t>, 4> d;
+  size_t n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
+  std::sort(d.begin(), d.begin() + n);
+  int64_t span = 1;
+  for (size_t i = 0; i < n; ++i) {
+    if (d[i].first < span) return false;
+    span = d[i].first * (d[i].second - 1) + span;
+  }
+  return true;
+}
+
+const at::Tensor* ints(PyObject* o, at::IntArrayRef shape, at::Device device) {
+  const at::Tensor* t = tensor(o);
+  return t && t->scalar_type() == at::kInt && t->sizes() == shape && t->device() == device && t->is_contiguous() ? t : nullptr;
+}
+
+// The descriptor of a valid PagedKV on the current device (ops._paged); `keys`: its key pages.
+bool paged(PyObject* o, dflash_paged_kv* d, const at::Tensor** keys, bool writes) {
+  if (Py_TYPE(o) != g_paged_type) return false;
+  const at::Tensor *k = tensor(PyTuple_GET_ITEM(o, 0)), *v = tensor(PyTuple_GET_ITEM(o, 1)), *t = tensor(PyTuple_GET_ITEM(o, 2));
+  if (!k || !v || !t || k->dim() != 4 || (k->scalar_type() != at::kBFloat16 && k->scalar_type() != at::kHalf) ||
+      v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() || v->device() != k->device() || !rows_aligned(*k) ||
+      !rows_aligned(*v) || t->dim() != 2 || t->scalar_type() != at::kInt || t->device() != k->device() || t->stride(1) != 1 ||
+      tracked(*k) || tracked(*v) || (writes && (!disjoint(*k) || !disjoint(*v))))
+    return false;
+  const at::Tensor* n = ints(PyTuple_GET_ITEM(o, 3), {t->size(0)}, k->device());
+  if (!n || k->device().index() != c10::hip::current_device()) return false;
+  *d = dflash_paged_kv{};
+  d->keys = k->data_ptr();
+  d->values = v->data_ptr();
+  d->table = static_cast<const int32_t*>(t->data_ptr());
+  d->lengths = static_cast<const int32_t*>(n->data_ptr());
+  d->sequences = t->size(0);
+  d->table_width = t->size(1);
+  d->table_stride = t->stride(0);
+  d->pages = k->size(0);
+  d->kv_heads = k->size(1);
+  d->page_size = k->size(2);
+  d->head_dim = k->size(3);
+  d->key_page_stride = k->stride(0);
+  d->key_head_stride = k->stride(1);
+  d->key_row_stride = k->stride(2);
+  d->value_page_stride = v->stride(0);
+  d->value_head_stride = v->stride(1);
+  d->value_row_stride = v->stride(2);
+  d->dtype = k->scalar_type() == at::kHalf ? DFLASH_DTYPE_F16 : DFLASH_DTYPE_BF16;
+  *keys = k;
+  return true;
+}
+
+// A block's rows of a cache (ops._token_rows); `heads` 0: any, `tokens` -1: any.
+const at::Tensor* token_rows(PyObject* o, const at::Tensor& keys, int64_t heads, int64_t tokens, dflash_rows* d) {
+  const at::Tensor* t = tensor(o);
+  if (!t || t->dim() != 3 || t->scalar_type() != keys.scalar_type() || t->device() != keys.device() || t->size(2) != keys.size(3) ||
+      t->size(1) < 1 || (heads && t->size(1) != heads) || (tokens >= 0 && t->size(0) != tokens) || !rows_aligned(*t) || tracked(*t))
+    return nullptr;
+  *d = dflash_rows{t->data_ptr(), t->stride(0), t->stride(1)};
+  return t;
+}
+
+// paged_append(cache, key, value, starts, query, inv_freq, positions, q_norm, k_norm, eps): the turned query, or True
+// without one
+PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 10)) return nullptr;
+  dflash_paged_kv c;
+  const at::Tensor* keys = nullptr;
+  if (!plain_state() || !paged(a[0], &c, &keys, true) || !PyFloat_CheckExact(a[9])) Py_RETURN_NONE;
+  const at::Device device = keys->device();
+  dflash_rows k, v, q;
+  const at::Tensor* key = token_rows(a[1], *keys, c.kv_heads, -1, &k);
+  if (!key) Py_RETURN_NONE;
+  const int64_t tokens = key->size(0);
+  const at::Tensor *value = token_rows(a[2], *keys, c.kv_heads, tokens, &v),
+                   *starts = ints(a[3], {c.sequences + 1}, device);
+  if (!value || !starts) Py_RETURN_NONE;
+  const at::Tensor *query = nullptr, *positions = nullptr, *vec[3] = {nullptr, nullptr, nullptr};
+  if (a[4] != Py_None && !(query = token_rows(a[4], *keys, 0, tokens, &q))) Py_RETURN_NONE;
+  if (a[6] != Py_None && (a[5] == Py_None || !(positions = ints(a[6], {tokens}, device)))) Py_RETURN_NONE;
+  if (a[7] != Py_None && !query) Py_RETURN_NONE;
+  const int at_[3] = {5, 7, 8};
+  for (int i = 0; i < 3; ++i) {
+    if (a[at_[i]] == Py_None) continue;
+    const at::Tensor* t = vec[i] = tensor(a[at_[i]]);
+    if (!t || t->scalar_type() != at::kFloat || t->dim() != 1 || t->device() != device || !t->is_contiguous() || tracked(*t) ||
+        (i > 0 && t->size(0) != c.head_dim))
+      Py_RETURN_NONE;
+  }
+  const int64_t heads = query ? query->size(1) : 0;
+  at::Tensor out;
+  if (query) out = make({tokens, heads, c.head_dim}, query->scalar_type(), device);
+  const auto f = [](const at::Tensor* t) { return t ? static_cast<const float*>(t->data_ptr()) : nullptr; };
+  void* st = stream_of(device);
+  const float eps = static_cast<float>(PyFloat_AS_DOUBLE(a[9]));
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.paged_append(&c, &k, &v, static_cast<const int32_t*>(starts->data_ptr()), tokens, query ? &q : nullptr, heads,
+                                f(vec[1]), f(vec[2]), f(vec[0]), vec[0] ? 2 * vec[0]->size(0) : 0,
+                                positions ? static_cast<const int32_t*>(positions->data_ptr()) : nullptr, eps,
+                                query ? out.data_ptr() : nullptr, st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_paged_append", status);
+  if (!query) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(query, prefix, cache, starts, scale, causal, out, workspace): prefix None: without one
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 8)) return nullptr;
+  dflash_paged_kv c, before;
+  const at::Tensor *keys = nullptr, *front = nullptr;
+  if (!plain_state() || !paged(a[2], &c, &keys, false) || !PyFloat_CheckExact(a[4]) || !PyBool_Check(a[5])) Py_RETURN_NONE;
+  const at::Device device = keys->device();
+  if (a[1] != Py_None && (!paged(a[1], &before, &front, false) || before.sequences != 1 || before.kv_heads != c.kv_heads ||
+                          before.head_dim != c.head_dim || before.dtype != c.dtype || front->device() != device))
+    Py_RETURN_NONE;
+  dflash_rows q;
+  const at::Tensor* query = token_rows(a[0], *keys, 0, -1, &q);
+  const at::Tensor* starts = query ? ints(a[3], {c.sequences + 1}, device) : nullptr;
+  if (!starts || query->size(1) % c.kv_heads) Py_RETURN_NONE;
+  const int64_t tokens = query->size(0), heads = query->size(1);
+  at::Tensor out, ws;
+  if (a[6] == Py_None) {
+    out = make({tokens, heads, c.head_dim}, query->scalar_type(), device);
+  } else {
+    const at::Tensor* given = exactly(a[6], query->scalar_type(), {tokens, heads, c.head_dim}, device);
+    if (!given || tracked(*given)) Py_RETURN_NONE;
+    out = *given;
+  }
+  const size_t need = g_entry.paged_attention_workspace_bytes(tokens, heads, c.kv_heads, c.head_dim, c.sequences, front != nullptr);
+  if (!workspace_of(a[7], need, device, &ws)) Py_RETURN_NONE;
+  void* st = stream_of(device);
+  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(a[4]));
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.paged_attention(&c, front ? &before : nullptr, &q, static_cast<const int32_t*>(starts->data_ptr()), tokens, heads,
+                                   scale, a[5] == Py_True, out.data_ptr(), ws.data_ptr(), ws.numel(), st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_paged_attention", status);
+  if (a[6] != Py_None) {
+    Py_INCREF(a[6]);
+    return a[6];
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(PackedW4, SharedExpert, PagedKV, _lib.check, address of an entry by name)
 PyObject* bind(PyObject*, PyObject* args) {
-  PyObject *packed, *shared, *check, *find;
-  if (!PyArg_ParseTuple(args, "O!O!OO", &PyType_Type, &packed, &PyType_Type, &shared, &check, &find)) return nullptr;
+  PyObject *packed, *shared, *cache, *check, *find;
+  if (!PyArg_ParseTuple(args, "O!O!O!OO", &PyType_Type, &packed, &PyType_Type, &shared, &PyType_Type, &cache, &check, &find))
+    return nullptr;
   bool ok = true;
   const auto get = [&](const char* name, auto& fn) {
     PyObject* v = ok ? PyObject_CallFunction(find, "s", name) : nullptr;
@@ -441,21 +609,27 @@ PyObject* bind(PyObject*, PyObject* args) {
   get("dflash_rms_norm", g_entry.rms_norm);
   get("dflash_attention_workspace_bytes", g_entry.attention_workspace_bytes);
   get("dflash_attention_mixer", g_entry.attention);
+  get("dflash_paged_append", g_entry.paged_append);
+  get("dflash_paged_attention_workspace_bytes", g_entry.paged_attention_workspace_bytes);
+  get("dflash_paged_attention", g_entry.paged_attention);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "bind: an entry has no address");
     return nullptr;
   }
   Py_INCREF(packed);
   Py_INCREF(shared);
+  Py_INCREF(cache);
   Py_INCREF(check);
   g_check = check;
   g_packed_type = reinterpret_cast<PyTypeObject*>(packed);
   g_shared_type = reinterpret_cast<PyTypeObject*>(shared);
+  g_paged_type = reinterpret_cast<PyTypeObject*>(cache);
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(linear), FAST(moe), FAST(gdn), FAST(attention), FAST(commit), FAST(rms_norm),
+                         FAST(paged_append), FAST(paged_attention),
                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dflash_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

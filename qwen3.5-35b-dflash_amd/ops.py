@@ -419,6 +419,10 @@ def paged_append(cache: PagedKV, key: torch.Tensor, value: torch.Tensor, starts:
     sequence).  fp32 inside, one rounding.  ``key``, ``value`` and ``query`` may be views of one projection's rows.  No two
     sequences may hold the same page where rows of the block go.  A table entry that is no page leaves its rows out.
     """
+    if _plain(key) and (host := _lib.host()):
+        done = host.paged_append(cache, key, value, starts, query, inv_freq, positions, q_norm, k_norm, eps)
+        if done is not None:
+            return None if done is True else done
     desc, device, lengths = _paged(cache, "paged_append cache")
     kv = cache.keys.shape[1]
     if not _disjoint(cache.keys) or not _disjoint(cache.values):
@@ -457,6 +461,10 @@ def paged_append(cache: PagedKV, key: torch.Tensor, value: torch.Tensor, starts:
 
 
 def _paged_attention(name: str, query, prefix: Optional[PagedKV], cache: PagedKV, starts, scale, causal, out, workspace):
+    if _plain(query) and (host := _lib.host()):
+        done = host.paged_attention(query, prefix, cache, starts, scale, causal, out, workspace)
+        if done is not None:
+            return done
     desc, device, lengths = _paged(cache, f"{name} cache")
     before = None
     if prefix is not None:

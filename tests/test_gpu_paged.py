@@ -446,3 +446,45 @@ def test_a_run_of_prompt_and_decode_steps(pkg, device, shared):
                 want, size, most = pu.attend(turned[at:at + t, h].double().cpu(), kk[:, h // 8], vv[:, h // 8], seen, scale)
                 check(got[at:at + t, h], want, pu.bound(dtype, dim, scale, size, most, kk.shape[0]))
             at += t
+
+
+def test_the_native_and_the_python_form_take_the_same_calls(pkg, device, monkeypatch):
+    """Bit for bit the same result; what the native form leaves to the Python form comes out as there."""
+    native = pkg._lib.host()
+    batch = pu.Batch(pkg, device, SPANS["blocks"], page=16, dtype=BF16, seed=16, spare=1, **SMALL)
+    prefix = pu.Batch(pkg, device, [(0, 90)], page=16, dtype=BF16, seed=17, **SMALL)
+    rows = torch.randn((batch.total, 2, 128), device=device).to(BF16)
+    inv, norm = 10000.0 ** -(torch.arange(16, device=device) / 16), torch.rand((128,), device=device)
+    where = torch.arange(batch.total, dtype=torch.int32, device=device)
+    c, q, s = batch.cache, batch.q, batch.s
+
+    def calls():
+        got = [pkg.ops.paged_append(c, rows, rows, s, query=q, inv_freq=inv, positions=where, q_norm=norm, k_norm=norm),
+               pkg.ops.paged_append(c, rows, rows, s), c.keys.clone()]
+        out = torch.zeros_like(q)
+        got += [pkg.ops.paged_attention(q, c, s, scale=0.1, causal=False), pkg.ops.paged_attention(q, c, s, scale=0.1, out=out), out,
+                pkg.ops.shared_prefix_attention(q, prefix.cache, c, s, scale=0.1)]
+        return got
+
+    got = calls()
+    assert native.paged_append(c, rows, rows, s, q, inv, where, norm, norm, 1e-6) is not None
+    assert native.paged_append(c, rows, rows, s, None, None, None, None, None, 1e-6) is True
+    assert native.paged_attention(q, prefix.cache, c, s, 0.1, True, None, None) is not None
+    with monkeypatch.context() as m:
+        m.setattr(pkg.ops, "_plain", lambda x: False)
+        want = calls()
+    for a, b in zip(got, want):
+        assert a is b is None or torch.equal(a[:batch.tokens].view(torch.int16), b[:batch.tokens].view(torch.int16))
+    odd = torch.empty((batch.total, 4, 129), dtype=BF16, device=device)[..., 1:]
+    odd.copy_(q)
+    wide = torch.zeros((4, 6), dtype=torch.int32, device=device)
+    for args in ((odd, None, c, s, 0.1, True, None, None), (q, None, tuple(c), s, 0.1, True, None, None),
+                 (q, None, c, wide[:, 0], 0.1, True, None, None), (q, None, c, s, 1, True, None, None),
+                 (q, c, c, s, 0.1, True, None, None), (q.clone().requires_grad_(), None, c, s, 0.1, True, None, None),
+                 (q, None, c._replace(lengths=c.lengths.long()), s, 0.1, True, None, None)):
+        assert native.paged_attention(*args) is None
+    for args in ((c, rows, rows[:3], s, None, None, None, None, None, 1e-6), (c, rows, rows, s, None, None, where, None, None, 1e-6),
+                 (c, rows, rows, s, None, None, None, norm, None, 1e-6), (c, rows, rows, s, None, None, None, None, norm[:64], 1e-6),
+                 (c._replace(keys=c.keys[:1].expand(4, -1, -1, -1), values=c.values[:4]), rows, rows, s, None, None, None, None, None,
+                  1e-6)):
+        assert native.paged_append(*args) is None
