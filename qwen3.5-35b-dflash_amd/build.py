@@ -33,6 +33,10 @@ FLAGS = (
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 )
 
+# The attention kernels of head dim 256 hold 128 accumulators a lane that vector instructions rescale now and then: with
+# matrix instructions that take them from the accumulation registers they would be copied there and back at every step.
+SOURCE_FLAGS = {"csrc/paged.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form=1")}
+
 
 def _hipcc() -> str:
     path = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -90,7 +94,7 @@ def build(verbose: bool = False, timeline: bool = False) -> Path:
         objects, procs = [], []
         for src in SOURCES:
             obj = Path(tmp) / (Path(src).stem + ".o")
-            cmd = [hipcc, *flags, "-c", str(PACKAGE_DIR / src), "-o", str(obj)]
+            cmd = [hipcc, *flags, *SOURCE_FLAGS.get(src, ()), "-c", str(PACKAGE_DIR / src), "-o", str(obj)]
             objects.append(obj)
             procs.append(_start(cmd))
         host = Path(tmp) / HOST_LIBRARY.name

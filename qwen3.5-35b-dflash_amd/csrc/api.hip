@@ -1106,6 +1106,8 @@ int check_paged(const dflash_paged_kv* c, const char* name) {
   for (int64_t s : {c->key_page_stride, c->key_head_stride, c->key_row_stride, c->value_page_stride, c->value_head_stride,
                     c->value_row_stride})
     if (s < 0 || s % 8) return bad("strides must be multiples of 8, not negative");
+  if (c->key_row_stride > (1 << 26) || c->value_row_stride > (1 << 26))  // a 16-row group's offsets stay in 32 bits
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": row strides above 2^26 elements");
   if (c->sequences == 0) return DFLASH_OK;  // an empty table and lengths have no address
   if (!c->keys || !c->values || !c->table || !c->lengths) return bad("NULL pointer");
   if (!aligned16(c->keys) || !aligned16(c->values)) return bad("keys and values must be 16-byte aligned");
@@ -1141,7 +1143,7 @@ dflash::PagedSide paged_side(const dflash_paged_kv* c) {
 struct PagedLayout {
   size_t part[2], ml[2], info[2], total;
   int64_t rows[2];  // partial rows of the own-keys and the prefix stage
-  int slots[2];
+  int slots[2], tile[2];
 };
 bool paged_shape_ok(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B) {
   return T >= 0 && heads > 0 && heads <= 1024 && kv > 0 && heads % kv == 0 && (D == 128 || D == 256) && B >= 0 &&
@@ -1151,8 +1153,8 @@ PagedLayout paged_layout(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_
   PagedLayout L{};
   Carver c;
   for (int g = 0; g < (prefix ? 2 : 1); ++g) {
-    const int64_t tile = dflash::paged_tile_rows();
-    L.slots[g] = 2 * cu_count();
+    const int64_t tile = L.tile[g] = dflash::paged_tile_rows(T, g ? 1 : B, heads / kv);
+    L.slots[g] = dflash::paged_slots(L.tile[g], static_cast<int>(D), cu_count());
     const int64_t tiles = g ? dflash::ceil_div(T * (heads / kv), tile) : dflash::max_tiles(T, B, heads / kv, tile);
     L.rows[g] = dflash::max_partial_tiles(tiles, kv, L.slots[g], prefix) * tile;
     L.part[g] = c.take(4 * static_cast<size_t>(L.rows[g]) * D);
@@ -1264,7 +1266,8 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
     p.query_token = query->token_stride;
     p.query_head = query->head_stride;
     p.out = static_cast<uint16_t*>(out);
-    p.own_tile_rows = p.prefix_tile_rows = dflash::paged_tile_rows();
+    p.own_tile_rows = L.tile[0];
+    p.prefix_tile_rows = L.tile[1];
     const auto stage = [&](int g) {
       p.slots = L.slots[g];
       p.part = at<float>(workspace, L.part[g]);

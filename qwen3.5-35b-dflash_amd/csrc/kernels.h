@@ -403,7 +403,8 @@ struct PagedParams {
   int own_tile_rows, prefix_tile_rows;
   int64_t part_rows[2];           // rows that part and prefix_part hold
 };
-int paged_tile_rows();
+int paged_tile_rows(int64_t tokens, int64_t sequences, int64_t group);
+int paged_slots(int tile_rows, int head_dim, int cus);
 void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStream_t stream);
 // `before`: the prefix stage's parameters (read where p.merge_prefix)
 void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, const PagedParams& before, hipStream_t stream);

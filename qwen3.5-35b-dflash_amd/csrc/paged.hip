@@ -12,6 +12,8 @@
 // A probability is rounded to 16 bits for the product with V, as V itself is held; the sum l takes it unrounded.  Each is off by
 // at most half a step, and its error is weighed as the value it multiplies: that leaves the sum about as far off as the output's own
 // rounding does.
+#include <algorithm>
+
 #include "kernels.h"
 
 namespace dflash {
@@ -19,8 +21,14 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct Bf16 {
+  typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kExponent = 0x7F80;  // all ones: an infinity or NaN
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
   static __device__ __forceinline__ uint16_t from_f32(float v) { return f32_to_bf16(v); }
   static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -28,15 +36,21 @@ struct Bf16 {
   }
 };
 struct Fp16 {
+  typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kExponent = 0x7C00;
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ float to_f32(uint16_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, v)); }
   static __device__ __forceinline__ uint16_t from_f32(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
   static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <class E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return E::from_f32(a) | (static_cast<uint32_t>(E::from_f32(b)) << 16);
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), typename E::Pair));
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -402,6 +416,264 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(Page
   }
 }
 
+// ------------------------------------------------------------------ 128 rows, four waves of 32
+// For blocks of many rows.  A workgroup takes 64 keys at a time through LDS, two stages of keys and values; wave w has rows 32 w
+// to 32 w + 31 for all of them.  Scores transposed again: lane l holds query row l & 31 and keys 8 (e / 4) + 4 (l >> 5) + e % 4 of a
+// 32-key block (e: element of the 32x32 result), whose elements 8 s to 8 s + 7 are, as a reduction's octet l >> 5, the B operand of
+// O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's operand needs eight keys of a dim: the
+// values are transposed on their way into LDS, in the order of those octets (slot 2 s + (l >> 5)).
+// The rows' running maximum is a reference that moves only when a score exceeds it by 8 (weights reach 2^8, their relative precision
+// is the same): the accumulators are rescaled a few times a row instead of at every step.
+constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
+// 16-byte slot of a row with a swizzle that spreads both the transposing writes and the reads over the banks
+template <int D>
+__device__ __forceinline__ int value_slot(int dim, int slot) {
+  return dim * 8 + (slot ^ ((dim ^ (dim >> (D == 256 ? 3 : 2))) & 7));
+}
+template <int D, class E, bool kPrefix>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
+  constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR, VD = D / 32, VW = VD / 2;
+  __shared__ u32x4 kbuf[2][64 * SL];
+  __shared__ u32x4 vbuf[2][D * 8];
+  __shared__ int odd;  // a stage lacks values that are infinite or NaN
+  const int kvh = blockIdx.x % p.kv;
+  Share w;
+  if (!(kPrefix ? prefix_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)
+                : own_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)))
+    return;
+  const PagedSide& side = kPrefix ? p.prefix : p.own;
+  const bool causal = !kPrefix && p.causal;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+  const int rows = w.tokens * p.group, nrows = min(kLargeRows, rows - w.tile * kLargeRows);
+  const int row0 = w.tile * kLargeRows;
+  const int r = row0 + min(wave * 32 + l31, nrows - 1);
+  const int tok = r / p.group, head = kvh * p.group + r - tok * p.group;
+  const int visible = visible_keys(w.keys, w.tokens, tok, causal);
+  const int least = visible_keys(w.keys, w.tokens, uniform(row0 / p.group), causal);
+  const int n = visible_keys(w.keys, w.tokens, uniform((row0 + nrows - 1) / p.group), causal);
+  const int k0 = w.chunk * w.c * kLargeUnit, k1 = min(k0 + w.c * kLargeUnit, n);
+  const int steps = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
+
+  u32x4 q[KS];
+  {
+    const uint16_t* qr = p.query + (w.start + tok) * p.query_token + head * p.query_head + 8 * half;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qr + 16 * s);
+  }
+  if (tid == 0) odd = 0;
+
+  // staging: thread tid holds 16 bytes of key rows tid / SL, + KR, ..., and VD dims of the eight keys of slot tid / 32, which are
+  // 4 (slot % 2) + 0..3 and 8 more of the 16-key group slot / 2
+  const char* keys = reinterpret_cast<const char*>(side.keys + kvh * side.key_head);
+  const char* vals = reinterpret_cast<const char*>(side.values + kvh * side.value_head);
+  const int krow = static_cast<int>(2 * side.key_row), vrow = static_cast<int>(2 * side.value_row);  // bytes
+  const uint32_t kcol = tid % SL * 16, vcol = (tid & 31) * VD * 2;
+  const uint32_t koff = (tid / SL & 15) * krow + kcol, voff = 4 * half * vrow + vcol;
+  u32x4 ks[KP];
+  uint32_t vs[8][VW];
+  const auto load_value = [&](int i, const char* src) {
+    if (VW == 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+      for (int k = 0; k < VW; ++k) vs[i][k] = v[k];
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(src);
+      vs[i][0] = v.x;
+      vs[i][1] = v.y;
+    }
+  };
+  const auto load = [&](int key0) {
+    if (key0 + 64 <= n) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const PageAt at = page_at(side, w.table, key0 / 16 + g);
+        const char* base = keys + 2 * at.page * side.key_page + static_cast<int64_t>(at.row) * krow;
+#pragma unroll
+        for (int i = 0; i < KP / 4; ++i)
+          ks[g * (KP / 4) + i] = *reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(i * KR) * krow + koff);
+      }
+      const PageAt at = page_at(side, w.table, key0 / 16 + wave);
+      const char* base = vals + 2 * at.page * side.value_page + static_cast<int64_t>(at.row) * vrow;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) load_value(i, base + static_cast<int64_t>((i >> 2) * 8 + (i & 3)) * vrow + voff);
+    } else {  // the last tile: rows past the last key repeat it
+      const int last = (n - 1) / 16;
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int g = min(key0 / 16 + i * KR / 16, last);
+        const PageAt at = page_at(side, w.table, g);
+        ks[i] = *reinterpret_cast<const u32x4*>(keys + 2 * at.page * side.key_page +
+                                                (at.row + min((i * KR + tid / SL) & 15, n - 1 - 16 * g)) * static_cast<int64_t>(krow) + kcol);
+      }
+      const int g = min(key0 / 16 + wave, last);
+      const PageAt at = page_at(side, w.table, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        load_value(i, vals + 2 * at.page * side.value_page +
+                          (at.row + min((i >> 2) * 8 + 4 * half + (i & 3), n - 1 - 16 * g)) * static_cast<int64_t>(vrow) + vcol);
+    }
+  };
+  const auto store = [&](int stage, int key0) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const int row = i * KR + tid / SL;
+      kbuf[stage][row * SL + ((tid % SL) ^ (row & (SL - 1)))] = ks[i];
+    }
+    if (key0 + 64 > least) {
+      // Some row masks some of these keys: its weights there are 0, but 0 times an infinite or NaN value is not.  Such values, and
+      // keys past the last one, are staged as zeros.
+      bool wild = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = key0 + 16 * wave + (i >> 2) * 8 + 4 * half + (i & 3) < n;
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const uint32_t x = in ? vs[i][k] : 0, high = E::kExponent << 16;
+          const bool a = (x & E::kExponent) == E::kExponent, b = (x & high) == high;
+          wild |= a || b;
+          vs[i][k] = x & (a ? 0xFFFF0000u : ~0u) & (b ? 0xFFFFu : ~0u);
+        }
+      }
+      if (wild) odd = 1;
+    }
+#pragma unroll
+    for (int d = 0; d < VD; ++d) {
+      u32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = __builtin_amdgcn_perm(vs[2 * i + 1][d >> 1], vs[2 * i][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+      vbuf[stage][value_slot<D>((tid & 31) * VD + d, tid >> 5)] = v;
+    }
+  };
+
+  f32x16 o[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
+
+  if (steps > 0) {
+    load(k0);
+    __syncthreads();  // odd is cleared
+    store(0, k0);
+  }
+  __syncthreads();
+  if (wave * 32 >= nrows) {  // no rows: the wave only stages
+    for (int i = 1; i < steps; ++i) {
+      load(k0 + 64 * i);
+      store(i & 1, k0 + 64 * i);
+      __syncthreads();
+    }
+    return;
+  }
+  for (int i = 0; i < steps; ++i) {
+    const int key0 = k0 + 64 * i, stage = i & 1;
+    if (i + 1 < steps) load(key0 + 64);
+    f32x16 sc[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        sc[b] = E::mfma32(kbuf[stage][(32 * b + l31) * SL + ((2 * s + half) ^ (l31 & (SL - 1)))], q[s], sc[b]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const bool masked = key0 + 64 > least;
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (key0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= visible) sc[b][e] = -__builtin_inff();
+    }
+    float mc = sc[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mc = fmaxf(mc, sc[b][e]);
+    mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
+    // a row that has seen no key keeps weights of 0 (the exponent is -inf); a NaN score, which the maximum skips, makes l and
+    // o NaN, and so they stay
+    const bool move = (mc - m) * p.scale_log2 > 8.f || (m == -__builtin_inff() && mc > m);
+    if (__any(move)) {
+      const float to = move ? mc : m;
+      const float corr = __builtin_amdgcn_exp2f(__builtin_fmaf(m, p.scale_log2, to == -__builtin_inff() ? 0.f : -to * p.scale_log2));
+      l *= move ? corr : 1.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[c][e] *= move ? corr : 1.f;
+      m = to;
+    }
+    const float ref = m == -__builtin_inff() ? 0.f : m * p.scale_log2;
+    u32x4 pf[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], p.scale_log2, -ref));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e + 1], p.scale_log2, -ref));
+        l += x + y;
+        pf[2 * b + (e >> 3)][(e & 7) >> 1] = pack2<E>(x, y);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) o[c] = E::mfma32(vbuf[stage][value_slot<D>(32 * c + l31, 2 * s + half)], pf[s], o[c]);
+    if (i + 1 < steps) {
+      store(stage ^ 1, key0 + 64);
+      __syncthreads();
+    }
+  }
+  if (steps > 0 && odd) {
+    // the values left out of the stages: infinite or NaN in the rows that see them, whatever their (positive) weight
+    for (int key = k0 + max(0, (least - k0) / 64) * 64; key < k1; ++key) {
+      const PageAt at = page_at(side, w.table, key / 16);
+      const char* src = vals + 2 * at.page * side.value_page + static_cast<int64_t>(at.row + key % 16) * vrow;
+      if (key >= visible) continue;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(src + 2 * (32 * c + 2 * e + 4 * half));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t x = (y < 2 ? v.x : v.y) >> (16 * (y & 1)) & 0xFFFF;
+            if ((x & E::kExponent) == E::kExponent) o[c][e + y] += E::to_f32(x);
+          }
+        }
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (wave * 32 + l31 >= nrows) return;
+  const int64_t out = static_cast<int64_t>(w.start + tok) * p.heads + head;
+  if (w.partial >= 0) {
+    const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * kLargeRows + wave * 32 + l31;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(p.part + held * D + 32 * c + 2 * e + 4 * half) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
+    if (half == 0) {
+      p.ml[held] = make_float2(m, l);
+      if (w.chunk == 0) p.info[out] = make_int2(static_cast<int>(held), w.chunks);
+    }
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<uint2*>(p.out + out * D + 32 * c + 2 * e + 4 * half) =
+            make_uint2(pack2<E>(o[c][e] * inv, o[c][e + 1] * inv), pack2<E>(o[c][e + 2] * inv, o[c][e + 3] * inv));
+    if (half == 0 && w.chunk == 0) p.info[out] = make_int2(0, 0);
+  }
+}
+
 // ------------------------------------------------------------------ merge
 // kWaves waves per (token, head), D / 64 dims a lane; wave w takes the row's partial results w, w + kWaves, ...: first every maximum
 // and sum, a partial a lane, then their rows, several in flight.  The order of the additions depends on the sizes alone.
@@ -497,8 +769,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
 
 }  // namespace
 
-// Rows a stage's tiles have.
-int paged_tile_rows() { return kSmallRows; }
+// Rows of a stage's tiles, by the rows a sequence has on average: up to 32 take the kernel of 16 rows, whose waves share the
+// keys out; more take the one of 128, whose waves share the keys' way through LDS.
+int paged_tile_rows(int64_t tokens, int64_t sequences, int64_t group) {
+  const int64_t blocks = std::max<int64_t>(1, std::min(tokens, sequences));
+  return tokens * group > 32 * blocks ? kLargeRows : kSmallRows;
+}
+// Workgroups that a stage's work is cut for: as many as run at once.
+int paged_slots(int tile_rows, int head_dim, int cus) { return tile_rows == kLargeRows && head_dim == 256 ? cus : 2 * cus; }
 
 template <int D, class E>
 static void launch_append(const AppendParams& p, hipStream_t stream) {
@@ -512,16 +790,19 @@ void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStre
   else bf16 ? launch_append<128, Bf16>(p, stream) : launch_append<128, Fp16>(p, stream);
 }
 
+template <int D, class E, bool kPrefix>
+static void launch_stage(const PagedParams& p, int tile_rows, int64_t tiles, hipStream_t stream) {
+  const dim3 grid(max_chunks(tiles, p.kv, p.slots) * p.kv);
+  if (tile_rows == kLargeRows) hipLaunchKernelGGL((paged_large_kernel<D, E, kPrefix>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((paged_small_kernel<D, E, kPrefix>), grid, dim3(256), 0, stream, p);
+}
 template <int D, class E>
 static void launch_attend(const PagedParams& p, const PagedParams& before, hipStream_t stream) {
-  if (p.merge_prefix) {
-    const int64_t tiles = seq_tiles(p.T, p.group, kSmallRows);
-    hipLaunchKernelGGL((paged_small_kernel<D, E, true>), dim3(max_chunks(tiles, p.kv, before.slots) * p.kv), dim3(256), 0,
-                       stream, before);
-  }
-  const int64_t tiles = max_tiles(p.T, p.B, p.group, kSmallRows);
-  hipLaunchKernelGGL((paged_small_kernel<D, E, false>), dim3(max_chunks(tiles, p.kv, p.slots) * p.kv), dim3(256), 0, stream, p);
-  if (!p.merge_prefix && p.own.capacity <= kSmallUnit) return;  // one chunk a tile: nothing to merge
+  const int own = p.own_tile_rows, front = p.prefix_tile_rows;
+  if (p.merge_prefix) launch_stage<D, E, true>(before, front, seq_tiles(p.T, p.group, front), stream);
+  launch_stage<D, E, false>(p, own, max_tiles(p.T, p.B, p.group, own), stream);
+  const int least = own == kLargeRows ? kLargeUnit * kLargeLeast : kSmallUnit;
+  if (!p.merge_prefix && p.own.capacity <= least) return;  // one chunk a tile: nothing to merge
   const int64_t rows = static_cast<int64_t>(p.T) * p.heads;
   // few rows may be in many chunks: four waves a row
   if (rows <= 4096) hipLaunchKernelGGL((paged_merge_kernel<D, E, 4>), dim3(rows), dim3(256), 0, stream, p);
