@@ -13,6 +13,7 @@
 // at most half a step, and its error is weighed as the value it multiplies: that leaves the sum about as far off as the output's own
 // rounding does.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -417,24 +418,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(Page
 }
 
 // ------------------------------------------------------------------ 128 rows, four waves of 32
-// For blocks of many rows.  A workgroup takes 64 keys at a time through LDS, two stages of keys and values; wave w has rows 32 w
-// to 32 w + 31 for all of them.  Scores transposed again: lane l holds query row l & 31 and keys 8 (e / 4) + 4 (l >> 5) + e % 4 of a
-// 32-key block (e: element of the 32x32 result), whose elements 8 s to 8 s + 7 are, as a reduction's octet l >> 5, the B operand of
-// O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's operand needs eight keys of a dim: the
-// values are transposed on their way into LDS, in the order of those octets (slot 2 s + (l >> 5)).
+// For blocks of many rows.  A workgroup takes 64 keys at a time through LDS, two stages of keys and values, loaded straight into
+// it a step ahead; wave w has rows 32 w to 32 w + 31 for all of them.  Scores transposed again: lane l holds query row l & 31 and
+// keys 8 (e / 4) + 4 (l >> 5) + e % 4 of a 32-key block (e: element of the 32x32 result), whose elements 8 s to 8 s + 7 are, as a
+// reduction's octet l >> 5, the B operand of O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's
+// operand needs eight keys of a dim: two transposing LDS reads of four keys each.
 // The rows' running maximum is a reference that moves only when a score exceeds it by 8 (weights reach 2^8, their relative precision
 // is the same): the accumulators are rescaled a few times a row instead of at every step.
-constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
-// 16-byte slot of a row with a swizzle that spreads both the transposing writes and the reads over the banks
-template <int D>
-__device__ __forceinline__ int value_slot(int dim, int slot) {
-  return dim * 8 + (slot ^ ((dim ^ (dim >> (D == 256 ? 3 : 2))) & 7));
+// A run of n matrix instructions that take one operand each from LDS: use(i, read(i)) for all i, each read kAhead instructions ahead of
+// its use.  Left to itself the compiler puts each read right before its use and waits for it (a read takes four times as long as
+// the instruction), so the order is fixed.
+template <int n, int kAhead, class Read, class Use>
+__device__ __forceinline__ void feed(const Read& read, const Use& use) {
+  u32x4 f[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) f[i] = read(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const u32x4 now = f[i % kAhead];
+    use(i, now);
+    if (i + kAhead < n) f[i % kAhead] = read(i + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
+// Four keys of one dim a lane: lane j of 16 gives the place of row j / 4, dims 4 (j % 4) on, and gets dim j of the four rows.
+__device__ __forceinline__ uint2 read_turned(const char* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
+}
+// 16 bytes a lane from global memory to 1 KB of LDS, lane by lane.
+__device__ __forceinline__ void copy_to_lds(const char* src, char* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16,
+                                   0, 0);
+}
+constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
 template <int D, class E, bool kPrefix>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
-  constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR, VD = D / 32, VW = VD / 2;
-  __shared__ u32x4 kbuf[2][64 * SL];
-  __shared__ u32x4 vbuf[2][D * 8];
+  constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR;
+  constexpr int kStage = 64 * D * 2;  // bytes of a stage of keys or values
+  constexpr int kAhead = 4;
+  __shared__ __align__(16) char lds[4 * kStage];  // keys of both stages, then values
   __shared__ int odd;  // a stage lacks values that are infinite or NaN
   const int kvh = blockIdx.x % p.kv;
   Share w;
@@ -462,89 +486,74 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   }
   if (tid == 0) odd = 0;
 
-  // staging: thread tid holds 16 bytes of key rows tid / SL, + KR, ..., and VD dims of the eight keys of slot tid / 32, which are
-  // 4 (slot % 2) + 0..3 and 8 more of the 16-key group slot / 2
+  // Staging: thread tid loads 16-byte slot tid % SL of rows tid / SL, + KR, ... of keys and values.  A 16-row group's place is a 64-bit
+  // offset that is found a step ahead, group g of the step in lane g; rows inside it are 32-bit offsets that do not change.
+  // LDS: slot c of row r holds 16-byte piece c ^ (r % 16) of the keys, c ^ 4 (r % 8 or 4) of the values, so that neither kind of read
+  // puts two of the lanes that read together on one bank; the loads permute the pieces, since their own order in LDS is fixed.
   const char* keys = reinterpret_cast<const char*>(side.keys + kvh * side.key_head);
   const char* vals = reinterpret_cast<const char*>(side.values + kvh * side.value_head);
   const int krow = static_cast<int>(2 * side.key_row), vrow = static_cast<int>(2 * side.value_row);  // bytes
-  const uint32_t kcol = tid % SL * 16, vcol = (tid & 31) * VD * 2;
-  const uint32_t koff = (tid / SL & 15) * krow + kcol, voff = 4 * half * vrow + vcol;
-  u32x4 ks[KP];
-  uint32_t vs[8][VW];
-  const auto load_value = [&](int i, const char* src) {
-    if (VW == 4) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(src);
+  const int slot = tid % SL, tr = tid / SL;
+  const uint32_t vcol = (slot ^ (tr & (D == 256 ? 7 : 3)) << 2) * 16;
+  const auto kcol = [&](int i) { return static_cast<uint32_t>((slot ^ ((tr + i * KR) & 15)) * 16); };
+  uint32_t koff[KP / 4], voff[KP / 4];
 #pragma unroll
-      for (int k = 0; k < VW; ++k) vs[i][k] = v[k];
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(src);
-      vs[i][0] = v.x;
-      vs[i][1] = v.y;
-    }
+  for (int i = 0; i < KP / 4; ++i) {
+    koff[i] = (tr + i * KR) * krow + kcol(i);
+    voff[i] = (tr + i * KR) * vrow + vcol;
+  }
+  int page = 0, inside = 0;  // of group lane % 4 of the step to load next
+  const auto find = [&](int key0) {
+    const PageAt at = page_at(side, w.table, min(key0 / 16 + (lane & 3), (n - 1) / 16));
+    page = at.page;
+    inside = at.row;
   };
-  const auto load = [&](int key0) {
-    if (key0 + 64 <= n) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const PageAt at = page_at(side, w.table, key0 / 16 + g);
-        const char* base = keys + 2 * at.page * side.key_page + static_cast<int64_t>(at.row) * krow;
-#pragma unroll
-        for (int i = 0; i < KP / 4; ++i)
-          ks[g * (KP / 4) + i] = *reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(i * KR) * krow + koff);
-      }
-      const PageAt at = page_at(side, w.table, key0 / 16 + wave);
-      const char* base = vals + 2 * at.page * side.value_page + static_cast<int64_t>(at.row) * vrow;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) load_value(i, base + static_cast<int64_t>((i >> 2) * 8 + (i & 3)) * vrow + voff);
-    } else {  // the last tile: rows past the last key repeat it
-      const int last = (n - 1) / 16;
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int g = min(key0 / 16 + i * KR / 16, last);
-        const PageAt at = page_at(side, w.table, g);
-        ks[i] = *reinterpret_cast<const u32x4*>(keys + 2 * at.page * side.key_page +
-                                                (at.row + min((i * KR + tid / SL) & 15, n - 1 - 16 * g)) * static_cast<int64_t>(krow) + kcol);
-      }
-      const int g = min(key0 / 16 + wave, last);
-      const PageAt at = page_at(side, w.table, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        load_value(i, vals + 2 * at.page * side.value_page +
-                          (at.row + min((i >> 2) * 8 + 4 * half + (i & 3), n - 1 - 16 * g)) * static_cast<int64_t>(vrow) + vcol);
-    }
-  };
-  const auto store = [&](int stage, int key0) {
+  const auto load = [&](int stage, int key0) {
+    const int64_t kat = page * (2 * side.key_page) + static_cast<int64_t>(inside) * krow;
+    const int64_t vat = page * (2 * side.value_page) + static_cast<int64_t>(inside) * vrow;
+    const auto of = [](int64_t v, int g) {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), g);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32), g);
+      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    };
+    char* to = lds + stage * kStage + wave * 1024;
+    const bool tail = key0 + 64 > n;  // rows past the last key repeat it
 #pragma unroll
     for (int i = 0; i < KP; ++i) {
-      const int row = i * KR + tid / SL;
-      kbuf[stage][row * SL + ((tid % SL) ^ (row & (SL - 1)))] = ks[i];
-    }
-    if (key0 + 64 > least) {
-      // Some row masks some of these keys: its weights there are 0, but 0 times an infinite or NaN value is not.  Such values, and
-      // keys past the last one, are staged as zeros.
-      bool wild = false;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = key0 + 16 * wave + (i >> 2) * 8 + 4 * half + (i & 3) < n;
-#pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          const uint32_t x = in ? vs[i][k] : 0, high = E::kExponent << 16;
-          const bool a = (x & E::kExponent) == E::kExponent, b = (x & high) == high;
-          wild |= a || b;
-          vs[i][k] = x & (a ? 0xFFFF0000u : ~0u) & (b ? 0xFFFFu : ~0u);
-        }
+      uint32_t k = koff[i % (KP / 4)], v = voff[i % (KP / 4)];
+      if (tail) {
+        const int row = min((i * KR + tr) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16));
+        k = row * krow + kcol(i);
+        v = row * vrow + vcol;
       }
-      if (wild) odd = 1;
-    }
-#pragma unroll
-    for (int d = 0; d < VD; ++d) {
-      u32x4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = __builtin_amdgcn_perm(vs[2 * i + 1][d >> 1], vs[2 * i][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
-      vbuf[stage][value_slot<D>((tid & 31) * VD + d, tid >> 5)] = v;
+      copy_to_lds(keys + of(kat, i / (KP / 4)) + k, to + i * 4096);
+      copy_to_lds(vals + of(vat, i / (KP / 4)) + v, to + 2 * kStage + i * 4096);
     }
   };
+  // Some row masks some of a step's keys: its weights there are 0, but 0 times an infinite or NaN value is not.  Such values, and keys
+  // past the last one, become zeros in the stage.
+  const auto clean = [&](int stage, int key0) {
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      u32x4* at = reinterpret_cast<u32x4*>(lds + (2 + stage) * kStage + i * 4096 + tid * 16);
+      u32x4 v = *at;
+      const bool in = key0 + i * KR + tr < n;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t x = in ? v[k] : 0, high = E::kExponent << 16;
+        const bool a = (x & E::kExponent) == E::kExponent, b = (x & high) == high;
+        wild |= a || b;
+        v[k] = x & (a ? 0xFFFF0000u : ~0u) & (b ? 0xFFFFu : ~0u);
+      }
+      *at = v;
+    }
+    if (wild) odd = 1;
+    lds_barrier();
+  };
+  const uint32_t kr = l31 * (2 * D) + ((half ^ l31) & 15) * 16;
+  const int j15 = lane & 15, turn = D == 256 ? 4 * half + (j15 >> 2) : j15 >> 2;
+  const uint32_t vr = 2 * kStage + (4 * half + (j15 >> 2)) * (2 * D) + (2 * (lane >> 4 & 1) + (j15 >> 1 & 1)) * 16 + (j15 & 1) * 8 + turn * 64;
 
   f32x16 o[NC];
 #pragma unroll
@@ -554,34 +563,43 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
 
   if (steps > 0) {
-    load(k0);
-    __syncthreads();  // odd is cleared
-    store(0, k0);
+    find(k0);
+    load(0, k0);
+    find(k0 + 64);
   }
-  __syncthreads();
+  wait_vmem();
+  lds_barrier();
   if (wave * 32 >= nrows) {  // no rows: the wave only stages
-    for (int i = 1; i < steps; ++i) {
-      load(k0 + 64 * i);
-      store(i & 1, k0 + 64 * i);
-      __syncthreads();
+    for (int i = 0; i < steps; ++i) {
+      if (i + 1 < steps) {
+        load(~i & 1, k0 + 64 * (i + 1));
+        find(k0 + 64 * (i + 2));
+      }
+      if (k0 + 64 * (i + 1) > least) clean(i & 1, k0 + 64 * i);
+      wait_vmem();
+      lds_barrier();
     }
     return;
   }
-  for (int i = 0; i < steps; ++i) {
-    const int key0 = k0 + 64 * i, stage = i & 1;
-    if (i + 1 < steps) load(key0 + 64);
+  const auto step = [&](auto stage_, int i) {
+    constexpr int stage = decltype(stage_)::value;
+    const int key0 = k0 + 64 * i;
+    if (i + 1 < steps) {
+      load(stage ^ 1, key0 + 64);
+      find(key0 + 128);
+    }
+    if (key0 + 64 > least) clean(stage, key0);
     f32x16 sc[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        sc[b] = E::mfma32(kbuf[stage][(32 * b + l31) * SL + ((2 * s + half) ^ (l31 & (SL - 1)))], q[s], sc[b]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    const bool masked = key0 + 64 > least;
-    if (masked) {
+    feed<2 * KS, kAhead>(
+        [&](int i) {
+          return *reinterpret_cast<const u32x4*>(lds + ((kr ^ (32 * (i >> 1))) + (stage * kStage + (i & 1) * 64 * D)));
+        },
+        [&](int i, u32x4 k) { sc[i & 1] = E::mfma32(k, q[i >> 1], sc[i & 1]); });
+    if (key0 + 64 > least) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -609,24 +627,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     }
     const float ref = m == -__builtin_inff() ? 0.f : m * p.scale_log2;
     u32x4 pf[4];
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], p.scale_log2, -ref));
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e + 1], p.scale_log2, -ref));
-        l += x + y;
+        sum[0] += x;
+        sum[1] += y;
         pf[2 * b + (e >> 3)][(e & 7) >> 1] = pack2<E>(x, y);
       }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) o[c] = E::mfma32(vbuf[stage][value_slot<D>(32 * c + l31, 2 * s + half)], pf[s], o[c]);
-    if (i + 1 < steps) {
-      store(stage ^ 1, key0 + 64);
-      __syncthreads();
-    }
+    l += sum[0] + sum[1];
+    feed<4 * NC, kAhead>(
+        [&](int i) {
+          const char* at = lds + ((vr ^ (64 * (i % NC))) + (stage * kStage + i / NC * 32 * D));
+          const uint2 a = read_turned(at), b = read_turned(at + 16 * D);
+          return u32x4{a.x, a.y, b.x, b.y};
+        },
+        [&](int i, u32x4 v) { o[i % NC] = E::mfma32(v, pf[i / NC], o[i % NC]); });
+    wait_vmem();
+    lds_barrier();
+  };
+  for (int i = 0; i < steps; i += 2) {
+    step(std::integral_constant<int, 0>{}, i);
+    if (i + 1 < steps) step(std::integral_constant<int, 1>{}, i + 1);
   }
   if (steps > 0 && odd) {
     // the values left out of the stages: infinite or NaN in the rows that see them, whatever their (positive) weight
