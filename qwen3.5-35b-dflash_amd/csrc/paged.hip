@@ -457,7 +457,7 @@ template <int D, class E, bool kPrefix>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
   constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR;
   constexpr int kStage = 64 * D * 2;  // bytes of a stage of keys or values
-  constexpr int kAhead = 4;
+  constexpr int kAhead = D == 256 ? 4 : 3;
   __shared__ __align__(16) char lds[4 * kStage];  // keys of both stages, then values
   __shared__ int odd;  // a stage lacks values that are infinite or NaN
   const int kvh = blockIdx.x % p.kv;
@@ -482,7 +482,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   {
     const uint16_t* qr = p.query + (w.start + tok) * p.query_token + head * p.query_head + 8 * half;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qr + 16 * s);
+    for (int s = 0; s < KS; ++s) {
+      q[s] = *reinterpret_cast<const u32x4*>(qr + 16 * s);
+      // at head dim 256 the queries stay in the accumulation registers, where matrix instructions take them from
+      if constexpr (D == 256) asm volatile("" : "+a"(q[s]));
+    }
   }
   if (tid == 0) odd = 0;
 
@@ -502,32 +506,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     koff[i] = (tr + i * KR) * krow + kcol(i);
     voff[i] = (tr + i * KR) * vrow + vcol;
   }
-  int page = 0, inside = 0;  // of group lane % 4 of the step to load next
+  PageAt place = {0, 0}, ahead = {0, 0};  // of group lane % 4 of the step whose values, and whose keys, are loaded next
   const auto find = [&](int key0) {
-    const PageAt at = page_at(side, w.table, min(key0 / 16 + (lane & 3), (n - 1) / 16));
-    page = at.page;
-    inside = at.row;
+    place = ahead;
+    ahead = page_at(side, w.table, min(key0 / 16 + (lane & 3), (n - 1) / 16));
   };
-  const auto load = [&](int stage, int key0) {
-    const int64_t kat = page * (2 * side.key_page) + static_cast<int64_t>(inside) * krow;
-    const int64_t vat = page * (2 * side.value_page) + static_cast<int64_t>(inside) * vrow;
-    const auto of = [](int64_t v, int g) {
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), g);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32), g);
-      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-    };
-    char* to = lds + stage * kStage + wave * 1024;
+  const auto load = [&](bool values, const PageAt& at, int stage, int key0) {
+    const int stride = values ? vrow : krow;
+    const int64_t offset = at.page * (2 * (values ? side.value_page : side.key_page)) + static_cast<int64_t>(at.row) * stride;
+    char* to = lds + (stage + (values ? 2 : 0)) * kStage + wave * 1024;
     const bool tail = key0 + 64 > n;  // rows past the last key repeat it
 #pragma unroll
     for (int i = 0; i < KP; ++i) {
-      uint32_t k = koff[i % (KP / 4)], v = voff[i % (KP / 4)];
-      if (tail) {
-        const int row = min((i * KR + tr) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16));
-        k = row * krow + kcol(i);
-        v = row * vrow + vcol;
-      }
-      copy_to_lds(keys + of(kat, i / (KP / 4)) + k, to + i * 4096);
-      copy_to_lds(vals + of(vat, i / (KP / 4)) + v, to + 2 * kStage + i * 4096);
+      const int g = i / (KP / 4);
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(offset), g);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(offset) >> 32), g);
+      const char* base = (values ? vals : keys) + static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+      uint32_t off = values ? voff[i % (KP / 4)] : koff[i % (KP / 4)];
+      if (tail)
+        off = min((i * KR + tr) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16)) * stride + (values ? vcol : kcol(i));
+      copy_to_lds(base + off, to + i * 4096);
     }
   };
   // Some row masks some of a step's keys: its weights there are 0, but 0 times an infinite or NaN value is not.  Such values, and keys
@@ -551,9 +549,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     if (wild) odd = 1;
     lds_barrier();
   };
-  const uint32_t kr = l31 * (2 * D) + ((half ^ l31) & 15) * 16;
+  uint32_t kr = l31 * (2 * D) + ((half ^ l31) & 15) * 16;
   const int j15 = lane & 15, turn = D == 256 ? 4 * half + (j15 >> 2) : j15 >> 2;
-  const uint32_t vr = 2 * kStage + (4 * half + (j15 >> 2)) * (2 * D) + (2 * (lane >> 4 & 1) + (j15 >> 1 & 1)) * 16 + (j15 & 1) * 8 + turn * 64;
+  uint32_t vr = 2 * kStage + (4 * half + (j15 >> 2)) * (2 * D) + (2 * (lane >> 4 & 1) + (j15 >> 1 & 1)) * 16 + (j15 & 1) * 8 + turn * 64;
 
   f32x16 o[NC];
 #pragma unroll
@@ -562,55 +560,73 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
 
+  // Step i multiplies its weights with its values, and before that the next step's keys with the queries: the exponentials of the one
+  // stand between the matrix instructions of the other, and the maximum of the next scores between those of the values.  So keys are
+  // loaded two steps ahead, values one.
+  const auto fill = [&](int i) {  // what step i loads
+    if (i + 1 < steps) load(true, place, ~i & 1, k0 + 64 * (i + 1));
+    if (i + 2 < steps) load(false, ahead, i & 1, k0 + 64 * (i + 2));
+    find(k0 + 64 * (i + 3));
+  };
+  const auto arrive = [&]() {
+    wait_vmem();
+    lds_barrier();
+  };
   if (steps > 0) {
     find(k0);
-    load(0, k0);
+    load(false, ahead, 0, k0);
+    load(true, ahead, 0, k0);
     find(k0 + 64);
+    if (steps > 1) load(false, ahead, 1, k0 + 64);
+    find(k0 + 128);
   }
-  wait_vmem();
-  lds_barrier();
+  arrive();
   if (wave * 32 >= nrows) {  // no rows: the wave only stages
+    if (steps > 2) lds_barrier();
     for (int i = 0; i < steps; ++i) {
-      if (i + 1 < steps) {
-        load(~i & 1, k0 + 64 * (i + 1));
-        find(k0 + 64 * (i + 2));
-      }
+      fill(i);
       if (k0 + 64 * (i + 1) > least) clean(i & 1, k0 + 64 * i);
-      wait_vmem();
-      lds_barrier();
+      arrive();
     }
     return;
   }
-  const auto step = [&](auto stage_, int i) {
+  f32x16 sc[2][2];  // scores of even and odd steps, 32 keys each
+  const auto clear = [&](f32x16 (&t)[2]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t[b][e] = 0.f;
+  };
+  const auto hide = [&](f32x16 (&t)[2], int key0) {
+    if (key0 + 64 <= least) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (key0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= visible) t[b][e] = -__builtin_inff();
+  };
+  const auto key_at = [&](int stage, int i) {
+    return *reinterpret_cast<const u32x4*>(lds + ((kr ^ (32 * (i >> 1))) + (stage * kStage + (i & 1) * 64 * D)));
+  };
+  float mc = -__builtin_inff();  // maximum of the scores of the step to come
+  if (steps > 0) {
+    clear(sc[0]);
+    feed<2 * KS, kAhead>([&](int i) { return key_at(0, i); },
+                         [&](int i, u32x4 k) { sc[0][i & 1] = E::mfma32(k, q[i >> 1], sc[0][i & 1]); });
+    hide(sc[0], k0);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) mc = fmaxf(mc, sc[0][e >> 4][e & 15]);
+    if (steps > 2) lds_barrier();  // step 0 loads step 2's keys where these were
+  }
+  const auto step = [&](auto stage_, auto last_, int i) {
     constexpr int stage = decltype(stage_)::value;
+    constexpr bool more = !decltype(last_)::value;
     const int key0 = k0 + 64 * i;
-    if (i + 1 < steps) {
-      load(stage ^ 1, key0 + 64);
-      find(key0 + 128);
-    }
+    f32x16(&now)[2] = sc[stage];
+    f32x16(&next)[2] = sc[stage ^ 1];
+    fill(i);
     if (key0 + 64 > least) clean(stage, key0);
-    f32x16 sc[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
-    feed<2 * KS, kAhead>(
-        [&](int i) {
-          return *reinterpret_cast<const u32x4*>(lds + ((kr ^ (32 * (i >> 1))) + (stage * kStage + (i & 1) * 64 * D)));
-        },
-        [&](int i, u32x4 k) { sc[i & 1] = E::mfma32(k, q[i >> 1], sc[i & 1]); });
-    if (key0 + 64 > least) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (key0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= visible) sc[b][e] = -__builtin_inff();
-    }
-    float mc = sc[0][0];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mc = fmaxf(mc, sc[b][e]);
+    if constexpr (D == 256) asm volatile("" : "+v"(kr), "+v"(vr));  // no two dozen registers of places kept over the steps
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
     // a row that has seen no key keeps weights of 0 (the exponent is -inf); a NaN score, which the maximum skips, makes l and
     // o NaN, and so they stay
@@ -628,30 +644,60 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     const float ref = m == -__builtin_inff() ? 0.f : m * p.scale_log2;
     u32x4 pf[4];
     float sum[2] = {0.f, 0.f};
+    const auto weigh = [&](int e) {  // elements e and e + 1 of the step's 32
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][e & 15], p.scale_log2, -ref));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][(e & 15) + 1], p.scale_log2, -ref));
+      sum[0] += x;
+      sum[1] += y;
+      uint32_t both = pack2<E>(x, y);
+      asm volatile("" : "+v"(both));  // made here, between the matrix instructions, not where it is used
+      pf[e >> 3][(e & 7) >> 1] = both;
+    };
+    if constexpr (more) {
+      clear(next);
+      constexpr int kEach = KS / 8;  // instructions a pair of elements
+      feed<2 * KS, kAhead>([&](int k) { return key_at(stage ^ 1, k); },
+                           [&](int k, u32x4 v) {
+                             next[k & 1] = E::mfma32(v, q[k >> 1], next[k & 1]);
+                             if (k % kEach == 0) weigh(k / kEach * 2);
+                           });
+      hide(next, key0 + 64);
+    } else {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], p.scale_log2, -ref));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e + 1], p.scale_log2, -ref));
-        sum[0] += x;
-        sum[1] += y;
-        pf[2 * b + (e >> 3)][(e & 7) >> 1] = pack2<E>(x, y);
-      }
+      for (int e = 0; e < 32; e += 2) weigh(e);
+    }
     l += sum[0] + sum[1];
+    mc = -__builtin_inff();
     feed<4 * NC, kAhead>(
-        [&](int i) {
-          const char* at = lds + ((vr ^ (64 * (i % NC))) + (stage * kStage + i / NC * 32 * D));
+        [&](int k) {
+          const char* at = lds + ((vr ^ (64 * (k % NC))) + (stage * kStage + k / NC * 32 * D));
           const uint2 a = read_turned(at), b = read_turned(at + 16 * D);
           return u32x4{a.x, a.y, b.x, b.y};
         },
-        [&](int i, u32x4 v) { o[i % NC] = E::mfma32(v, pf[i / NC], o[i % NC]); });
-    wait_vmem();
-    lds_barrier();
+        [&](int k, u32x4 v) {
+          o[k % NC] = E::mfma32(v, pf[k / NC], o[k % NC]);
+          constexpr int kEach = NC / 4;  // instructions a pair of elements of the next scores
+          if (more && k % kEach == 0) {
+            const int e = k / kEach * 2;
+            mc = fmaxf(fmaxf(mc, next[e >> 4][e & 15]), next[e >> 4][(e & 15) + 1]);
+          }
+        });
+    arrive();
   };
-  for (int i = 0; i < steps; i += 2) {
-    step(std::integral_constant<int, 0>{}, i);
-    if (i + 1 < steps) step(std::integral_constant<int, 1>{}, i + 1);
+  if (steps > 0) {
+    const std::integral_constant<int, 0> even{};
+    const std::integral_constant<int, 1> uneven{};
+    int i = 0;
+    for (; i + 2 < steps; i += 2) {
+      step(even, std::false_type{}, i);
+      step(uneven, std::false_type{}, i + 1);
+    }
+    if (i + 1 < steps) {
+      step(even, std::false_type{}, i);
+      step(uneven, std::true_type{}, i + 1);
+    } else {
+      step(even, std::true_type{}, i);
+    }
   }
   if (steps > 0 && odd) {
     // the values left out of the stages: infinite or NaN in the rows that see them, whatever their (positive) weight
