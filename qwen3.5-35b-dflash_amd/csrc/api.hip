@@ -1259,6 +1259,7 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
     p.heads = static_cast<int>(heads);
     p.kv = static_cast<int>(kv);
     p.group = static_cast<int>(heads / kv);
+    p.by_group = dflash::fast_div(static_cast<uint32_t>(p.group));
     p.causal = causal != 0;
     p.merge_prefix = prefix != nullptr;
     p.scale_log2 = scale * 1.4426950408889634f;
@@ -1270,6 +1271,7 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
     p.prefix_tile_rows = L.tile[1];
     const auto stage = [&](int g) {
       p.slots = L.slots[g];
+      p.per_slot = 1.0 / L.slots[g];
       p.part = at<float>(workspace, L.part[g]);
       p.ml = at<float2>(workspace, L.ml[g]);
       p.info = at<int2>(workspace, L.info[g]);

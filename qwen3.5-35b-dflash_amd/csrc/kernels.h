@@ -386,7 +386,9 @@ struct PagedParams {
   PagedSide own, prefix;
   const int32_t* starts;          // [B + 1]
   int B, T, heads, kv, group, causal, merge_prefix;
+  FastDiv by_group;
   int slots;                      // workgroups that the work is cut for
+  double per_slot;                // 1 / slots
   float scale_log2;               // scale * log2(e)
   const uint16_t* query;
   int64_t query_token, query_head;

@@ -178,38 +178,45 @@ struct Share {
   const int32_t* table;
 };
 
+// Sum of a wave's 64 values and inclusive sums over its lanes, on the lanes' own data paths (a shuffle through LDS takes ten
+// times as long, and the search below is part of every workgroup's start).
+template <int kCtrl>
+__device__ __forceinline__ int shifted(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, 0xF, 0xF, true);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += shifted<0x111>(v);  // row_shr:1, within 16 lanes
+  v += shifted<0x112>(v);
+  v += shifted<0x114>(v);
+  v += shifted<0x118>(v);
+  const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31), c = __builtin_amdgcn_readlane(v, 47);
+  const int row = (threadIdx.x >> 4) & 3;
+  return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
 // Share `id` of the own-keys stage: every wave finds it by itself, 64 sequences at a time, one a lane.
 __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile_rows, int unit, int least, Share* out) {
   const int lane = threadIdx.x & 63;
   int64_t total = 0;
+  SeqSpan s{0, 0, 0};
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int64_t u = 0;
-    if (b0 + lane < p.B) {
-      const SeqSpan s = load_span(p, b0 + lane);
-      u = static_cast<int64_t>(seq_tiles(s.tokens, p.group, tile_rows)) * seq_units(s.keys, unit);
-    }
-    for (int o = 1; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
-    total += u;
+    s = SeqSpan{0, 0, 0};
+    if (b0 + lane < p.B) s = load_span(p, b0 + lane);
+    // tiles <= 2^18 and units <= 2^24: the product in two parts whose sums stay in 31 bits
+    const uint64_t u = static_cast<uint64_t>(seq_tiles(s.tokens, p.group, tile_rows)) * seq_units(s.keys, unit);
+    const int lo = wave_scan(static_cast<int>(u & 0xFFFFFF)), hi = wave_scan(static_cast<int>(u >> 24));
+    total += (static_cast<int64_t>(__builtin_amdgcn_readlane(hi, 63)) << 24) + __builtin_amdgcn_readlane(lo, 63);
   }
-  const int c = uniform(chunk_units(total, p.kv, p.slots, least));
+  const int c = uniform(chunk_units(total, p.kv, p.per_slot, least));
   int first = 0, held = 0;  // shares and partial tiles of the sequences before
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    SeqSpan s{0, 0, 0};
-    int n = 0, k = 1;
-    if (b0 + lane < p.B) {
-      s = load_span(p, b0 + lane);
-      k = tile_chunks(seq_units(s.keys, unit), c);
-      n = seq_tiles(s.tokens, p.group, tile_rows) * k;
+    if (p.B > 64) {
+      s = SeqSpan{0, 0, 0};
+      if (b0 + lane < p.B) s = load_span(p, b0 + lane);
     }
+    const int k = tile_chunks(seq_units(s.keys, unit), c), n = seq_tiles(s.tokens, p.group, tile_rows) * k;
     const int kept = k > 1 || p.merge_prefix ? n : 0;
-    int sum = n, sum_kept = kept;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int a = __shfl_up(sum, o, 64), d = __shfl_up(sum_kept, o, 64);
-      if (lane >= o) {
-        sum += a;
-        sum_kept += d;
-      }
-    }
+    const int sum = wave_scan(n), sum_kept = wave_scan(kept);
     const uint64_t m = __ballot(n > 0 && id < first + sum);
     if (m) {
       const int l = __builtin_ctzll(m);
@@ -218,7 +225,7 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
       out->start = __builtin_amdgcn_readlane(s.start, l);
       out->tokens = __builtin_amdgcn_readlane(s.tokens, l);
       out->keys = __builtin_amdgcn_readlane(s.keys, l);
-      out->tile = uniform(rest / chunks);
+      out->tile = uniform(static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks)));
       out->chunk = uniform(rest - out->tile * chunks);
       out->chunks = chunks;
       out->partial = chunks > 1 || p.merge_prefix
@@ -237,10 +244,11 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
 __device__ __forceinline__ bool prefix_share(const PagedParams& p, int id, int tile_rows, int unit, int least, Share* out) {
   const int keys = uniform(clampi(p.prefix.lengths[0], 0, p.prefix.capacity));
   const int tiles = seq_tiles(p.T, p.group, tile_rows), units = seq_units(keys, unit);
-  const int c = chunk_units(static_cast<int64_t>(tiles) * units, p.kv, p.slots, least);
-  const int chunks = tile_chunks(units, c);
+  const int c = uniform(chunk_units(static_cast<int64_t>(tiles) * units, p.kv, p.per_slot, least));
+  const int chunks = uniform(tile_chunks(units, c));
   if (id >= tiles * chunks) return false;
-  *out = Share{0, p.T, keys, id / chunks, id % chunks, chunks, id / chunks * chunks, c, p.prefix.table};
+  const int tile = uniform(static_cast<int>(static_cast<uint32_t>(id) / static_cast<uint32_t>(chunks)));
+  *out = Share{0, p.T, keys, tile, id - tile * chunks, chunks, tile * chunks, c, p.prefix.table};
   return true;
 }
 
@@ -255,7 +263,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(Page
   constexpr int NC = D / 16, KS = D / 32, VL = NC / 8, kPitch = D + 4;
   __shared__ __align__(16) float osum[4][16][kPitch];
   __shared__ float mx[4][16], ls[4][16];
-  const int kvh = blockIdx.x % p.kv;
+  const int kvh = uniform(static_cast<int>(blockIdx.x) % p.kv);
   Share w;
   if (!(kPrefix ? prefix_share(p, blockIdx.x / p.kv, kSmallRows, kSmallUnit, 1, &w)
                 : own_share(p, blockIdx.x / p.kv, kSmallRows, kSmallUnit, 1, &w)))
@@ -265,9 +273,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(Page
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, lr = lane & 15, kq = lane >> 4;
   const int rows = w.tokens * p.group, nrows = min(16, rows - w.tile * 16);
   const int r = w.tile * 16 + min(lr, nrows - 1);  // this lane's row in its block
-  const int tok = r / p.group, head = kvh * p.group + r - tok * p.group;
+  const int tok = divide(r, p.by_group), head = kvh * p.group + r - tok * p.group;
   const int visible = visible_keys(w.keys, w.tokens, tok, causal);
-  const int tok0 = uniform(w.tile * 16 / p.group), tok1 = uniform((w.tile * 16 + nrows - 1) / p.group);
+  const int tok0 = uniform(static_cast<int>(divide(w.tile * 16, p.by_group))), tok1 = uniform(static_cast<int>(divide(w.tile * 16 + nrows - 1, p.by_group)));
   const int least = visible_keys(w.keys, w.tokens, tok0, causal);  // keys that every row of the tile sees
   const int n = visible_keys(w.keys, w.tokens, tok1, causal);      // keys that some row sees
   const int k0 = w.chunk * w.c * kSmallUnit, k1 = min(k0 + w.c * kSmallUnit, n);
@@ -400,7 +408,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(Page
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) sum += ls[x][row] * factor(mx[x][row], Mr);
-    const int rr = w.tile * 16 + row, tk = rr / p.group, hd = kvh * p.group + rr - tk * p.group;
+    const int rr = w.tile * 16 + row, tk = divide(rr, p.by_group), hd = kvh * p.group + rr - tk * p.group;
     const int64_t out = static_cast<int64_t>(w.start + tk) * p.heads + hd;
     if (w.partial >= 0) {
       *reinterpret_cast<f32x4*>(p.part + (held + row) * D + c) = v;
@@ -447,20 +455,28 @@ __device__ __forceinline__ uint2 read_turned(const char* p) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
-// 16 bytes a lane from global memory to 1 KB of LDS, lane by lane.
-__device__ __forceinline__ void copy_to_lds(const char* src, char* dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16,
-                                   0, 0);
+// 16 bytes a lane from base + off to 1 KB of LDS at the wave's `dst`, lane by lane.  In assembly, so that the compiler does not put a
+// wait for every load into LDS before every read of it: what a read needs has arrived at the barrier before (arrive() below).  No
+// register is written but m0, which nothing else in this file uses.
+__device__ __forceinline__ void copy_to_lds(const char* base, uint32_t off, char* dst) {
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
+}
+// The thread's number, with nothing that was computed from it before: for what is rarely needed and would else stay in registers.
+__device__ __forceinline__ int thread_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
 template <int D, class E, bool kPrefix>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
   constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR;
   constexpr int kStage = 64 * D * 2;  // bytes of a stage of keys or values
-  constexpr int kAhead = D == 256 ? 4 : 3;
-  __shared__ __align__(16) char lds[4 * kStage];  // keys of both stages, then values
+  constexpr int kAhead = D == 256 ? 4 : 2;
+  __shared__ __align__(16) char keys0[kStage], keys1[kStage], values0[kStage], values1[kStage];
   __shared__ int odd;  // a stage lacks values that are infinite or NaN
-  const int kvh = blockIdx.x % p.kv;
+  const int kvh = uniform(static_cast<int>(blockIdx.x) % p.kv);
   Share w;
   if (!(kPrefix ? prefix_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)
                 : own_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)))
@@ -471,72 +487,65 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   const int rows = w.tokens * p.group, nrows = min(kLargeRows, rows - w.tile * kLargeRows);
   const int row0 = w.tile * kLargeRows;
   const int r = row0 + min(wave * 32 + l31, nrows - 1);
-  const int tok = r / p.group, head = kvh * p.group + r - tok * p.group;
+  const int tok = divide(r, p.by_group), head = kvh * p.group + r - tok * p.group;
   const int visible = visible_keys(w.keys, w.tokens, tok, causal);
-  const int least = visible_keys(w.keys, w.tokens, uniform(row0 / p.group), causal);
-  const int n = visible_keys(w.keys, w.tokens, uniform((row0 + nrows - 1) / p.group), causal);
+  const int least = visible_keys(w.keys, w.tokens, uniform(static_cast<int>(divide(row0, p.by_group))), causal);
+  const int n = visible_keys(w.keys, w.tokens, uniform(static_cast<int>(divide(row0 + nrows - 1, p.by_group))), causal);
   const int k0 = w.chunk * w.c * kLargeUnit, k1 = min(k0 + w.c * kLargeUnit, n);
   const int steps = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
 
-  u32x4 q[KS];
-  {
-    const uint16_t* qr = p.query + (w.start + tok) * p.query_token + head * p.query_head + 8 * half;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      q[s] = *reinterpret_cast<const u32x4*>(qr + 16 * s);
-      // at head dim 256 the queries stay in the accumulation registers, where matrix instructions take them from
-      if constexpr (D == 256) asm volatile("" : "+a"(q[s]));
-    }
-  }
   if (tid == 0) odd = 0;
 
   // Staging: thread tid loads 16-byte slot tid % SL of rows tid / SL, + KR, ... of keys and values.  A 16-row group's place is a 64-bit
-  // offset that is found a step ahead, group g of the step in lane g; rows inside it are 32-bit offsets that do not change.
+  // offset, looked up many steps ahead; rows inside it are 32-bit offsets that do not change.
   // LDS: slot c of row r holds 16-byte piece c ^ (r % 16) of the keys, c ^ 4 (r % 8 or 4) of the values, so that neither kind of read
   // puts two of the lanes that read together on one bank; the loads permute the pieces, since their own order in LDS is fixed.
   const char* keys = reinterpret_cast<const char*>(side.keys + kvh * side.key_head);
   const char* vals = reinterpret_cast<const char*>(side.values + kvh * side.value_head);
   const int krow = static_cast<int>(2 * side.key_row), vrow = static_cast<int>(2 * side.value_row);  // bytes
-  const int slot = tid % SL, tr = tid / SL;
-  const uint32_t vcol = (slot ^ (tr & (D == 256 ? 7 : 3)) << 2) * 16;
-  const auto kcol = [&](int i) { return static_cast<uint32_t>((slot ^ ((tr + i * KR) & 15)) * 16); };
+  const auto vcol = [](int t) { return static_cast<uint32_t>((t % SL ^ (t / SL & (D == 256 ? 7 : 3)) << 2) * 16); };
+  const auto kcol = [](int t, int i) { return static_cast<uint32_t>((t % SL ^ ((t / SL + i * KR) & 15)) * 16); };
   uint32_t koff[KP / 4], voff[KP / 4];
 #pragma unroll
   for (int i = 0; i < KP / 4; ++i) {
-    koff[i] = (tr + i * KR) * krow + kcol(i);
-    voff[i] = (tr + i * KR) * vrow + vcol;
+    koff[i] = (tid / SL + i * KR) * krow + kcol(tid, i);
+    voff[i] = (tid / SL + i * KR) * vrow + vcol(tid);
   }
-  PageAt place = {0, 0}, ahead = {0, 0};  // of group lane % 4 of the step whose values, and whose keys, are loaded next
-  const auto find = [&](int key0) {
-    place = ahead;
-    ahead = page_at(side, w.table, min(key0 / 16 + (lane & 3), (n - 1) / 16));
-  };
-  const auto load = [&](bool values, const PageAt& at, int stage, int key0) {
-    const int stride = values ? vrow : krow;
-    const int64_t offset = at.page * (2 * (values ? side.value_page : side.key_page)) + static_cast<int64_t>(at.row) * stride;
-    char* to = lds + (stage + (values ? 2 : 0)) * kStage + wave * 1024;
-    const bool tail = key0 + 64 > n;  // rows past the last key repeat it
+  // Groups' places, 64 of them (16 steps) a lookup, group lane of its block of steps.
+  const auto find = [&](int block) { return page_at(side, w.table, min(k0 / 16 + 64 * block + (thread_again() & 63), (n - 1) / 16)); };
+  const auto load = [&](auto values_, char* into, const PageAt& places, int step) {
+    constexpr bool values = decltype(values_)::value;
+    const int key0 = k0 + 64 * step;
+    const char* base[4];
 #pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const int g = i / (KP / 4);
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(offset), g);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(offset) >> 32), g);
-      const char* base = (values ? vals : keys) + static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-      uint32_t off = values ? voff[i % (KP / 4)] : koff[i % (KP / 4)];
-      if (tail)
-        off = min((i * KR + tr) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16)) * stride + (values ? vcol : kcol(i));
-      copy_to_lds(base + off, to + i * 4096);
+    for (int g = 0; g < 4; ++g) {
+      const int page = __builtin_amdgcn_readlane(places.page, 4 * (step & 15) + g);
+      const int row = __builtin_amdgcn_readlane(places.row, 4 * (step & 15) + g);
+      base[g] = (values ? vals : keys) + page * (2 * (values ? side.value_page : side.key_page)) + static_cast<int64_t>(row) * (values ? vrow : krow);
+    }
+    char* to = into + wave * 1024;
+    if (key0 + 64 <= n) {
+#pragma unroll
+      for (int i = 0; i < KP; ++i) copy_to_lds(base[i / (KP / 4)], (values ? voff : koff)[i % (KP / 4)], to + i * 4096);
+    } else {  // rows past the last key repeat it
+      const int t = thread_again();
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int row = min((i * KR + t / SL) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16));
+        copy_to_lds(base[i / (KP / 4)], row * (values ? vrow : krow) + (values ? vcol(t) : kcol(t, i)), to + i * 4096);
+      }
     }
   };
   // Some row masks some of a step's keys: its weights there are 0, but 0 times an infinite or NaN value is not.  Such values, and keys
   // past the last one, become zeros in the stage.
-  const auto clean = [&](int stage, int key0) {
+  const auto clean = [&](char* stage, int key0) {
     bool wild = false;
-#pragma unroll
+    const int t = thread_again();
+#pragma unroll 1
     for (int i = 0; i < KP; ++i) {
-      u32x4* at = reinterpret_cast<u32x4*>(lds + (2 + stage) * kStage + i * 4096 + tid * 16);
+      u32x4* at = reinterpret_cast<u32x4*>(stage + i * 4096 + t * 16);
       u32x4 v = *at;
-      const bool in = key0 + i * KR + tr < n;
+      const bool in = key0 + i * KR + t / SL < n;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t x = in ? v[k] : 0, high = E::kExponent << 16;
@@ -551,7 +560,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   };
   uint32_t kr = l31 * (2 * D) + ((half ^ l31) & 15) * 16;
   const int j15 = lane & 15, turn = D == 256 ? 4 * half + (j15 >> 2) : j15 >> 2;
-  uint32_t vr = 2 * kStage + (4 * half + (j15 >> 2)) * (2 * D) + (2 * (lane >> 4 & 1) + (j15 >> 1 & 1)) * 16 + (j15 & 1) * 8 + turn * 64;
+  uint32_t vr = (4 * half + (j15 >> 2)) * (2 * D) + (2 * (lane >> 4 & 1) + (j15 >> 1 & 1)) * 16 + (j15 & 1) * 8 + turn * 64;
 
   f32x16 o[NC];
 #pragma unroll
@@ -560,33 +569,59 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
 
-  // Step i multiplies its weights with its values, and before that the next step's keys with the queries: the exponentials of the one
-  // stand between the matrix instructions of the other, and the maximum of the next scores between those of the values.  So keys are
-  // loaded two steps ahead, values one.
-  const auto fill = [&](int i) {  // what step i loads
-    if (i + 1 < steps) load(true, place, ~i & 1, k0 + 64 * (i + 1));
-    if (i + 2 < steps) load(false, ahead, i & 1, k0 + 64 * (i + 2));
-    find(k0 + 64 * (i + 3));
+  // Step i multiplies the next step's keys with the queries, then its own weights with its values: the exponentials of its scores
+  // stand between the matrix instructions of the one, the maximum of the next scores between those of the other.  Each half ends
+  // with a barrier, after which the stage it read takes the keys, or values, of two steps on: every load has one and a half steps.
+  const std::false_type of_keys{};
+  const std::true_type of_values{};
+  PageAt here{0, 0}, after{0, 0};  // of the steps whose keys are loaded, and of the next 16
+  PageAt vhere{0, 0};              // of the step whose values are loaded, a step behind
+  const auto load_keys = [&](char* into, int t) {
+    if (t >= steps) return;
+    if (t > 0 && (t & 15) == 0) {
+      here = after;
+      after = find(t / 16 + 1);
+    }
+    load(of_keys, into, here, t);
   };
-  const auto arrive = [&]() {
-    wait_vmem();
+  const auto load_values = [&](char* into, int t) {
+    if (t >= steps) return;
+    if ((t & 15) == 0) vhere = here;
+    load(of_values, into, vhere, t);
+  };
+  // All but the last 2 KP loads have arrived, where that many are on their way behind the ones waited for; and every wave is here.
+  const auto arrive = [&](bool behind) {
+    if (behind) __builtin_amdgcn_s_waitcnt(KP == 8 ? 0x4F70 : 0x0F78);  // vmcnt(2 KP)
+    else wait_vmem();
     lds_barrier();
   };
+  u32x4 q[KS];
   if (steps > 0) {
-    find(k0);
-    load(false, ahead, 0, k0);
-    load(true, ahead, 0, k0);
-    find(k0 + 64);
-    if (steps > 1) load(false, ahead, 1, k0 + 64);
-    find(k0 + 128);
+    here = find(0);
+    const uint16_t* qr = p.query + (w.start + tok) * p.query_token + head * p.query_head + 8 * half;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qr + 16 * s);
+    load_keys(keys0, 0);
+    load_keys(keys1, 1);
+    load_values(values0, 0);
+    after = find(1);
+    // at head dim 256 the queries stay in the accumulation registers, where matrix instructions take them from
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) asm volatile("" : "+a"(q[s]));
+    }
   }
-  arrive();
+  arrive(false);
   if (wave * 32 >= nrows) {  // no rows: the wave only stages
-    if (steps > 2) lds_barrier();
+    if (steps > 0) lds_barrier();
+    load_keys(keys0, 2);
+    load_values(values1, 1);
     for (int i = 0; i < steps; ++i) {
-      fill(i);
-      if (k0 + 64 * (i + 1) > least) clean(i & 1, k0 + 64 * i);
-      arrive();
+      arrive(i + 2 < steps);
+      load_keys(i & 1 ? keys0 : keys1, i + 3);
+      if (k0 + 64 * (i + 1) > least) clean(i & 1 ? values1 : values0, k0 + 64 * i);
+      arrive(i + 3 < steps);
+      load_values(i & 1 ? values1 : values0, i + 2);
     }
     return;
   }
@@ -605,28 +640,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
       for (int e = 0; e < 16; ++e)
         if (key0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= visible) t[b][e] = -__builtin_inff();
   };
-  const auto key_at = [&](int stage, int i) {
-    return *reinterpret_cast<const u32x4*>(lds + ((kr ^ (32 * (i >> 1))) + (stage * kStage + (i & 1) * 64 * D)));
+  const auto key_at = [&](const char* from, int i) {
+    return *reinterpret_cast<const u32x4*>(from + ((kr ^ (32 * (i >> 1))) + (i & 1) * 64 * D));
   };
   float mc = -__builtin_inff();  // maximum of the scores of the step to come
   if (steps > 0) {
     clear(sc[0]);
-    feed<2 * KS, kAhead>([&](int i) { return key_at(0, i); },
+    feed<2 * KS, kAhead>([&](int i) { return key_at(keys0, i); },
                          [&](int i, u32x4 k) { sc[0][i & 1] = E::mfma32(k, q[i >> 1], sc[0][i & 1]); });
     hide(sc[0], k0);
 #pragma unroll
     for (int e = 0; e < 32; ++e) mc = fmaxf(mc, sc[0][e >> 4][e & 15]);
-    if (steps > 2) lds_barrier();  // step 0 loads step 2's keys where these were
+    lds_barrier();
+    load_keys(keys0, 2);
+    load_values(values1, 1);
   }
-  const auto step = [&](auto stage_, auto last_, int i) {
+  const auto step = [&](auto stage_, int i) {
     constexpr int stage = decltype(stage_)::value;
-    constexpr bool more = !decltype(last_)::value;
+    char* const other = stage ? keys0 : keys1;      // the next step's keys
+    char* const held = stage ? values1 : values0;   // this step's values
     const int key0 = k0 + 64 * i;
     f32x16(&now)[2] = sc[stage];
     f32x16(&next)[2] = sc[stage ^ 1];
-    fill(i);
-    if (key0 + 64 > least) clean(stage, key0);
-    if constexpr (D == 256) asm volatile("" : "+v"(kr), "+v"(vr));  // no two dozen registers of places kept over the steps
+    asm volatile("" : "+v"(kr), "+v"(vr));  // no two dozen registers of places kept over the steps
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
     // a row that has seen no key keeps weights of 0 (the exponent is -inf); a NaN score, which the maximum skips, makes l and
     // o NaN, and so they stay
@@ -653,63 +689,54 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
       asm volatile("" : "+v"(both));  // made here, between the matrix instructions, not where it is used
       pf[e >> 3][(e & 7) >> 1] = both;
     };
-    if constexpr (more) {
-      clear(next);
-      constexpr int kEach = KS / 8;  // instructions a pair of elements
-      feed<2 * KS, kAhead>([&](int k) { return key_at(stage ^ 1, k); },
-                           [&](int k, u32x4 v) {
-                             next[k & 1] = E::mfma32(v, q[k >> 1], next[k & 1]);
-                             if (k % kEach == 0) weigh(k / kEach * 2);
-                           });
-      hide(next, key0 + 64);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) weigh(e);
-    }
+    clear(next);
+    constexpr int kPairK = KS / 8, kPairV = NC / 4;  // matrix instructions a pair of elements
+    feed<2 * KS, kAhead>([&](int k) { return key_at(other, k); },
+                         [&](int k, u32x4 v) {
+                           next[k & 1] = E::mfma32(v, q[k >> 1], next[k & 1]);
+                           if (k % kPairK == 0) weigh(k / kPairK * 2);
+                         });
+    hide(next, key0 + 64);
     l += sum[0] + sum[1];
     mc = -__builtin_inff();
+    arrive(i + 2 < steps);
+    load_keys(other, i + 3);
+    if (key0 + 64 > least) clean(held, key0);
     feed<4 * NC, kAhead>(
         [&](int k) {
-          const char* at = lds + ((vr ^ (64 * (k % NC))) + (stage * kStage + k / NC * 32 * D));
+          const char* at = held + ((vr ^ (64 * (k % NC))) + k / NC * 32 * D);
           const uint2 a = read_turned(at), b = read_turned(at + 16 * D);
           return u32x4{a.x, a.y, b.x, b.y};
         },
         [&](int k, u32x4 v) {
           o[k % NC] = E::mfma32(v, pf[k / NC], o[k % NC]);
-          constexpr int kEach = NC / 4;  // instructions a pair of elements of the next scores
-          if (more && k % kEach == 0) {
-            const int e = k / kEach * 2;
+          if (k % kPairV == 0) {
+            const int e = k / kPairV * 2;
             mc = fmaxf(fmaxf(mc, next[e >> 4][e & 15]), next[e >> 4][(e & 15) + 1]);
           }
         });
-    arrive();
+    arrive(i + 3 < steps);
+    load_values(held, i + 2);
   };
-  if (steps > 0) {
-    const std::integral_constant<int, 0> even{};
-    const std::integral_constant<int, 1> uneven{};
-    int i = 0;
-    for (; i + 2 < steps; i += 2) {
-      step(even, std::false_type{}, i);
-      step(uneven, std::false_type{}, i + 1);
-    }
-    if (i + 1 < steps) {
-      step(even, std::false_type{}, i);
-      step(uneven, std::true_type{}, i + 1);
-    } else {
-      step(even, std::true_type{}, i);
-    }
+  // the last step multiplies keys that are none: code of its own for it would cost more than that
+  for (int i = 0; i < steps; i += 2) {
+    step(std::integral_constant<int, 0>{}, i);
+    if (i + 1 < steps) step(std::integral_constant<int, 1>{}, i + 1);
   }
+  const int again = thread_again();  // the lane's row once more
+  const int part = again >> 5 & 1, mine = (again >> 6) * 32 + (again & 31), at_row = row0 + min(mine, nrows - 1);
+  const int at_token = divide(at_row, p.by_group), at_head = kvh * p.group + at_row - at_token * p.group;
   if (steps > 0 && odd) {
     // the values left out of the stages: infinite or NaN in the rows that see them, whatever their (positive) weight
     for (int key = k0 + max(0, (least - k0) / 64) * 64; key < k1; ++key) {
       const PageAt at = page_at(side, w.table, key / 16);
       const char* src = vals + 2 * at.page * side.value_page + static_cast<int64_t>(at.row + key % 16) * vrow;
-      if (key >= visible) continue;
+      if (key >= visible_keys(w.keys, w.tokens, at_token, causal)) continue;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const uint2 v = *reinterpret_cast<const uint2*>(src + 2 * (32 * c + 2 * e + 4 * half));
+          const uint2 v = *reinterpret_cast<const uint2*>(src + 2 * (32 * c + 2 * e + 4 * part));
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const uint32_t x = (y < 2 ? v.x : v.y) >> (16 * (y & 1)) & 0xFFFF;
@@ -720,16 +747,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   }
 
   l += __shfl_xor(l, 32, 64);
-  if (wave * 32 + l31 >= nrows) return;
-  const int64_t out = static_cast<int64_t>(w.start + tok) * p.heads + head;
+  if (mine >= nrows) return;
+  const int64_t out = static_cast<int64_t>(w.start + at_token) * p.heads + at_head;
   if (w.partial >= 0) {
-    const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * kLargeRows + wave * 32 + l31;
+    const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * kLargeRows + mine;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>(p.part + held * D + 32 * c + 2 * e + 4 * half) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
-    if (half == 0) {
+        *reinterpret_cast<f32x4*>(p.part + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
+    if (part == 0) {
       p.ml[held] = make_float2(m, l);
       if (w.chunk == 0) p.info[out] = make_int2(static_cast<int>(held), w.chunks);
     }
@@ -739,103 +766,112 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<uint2*>(p.out + out * D + 32 * c + 2 * e + 4 * half) =
+        *reinterpret_cast<uint2*>(p.out + out * D + 32 * c + 2 * e + 4 * part) =
             make_uint2(pack2<E>(o[c][e] * inv, o[c][e + 1] * inv), pack2<E>(o[c][e + 2] * inv, o[c][e + 3] * inv));
-    if (half == 0 && w.chunk == 0) p.info[out] = make_int2(0, 0);
+    if (part == 0 && w.chunk == 0) p.info[out] = make_int2(0, 0);
   }
 }
 
 // ------------------------------------------------------------------ merge
-// kWaves waves per (token, head), D / 64 dims a lane; wave w takes the row's partial results w, w + kWaves, ...: first every maximum
-// and sum, a partial a lane, then their rows, several in flight.  The order of the additions depends on the sizes alone.
-template <int D, class E, int kWaves>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
-  constexpr int F = D / 64, kFlight = 8, kRows = 4 / kWaves;
-  __shared__ float om[4][D], lm[4];
-  __shared__ float mm[4];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = wave % kWaves;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + wave / kWaves;
-  const int t = static_cast<int>(row / p.heads);
-  // rows of tokens in no sequence are not written (with one row a workgroup and several waves this holds for all of them)
-  const bool covered = t < p.T && t >= p.starts[0] && t < p.starts[p.B];
+// kWaves waves per (token, head), D / 64 dims a lane; wave w takes the row's partial results w, w + kWaves, ..., eight in flight, and
+// the waves' sums meet in LDS.  The order of the additions depends on the sizes alone.  A wave that has rows to itself (kWaves 1)
+// looks at kRows of them at once and takes those that are in parts.
+template <int D, class E, int kWaves, int kRows>
+__global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_kernel(PagedParams p) {
+  static_assert(kWaves == 1 || kRows == 1, "waves that share rows meet once");
+  constexpr int F = D / 64, kFlight = 8;
+  __shared__ float om[kWaves == 1 ? 1 : kWaves][D], lm[kWaves], mm[kWaves];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = kWaves == 1 ? 0 : wave;
+  const int64_t row0 = kWaves == 1 ? (static_cast<int64_t>(blockIdx.x) * 4 + wave) * kRows : blockIdx.x;
+  const int64_t rows = static_cast<int64_t>(p.T) * p.heads;
+  // rows of tokens in no sequence are not written
+  const int64_t from = static_cast<int64_t>(p.starts[0]) * p.heads, to = static_cast<int64_t>(p.starts[p.B]) * p.heads;
   int2 range[2] = {make_int2(0, 0), make_int2(0, 0)};
-  if (covered) {
-    range[0] = p.info[row];
-    if (p.merge_prefix) range[1] = p.prefix_info[row];
+  {
+    const int64_t row = row0 + lane % kRows;
+    if (row < rows) {
+      range[0] = p.info[row];
+      if (p.merge_prefix) range[1] = p.prefix_info[row];
+    }
+    if (row < from || row >= to) range[0].y = 0;
   }
-  const bool any = covered && range[0].y > 0;
-  if (kWaves == 1 && !any) return;
-  if (kWaves > 1 && !any) return;  // the same for all waves: they share the row
-  float M = -__builtin_inff();
-  const int tile[2] = {p.own_tile_rows, p.prefix_tile_rows};
+  uint64_t todo = __ballot(range[0].y > 0 && lane < kRows);
+  for (; todo; todo &= todo - 1) {
+    const int at = __builtin_ctzll(todo);
+    const int64_t row = row0 + at;
+    float M = -__builtin_inff(), l = 0.f, acc[F];
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    // whatever the sequences' starts held, nothing outside the partial results is read
-    const int64_t last = range[g].x + static_cast<int64_t>(range[g].y - 1) * tile[g] * p.kv;
-    if (range[g].x < 0 || range[g].y < 0 || last >= p.part_rows[g]) range[g].y = 0;
-    const float2* ml = g ? p.prefix_ml : p.ml;
-    for (int i = part + kWaves * lane; i < range[g].y; i += 64 * kWaves)
-      M = fmaxf(M, ml[range[g].x + static_cast<int64_t>(i) * tile[g] * p.kv].x);
-  }
+    for (int i = 0; i < F; ++i) acc[i] = 0.f;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  const float ref = M == -__builtin_inff() ? 0.f : M * p.scale_log2;
-  float l = 0.f, acc[F];
+    for (int g = 0; g < 2; ++g) {
+      if (g == 1 && !p.merge_prefix) break;
+      const int first = __builtin_amdgcn_readlane(range[g].x, at);
+      int chunks = __builtin_amdgcn_readlane(range[g].y, at);
+      // whatever the sequences' starts held, nothing outside the partial results is read
+      const int64_t stride = static_cast<int64_t>(g ? p.prefix_tile_rows : p.own_tile_rows) * p.kv;
+      if (first < 0 || chunks < 0 || first + (chunks - 1) * stride >= p.part_rows[g]) chunks = 0;
+      const float2* ml = g ? p.prefix_ml : p.ml;
+      const float* data = (g ? p.prefix_part : p.part) + lane * F;
+      const int64_t step = stride * kWaves, base = first + part * stride;
+      const int count = (chunks - part + kWaves - 1) / kWaves;
+      for (int i0 = 0; i0 < count; i0 += kFlight) {
+        float x[kFlight][F];
+        float2 v[kFlight];
 #pragma unroll
-  for (int i = 0; i < F; ++i) acc[i] = 0.f;
+        for (int i = 0; i < kFlight; ++i) {
+          const int64_t r = base + min(i0 + i, count - 1) * step;
+          v[i] = ml[r];
+          if (i0 + i >= count) v[i] = make_float2(-__builtin_inff(), 0.f);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const float2* ml = g ? p.prefix_ml : p.ml;
-    const float* rows = (g ? p.prefix_part : p.part) + lane * F;
-    const int64_t step = static_cast<int64_t>(tile[g]) * p.kv * kWaves;
-    const int64_t base = range[g].x + static_cast<int64_t>(part) * tile[g] * p.kv;
-    const int count = (range[g].y - part + kWaves - 1) / kWaves;
-    for (int i0 = 0; i0 < count; i0 += kFlight) {
-      float x[kFlight][F];
-      float2 v[kFlight];
+          for (int f = 0; f < F; ++f) x[i][f] = data[r * D + f];
+        }
+        float top = M;
 #pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        const int64_t at = base + min(i0 + i, count - 1) * step;
-        v[i] = ml[at];
+        for (int i = 0; i < kFlight; ++i) top = fmaxf(top, v[i].x);
+        const float ref = top == -__builtin_inff() ? 0.f : top * p.scale_log2;
+        const float corr = __builtin_amdgcn_exp2f(__builtin_fmaf(M, p.scale_log2, -ref));
+        M = top;
+        l *= corr;
 #pragma unroll
-        for (int f = 0; f < F; ++f) x[i][f] = rows[at * D + f];
+        for (int k = 0; k < F; ++k) acc[k] *= corr;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+          if (v[i].y == 0.f) continue;  // no key of this row in that chunk, whose row may hold anything
+          const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(v[i].x, p.scale_log2, -ref));
+          l += v[i].y * f;
+#pragma unroll
+          for (int k = 0; k < F; ++k) acc[k] += x[i][k] * f;
+        }
+      }
+    }
+    if (kWaves > 1) {  // the same rows in all waves: they share one
+      if (lane == 0) {
+        lm[part] = l;
+        mm[part] = M;
       }
 #pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        if (i0 + i >= count || v[i].y == 0.f) continue;  // no key of this row in that chunk
-        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(v[i].x, p.scale_log2, -ref));
-        l += v[i].y * f;
+      for (int k = 0; k < F; ++k) om[part][lane * F + k] = acc[k];
+      __syncthreads();
+      if (wave) return;
 #pragma unroll
-        for (int k = 0; k < F; ++k) acc[k] += x[i][k] * f;
+      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mm[w]);
+      const float ref = M == -__builtin_inff() ? 0.f : M * p.scale_log2;
+      l = 0.f;
+#pragma unroll
+      for (int k = 0; k < F; ++k) acc[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(mm[w], p.scale_log2, -ref));
+        l += lm[w] * f;
+#pragma unroll
+        for (int k = 0; k < F; ++k) acc[k] += om[w][lane * F + k] * f;
       }
     }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + row * D + lane * F);
+#pragma unroll
+    for (int k = 0; k < F; k += 2) out[k / 2] = pack2<E>(acc[k] * inv, acc[k + 1] * inv);
   }
-  if (kWaves > 1) {
-    if (lane == 0) {
-      lm[wave] = l;
-      mm[wave] = M;
-    }
-#pragma unroll
-    for (int k = 0; k < F; ++k) om[wave][lane * F + k] = acc[k];
-    __syncthreads();
-    if (wave) return;
-    M = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3]));
-    const float all = M == -__builtin_inff() ? 0.f : M * p.scale_log2;
-    l = 0.f;
-#pragma unroll
-    for (int k = 0; k < F; ++k) acc[k] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(mm[w], p.scale_log2, -all));
-      l += lm[w] * f;
-#pragma unroll
-      for (int k = 0; k < F; ++k) acc[k] += om[w][lane * F + k] * f;
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint32_t* out = reinterpret_cast<uint32_t*>(p.out + row * D + lane * F);
-#pragma unroll
-  for (int k = 0; k < F; k += 2) out[k / 2] = pack2<E>(acc[k] * inv, acc[k + 1] * inv);
 }
 
 }  // namespace
@@ -875,9 +911,10 @@ static void launch_attend(const PagedParams& p, const PagedParams& before, hipSt
   const int least = own == kLargeRows ? kLargeUnit * kLargeLeast : kSmallUnit;
   if (!p.merge_prefix && p.own.capacity <= least) return;  // one chunk a tile: nothing to merge
   const int64_t rows = static_cast<int64_t>(p.T) * p.heads;
-  // few rows may be in many chunks: four waves a row
-  if (rows <= 4096) hipLaunchKernelGGL((paged_merge_kernel<D, E, 4>), dim3(rows), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((paged_merge_kernel<D, E, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+  // few rows may be in many chunks: eight waves a row; many rows are mostly in one: sixteen rows a wave
+  if (rows <= 512) hipLaunchKernelGGL((paged_merge_kernel<D, E, 8, 1>), dim3(rows), dim3(512), 0, stream, p);
+  else if (rows <= 16384) hipLaunchKernelGGL((paged_merge_kernel<D, E, 1, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((paged_merge_kernel<D, E, 1, 16>), dim3((rows + 63) / 64), dim3(256), 0, stream, p);
 }
 void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, const PagedParams& before, hipStream_t stream) {
   if (head_dim == 256) bf16 ? launch_attend<256, Bf16>(p, before, stream) : launch_attend<256, Fp16>(p, before, stream);

@@ -46,20 +46,20 @@ DFLASH_HD SeqSpan seq_span(int start, int end, int length, int T, int capacity) 
   return s;
 }
 
-// Row tiles of a sequence, and its (tile, unit) pairs.
-DFLASH_HD int seq_tiles(int tokens, int group, int tile_rows) {
-  return static_cast<int>(ceil_div(static_cast<int64_t>(tokens) * group, tile_rows));
-}
-DFLASH_HD int seq_units(int keys, int unit) { return static_cast<int>(ceil_div(keys, unit)); }
+// Row tiles of a sequence (tokens * group <= 2^22), and units of its keys.
+DFLASH_HD int seq_tiles(int tokens, int group, int tile_rows) { return (tokens * group + tile_rows - 1) / tile_rows; }
+DFLASH_HD int seq_units(int keys, int unit) { return (keys + unit - 1) / unit; }
 
-// Units a chunk, for `total` (tile, unit) pairs of all sequences per KV head.
-DFLASH_HD int chunk_units(int64_t total, int kv, int slots, int least) {
-  const int64_t c = ceil_div(total * kv, slots);
-  return static_cast<int>(c < least ? least : c);
+// Units a chunk, for `total` (tile, unit) pairs of all sequences per KV head: at least total * kv / slots, whatever the
+// product's rounding (a 64-bit division would take longer than the rest of the search).
+DFLASH_HD int chunk_units(int64_t total, int kv, double per_slot, int least) {
+  const double c = static_cast<double>(total) * kv * per_slot;
+  const int up = c < 1e9 ? static_cast<int>(c) + 1 : 1000000001;
+  return up < least ? least : up;
 }
 // Chunks a tile: one at least, which writes the rows of a sequence without keys.
 DFLASH_HD int tile_chunks(int units, int c) {
-  const int k = static_cast<int>(ceil_div(units, c));
+  const int k = static_cast<int>(static_cast<uint32_t>(units + c - 1) / static_cast<uint32_t>(c));
   return k < 1 ? 1 : k;
 }
 

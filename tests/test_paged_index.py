@@ -23,7 +23,7 @@ void span(int start, int end, int length, int T, int capacity, int* out) {
 }
 int tiles(int tokens, int group, int rows) { return seq_tiles(tokens, group, rows); }
 int units(int keys, int unit) { return seq_units(keys, unit); }
-int chunk(int64_t total, int kv, int slots, int least) { return chunk_units(total, kv, slots, least); }
+int chunk(int64_t total, int kv, int slots, int least) { return chunk_units(total, kv, 1.0 / slots, least); }
 int chunks(int units, int c) { return tile_chunks(units, c); }
 int visible(int keys, int tokens, int i, int causal) { return visible_keys(keys, tokens, i, causal); }
 int64_t tile_bound(int64_t T, int64_t B, int64_t group, int64_t rows) { return max_tiles(T, B, group, rows); }
@@ -119,6 +119,16 @@ def test_shares_cover_every_row_and_key_once(index, rows, unit, least, always):
         assert not seen
         partial = [s[4] for s in shares if s[4] >= 0]
         assert partial == list(range(len(partial)))
+
+
+def test_chunks_are_long_enough_at_any_size(index):
+    """c slots >= total kv, which the bounds above rest on, also where the product is rounded; and no chunk much longer."""
+    rng = random.Random(3)
+    for _ in range(20000):
+        total, kv = rng.randrange(1, 1 << rng.randrange(1, 45)), rng.choice((1, 2, 3, 8, 31))
+        slots = rng.choice((1, 7, 256, 304, 512, 1024))
+        c = index.chunk(total, kv, slots, 1)
+        assert c > 1000000000 or total * kv <= c * slots <= total * kv + slots, (total, kv, slots, c)
 
 
 def test_a_row_tile_too_few_is_seen(index):
