@@ -511,28 +511,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     koff[i] = (tid / SL + i * KR) * krow + kcol(tid, i);
     voff[i] = (tid / SL + i * KR) * vrow + vcol(tid);
   }
-  // Groups' places, 64 of them (16 steps) a lookup, group lane of its block of steps.
-  const auto find = [&](int block) { return page_at(side, w.table, min(k0 / 16 + 64 * block + (thread_again() & 63), (n - 1) / 16)); };
-  const auto load = [&](auto values_, char* into, const PageAt& places, int step) {
-    constexpr bool values = decltype(values_)::value;
-    const int key0 = k0 + 64 * step;
-    const char* base[4];
+  // Groups' places, 64 of them (16 steps) a lookup, group lane of its block of steps: byte offsets of keys and values.
+  struct Places {
+    int64_t k, v;
+  };
+  const auto find = [&](int block) {
+    const PageAt at = page_at(side, w.table, min(k0 / 16 + 64 * block + (thread_again() & 63), (n - 1) / 16));
+    return Places{at.page * (2 * side.key_page) + static_cast<int64_t>(at.row) * krow,
+                  at.page * (2 * side.value_page) + static_cast<int64_t>(at.row) * vrow};
+  };
+  struct Bases {
+    const char* g[4];  // of the step's four groups
+  };
+  const auto bases = [&](const char* from, int64_t places, int step) {
+    Bases b;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int page = __builtin_amdgcn_readlane(places.page, 4 * (step & 15) + g);
-      const int row = __builtin_amdgcn_readlane(places.row, 4 * (step & 15) + g);
-      base[g] = (values ? vals : keys) + page * (2 * (values ? side.value_page : side.key_page)) + static_cast<int64_t>(row) * (values ? vrow : krow);
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(places), 4 * (step & 15) + g);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(places) >> 32), 4 * (step & 15) + g);
+      b.g[g] = from + static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
     }
-    char* to = into + wave * 1024;
+    return b;
+  };
+  const auto piece = [&](auto values_, char* into, const Bases& b, int i) {
+    copy_to_lds(b.g[i / (KP / 4)], (decltype(values_)::value ? voff : koff)[i % (KP / 4)], into + wave * 1024 + i * 4096);
+  };
+  const auto load = [&](auto values_, char* into, int64_t places, int step) {
+    constexpr bool values = decltype(values_)::value;
+    const int key0 = k0 + 64 * step;
+    const Bases b = bases(values ? vals : keys, places, step);
     if (key0 + 64 <= n) {
 #pragma unroll
-      for (int i = 0; i < KP; ++i) copy_to_lds(base[i / (KP / 4)], (values ? voff : koff)[i % (KP / 4)], to + i * 4096);
+      for (int i = 0; i < KP; ++i) piece(values_, into, b, i);
     } else {  // rows past the last key repeat it
       const int t = thread_again();
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
         const int row = min((i * KR + t / SL) & 15, n - 1 - 16 * min(key0 / 16 + i * KR / 16, (n - 1) / 16));
-        copy_to_lds(base[i / (KP / 4)], row * (values ? vrow : krow) + (values ? vcol(t) : kcol(t, i)), to + i * 4096);
+        copy_to_lds(b.g[i / (KP / 4)], row * (values ? vrow : krow) + (values ? vcol(t) : kcol(t, i)), into + wave * 1024 + i * 4096);
       }
     }
   };
@@ -574,19 +590,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
   // with a barrier, after which the stage it read takes the keys, or values, of two steps on: every load has one and a half steps.
   const std::false_type of_keys{};
   const std::true_type of_values{};
-  PageAt here{0, 0}, after{0, 0};  // of the steps whose keys are loaded, and of the next 16
-  PageAt vhere{0, 0};              // of the step whose values are loaded, a step behind
-  const auto load_keys = [&](char* into, int t) {
-    if (t >= steps) return;
+  Places here{0, 0}, after{0, 0};  // of the steps whose keys are loaded, and of the next 16
+  int64_t vhere = 0;               // of the step whose values are loaded, a step behind
+  const auto turn_keys = [&](int t) {
     if (t > 0 && (t & 15) == 0) {
       here = after;
       after = find(t / 16 + 1);
     }
-    load(of_keys, into, here, t);
+  };
+  const auto turn_values = [&](int t) {
+    if ((t & 15) == 0) vhere = here.v;
+  };
+  const auto load_keys = [&](char* into, int t) {
+    if (t >= steps) return;
+    turn_keys(t);
+    load(of_keys, into, here.k, t);
   };
   const auto load_values = [&](char* into, int t) {
     if (t >= steps) return;
-    if ((t & 15) == 0) vhere = here;
+    turn_values(t);
     load(of_values, into, vhere, t);
   };
   // All but the last 2 KP loads have arrived, where that many are on their way behind the ones waited for; and every wave is here.
@@ -653,10 +675,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     for (int e = 0; e < 32; ++e) mc = fmaxf(mc, sc[0][e >> 4][e & 15]);
     lds_barrier();
     load_keys(keys0, 2);
-    load_values(values1, 1);
   }
-  const auto step = [&](auto stage_, int i) {
+  const auto step = [&](auto stage_, auto inner_, int i) {
     constexpr int stage = decltype(stage_)::value;
+    constexpr bool inner = decltype(inner_)::value;  // whole tiles follow: the loads stand between the matrix instructions too
     char* const other = stage ? keys0 : keys1;      // the next step's keys
     char* const held = stage ? values1 : values0;   // this step's values
     const int key0 = k0 + 64 * i;
@@ -691,16 +713,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     };
     clear(next);
     constexpr int kPairK = KS / 8, kPairV = NC / 4;  // matrix instructions a pair of elements
+    char* const ahead = stage ? values0 : values1;   // the next step's values
+    Bases b;
+    if constexpr (inner) {
+      turn_values(i + 1);
+      b = bases(vals, vhere, i + 1);
+    }
     feed<2 * KS, kAhead>([&](int k) { return key_at(other, k); },
                          [&](int k, u32x4 v) {
                            next[k & 1] = E::mfma32(v, q[k >> 1], next[k & 1]);
                            if (k % kPairK == 0) weigh(k / kPairK * 2);
+                           if constexpr (inner) {
+                             if (k % 4 == 1) piece(of_values, ahead, b, k / 4);
+                           }
                          });
     hide(next, key0 + 64);
     l += sum[0] + sum[1];
     mc = -__builtin_inff();
-    arrive(i + 2 < steps);
-    load_keys(other, i + 3);
+    arrive(inner || i + 2 < steps);
+    if constexpr (inner) {
+      turn_keys(i + 3);
+      b = bases(keys, here.k, i + 3);
+    } else {
+      load_keys(other, i + 3);
+    }
     if (key0 + 64 > least) clean(held, key0);
     feed<4 * NC, kAhead>(
         [&](int k) {
@@ -714,14 +750,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
             const int e = k / kPairV * 2;
             mc = fmaxf(fmaxf(mc, next[e >> 4][e & 15]), next[e >> 4][(e & 15) + 1]);
           }
+          if constexpr (inner) {
+            if (k % 4 == 1) piece(of_keys, other, b, k / 4);
+          }
         });
-    arrive(i + 3 < steps);
-    load_values(held, i + 2);
+    arrive(inner || i + 3 < steps);
+    if constexpr (!inner) load_values(held, i + 2);
   };
   // the last step multiplies keys that are none: code of its own for it would cost more than that
-  for (int i = 0; i < steps; i += 2) {
-    step(std::integral_constant<int, 0>{}, i);
-    if (i + 1 < steps) step(std::integral_constant<int, 1>{}, i + 1);
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> uneven{};
+  int i = 0;
+  for (; i + 5 < steps; i += 2) {
+    step(even, std::true_type{}, i);
+    step(uneven, std::true_type{}, i + 1);
+  }
+  load_values(values1, i + 1);
+  for (; i < steps; i += 2) {
+    step(even, std::false_type{}, i);
+    if (i + 1 < steps) step(uneven, std::false_type{}, i + 1);
   }
   const int again = thread_again();  // the lane's row once more
   const int part = again >> 5 & 1, mine = (again >> 6) * 32 + (again & 31), at_row = row0 + min(mine, nrows - 1);
