@@ -259,7 +259,7 @@ __device__ __forceinline__ bool prefix_share(const PagedParams& p, int id, int t
 // registers, so V needs no transpose and neither operand passes through LDS.
 constexpr int kSmallRows = 16, kSmallUnit = 128;  // keys a round of the four waves
 template <int D, class E, bool kPrefix>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_small_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, 2) void paged_small_kernel(PagedParams p) {
   constexpr int NC = D / 16, KS = D / 32, VL = NC / 8, kPitch = D + 4;
   __shared__ __align__(16) float osum[4][16][kPitch];
   __shared__ float mx[4][16], ls[4][16];
