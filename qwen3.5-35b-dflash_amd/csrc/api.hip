@@ -1143,7 +1143,7 @@ dflash::PagedSide paged_side(const dflash_paged_kv* c) {
 struct PagedLayout {
   size_t part[2], ml[2], info[2], total;
   int64_t rows[2];  // partial rows of the own-keys and the prefix stage
-  int slots[2], tile[2];
+  int slots, tile[2];
 };
 bool paged_shape_ok(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B) {
   return T >= 0 && heads > 0 && heads <= 1024 && kv > 0 && heads % kv == 0 && (D == 128 || D == 256) && B >= 0 &&
@@ -1152,11 +1152,11 @@ bool paged_shape_ok(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B) 
 PagedLayout paged_layout(int64_t T, int64_t heads, int64_t kv, int64_t D, int64_t B, bool prefix) {
   PagedLayout L{};
   Carver c;
+  L.slots = dflash::paged_slots(dflash::paged_tile_rows(T, prefix ? 1 : B, heads / kv), static_cast<int>(D), cu_count());
   for (int g = 0; g < (prefix ? 2 : 1); ++g) {
     const int64_t tile = L.tile[g] = dflash::paged_tile_rows(T, g ? 1 : B, heads / kv);
-    L.slots[g] = dflash::paged_slots(L.tile[g], static_cast<int>(D), cu_count());
     const int64_t tiles = g ? dflash::ceil_div(T * (heads / kv), tile) : dflash::max_tiles(T, B, heads / kv, tile);
-    L.rows[g] = dflash::max_partial_tiles(tiles, kv, L.slots[g], prefix) * tile;
+    L.rows[g] = dflash::max_partial_tiles(tiles, kv, L.slots, prefix) * tile;
     L.part[g] = c.take(4 * static_cast<size_t>(L.rows[g]) * D);
     L.ml[g] = c.take(8 * static_cast<size_t>(L.rows[g]));
     L.info[g] = c.take(8 * static_cast<size_t>(T) * heads);
@@ -1269,25 +1269,17 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
     p.out = static_cast<uint16_t*>(out);
     p.own_tile_rows = L.tile[0];
     p.prefix_tile_rows = L.tile[1];
-    const auto stage = [&](int g) {
-      p.slots = L.slots[g];
-      p.per_slot = 1.0 / L.slots[g];
-      p.part = at<float>(workspace, L.part[g]);
-      p.ml = at<float2>(workspace, L.ml[g]);
-      p.info = at<int2>(workspace, L.info[g]);
-    };
+    p.slots = L.slots;
+    p.per_slot = 1.0 / L.slots;
+    p.part = at<float>(workspace, L.part[0]);
+    p.ml = at<float2>(workspace, L.ml[0]);
+    p.info = at<int2>(workspace, L.info[0]);
+    p.prefix_part = at<float>(workspace, L.part[1]);
+    p.prefix_ml = at<float2>(workspace, L.ml[1]);
+    p.prefix_info = at<int2>(workspace, L.info[1]);
     p.part_rows[0] = L.rows[0];
     p.part_rows[1] = L.rows[1];
-    dflash::PagedParams before = p;
-    if (prefix) {
-      stage(1);
-      before = p;
-      p.prefix_part = p.part;
-      p.prefix_ml = p.ml;
-      p.prefix_info = p.info;
-    }
-    stage(0);
-    dflash::launch_paged_attention(static_cast<int>(D), cache->dtype == DFLASH_DTYPE_BF16, p, before,
+    dflash::launch_paged_attention(static_cast<int>(D), cache->dtype == DFLASH_DTYPE_BF16, p,
                                    static_cast<hipStream_t>(stream));
     return launch_status("paged attention");
   } catch (...) {

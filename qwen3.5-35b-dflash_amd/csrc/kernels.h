@@ -393,22 +393,20 @@ struct PagedParams {
   const uint16_t* query;
   int64_t query_token, query_head;
   uint16_t* out;                  // [T][heads][head_dim]
-  // partial results of this stage: rows of unnormalised sums, their maximum and sum, and per (token, head) the first
-  // row and how many (partial tiles of tile_rows rows, tile_rows * kv rows apart)
+  // partial results: rows of unnormalised sums, their maximum and sum, and per (token, head) the first row and how many
+  // (partial tiles of own_tile_rows rows, own_tile_rows * kv rows apart); and the prefix's
   float* part;
   float2* ml;
   int2* info;
-  // the prefix stage's, for the merge
-  const float* prefix_part;
-  const float2* prefix_ml;
-  const int2* prefix_info;
+  float* prefix_part;
+  float2* prefix_ml;
+  int2* prefix_info;
   int own_tile_rows, prefix_tile_rows;
   int64_t part_rows[2];           // rows that part and prefix_part hold
 };
 int paged_tile_rows(int64_t tokens, int64_t sequences, int64_t group);
 int paged_slots(int tile_rows, int head_dim, int cus);
 void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStream_t stream);
-// `before`: the prefix stage's parameters (read where p.merge_prefix)
-void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, const PagedParams& before, hipStream_t stream);
+void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, hipStream_t stream);
 
 }  // namespace dflash

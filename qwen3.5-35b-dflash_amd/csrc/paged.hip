@@ -194,20 +194,37 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
 }
 
-// Share `id` of the own-keys stage: every wave finds it by itself, 64 sequences at a time, one a lane.
-__device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile_rows, int unit, int least, Share* out) {
+// Row tiles of all sequences, and the (tile, unit of keys) pairs; `last` keeps what the lane found of the last 64 sequences.
+struct Work {
+  int tiles;
+  double units;
+};
+__device__ __forceinline__ Work own_work(const PagedParams& p, int tile_rows, int unit, SeqSpan* last) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  SeqSpan s{0, 0, 0};
+  Work w{0, 0.0};
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    s = SeqSpan{0, 0, 0};
-    if (b0 + lane < p.B) s = load_span(p, b0 + lane);
+    *last = SeqSpan{0, 0, 0};
+    if (b0 + lane < p.B) *last = load_span(p, b0 + lane);
+    const int tiles = seq_tiles(last->tokens, p.group, tile_rows);
     // tiles <= 2^18 and units <= 2^24: the product in two parts whose sums stay in 31 bits
-    const uint64_t u = static_cast<uint64_t>(seq_tiles(s.tokens, p.group, tile_rows)) * seq_units(s.keys, unit);
+    const uint64_t u = static_cast<uint64_t>(tiles) * seq_units(last->keys, unit);
     const int lo = wave_scan(static_cast<int>(u & 0xFFFFFF)), hi = wave_scan(static_cast<int>(u >> 24));
-    total += (static_cast<int64_t>(__builtin_amdgcn_readlane(hi, 63)) << 24) + __builtin_amdgcn_readlane(lo, 63);
+    w.units += static_cast<double>((static_cast<int64_t>(__builtin_amdgcn_readlane(hi, 63)) << 24) + __builtin_amdgcn_readlane(lo, 63));
+    w.tiles += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   }
-  const int c = uniform(chunk_units(total, p.kv, p.per_slot, least));
+  return w;
+}
+// The prefix as a sequence whose block is the whole batch.
+__device__ __forceinline__ Work front_work(const PagedParams& p, int tile_rows, int unit, int* keys) {
+  *keys = uniform(clampi(p.prefix.lengths[0], 0, p.prefix.capacity));
+  const int tiles = seq_tiles(p.T, p.group, tile_rows);
+  return Work{tiles, static_cast<double>(static_cast<int64_t>(tiles) * seq_units(*keys, unit))};
+}
+
+// Share `id` of the sequences' own keys in chunks of c units: every wave finds it by itself, 64 sequences at a time, one a lane.
+// `s`: what own_work left.
+__device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile_rows, int unit, int c, SeqSpan s, Share* out) {
+  const int lane = threadIdx.x & 63;
   int first = 0, held = 0;  // shares and partial tiles of the sequences before
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) {
@@ -240,16 +257,11 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
   return false;
 }
 
-// Share `id` of the prefix stage: one sequence whose block is the whole batch.
-__device__ __forceinline__ bool prefix_share(const PagedParams& p, int id, int tile_rows, int unit, int least, Share* out) {
-  const int keys = uniform(clampi(p.prefix.lengths[0], 0, p.prefix.capacity));
-  const int tiles = seq_tiles(p.T, p.group, tile_rows), units = seq_units(keys, unit);
-  const int c = uniform(chunk_units(static_cast<int64_t>(tiles) * units, p.kv, p.per_slot, least));
-  const int chunks = uniform(tile_chunks(units, c));
-  if (id >= tiles * chunks) return false;
-  const int tile = uniform(static_cast<int>(static_cast<uint32_t>(id) / static_cast<uint32_t>(chunks)));
-  *out = Share{0, p.T, keys, tile, id - tile * chunks, chunks, tile * chunks, c, p.prefix.table};
-  return true;
+// The thread's number, with nothing that was computed from it before: for what is rarely needed and would else stay in registers.
+__device__ __forceinline__ int thread_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 // ------------------------------------------------------------------ 16 rows, four waves over the keys
@@ -258,19 +270,17 @@ __device__ __forceinline__ bool prefix_share(const PagedParams& p, int id, int t
 // operand needs eight keys of one dim per lane: a lane loads D / 16 neighbouring dims of its eight keys and pairs halves in
 // registers, so V needs no transpose and neither operand passes through LDS.
 constexpr int kSmallRows = 16, kSmallUnit = 128;  // keys a round of the four waves
-template <int D, class E, bool kPrefix>
-__global__ __launch_bounds__(256, 2) void paged_small_kernel(PagedParams p) {
-  constexpr int NC = D / 16, KS = D / 32, VL = NC / 8, kPitch = D + 4;
-  __shared__ __align__(16) float osum[4][16][kPitch];
-  __shared__ float mx[4][16], ls[4][16];
-  const int kvh = uniform(static_cast<int>(blockIdx.x) % p.kv);
-  Share w;
-  if (!(kPrefix ? prefix_share(p, blockIdx.x / p.kv, kSmallRows, kSmallUnit, 1, &w)
-                : own_share(p, blockIdx.x / p.kv, kSmallRows, kSmallUnit, 1, &w)))
-    return;
-  const PagedSide& side = kPrefix ? p.prefix : p.own;
-  const bool causal = !kPrefix && p.causal;
-  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, lr = lane & 15, kq = lane >> 4;
+template <int D>
+constexpr int kSmallPitch = D + 4;
+template <int D>
+constexpr int kSmallArea = 16 * kSmallPitch<D> * 4;  // bytes a wave's sums take
+// `areas`: LDS of kSmallArea bytes for each wave.
+template <int D, class E>
+__device__ __forceinline__ void small_share(const PagedParams& p, const Share& w, bool on_front, int kvh, char* const (&areas)[4], float (&mx)[4][16], float (&ls)[4][16]) {
+  constexpr int NC = D / 16, KS = D / 32, VL = NC / 8, kPitch = kSmallPitch<D>;
+  const PagedSide& side = on_front ? p.prefix : p.own;
+  const bool causal = !on_front && p.causal;
+  const int tid = thread_again(), wave = uniform(tid >> 6), lane = tid & 63, lr = lane & 15, kq = lane >> 4;
   const int rows = w.tokens * p.group, nrows = min(16, rows - w.tile * 16);
   const int r = w.tile * 16 + min(lr, nrows - 1);  // this lane's row in its block
   const int tok = divide(r, p.by_group), head = kvh * p.group + r - tok * p.group;
@@ -391,19 +401,21 @@ __global__ __launch_bounds__(256, 2) void paged_small_kernel(PagedParams p) {
   };
   const float M = fmaxf(fmaxf(mx[0][lr], mx[1][lr]), fmaxf(mx[2][lr], mx[3][lr]));
   const float f = factor(m, M);
+  float* const mine = reinterpret_cast<float*>(wave == 0 ? areas[0] : wave == 1 ? areas[1] : wave == 2 ? areas[2] : areas[3]) + lr * kPitch;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int c = 0; c < NC; c += 4)
-      *reinterpret_cast<f32x4*>(&osum[wave][lr][NC * (4 * kq + e) + c]) =
+      *reinterpret_cast<f32x4*>(mine + NC * (4 * kq + e) + c) =
           f32x4{o[c][e] * f, o[c + 1][e] * f, o[c + 2][e] * f, o[c + 3][e] * f};
   __syncthreads();
   const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * 16;
   for (int i = tid; i < nrows * (D / 4); i += 256) {
     const int row = i / (D / 4), c = i % (D / 4) * 4;
-    f32x4 v = *reinterpret_cast<const f32x4*>(&osum[0][row][c]);
+    const int at = 4 * (row * kPitch + c);
+    f32x4 v = *reinterpret_cast<const f32x4*>(areas[0] + at);
 #pragma unroll
-    for (int x = 1; x < 4; ++x) v += *reinterpret_cast<const f32x4*>(&osum[x][row][c]);
+    for (int x = 1; x < 4; ++x) v += *reinterpret_cast<const f32x4*>(areas[x] + at);
     const float Mr = fmaxf(fmaxf(mx[0][row], mx[1][row]), fmaxf(mx[2][row], mx[3][row]));
     float sum = 0.f;
 #pragma unroll
@@ -411,16 +423,16 @@ __global__ __launch_bounds__(256, 2) void paged_small_kernel(PagedParams p) {
     const int rr = w.tile * 16 + row, tk = divide(rr, p.by_group), hd = kvh * p.group + rr - tk * p.group;
     const int64_t out = static_cast<int64_t>(w.start + tk) * p.heads + hd;
     if (w.partial >= 0) {
-      *reinterpret_cast<f32x4*>(p.part + (held + row) * D + c) = v;
+      *reinterpret_cast<f32x4*>((on_front ? p.prefix_part : p.part) + (held + row) * D + c) = v;
       if (c == 0) {
-        p.ml[held + row] = make_float2(Mr, sum);
-        if (w.chunk == 0) p.info[out] = make_int2(static_cast<int>(held) + row, w.chunks);
+        (on_front ? p.prefix_ml : p.ml)[held + row] = make_float2(Mr, sum);
+        if (w.chunk == 0) (on_front ? p.prefix_info : p.info)[out] = make_int2(static_cast<int>(held) + row, w.chunks);
       }
     } else {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
       *reinterpret_cast<uint2*>(p.out + out * D + c) =
           make_uint2(pack2<E>(v[0] * inv, v[1] * inv), pack2<E>(v[2] * inv, v[3] * inv));
-      if (c == 0 && w.chunk == 0) p.info[out] = make_int2(0, 0);
+      if (c == 0 && w.chunk == 0) (on_front ? p.prefix_info : p.info)[out] = make_int2(0, 0);
     }
   }
 }
@@ -462,25 +474,14 @@ __device__ __forceinline__ void copy_to_lds(const char* base, uint32_t off, char
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
 }
-// The thread's number, with nothing that was computed from it before: for what is rarely needed and would else stay in registers.
-__device__ __forceinline__ int thread_again() {
-  int t = threadIdx.x;
-  asm volatile("" : "+v"(t));
-  return t;
-}
 constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
+template <int D>
+constexpr int kStage = 64 * D * 2;  // bytes of a stage of keys or values
+// `odd`: set where a stage lacks values that are infinite or NaN.
 template <int D, class E, bool kPrefix>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
+__device__ __forceinline__ void large_share(const PagedParams& p, const Share& w, int kvh, char* const keys0, char* const keys1, char* const values0, char* const values1, int& odd) {
   constexpr int KS = D / 16, NC = D / 32, SL = D / 8, KR = 256 / SL, KP = 64 / KR;
-  constexpr int kStage = 64 * D * 2;  // bytes of a stage of keys or values
   constexpr int kAhead = D == 256 ? 4 : 2;
-  __shared__ __align__(16) char keys0[kStage], keys1[kStage], values0[kStage], values1[kStage];
-  __shared__ int odd;  // a stage lacks values that are infinite or NaN
-  const int kvh = uniform(static_cast<int>(blockIdx.x) % p.kv);
-  Share w;
-  if (!(kPrefix ? prefix_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)
-                : own_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, kLargeLeast, &w)))
-    return;
   const PagedSide& side = kPrefix ? p.prefix : p.own;
   const bool causal = !kPrefix && p.causal;
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -802,10 +803,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>(p.part + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
+        *reinterpret_cast<f32x4*>((kPrefix ? p.prefix_part : p.part) + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
     if (part == 0) {
-      p.ml[held] = make_float2(m, l);
-      if (w.chunk == 0) p.info[out] = make_int2(static_cast<int>(held), w.chunks);
+      (kPrefix ? p.prefix_ml : p.ml)[held] = make_float2(m, l);
+      if (w.chunk == 0) (kPrefix ? p.prefix_info : p.info)[out] = make_int2(static_cast<int>(held), w.chunks);
     }
   } else {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -815,8 +816,74 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(Page
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<uint2*>(p.out + out * D + 32 * c + 2 * e + 4 * part) =
             make_uint2(pack2<E>(o[c][e] * inv, o[c][e + 1] * inv), pack2<E>(o[c][e + 2] * inv, o[c][e + 3] * inv));
-    if (part == 0 && w.chunk == 0) p.info[out] = make_int2(0, 0);
+    if (part == 0 && w.chunk == 0) (kPrefix ? p.prefix_info : p.info)[out] = make_int2(0, 0);
   }
+}
+
+// ------------------------------------------------------------------ the kernels
+template <int D, class E>
+__global__ __launch_bounds__(256, 2) void paged_small_kernel(PagedParams p) {
+  __shared__ __align__(16) char s0[kSmallArea<D>], s1[kSmallArea<D>], s2[kSmallArea<D>], s3[kSmallArea<D>];
+  __shared__ float mx[4][16], ls[4][16];
+  SeqSpan last{0, 0, 0};
+  const int c = uniform(chunk_units(own_work(p, kSmallRows, kSmallUnit, &last).units, p.kv, p.per_slot, 1));
+  Share w;
+  if (!own_share(p, blockIdx.x / p.kv, kSmallRows, kSmallUnit, c, last, &w)) return;
+  small_share<D, E>(p, w, false, uniform(static_cast<int>(blockIdx.x) % p.kv), {s0, s1, s2, s3}, mx, ls);
+}
+template <int D, class E>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_large_kernel(PagedParams p) {
+  __shared__ __align__(16) char keys0[kStage<D>], keys1[kStage<D>], values0[kStage<D>], values1[kStage<D>];
+  __shared__ int odd;
+  SeqSpan last{0, 0, 0};
+  const int c = uniform(chunk_units(own_work(p, kLargeRows, kLargeUnit, &last).units, p.kv, p.per_slot, kLargeLeast));
+  Share w;
+  if (!own_share(p, blockIdx.x / p.kv, kLargeRows, kLargeUnit, c, last, &w)) return;
+  large_share<D, E, false>(p, w, uniform(static_cast<int>(blockIdx.x) % p.kv), keys0, keys1, values0, values1, odd);
+}
+// The prefix and the sequences' own keys in one launch: what multiplies much and what reads many bytes run side by side, and
+// neither waits for the other's slowest share.  The workgroups that run at once are divided by the two sides' work; the prefix's
+// shares, all alike, come first, and the sequences' take what places are left.
+template <int D, class E, bool kOwnLarge, bool kFrontLarge>
+__global__ __launch_bounds__(256, kFrontLarge && D == 256 ? 1 : 2) void paged_pair_kernel(PagedParams p) {
+  static_assert(kFrontLarge || !kOwnLarge, "the prefix has the rows of all sequences");
+  constexpr int kArea = kFrontLarge ? kStage<D> : kSmallArea<D>;
+  static_assert(kArea >= kSmallArea<D>, "either fits");
+  constexpr int kOwnRows = kOwnLarge ? kLargeRows : kSmallRows, kOwnUnit = kOwnLarge ? kLargeUnit : kSmallUnit;
+  constexpr int kFrontRows = kFrontLarge ? kLargeRows : kSmallRows, kFrontUnit = kFrontLarge ? kLargeUnit : kSmallUnit;
+  // Time of a unit of own keys, and of a row tile's start and end, in units of the prefix: a 128-row step takes about 1.8 us and
+  // its kernel's start and end 14, a 16-row round 3 us or, when memory is the limit, 6, its start and end 8.  Measured from 1.2
+  // to 4 and 1 to 8: 64 sequences behind 8192 shared keys 37.5 to 40.8 us (38.9 here), 256 behind 32768 200 to 219 (200).
+  constexpr float kUnitCost = kOwnLarge == kFrontLarge ? 1.f : 3.f, kStartCost = kOwnLarge ? 8.f : kFrontLarge ? 4.5f : 2.f;
+  __shared__ __align__(16) char s0[kArea], s1[kArea], s2[kArea], s3[kArea];
+  __shared__ float mx[4][16], ls[4][16];
+  __shared__ int odd;
+  const int kvh = uniform(static_cast<int>(blockIdx.x) % p.kv), id = blockIdx.x / p.kv;
+  int keys;
+  SeqSpan last{0, 0, 0};
+  const Work front = front_work(p, kFrontRows, kFrontUnit, &keys), own = own_work(p, kOwnRows, kOwnUnit, &last);
+  const float own_cost = static_cast<float>(own.units) * kUnitCost + static_cast<float>(own.tiles) * kStartCost;
+  const float places = static_cast<float>(p.slots), tiles = static_cast<float>(own.tiles * p.kv);
+  float for_own = places * own_cost / (own_cost + static_cast<float>(front.units) + 1.f);
+  if (for_own < tiles) for_own = tiles / rintf(tiles / for_own);  // as many row tiles to each place
+  for_own = fminf(fmaxf(for_own, 1.f), places - 1.f);
+  const float above = 1.000001f;  // more than the quotients' roundings take off
+  const int c0 = uniform(chunk_units(front.units, p.kv, above / (places - for_own), kFrontLarge ? kLargeLeast : 1));
+  const int chunks = uniform(tile_chunks(seq_units(keys, kFrontUnit), c0)), shares = front.tiles * chunks;
+  Share w;
+  if (id < shares) {
+    const int tile = uniform(static_cast<int>(static_cast<uint32_t>(id) / static_cast<uint32_t>(chunks)));
+    w = Share{0, p.T, keys, tile, id - tile * chunks, chunks, tile * chunks, c0, p.prefix.table};
+    if constexpr (kFrontLarge) {
+      large_share<D, E, true>(p, w, kvh, s0, s1, s2, s3, odd);
+      return;
+    }
+  } else {
+    const int c1 = uniform(chunk_units(own.units, p.kv, above / for_own, kOwnLarge ? kLargeLeast : 1));
+    if (!own_share(p, id - shares, kOwnRows, kOwnUnit, c1, last, &w)) return;
+    if constexpr (kOwnLarge) large_share<D, E, false>(p, w, kvh, s0, s1, s2, s3, odd);
+  }
+  if constexpr (!kOwnLarge) small_share<D, E>(p, w, !kFrontLarge && id < shares, kvh, {s0, s1, s2, s3}, mx, ls);
 }
 
 // ------------------------------------------------------------------ merge
@@ -944,17 +1011,16 @@ void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStre
   else bf16 ? launch_append<128, Bf16>(p, stream) : launch_append<128, Fp16>(p, stream);
 }
 
-template <int D, class E, bool kPrefix>
-static void launch_stage(const PagedParams& p, int tile_rows, int64_t tiles, hipStream_t stream) {
-  const dim3 grid(max_chunks(tiles, p.kv, p.slots) * p.kv);
-  if (tile_rows == kLargeRows) hipLaunchKernelGGL((paged_large_kernel<D, E, kPrefix>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((paged_small_kernel<D, E, kPrefix>), grid, dim3(256), 0, stream, p);
-}
 template <int D, class E>
-static void launch_attend(const PagedParams& p, const PagedParams& before, hipStream_t stream) {
+static void launch_attend(const PagedParams& p, hipStream_t stream) {
   const int own = p.own_tile_rows, front = p.prefix_tile_rows;
-  if (p.merge_prefix) launch_stage<D, E, true>(before, front, seq_tiles(p.T, p.group, front), stream);
-  launch_stage<D, E, false>(p, own, max_tiles(p.T, p.B, p.group, own), stream);
+  const int64_t tiles = max_tiles(p.T, p.B, p.group, own) + (p.merge_prefix ? seq_tiles(p.T, p.group, front) : 0);
+  const dim3 grid(max_chunks(tiles, p.kv, p.slots) * p.kv), block(256);
+  if (p.merge_prefix && own == kLargeRows) hipLaunchKernelGGL((paged_pair_kernel<D, E, true, true>), grid, block, 0, stream, p);
+  else if (p.merge_prefix && front == kLargeRows) hipLaunchKernelGGL((paged_pair_kernel<D, E, false, true>), grid, block, 0, stream, p);
+  else if (p.merge_prefix) hipLaunchKernelGGL((paged_pair_kernel<D, E, false, false>), grid, block, 0, stream, p);
+  else if (own == kLargeRows) hipLaunchKernelGGL((paged_large_kernel<D, E>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((paged_small_kernel<D, E>), grid, block, 0, stream, p);
   const int least = own == kLargeRows ? kLargeUnit * kLargeLeast : kSmallUnit;
   if (!p.merge_prefix && p.own.capacity <= least) return;  // one chunk a tile: nothing to merge
   const int64_t rows = static_cast<int64_t>(p.T) * p.heads;
@@ -963,9 +1029,9 @@ static void launch_attend(const PagedParams& p, const PagedParams& before, hipSt
   else if (rows <= 16384) hipLaunchKernelGGL((paged_merge_kernel<D, E, 1, 1>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((paged_merge_kernel<D, E, 1, 16>), dim3((rows + 63) / 64), dim3(256), 0, stream, p);
 }
-void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, const PagedParams& before, hipStream_t stream) {
-  if (head_dim == 256) bf16 ? launch_attend<256, Bf16>(p, before, stream) : launch_attend<256, Fp16>(p, before, stream);
-  else bf16 ? launch_attend<128, Bf16>(p, before, stream) : launch_attend<128, Fp16>(p, before, stream);
+void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, hipStream_t stream) {
+  if (head_dim == 256) bf16 ? launch_attend<256, Bf16>(p, stream) : launch_attend<256, Fp16>(p, stream);
+  else bf16 ? launch_attend<128, Bf16>(p, stream) : launch_attend<128, Fp16>(p, stream);
 }
 
 }  // namespace dflash

@@ -52,8 +52,8 @@ DFLASH_HD int seq_units(int keys, int unit) { return (keys + unit - 1) / unit; }
 
 // Units a chunk, for `total` (tile, unit) pairs of all sequences per KV head: at least total * kv / slots, whatever the
 // product's rounding (a 64-bit division would take longer than the rest of the search).
-DFLASH_HD int chunk_units(int64_t total, int kv, double per_slot, int least) {
-  const double c = static_cast<double>(total) * kv * per_slot;
+DFLASH_HD int chunk_units(double total, int kv, double per_slot, int least) {
+  const double c = total * kv * per_slot;
   const int up = c < 1e9 ? static_cast<int>(c) + 1 : 1000000001;
   return up < least ? least : up;
 }
