@@ -101,6 +101,26 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const SeqSpan s = seq_span(p.starts[b], p.starts[b + 1], p.side.lengths[b], p.T, p.side.capacity);
   if (t < s.start || t >= s.start + s.tokens) return;
   const int row = s.keys - s.tokens + t - s.start;
+  const int all = p.heads + 2 * p.kv, c = (tid % L) * 8, step = gridDim.y * kHeads;
+  const auto read = [&](int j) {
+    const bool is_q = j < p.heads, is_v = j >= p.heads + p.kv;
+    const int h = is_q ? j : is_v ? j - p.heads - p.kv : j - p.heads;
+    const uint16_t* src = is_q ? p.query + t * p.query_token + h * p.query_head
+                        : is_v ? p.value + t * p.value_token + h * p.value_head
+                               : p.key + t * p.key_token + h * p.key_head;
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + c));  // read once
+  };
+  // the first heads are on their way while the angles are made, the next while heads are turned
+  int j = blockIdx.y * kHeads + tid / L;
+  u32x4 next{0, 0, 0, 0};
+  if (j < all) next = read(j);
+  int page = -1, inside = 0;  // where the token's rows go; -1: nowhere
+  if (row >= 0) {
+    const int i = divide(row >> 4, p.side.groups_per_page);
+    page = p.side.table[b * p.side.table_stride + i];
+    inside = row - i * p.side.page_groups * 16;
+    if (page >= p.side.pages) page = -1;
+  }
   if (p.half) {
     const int position = p.positions ? p.positions[t] : row;
     for (int i = tid; i < p.half; i += 256) {
@@ -112,14 +132,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     }
   }
   __syncthreads();
-  const int all = p.heads + 2 * p.kv, c = (tid % L) * 8;
-  for (int j = blockIdx.y * kHeads + tid / L; j < all; j += gridDim.y * kHeads) {
+  for (; j < all; j += step) {
     const bool is_q = j < p.heads, is_v = j >= p.heads + p.kv;
     const int h = is_q ? j : is_v ? j - p.heads - p.kv : j - p.heads;
-    const uint16_t* src = is_q ? p.query + t * p.query_token + h * p.query_head
-                        : is_v ? p.value + t * p.value_token + h * p.value_head
-                               : p.key + t * p.key_token + h * p.key_head;
-    const u32x4 raw = *reinterpret_cast<const u32x4*>(src + c);
+    const u32x4 raw = next;
+    if (j + step < all) next = read(j + step);
     u32x4 out = raw;
     if (!is_v) {
       float v[8];
@@ -157,14 +174,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     }
     if (is_q) {
       *reinterpret_cast<u32x4*>(p.query_out + (static_cast<int64_t>(t) * p.heads + h) * D + c) = out;
-    } else if (row >= 0) {
-      const int i = divide(row >> 4, p.side.groups_per_page), page = p.side.table[b * p.side.table_stride + i];
-      const int inside = row - i * p.side.page_groups * 16;
-      if (page >= 0 && page < p.side.pages) {
-        uint16_t* dst = is_v ? p.values + page * p.side.value_page + h * p.side.value_head + inside * p.side.value_row
-                             : p.keys + page * p.side.key_page + h * p.side.key_head + inside * p.side.key_row;
-        *reinterpret_cast<u32x4*>(dst + c) = out;
-      }
+    } else if (page >= 0) {
+      uint16_t* dst = is_v ? p.values + page * p.side.value_page + h * p.side.value_head + inside * p.side.value_row
+                           : p.keys + page * p.side.key_page + h * p.side.key_head + inside * p.side.key_row;
+      *reinterpret_cast<u32x4*>(dst + c) = out;
     }
   }
 }
@@ -1004,7 +1017,7 @@ static void launch_append(const AppendParams& p, hipStream_t stream) {
   // a token's heads over several workgroups while there are few tokens: each makes the token's angles itself
   constexpr int kHeads = 256 / (D / 8);
   const int all = (p.heads + 2 * p.kv + kHeads - 1) / kHeads;
-  hipLaunchKernelGGL((paged_append_kernel<D, E>), dim3(p.T, p.T <= 256 ? all : 1), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((paged_append_kernel<D, E>), dim3(p.T, p.T <= 1024 ? all : 1), dim3(256), 0, stream, p);
 }
 void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStream_t stream) {
   if (head_dim == 256) bf16 ? launch_append<256, Bf16>(p, stream) : launch_append<256, Fp16>(p, stream);
