@@ -255,8 +255,10 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
       out->start = __builtin_amdgcn_readlane(s.start, l);
       out->tokens = __builtin_amdgcn_readlane(s.tokens, l);
       out->keys = __builtin_amdgcn_readlane(s.keys, l);
-      out->tile = uniform(static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks)));
-      out->chunk = uniform(rest - out->tile * chunks);
+      // last tile first: where the block's tokens mask what follows them, the later tiles have more keys
+      const int tile = static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks));
+      out->tile = uniform(__builtin_amdgcn_readlane(n, l) / chunks - 1 - tile);
+      out->chunk = uniform(rest - tile * chunks);
       out->chunks = chunks;
       out->partial = chunks > 1 || p.merge_prefix
                          ? uniform(held + __builtin_amdgcn_readlane(sum_kept - kept, l) + out->tile * chunks) : -1;
