@@ -235,7 +235,9 @@ __device__ __forceinline__ Work front_work(const PagedParams& p, int tile_rows, 
 }
 
 // Share `id` of the sequences' own keys in chunks of c units: every wave finds it by itself, 64 sequences at a time, one a lane.
-// `s`: what own_work left.
+// `s`: what own_work left.  A sequence's last tiles come first: where the block's tokens mask what follows them, later tiles have more
+// keys, and the longest should not start last.  (All sequences' tiles in one order by their place: 1% faster with prompts of 442 to
+// 2222 tokens, not kept.)
 __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile_rows, int unit, int c, SeqSpan s, Share* out) {
   const int lane = threadIdx.x & 63;
   int first = 0, held = 0;  // shares and partial tiles of the sequences before
@@ -252,19 +254,21 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
       const int l = __builtin_ctzll(m);
       const int rest = id - (first + __builtin_amdgcn_readlane(sum - n, l));
       const int chunks = __builtin_amdgcn_readlane(k, l);
+      const uint32_t tiles = __builtin_amdgcn_readlane(n, l) / static_cast<uint32_t>(chunks);
+      const uint32_t before = static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks);
+      const int chunk = rest - before * chunks;
       out->start = __builtin_amdgcn_readlane(s.start, l);
       out->tokens = __builtin_amdgcn_readlane(s.tokens, l);
       out->keys = __builtin_amdgcn_readlane(s.keys, l);
-      // last tile first: where the block's tokens mask what follows them, the later tiles have more keys
-      const int tile = static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks));
-      out->tile = uniform(__builtin_amdgcn_readlane(n, l) / chunks - 1 - tile);
-      out->chunk = uniform(rest - tile * chunks);
+      out->tile = uniform(static_cast<int>(tiles - 1 - before));
+      out->chunk = uniform(chunk);
       out->chunks = chunks;
       out->partial = chunks > 1 || p.merge_prefix
                          ? uniform(held + __builtin_amdgcn_readlane(sum_kept - kept, l) + out->tile * chunks) : -1;
       out->c = c;
       out->table = p.own.table + static_cast<int64_t>(b0 + l) * p.own.table_stride;
-      return true;
+      // blocks that overlap (starts that are no such thing) may have more tiles than there is room for
+      return out->partial < 0 || static_cast<int64_t>(out->partial + chunk + 1) * p.kv * tile_rows <= p.part_rows[0];
     }
     first += __builtin_amdgcn_readlane(sum, 63);
     held += __builtin_amdgcn_readlane(sum_kept, 63);

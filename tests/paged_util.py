@@ -45,10 +45,8 @@ class Batch:
         """Rows of sequence b, [rows, kv, dim], in 64 bits."""
         n = self.spans[b][1]
         pool = self.host[name].double()
-        out = torch.empty((n, self.kv, self.dim), dtype=torch.float64)
-        for r in range(n):
-            out[r] = pool[self.table[b, r // self.page].item(), :, r % self.page]
-        return out
+        r = torch.arange(n)
+        return pool[self.table[b, r // self.page].long(), :, r % self.page].reshape(n, self.kv, self.dim)
 
 
 def attend(q, k, v, seen, scale):
@@ -96,6 +94,29 @@ def bound(dtype, dim, scale, size, most, keys):
     weight = (dim + 6) * 2.0 ** -24 * scale * most + 2.0 ** -22
     relative = 2 * UNIT[dtype] * (1 + UNIT[dtype]) + 2 * weight + 2 * (keys + 16) * 2.0 ** -24
     return relative * size + (keys + 1) * TINY[dtype] * 8        # |v| stays under 8
+
+
+def expected_wide(batch, scale, causal, device, prefix=None):
+    """expected() on the device, a head at a time over all rows of a sequence (values must be finite)."""
+    shape = (batch.tokens, batch.heads, batch.dim)
+    out, size = torch.zeros(shape, dtype=torch.float64), torch.zeros(shape, dtype=torch.float64)
+    most, keys, at, group = 0.0, 1, 0, batch.heads // batch.kv
+    for b, (t, n) in enumerate(batch.spans):
+        k, v, front = batch.rows(b), batch.rows(b, "values"), 0
+        if prefix is not None:
+            front = prefix.spans[0][1]
+            k, v = torch.cat((prefix.rows(0), k)), torch.cat((prefix.rows(0, "values"), v))
+        seen = front + (torch.arange(n - t, n) + 1 if causal else torch.full((t,), n)).clamp(min=0)
+        hidden = torch.arange(front + n)[None] >= seen[:, None]
+        hidden, k, v = hidden.to(device), k.to(device), v.to(device)
+        for h in range(batch.heads):
+            q, kh, vh = batch.query[at:at + t, h].double().to(device), k[:, h // group].contiguous(), v[:, h // group].contiguous()
+            p = torch.softmax((scale * (q @ kh.T.contiguous())).masked_fill(hidden, -float("inf")), 1).nan_to_num(0.0)
+            out[at:at + t, h], size[at:at + t, h] = (p @ vh).cpu(), (p @ vh.abs()).cpu()
+            if t and front + n:
+                most = max(most, float((q.abs() @ kh.abs().T.contiguous()).masked_fill(hidden, 0.0).max()))
+        keys, at = max(keys, front + n), at + t
+    return out, size, most, keys
 
 
 def turned(x, weight, inv_freq, positions, eps):

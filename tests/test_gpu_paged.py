@@ -20,8 +20,8 @@ def check(got, want, limit, what=""):
     assert worst <= 0, (what, worst)
 
 
-def attended(pkg, batch, causal, prefix=None, scale=None):
-    """The operator's result over a batch, checked against 64 bits; rows of tokens in no sequence stay."""
+def attended(pkg, batch, causal, prefix=None, scale=None, wide=False):
+    """The operator's result over a batch, checked against 64 bits (``wide``: on the device); rows of tokens in no sequence stay."""
     scale = batch.dim ** -0.5 if scale is None else scale
     out = torch.full((batch.total, batch.heads, batch.dim), 7.0, dtype=batch.dtype, device=batch.q.device)
     if prefix is None:
@@ -29,7 +29,8 @@ def attended(pkg, batch, causal, prefix=None, scale=None):
     else:
         got = pkg.ops.shared_prefix_attention(batch.q, prefix.cache, batch.cache, batch.s, scale=scale, causal=causal, out=out)
     assert got is out
-    want, size, most, keys = pu.expected(batch, scale, causal, prefix)
+    want, size, most, keys = (pu.expected_wide(batch, scale, causal, batch.q.device, prefix) if wide
+                              else pu.expected(batch, scale, causal, prefix))
     check(got[:batch.tokens], want, pu.bound(batch.dtype, batch.dim, scale, size, most, keys), str(batch.spans[:4]))
     assert (got[batch.tokens:] == 7.0).all()
     return got
@@ -59,6 +60,52 @@ def test_attention(pkg, device, spans, shape, page, dtype, causal):
 def test_attention_over_many_chunks(pkg, device, shape):
     attended(pkg, pu.Batch(pkg, device, [(1, 5003)], page=64, dtype=BF16, seed=1, **shape), True)
     attended(pkg, pu.Batch(pkg, device, [(3, 4099), (1, 9), (16, 700)], page=16, dtype=FP16, seed=2, **shape), True)
+
+
+# Row tiles of 128: chunks longer than 16 and 32 steps of 64 keys, chunks that end inside a step and inside a page
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape,page,spans", [
+    (MODEL, 64, [(600, 4100)]), (MODEL, 16, [(513, 2900), (40, 41), (129, 1411)]), (SMALL, 64, [(1500, 4100)]),
+    (dict(heads=32, kv=8, dim=128), 16, [(700, 2950)]), (dict(heads=1, kv=1, dim=128), 16, [(333, 700)]),
+    (dict(heads=7, kv=1, dim=256), 32, [(90, 9001)])])
+def test_attention_of_many_rows(pkg, device, shape, page, spans, causal):
+    attended(pkg, pu.Batch(pkg, device, spans, page=page, dtype=BF16, seed=len(spans), spare=1, **shape), causal, wide=True)
+
+
+@pytest.mark.parametrize("shape", [dict(heads=32, kv=8, dim=128), MODEL, dict(heads=8, kv=8, dim=256)])
+@pytest.mark.parametrize("spans", [[(900, 900), (130, 1000), (0, 0), (1800, 1800), (5, 5)], [(60, 64 + 7 * b) for b in range(66)],
+                                   [(33, 33)] * 64])
+def test_more_row_tiles_than_workgroups_at_once(pkg, device, shape, spans):
+    """Several to a place, of more and of fewer sequences than lanes, and more than 16384 rows to merge."""
+    attended(pkg, pu.Batch(pkg, device, spans, page=16, dtype=FP16, seed=3, spare=1, **shape), True, wide=True)
+
+
+@pytest.mark.parametrize("shape", [MODEL, SMALL])
+@pytest.mark.parametrize("tokens,rows", [(20, 301), (40, 1003), (128, 4001)])
+def test_many_rows_over_a_page_of_any_size(pkg, device, shape, tokens, rows):
+    batch = pu.Batch(pkg, device, [(tokens, rows), (tokens, tokens + 5)], page=rows, dtype=BF16, seed=5, one_page=True, **shape)
+    attended(pkg, batch, True, wide=True)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("shape", [MODEL, SMALL, dict(heads=2, kv=2, dim=256)])
+def test_a_value_among_many_counts_only_where_it_is_seen(pkg, device, shape, bad):
+    """Values that are NaN or infinite inside blocks of hundreds of tokens, in the first, an inner and the last step and chunk."""
+    tokens, keys = 500, 2113
+    batch = pu.Batch(pkg, device, [(tokens, keys), (1, 9)], page=16, dtype=BF16, seed=17, **shape)
+    scale, pool = batch.dim ** -0.5, batch.cache.values
+    for i in (0, 1, 63, 64, 250, 498, 499):
+        row = keys - tokens + i
+        at = (batch.table[0, row // 16].item(), slice(None), row % 16, 5)
+        kept = pool[at].clone()
+        pool[at] = 0.0
+        want = pkg.ops.paged_attention(batch.q, batch.cache, batch.s, scale=scale)
+        pool[at] = bad
+        got = pkg.ops.paged_attention(batch.q, batch.cache, batch.s, scale=scale)
+        pool[at] = kept
+        assert not torch.isfinite(got[i:tokens, :, 5]).any(), i
+        got[i:tokens, :, 5] = want[i:tokens, :, 5]
+        assert torch.equal(got, want), i
 
 
 @pytest.mark.parametrize("count", [64, 65, 150])
@@ -180,6 +227,17 @@ def test_many_sequences_behind_a_long_prefix(pkg, device):
     batch = pu.Batch(pkg, device, [(1, b % 40) for b in range(90)], page=16, dtype=BF16, seed=13, **SMALL)
     prefix = pu.Batch(pkg, device, [(0, 2500)], page=64, dtype=BF16, seed=14, **SMALL)
     attended(pkg, batch, True, prefix)
+
+
+@pytest.mark.parametrize("shape", [MODEL, dict(heads=32, kv=8, dim=128)])
+@pytest.mark.parametrize("spans,rows", [([(1, 300 + b) for b in range(64)], 4097), ([(1, (37 * b) % 600) for b in range(130)], 2003),
+                                        ([(50, 50 + 9 * b) for b in range(12)], 3003), ([(1, 2)] * 3, 7000),
+                                        ([(300, 2500)], 40), ([(1, 5000), (1, 1)], 33)])
+def test_prefixes_and_own_keys_of_many_sizes(pkg, device, shape, spans, rows):
+    """Much of the one and little of the other: their shares of the workgroups."""
+    batch = pu.Batch(pkg, device, spans, page=16, dtype=BF16, seed=rows, spare=1, **shape)
+    prefix = pu.Batch(pkg, device, [(0, rows)], page=64, dtype=BF16, seed=rows + 1, **shape)
+    attended(pkg, batch, True, prefix, wide=True)
 
 
 # ------------------------------------------------------------------ append
@@ -347,6 +405,44 @@ def test_starts_that_are_no_such_thing_stay_inside(pkg, device):
             pkg.ops.paged_append(cache, rows, rows, s)
     torch.cuda.synchronize()
     assert (keep[16:] == 3).all()
+
+
+@pytest.mark.parametrize("shape,tokens", [(MODEL, 700), (SMALL, 40), (MODEL, 12)])
+def test_overlapping_blocks_stay_inside_the_workspace(pkg, device, shape, tokens):
+    """Starts out of order, so that sequences' blocks hold more rows than the batch: nothing behind the workspace is written."""
+    batch = pu.Batch(pkg, device, [(tokens, 3 * tokens + 900)] + [(0, 1200)] * 7, page=16, dtype=BF16, seed=19, **shape)
+    prefix = pu.Batch(pkg, device, [(0, 500)], page=16, dtype=BF16, seed=20, **shape)
+    wild = torch.tensor([0, tokens] * 4 + [0], dtype=torch.int32, device=device)
+    for front in (None, prefix):
+        size = pkg.ops.paged_attention_workspace_bytes(tokens, batch.heads, batch.kv, batch.dim, 8, front is not None)
+        room = torch.full((size + (1 << 24),), 0x5A, dtype=torch.uint8, device=device)
+        out = torch.zeros((tokens + 64, batch.heads, batch.dim), dtype=BF16, device=device)
+        if front is None:
+            pkg.ops.paged_attention(batch.q, batch.cache, wild, scale=0.1, out=out[:tokens], workspace=room)
+        else:
+            pkg.ops.shared_prefix_attention(batch.q, front.cache, batch.cache, wild, scale=0.1, out=out[:tokens], workspace=room)
+        assert (room[size:] == 0x5A).all() and (out[tokens:] == 0).all()
+
+
+def test_two_streams_at_once(pkg, device):
+    """Calls on two streams side by side, each with what it allocates itself, give what they give alone."""
+    big = pu.Batch(pkg, device, [(600, 2100)], page=16, dtype=BF16, seed=21, **MODEL)
+    small = pu.Batch(pkg, device, [(1, 900 + b) for b in range(24)], page=16, dtype=BF16, seed=22, **MODEL)
+    prefix = pu.Batch(pkg, device, [(0, 1500)], page=64, dtype=BF16, seed=23, **MODEL)
+    calls = (lambda: pkg.ops.paged_attention(big.q, big.cache, big.s, scale=0.06),
+             lambda: pkg.ops.shared_prefix_attention(small.q, prefix.cache, small.cache, small.s, scale=0.06))
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], [[], []]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, call in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for one, many in zip(alone, got):
+        assert all(torch.equal(one, other) for other in many)
 
 
 def test_other_stream_and_repeats(pkg, device):

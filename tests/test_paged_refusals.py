@@ -26,7 +26,8 @@ BAD_CACHES = [
     (dict(kv_heads=0), 1, "out of range"), (dict(kv_heads=1025), 1, "out of range"), (dict(sequences=-1), 1, "out of range"),
     (dict(sequences=(1 << 20) + 1), 1, "out of range"), (dict(pages=1 << 31), 1, "out of range"),
     (dict(table_stride=-4), 1, "out of range"), (dict(key_row_stride=129), 1, "multiples of 8"),
-    (dict(value_page_stride=-8), 1, "multiples of 8"), (dict(keys=0), 1, "NULL"), (dict(lengths=0), 1, "NULL"),
+    (dict(value_page_stride=-8), 1, "multiples of 8"), (dict(key_row_stride=(1 << 26) + 8), 2, "2\\^26"),
+    (dict(value_row_stride=1 << 40), 2, "2\\^26"), (dict(keys=0), 1, "NULL"), (dict(lengths=0), 1, "NULL"),
     (dict(values=ADDRESS + 8), 1, "aligned")]
 
 
