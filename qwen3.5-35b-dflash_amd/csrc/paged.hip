@@ -214,18 +214,20 @@ struct Work {
 };
 __device__ __forceinline__ Work own_work(const PagedParams& p, int tile_rows, int unit, SeqSpan* last) {
   const int lane = threadIdx.x & 63;
-  Work w{0, 0.0};
+  int tiles = 0;
+  uint64_t units = 0;
+#pragma unroll 4
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     *last = SeqSpan{0, 0, 0};
     if (b0 + lane < p.B) *last = load_span(p, b0 + lane);
-    const int tiles = seq_tiles(last->tokens, p.group, tile_rows);
-    // tiles <= 2^18 and units <= 2^24: the product in two parts whose sums stay in 31 bits
-    const uint64_t u = static_cast<uint64_t>(tiles) * seq_units(last->keys, unit);
-    const int lo = wave_scan(static_cast<int>(u & 0xFFFFFF)), hi = wave_scan(static_cast<int>(u >> 24));
-    w.units += static_cast<double>((static_cast<int64_t>(__builtin_amdgcn_readlane(hi, 63)) << 24) + __builtin_amdgcn_readlane(lo, 63));
-    w.tiles += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+    const int t = seq_tiles(last->tokens, p.group, tile_rows);
+    tiles += t;
+    units += static_cast<uint64_t>(t) * seq_units(last->keys, unit);
   }
-  return w;
+  // in two parts whose sums stay in 31 bits
+  const int lo = wave_scan(static_cast<int>(units & 0xFFFFFF)), hi = wave_scan(static_cast<int>(units >> 24));
+  return Work{__builtin_amdgcn_readlane(wave_scan(tiles), 63),
+              __builtin_amdgcn_readlane(hi, 63) * 16777216.0 + __builtin_amdgcn_readlane(lo, 63)};
 }
 // The prefix as a sequence whose block is the whole batch.
 __device__ __forceinline__ Work front_work(const PagedParams& p, int tile_rows, int unit, int* keys) {
@@ -240,15 +242,16 @@ __device__ __forceinline__ Work front_work(const PagedParams& p, int tile_rows, 
 // 2222 tokens, not kept.)
 __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile_rows, int unit, int c, SeqSpan s, Share* out) {
   const int lane = threadIdx.x & 63;
-  int first = 0, held = 0;  // shares and partial tiles of the sequences before
+  int first = 0, held = 0;  // shares of the sequences before; partial tiles of those that this lane had
+  const auto at = [&](int b) { return b < p.B ? load_span(p, b) : SeqSpan{0, 0, 0}; };
+  SeqSpan next = s;
+  if (p.B > 64) next = at(lane);
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    if (p.B > 64) {
-      s = SeqSpan{0, 0, 0};
-      if (b0 + lane < p.B) s = load_span(p, b0 + lane);
-    }
+    s = next;
+    if (b0 + 64 < p.B) next = at(b0 + 64 + lane);
     const int k = tile_chunks(seq_units(s.keys, unit), c), n = seq_tiles(s.tokens, p.group, tile_rows) * k;
     const int kept = k > 1 || p.merge_prefix ? n : 0;
-    const int sum = wave_scan(n), sum_kept = wave_scan(kept);
+    const int sum = wave_scan(n);
     const uint64_t m = __ballot(n > 0 && id < first + sum);
     if (m) {
       const int l = __builtin_ctzll(m);
@@ -257,6 +260,7 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
       const uint32_t tiles = __builtin_amdgcn_readlane(n, l) / static_cast<uint32_t>(chunks);
       const uint32_t before = static_cast<uint32_t>(rest) / static_cast<uint32_t>(chunks);
       const int chunk = rest - before * chunks;
+      const int partial = __builtin_amdgcn_readlane(wave_scan(held + (lane < l ? kept : 0)), 63);
       out->start = __builtin_amdgcn_readlane(s.start, l);
       out->tokens = __builtin_amdgcn_readlane(s.tokens, l);
       out->keys = __builtin_amdgcn_readlane(s.keys, l);
@@ -264,14 +268,14 @@ __device__ __forceinline__ bool own_share(const PagedParams& p, int id, int tile
       out->chunk = uniform(chunk);
       out->chunks = chunks;
       out->partial = chunks > 1 || p.merge_prefix
-                         ? uniform(held + __builtin_amdgcn_readlane(sum_kept - kept, l) + out->tile * chunks) : -1;
+                         ? uniform(partial + out->tile * chunks) : -1;
       out->c = c;
       out->table = p.own.table + static_cast<int64_t>(b0 + l) * p.own.table_stride;
       // blocks that overlap (starts that are no such thing) may have more tiles than there is room for
       return out->partial < 0 || static_cast<int64_t>(out->partial + chunk + 1) * p.kv * tile_rows <= p.part_rows[0];
     }
     first += __builtin_amdgcn_readlane(sum, 63);
-    held += __builtin_amdgcn_readlane(sum_kept, 63);
+    held += kept;
   }
   return false;
 }
