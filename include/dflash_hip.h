@@ -321,7 +321,7 @@ int dflash_attention_mixer(const dflash_attention* a, const float* hidden, int64
  * the pool: attention reads the nearest page instead, append leaves such rows out.  Lengths are taken as at most
  * table_width * page_size.
  * Constraints: head_dim 128 or 256, dtype BF16 or F16, page_size % 16 == 0 or table_width == 1,
- * page_size <= 2^30, table_width * page_size <= 2^30.
+ * page_size <= 2^30, table_width * page_size <= 2^30, row strides <= 2^26.
  */
 typedef struct dflash_paged_kv {
   void* keys;

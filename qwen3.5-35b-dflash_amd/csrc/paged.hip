@@ -80,6 +80,8 @@ __device__ __forceinline__ PageAt page_at(const PagedSide& s, const int32_t* tab
 // One workgroup per (token, slice of its heads); D / 8 lanes a head row, 8 features a lane.  The token's cosines and sines are
 // made once for all its heads: 64-bit products and reduction by 2 pi (positions reach 2^31, where a 32-bit angle is off by
 // more than a turn), then fp32 functions of the remainder.
+// Bound: memory, behind it the angles' latency, which the first heads' loads cover: 15005 tokens of 48 rows at head dim 128, 218 MB,
+// 52.5 us (4.15 TB/s; a large copy 4.64); few tokens: the launch and the chain starts - table - store, 5.1 us for one.
 template <int D, class E>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int L = D / 8, kHeads = 256 / L;
@@ -292,6 +294,10 @@ __device__ __forceinline__ int thread_again() {
 // 16-key tiles, which, with those eight keys as the reduction's octet l >> 4, is the B operand of O^T = V^T P^T as it stands.  The A
 // operand needs eight keys of one dim per lane: a lane loads D / 16 neighbouring dims of its eight keys and pairs halves in
 // registers, so V needs no transpose and neither operand passes through LDS.
+// Bound: memory.  A wave has a round's 32 keys and values in flight, two workgroups a CU: one at head dim 256 (300 registers
+// instead of 256) takes 130 us instead of 120 for 64 sequences of up to 8192 keys, 572 MB (4.8 TB/s); streaming loads 132,
+// the rounds' places looked up eight rounds ahead 137.  One row behind 131072 keys, 268 MB: 43.5 us.  Few keys: latency,
+// 8 us for a row behind 4000.
 constexpr int kSmallRows = 16, kSmallUnit = 128;  // keys a round of the four waves
 template <int D>
 constexpr int kSmallPitch = D + 4;
@@ -466,6 +472,11 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // keys 8 (e / 4) + 4 (l >> 5) + e % 4 of a 32-key block (e: element of the 32x32 result), whose elements 8 s to 8 s + 7 are, as a
 // reduction's octet l >> 5, the B operand of O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's
 // operand needs eight keys of a dim: two transposing LDS reads of four keys each.
+// Bound: matrix instructions and LDS reads, which take about as long (a wave reads every key and value for its 32 rows; 64 rows a
+// wave would halve the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of
+// 256: 243 us, 990 TFLOP/s (a large library product 1305); prompts of 442 to 2222 tokens, 32 heads of 128: 132 us,
+// 656, of which a workgroup's start and end take a quarter at 13 steps on average.  Started cold, a launch spends about 14 us
+// before and behind its steps, most of it fetching code that runs once.
 // The rows' running maximum is a reference that moves only when a score exceeds it by 8 (weights reach 2^8, their relative precision
 // is the same): the accumulators are rescaled a few times a row instead of at every step.
 // A run of n matrix instructions that take one operand each from LDS: use(i, read(i)) for all i, each read kAhead instructions ahead of
@@ -913,6 +924,9 @@ __global__ __launch_bounds__(256, kFrontLarge && D == 256 ? 1 : 2) void paged_pa
 // kWaves waves per (token, head), D / 64 dims a lane; wave w takes the row's partial results w, w + kWaves, ..., eight in flight, and
 // the waves' sums meet in LDS.  The order of the additions depends on the sizes alone.  A wave that has rows to itself (kWaves 1)
 // looks at kRows of them at once and takes those that are in parts.
+// Bound: latency (info, then the parts): 4.7 us where nothing is in parts, 6 to 9 where all is.  Eight waves a row instead of one: 62
+// instead of 83 us for a row behind 131072 keys, 17.6 instead of 20.9 for 8 blocks of 2 behind 4096 (both kernels); sixteen rows a
+// wave instead of one: 2 us less for 32768 rows that are in one part each.
 template <int D, class E, int kWaves, int kRows>
 __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_kernel(PagedParams p) {
   static_assert(kWaves == 1 || kRows == 1, "waves that share rows meet once");
@@ -1013,11 +1027,14 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_k
 
 }  // namespace
 
-// Rows of a stage's tiles, by the rows a sequence has on average: up to 32 take the kernel of 16 rows, whose waves share the
-// keys out; more take the one of 128, whose waves share the keys' way through LDS.
+// Rows of a side's tiles, by the rows a sequence has on average: up to 20 take the kernel of 16 rows, whose waves share the
+// keys out; more, which would be two such tiles or several, take the one of 128, whose waves share the keys' way through LDS.  16 and
+// 128 rows, us: 64 sequences behind 4096 keys, 16 rows each 106 and 105, 24 rows 164 and 106, 32 rows 167 and 108; 8 sequences,
+// 16 rows 24 and 25, 24 rows 32 and 26, 128 rows at most 32 and 28.5; of unlike blocks, 64 of 18 rows on average 75 and 90, 8 of
+// 21 25 and 23, 64 of 31 115 and 93; 16 sequences of 24 rows behind 1000 keys 17 and 21; one row 13 and 18.
 int paged_tile_rows(int64_t tokens, int64_t sequences, int64_t group) {
   const int64_t blocks = std::max<int64_t>(1, std::min(tokens, sequences));
-  return tokens * group > 32 * blocks ? kLargeRows : kSmallRows;
+  return tokens * group > 20 * blocks ? kLargeRows : kSmallRows;
 }
 // Workgroups that a stage's work is cut for: as many as run at once.
 int paged_slots(int tile_rows, int head_dim, int cus) { return tile_rows == kLargeRows && head_dim == 256 ? cus : 2 * cus; }

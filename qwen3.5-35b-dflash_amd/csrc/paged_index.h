@@ -3,7 +3,7 @@
 //
 // Attention work is cut in two directions.  A sequence's block gives ceil(tokens * group / R) row tiles of R rows (row =
 // token * group + head in group) per KV head.  A tile's keys are cut into chunks of `c` units of `unit` keys, with one c
-// for the whole batch: c = max(c_min, ceil(U * kv / slots)), U = sum over sequences of tiles * ceil(keys / unit).  Equal
+// for the whole batch: c = max(c_min, U * kv / slots rounded up), U = sum over sequences of tiles * ceil(keys / unit).  Equal
 // chunks keep the workgroups alike whatever the lengths are, and there are at most slots / kv + tiles of them per KV
 // head, which bounds the grid without knowing a length on the host.
 #pragma once
