@@ -5,7 +5,7 @@ The directory name is not a Python identifier; load it under the alias
 ``bench.py``).  Modules:
 
 * ``fused_ops`` -- FusedOps ABI-v1 adapter module (the drop-in seam)
-* ``ops``       -- PyTorch-ROCm wrappers over the C ABI
+* ``ops``       -- PyTorch-ROCm wrappers over the C ABI, the operators of the paged cache of many sequences among them
 * ``packing``   -- ``PackedW4`` / ``SharedExpert`` types and the int4 packer
 * ``plan``      -- tensor inventory of the target (names, shapes, which are int4)
 * ``layers``    -- non-hot decoder arithmetic (delta rule, norms, rotary, attention)
