@@ -318,8 +318,8 @@ int dflash_attention_mixer(const dflash_attention* a, const float* hidden, int64
  * lengths[b] counts the rows of sequence b, those of the block that a call appends or attends with included.
  * table and lengths are read on the device when the call runs: a captured call follows their later values.  Table
  * entries behind a sequence's last row are not read.  An entry outside [0, pages) within it is never followed out of
- * the pool: attention reads the nearest page instead, append leaves such rows out.  Lengths are taken as at most
- * table_width * page_size.
+ * the pool: attention reads the nearest page instead, append leaves such rows out.  Attention takes lengths as at most
+ * table_width * page_size; append leaves out rows past that.
  * Constraints: head_dim 128 or 256, dtype BF16 or F16, page_size % 16 == 0 or table_width == 1,
  * page_size <= 2^30, table_width * page_size <= 2^30, row strides <= 2^26.
  */
@@ -347,7 +347,8 @@ typedef struct dflash_rows {
  * Append a block's K and V rows to their sequences' pages, with the Q/K norm and the position rotation on the way
  * (model/qwen35_moe_dflash/fused/model.py:265-294).  Tokens [starts[b], starts[b + 1]) of the block are the last ones of
  * sequence b: token i of them goes to row lengths[b] - (starts[b + 1] - starts[b]) + i.  starts: int32 [sequences + 1] on
- * the device, ascending from 0 to at most `tokens`; tokens past starts[sequences] are left out, as are rows before 0.
+ * the device, ascending from 0 to at most `tokens`; tokens past starts[sequences] are left out, as are rows before 0 (their
+ * queries are turned all the same).
  *   n = x / sqrt(mean(x^2) + eps) * (norm + 1)       (q_norm, k_norm: fp32 [head_dim] or NULL: n = x)
  *   y_i = n_i cos(a_i) - n_{i+h} sin(a_i), y_{i+h} = n_{i+h} cos(a_i) + n_i sin(a_i)  for i < h = rotary_dim / 2,
  *   a_i = position * inv_freq_i (inv_freq fp32 [h]; NULL: y = n); position: positions[token] (int32 [tokens]) or, NULL, the

@@ -102,7 +102,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   if (b == p.B) return;
   const SeqSpan s = seq_span(p.starts[b], p.starts[b + 1], p.side.lengths[b], p.T, p.side.capacity);
   if (t < s.start || t >= s.start + s.tokens) return;
-  const int row = s.keys - s.tokens + t - s.start;
+  // of the length as it stands, not the most that the table holds: rows past that have no page
+  const int64_t row = static_cast<int64_t>(p.side.lengths[b]) - s.tokens + t - s.start;
   const int all = p.heads + 2 * p.kv, c = (tid % L) * 8, step = gridDim.y * kHeads;
   const auto read = [&](int j) {
     const bool is_q = j < p.heads, is_v = j >= p.heads + p.kv;
@@ -117,14 +118,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   u32x4 next{0, 0, 0, 0};
   if (j < all) next = read(j);
   int page = -1, inside = 0;  // where the token's rows go; -1: nowhere
-  if (row >= 0) {
-    const int i = divide(row >> 4, p.side.groups_per_page);
+  if (row >= 0 && row < p.side.capacity) {
+    const int i = divide(static_cast<uint32_t>(row) >> 4, p.side.groups_per_page);
     page = p.side.table[b * p.side.table_stride + i];
-    inside = row - i * p.side.page_groups * 16;
+    inside = static_cast<int>(row) - i * p.side.page_groups * 16;
     if (page >= p.side.pages) page = -1;
   }
   if (p.half) {
-    const int position = p.positions ? p.positions[t] : row;
+    const int64_t position = p.positions ? p.positions[t] : row;
     for (int i = tid; i < p.half; i += 256) {
       const double a = static_cast<double>(position) * static_cast<double>(p.inv_freq[i]);
       const double turns = rint(a * 0.15915494309189535);

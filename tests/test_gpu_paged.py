@@ -346,6 +346,24 @@ def test_append_leaves_out_rows_without_a_page(pkg, device):
         assert torch.equal(batch.cache.keys.view(torch.int16), want.view(torch.int16)), wild
 
 
+@pytest.mark.parametrize("length", [48, 49, 55, 67, 68, 1 << 30, (1 << 31) - 1])
+def test_append_past_the_last_page_leaves_the_rest_alone(pkg, device, length):
+    """A sequence longer than its table has pages for: rows that have a place go there, no other row changes."""
+    batch = pu.Batch(pkg, device, [(20, 48)], page=16, dtype=BF16, seed=6, **SMALL)
+    rows = torch.randn((20, 2, 128), device=device).to(BF16)
+    cache = batch.cache._replace(table=batch.cache.table[:, :3].contiguous(),
+                                 lengths=torch.tensor([length], dtype=torch.int32, device=device))
+    want = {name: getattr(cache, name).clone() for name in ("keys", "values")}
+    for i in range(20):
+        row = length - 20 + i
+        if row < 48:
+            for pool in want.values():
+                pool[cache.table[0, row // 16].item(), :, row % 16] = rows[i]
+    pkg.ops.paged_append(cache, rows, rows, batch.s)
+    for name, pool in want.items():
+        assert torch.equal(getattr(cache, name).view(torch.int16), pool.view(torch.int16)), name
+
+
 # ------------------------------------------------------------------ refusals, streams, graphs, runs
 def test_python_refusals(pkg, device):
     ops = pkg.ops
