@@ -373,7 +373,7 @@ int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, co
  * tokens, before the sequence's own, and are read once for the whole batch.  Same kv_heads, head_dim and dtype; pages of
  * its own kind, of the same pool or another.
  * out [tokens][heads][head_dim], the query's dtype.  Constraints: heads <= 1024, heads % kv_heads == 0, tokens * heads <=
- * 2^22, sequences <= 2^20, scale > 0 and finite.  The workspace depends on the sizes alone, not on the lengths.
+ * 2^22, sequences <= 2^20, 0 < scale <= 2e38.  The workspace depends on the sizes alone, not on the lengths.
  */
 size_t dflash_paged_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                               int64_t sequences, int has_prefix);

@@ -1242,8 +1242,8 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
       if (prefix->sequences != 1 || prefix->kv_heads != kv || prefix->head_dim != D || prefix->dtype != cache->dtype)
         return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: the prefix is one sequence with the cache's kv_heads, head_dim and dtype");
     }
-    if (!(scale > 0.0f) || scale > 3.0e38f)
-      return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: scale must be positive and finite");
+    if (!(scale > 0.0f) || scale > 2.0e38f)  // times log2(e) it has to stay finite
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: scale must be positive, at most 2e38");
     if (T == 0 || B == 0) return DFLASH_OK;
     if (int r = check_rows(query, "paged attention query")) return r;
     if (!starts || !out || !aligned16(out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged attention: NULL starts, or NULL or misaligned out");

@@ -84,7 +84,7 @@ def test_attention_refusals(pkg):
             (dict(heads=3), "multiple of kv_heads"), (dict(heads=0), "multiple of kv_heads"), (dict(heads=2048), "at most 1024"),
             (dict(tokens=-1), "at most"), (dict(tokens=1 << 21), "2\\^22"), (dict(tokens=1 << 62), "2\\^22"),
             (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
-            (dict(scale=float("inf")), "scale"), (dict(query=_rows(lib, 0)), "query"), (dict(starts=None), "starts"),
+            (dict(scale=float("inf")), "scale"), (dict(scale=2.5e38), "scale"), (dict(query=_rows(lib, 0)), "query"), (dict(starts=None), "starts"),
             (dict(out=None), "out"), (dict(out=ADDRESS + 8), "out"), (dict(ws=None), "workspace"),
             (dict(ws=ADDRESS + 8), "workspace"), (dict(size=need - 1), "workspace"),
             (dict(prefix=_cache(lib)), "one sequence"), (dict(prefix=_cache(lib, sequences=1, kv_heads=4)), "kv_heads"),
