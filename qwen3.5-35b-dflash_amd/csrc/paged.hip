@@ -475,8 +475,8 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // operand needs eight keys of a dim: two transposing LDS reads of four keys each.
 // Bound: matrix instructions and LDS reads, which take about as long (a wave reads every key and value for its 32 rows; 64 rows a
 // wave would halve the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of
-// 256: 243 us, 990 TFLOP/s (a large library product 1305); prompts of 442 to 2222 tokens, 32 heads of 128: 132 us,
-// 656, of which a workgroup's start and end take a quarter at 13 steps on average.  Started cold, a launch spends about 14 us
+// 256: 242 us, 995 TFLOP/s (a large library product 1305); prompts of 442 to 2222 tokens, 32 heads of 128: 131 us,
+// 658, of which a workgroup's start and end take a quarter at 13 steps on average.  Started cold, a launch spends about 14 us
 // before and behind its steps, most of it fetching code that runs once.
 // The rows' running maximum is a reference that moves only when a score exceeds it by 8 (weights reach 2^8, their relative precision
 // is the same): the accumulators are rescaled a few times a row instead of at every step.
@@ -714,7 +714,9 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
   }
   const auto step = [&](auto stage_, auto inner_, int i) {
     constexpr int stage = decltype(stage_)::value;
-    constexpr bool inner = decltype(inner_)::value;  // whole tiles follow: the loads stand between the matrix instructions too
+    // Whole steps follow: the loads stand between the matrix instructions too.  And no row masks any of this step's keys or the next's:
+    // a tile has 128 tokens at most, so that all rows see all but the last 127 keys, and five steps follow.
+    constexpr bool inner = decltype(inner_)::value;
     char* const other = stage ? keys0 : keys1;      // the next step's keys
     char* const held = stage ? values1 : values0;   // this step's values
     const int key0 = k0 + 64 * i;
@@ -763,7 +765,7 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
                              if (k % 4 == 1) piece(of_values, ahead, b, k / 4);
                            }
                          });
-    hide(next, key0 + 64);
+    if constexpr (!inner) hide(next, key0 + 64);
     l += sum[0] + sum[1];
     mc = -__builtin_inff();
     arrive(inner || i + 2 < steps);
@@ -773,7 +775,9 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
     } else {
       load_keys(other, i + 3);
     }
-    if (key0 + 64 > least) clean(held, key0);
+    if constexpr (!inner) {
+      if (key0 + 64 > least) clean(held, key0);
+    }
     feed<4 * NC, kAhead>(
         [&](int k) {
           const char* at = held + ((vr ^ (64 * (k % NC))) + k / NC * 32 * D);
