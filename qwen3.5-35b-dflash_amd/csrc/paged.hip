@@ -318,7 +318,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
   const int tok0 = uniform(static_cast<int>(divide(w.tile * 16, p.by_group))), tok1 = uniform(static_cast<int>(divide(w.tile * 16 + nrows - 1, p.by_group)));
   const int least = visible_keys(w.keys, w.tokens, tok0, causal);  // keys that every row of the tile sees
   const int n = visible_keys(w.keys, w.tokens, tok1, causal);      // keys that some row sees
-  const int k0 = w.chunk * w.c * kSmallUnit, k1 = min(k0 + w.c * kSmallUnit, n);
+  const int k0 = w.chunk * w.c * kSmallUnit, k1 = chunk_end(k0, w.c, kSmallUnit, n);
 
   u32x4 q[KS];
   {
@@ -527,7 +527,7 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
   const int visible = visible_keys(w.keys, w.tokens, tok, causal);
   const int least = visible_keys(w.keys, w.tokens, uniform(static_cast<int>(divide(row0, p.by_group))), causal);
   const int n = visible_keys(w.keys, w.tokens, uniform(static_cast<int>(divide(row0 + nrows - 1, p.by_group))), causal);
-  const int k0 = w.chunk * w.c * kLargeUnit, k1 = min(k0 + w.c * kLargeUnit, n);
+  const int k0 = w.chunk * w.c * kLargeUnit, k1 = chunk_end(k0, w.c, kLargeUnit, n);
   const int steps = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
 
   if (tid == 0) odd = 0;

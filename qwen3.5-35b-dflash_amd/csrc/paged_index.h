@@ -62,6 +62,11 @@ DFLASH_HD int tile_chunks(int units, int c) {
   const int k = static_cast<int>(static_cast<uint32_t>(units + c - 1) / static_cast<uint32_t>(c));
   return k < 1 ? 1 : k;
 }
+// End of the chunk of c units that starts at key k0, among n keys (c may be far more than they have).
+DFLASH_HD int chunk_end(int k0, int c, int unit, int n) {
+  const int64_t end = k0 + static_cast<int64_t>(c) * unit;
+  return end < n ? static_cast<int>(end) : n;
+}
 
 // Keys that token i of a block of `tokens` sees (causal: itself and what lies before it).
 DFLASH_HD int visible_keys(int keys, int tokens, int i, bool causal) {

@@ -25,6 +25,7 @@ int tiles(int tokens, int group, int rows) { return seq_tiles(tokens, group, row
 int units(int keys, int unit) { return seq_units(keys, unit); }
 int chunk(int64_t total, int kv, int slots, int least) { return chunk_units(total, kv, 1.0 / slots, least); }
 int chunks(int units, int c) { return tile_chunks(units, c); }
+int chunk_last(int k0, int c, int unit, int n) { return chunk_end(k0, c, unit, n); }
 int visible(int keys, int tokens, int i, int causal) { return visible_keys(keys, tokens, i, causal); }
 int64_t tile_bound(int64_t T, int64_t B, int64_t group, int64_t rows) { return max_tiles(T, B, group, rows); }
 int64_t chunk_bound(int64_t tiles, int64_t kv, int64_t slots) { return max_chunks(tiles, kv, slots); }
@@ -129,6 +130,13 @@ def test_chunks_are_long_enough_at_any_size(index):
         slots = rng.choice((1, 7, 256, 304, 512, 1024))
         c = index.chunk(total, kv, slots, 1)
         assert c > 1000000000 or total * kv <= c * slots <= total * kv + slots, (total, kv, slots, c)
+
+
+def test_a_chunk_ends_at_the_last_key_at_any_size(index):
+    for c in (1, 7, 1 << 23, 1 << 25, 1 << 26, 1_000_000_001):
+        for unit in (64, 128):
+            for k0, n in ((0, 1), (0, 1 << 30), (unit, 5), ((1 << 30) - unit, 1 << 30), (0, 0)):
+                assert index.chunk_last(k0, c, unit, n) == min(k0 + c * unit, n)
 
 
 def test_a_row_tile_too_few_is_seen(index):
