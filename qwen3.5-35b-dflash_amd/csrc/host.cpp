@@ -129,7 +129,8 @@ bool workspace_of(PyObject* o, size_t need, at::Device device, at::Tensor* ws) {
     return true;
   }
   const at::Tensor* t = tensor(o);
-  if (!t || t->scalar_type() != at::kByte || t->device() != device || static_cast<size_t>(t->numel()) < need) return false;
+  if (!t || t->scalar_type() != at::kByte || t->device() != device || static_cast<size_t>(t->numel()) < need || !t->is_contiguous())
+    return false;
   *ws = *t;
   return true;
 }

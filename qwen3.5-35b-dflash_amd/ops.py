@@ -63,8 +63,10 @@ def _desc(w: PackedW4) -> _lib.W4Desc:
 
 def _workspace(nbytes: int, device: torch.device, workspace: Optional[torch.Tensor]) -> torch.Tensor:
     if workspace is not None:
-        if workspace.dtype != torch.uint8 or workspace.numel() < nbytes or workspace.device != device:
-            raise ValueError(f"workspace must be a uint8 tensor of at least {nbytes} bytes on {device}")
+        # its bytes are written one after the other: an expanded or strided tensor counts more than it has there
+        if (workspace.dtype != torch.uint8 or workspace.numel() < nbytes or workspace.device != device
+                or not workspace.is_contiguous()):
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
         return workspace
     return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
 
