@@ -393,8 +393,8 @@ struct PagedParams {
   const uint16_t* query;
   int64_t query_token, query_head;
   uint16_t* out;                  // [T][heads][head_dim]
-  // partial results: rows of unnormalised sums, their maximum and sum, and per (token, head) the first row and how many
-  // (partial tiles of own_tile_rows rows, own_tile_rows * kv rows apart); and the prefix's
+  // partial results: rows of unnormalised sums, their reference (in units of log2) and sum of weights, and per (token, head) the
+  // first row and how many (partial tiles of own_tile_rows rows, own_tile_rows * kv rows apart); and the prefix's
   float* part;
   float2* ml;
   int2* info;

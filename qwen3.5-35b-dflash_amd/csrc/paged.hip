@@ -12,6 +12,15 @@
 // A probability is rounded to 16 bits for the product with V, as V itself is held; the sum l takes it unrounded.  Each is off by
 // at most half a step, and its error is weighed as the value it multiplies: that leaves the sum about as far off as the output's own
 // rounding does.
+//
+// The reference.  A probability is held as 2^(s_j log2 e - r + bias) with a reference r of its row, in units of log2; partial results
+// keep the r that their l and o belong to, and merge by it whatever it is.  In bf16, which has the range of fp32, r is a maximum and bias 0.
+// fp16 has its precision from 2^-14 to 2^16 only.  There the bias puts the largest weight at 2^15 at most, and r follows the keys
+// down as well as up: where all of a step's keys weigh less than 2^-kFall of it, as those behind one key that takes nearly all of the
+// softmax do, r falls to their maximum, and l and o, which have the range of fp32, are scaled up to it (r at most kReach below the row's
+// largest score: with weights of 2^15, values of 2^16 and 2^30 keys the sums stay under 2^105).  So a weight keeps its
+// precision unless it is less than 2^-17 of another of the same 32 or 64 keys, where it is off by 2^-28 of that one at most, or 2^-65 of
+// the row's largest.
 #include <algorithm>
 #include <type_traits>
 
@@ -27,6 +36,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 struct Bf16 {
   typedef __bf16 Pair __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kExponent = 0x7F80;  // all ones: an infinity or NaN
+  static constexpr bool kNarrow = false;         // the reference of weights never falls
+  static constexpr int kRise = 8;                // 128-row kernel: how far scores may exceed the reference
+  static constexpr int kSmallBias = 0, kLargeBias = 0;
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -39,6 +51,9 @@ struct Bf16 {
 struct Fp16 {
   typedef _Float16 Pair __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kExponent = 0x7C00;
+  static constexpr bool kNarrow = true;
+  static constexpr int kRise = 4;
+  static constexpr int kSmallBias = 15, kLargeBias = 15 - kRise;
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -53,6 +68,12 @@ template <class E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), typename E::Pair));
 }
+
+constexpr float kFall = 8.f, kReach = 40.f;
+// 2^-bias, which takes the bias out of the sums that partial results keep.
+constexpr float unbiased(int bias) { return bias ? 0.5f * unbiased(bias - 1) : 1.f; }
+// The number that is subtracted: a row that has seen no key keeps weights of 0 (the exponent is -inf).
+__device__ __forceinline__ float reference(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
@@ -331,7 +352,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
   f32x4 o[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), l = 0.f, peak = -__builtin_inff();  // the row's reference, sum of weights and largest score
 
   for (int j0 = k0 + 32 * wave; j0 < k1; j0 += kSmallUnit) {
     u32x4 kf[2][KS], vf[8][VL];
@@ -362,15 +383,20 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     float mc = fmaxf(fmaxf(fmaxf(s8[0], s8[1]), fmaxf(s8[2], s8[3])), fmaxf(fmaxf(s8[4], s8[5]), fmaxf(s8[6], s8[7])));
     mc = fmaxf(mc, __shfl_xor(mc, 16, 64));
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
-    const float mn = fmaxf(m, mc);
-    // a row that has seen no key keeps weights of 0 (the exponent is -inf); a NaN score, which the maximum skips, makes l and
-    // o NaN, and so they stay
-    const float ref = mn == -__builtin_inff() ? 0.f : mn * p.scale_log2;
-    const float corr = __builtin_amdgcn_exp2f(__builtin_fmaf(m, p.scale_log2, -ref));
+    const float top = mc * p.scale_log2;
+    float mn = fmaxf(m, top);
+    if constexpr (E::kNarrow) {
+      peak = fmaxf(peak, top);
+      const bool fall = (m - top > kFall) & (top > -__builtin_inff());
+      mn = fall ? fmaxf(top, peak - kReach) : mn;
+    }
+    // a NaN score, which the maximum skips, makes l and o NaN, and so they stay
+    const float ref = reference(mn);
+    const float corr = __builtin_amdgcn_exp2f(m - ref);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s8[i], p.scale_log2, -ref));
+      s8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s8[i], p.scale_log2, E::kSmallBias - ref));
       sum += s8[i];
     }
     sum += __shfl_xor(sum, 16, 64);
@@ -419,16 +445,14 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
       }
     }
   }
-  // merge the four waves: each scales its sums to the workgroup's maximum (a wave without keys has sums of 0, not only a
+  // merge the four waves: each scales its sums to the workgroup's largest reference (a wave without keys has sums of 0, not only a
   // maximum of -inf: with scores that are all NaN its sums are NaN and stay in)
   if (kq == 0) {
     mx[wave][lr] = m;
     ls[wave][lr] = l;
   }
   __syncthreads();
-  const auto factor = [&](float mw, float M) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(mw, p.scale_log2, M == -__builtin_inff() ? 0.f : -M * p.scale_log2));
-  };
+  const auto factor = [&](float mw, float M) { return __builtin_amdgcn_exp2f(mw - reference(M)); };
   const float M = fmaxf(fmaxf(mx[0][lr], mx[1][lr]), fmaxf(mx[2][lr], mx[3][lr]));
   const float f = factor(m, M);
   float* const mine = reinterpret_cast<float*>(wave == 0 ? areas[0] : wave == 1 ? areas[1] : wave == 2 ? areas[2] : areas[3]) + lr * kPitch;
@@ -453,6 +477,8 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     const int rr = w.tile * 16 + row, tk = divide(rr, p.by_group), hd = kvh * p.group + rr - tk * p.group;
     const int64_t out = static_cast<int64_t>(w.start + tk) * p.heads + hd;
     if (w.partial >= 0) {
+      v *= unbiased(E::kSmallBias);
+      sum *= unbiased(E::kSmallBias);
       *reinterpret_cast<f32x4*>((on_front ? p.prefix_part : p.part) + (held + row) * D + c) = v;
       if (c == 0) {
         (on_front ? p.prefix_ml : p.ml)[held + row] = make_float2(Mr, sum);
@@ -478,8 +504,8 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // 256: 242 us, 995 TFLOP/s (a large library product 1305); prompts of 442 to 2222 tokens, 32 heads of 128: 131 us,
 // 658, of which a workgroup's start and end take a quarter at 13 steps on average.  Started cold, a launch spends about 14 us
 // before and behind its steps, most of it fetching code that runs once.
-// The rows' running maximum is a reference that moves only when a score exceeds it by 8 (weights reach 2^8, their relative precision
-// is the same): the accumulators are rescaled a few times a row instead of at every step.
+// The rows' reference moves only when a score exceeds it by kRise (weights reach 2^kRise, their relative precision is the same): the
+// accumulators are rescaled a few times a row instead of at every step.
 // A run of n matrix instructions that take one operand each from LDS: use(i, read(i)) for all i, each read kAhead instructions ahead of
 // its use.  Left to itself the compiler puts each read right before its use and waits for it (a read takes four times as long as
 // the instruction), so the order is fixed.
@@ -620,6 +646,7 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
+  float peak = -__builtin_inff();        // the row's largest score so far, where the reference may fall
 
   // Step i multiplies the next step's keys with the queries, then its own weights with its values: the exponentials of its scores
   // stand between the matrix instructions of the one, the maximum of the next scores between those of the other.  Each half ends
@@ -724,12 +751,18 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
     f32x16(&next)[2] = sc[stage ^ 1];
     asm volatile("" : "+v"(kr), "+v"(vr));  // no two dozen registers of places kept over the steps
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
-    // a row that has seen no key keeps weights of 0 (the exponent is -inf); a NaN score, which the maximum skips, makes l and
-    // o NaN, and so they stay
-    const bool move = (mc - m) * p.scale_log2 > 8.f || (m == -__builtin_inff() && mc > m);
+    // a NaN score, which the maximum skips, makes l and o NaN, and so they stay
+    const float top = mc * p.scale_log2;
+    bool move = top - m > E::kRise;  // the first key's too, from -inf; not where both are
+    float to = top;
+    if constexpr (E::kNarrow) {
+      peak = fmaxf(peak, top);
+      move |= (m - top > kFall) & (top > -__builtin_inff()) & (m > peak - kReach);
+      to = fmaxf(top, peak - kReach);
+    }
     if (__any(move)) {
-      const float to = move ? mc : m;
-      const float corr = __builtin_amdgcn_exp2f(__builtin_fmaf(m, p.scale_log2, to == -__builtin_inff() ? 0.f : -to * p.scale_log2));
+      if (!move) to = m;
+      const float corr = __builtin_amdgcn_exp2f(m - reference(to));
       l *= move ? corr : 1.f;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -737,7 +770,7 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
         for (int e = 0; e < 16; ++e) o[c][e] *= move ? corr : 1.f;
       m = to;
     }
-    const float ref = m == -__builtin_inff() ? 0.f : m * p.scale_log2;
+    const float ref = reference(m) - E::kLargeBias;
     u32x4 pf[4];
     float sum[2] = {0.f, 0.f};
     const auto weigh = [&](int e) {  // elements e and e + 1 of the step's 32
@@ -838,13 +871,14 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
   const int64_t out = static_cast<int64_t>(w.start + at_token) * p.heads + at_head;
   if (w.partial >= 0) {
     const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * kLargeRows + mine;
+    constexpr float by = unbiased(E::kLargeBias);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>((kPrefix ? p.prefix_part : p.part) + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
+        *reinterpret_cast<f32x4*>((kPrefix ? p.prefix_part : p.part) + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e] * by, o[c][e + 1] * by, o[c][e + 2] * by, o[c][e + 3] * by};
     if (part == 0) {
-      (kPrefix ? p.prefix_ml : p.ml)[held] = make_float2(m, l);
+      (kPrefix ? p.prefix_ml : p.ml)[held] = make_float2(m, l * by);
       if (w.chunk == 0) (kPrefix ? p.prefix_info : p.info)[out] = make_int2(static_cast<int>(held), w.chunks);
     }
   } else {
@@ -984,8 +1018,8 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_k
         float top = M;
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) top = fmaxf(top, v[i].x);
-        const float ref = top == -__builtin_inff() ? 0.f : top * p.scale_log2;
-        const float corr = __builtin_amdgcn_exp2f(__builtin_fmaf(M, p.scale_log2, -ref));
+        const float ref = reference(top);
+        const float corr = __builtin_amdgcn_exp2f(M - ref);
         M = top;
         l *= corr;
 #pragma unroll
@@ -993,7 +1027,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_k
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
           if (v[i].y == 0.f) continue;  // no key of this row in that chunk, whose row may hold anything
-          const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(v[i].x, p.scale_log2, -ref));
+          const float f = __builtin_amdgcn_exp2f(v[i].x - ref);
           l += v[i].y * f;
 #pragma unroll
           for (int k = 0; k < F; ++k) acc[k] += x[i][k] * f;
@@ -1011,13 +1045,13 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_k
       if (wave) return;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mm[w]);
-      const float ref = M == -__builtin_inff() ? 0.f : M * p.scale_log2;
+      const float ref = reference(M);
       l = 0.f;
 #pragma unroll
       for (int k = 0; k < F; ++k) acc[k] = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(mm[w], p.scale_log2, -ref));
+        const float f = __builtin_amdgcn_exp2f(mm[w] - ref);
         l += lm[w] * f;
 #pragma unroll
         for (int k = 0; k < F; ++k) acc[k] += om[w][lane * F + k] * f;
