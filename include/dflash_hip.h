@@ -366,8 +366,8 @@ int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, co
  * Attention of a batch of blocks over a paged cache (the math of FusedOps.attention,
  * model/qwen35_moe_dflash/fused/ops.py:25-123, per sequence): out[token][head] = sum_j softmax_j(scale q.k_j) v_j.
  * Tokens [starts[b], starts[b + 1]) are the last of sequence b's lengths[b] rows; causal: token i of them sees the rows up to
- * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums, weights
- * rounded to 16 bits for their product with V.  A row that sees no key gives zeros; rows of tokens in no sequence are not
+ * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums; weights
+ * as the sum of two 16-bit parts (2^-16 of a weight at most is left out in bf16, 2^-22 in fp16).  A row that sees no key gives zeros; rows of tokens in no sequence are not
  * written.  Masked keys and values count for nothing, NaN and infinities among them.
  * prefix (NULL: none): a cache of one sequence that every sequence of the batch continues.  Its rows are visible to all
  * tokens, before the sequence's own, and are read once for the whole batch.  Same kv_heads, head_dim and dtype; pages of

@@ -9,18 +9,18 @@
 // s_j = scale q.k_j in fp32 from exact products of 16-bit values; a row that sees no key gives zeros.  Partial results
 // over disjoint keys merge as m = max m_i, l = sum l_i e^{m_i - m}, o = sum o_i e^{m_i - m}: chunks of a long sequence, and a
 // prefix that all sequences share, whose keys are taken once for the stacked rows of the whole batch.
-// A probability is rounded to 16 bits for the product with V, as V itself is held; the sum l takes it unrounded.  Each is off by
-// at most half a step, and its error is weighed as the value it multiplies: that leaves the sum about as far off as the output's own
-// rounding does.
+// A probability takes part in the product with V as two 16-bit parts, its rounding and the rounding of what that leaves: off by 2^-16 of
+// itself in bf16, 2^-22 in fp16, so that what an output is off by is its own rounding (1.66e-3 of the norm in bf16, 2.0e-4 in fp16, for
+// values from N(0, 1)).  With one part it would be 2.0e-3 to 2.3e-3 and 2.6e-4; the second costs matrix instructions, a third of those of
+// the 128-row kernel: 322 instead of 237 us for its largest case below, 124 instead of 121 for decode of 64 sequences.
 //
 // The reference.  A probability is held as 2^(s_j log2 e - r + bias) with a reference r of its row, in units of log2; partial results
 // keep the r that their l and o belong to, and merge by it whatever it is.  In bf16, which has the range of fp32, r is a maximum and bias 0.
 // fp16 has its precision from 2^-14 to 2^16 only.  There the bias puts the largest weight at 2^15 at most, and r follows the keys
 // down as well as up: where all of a step's keys weigh less than 2^-kFall of it, as those behind one key that takes nearly all of the
 // softmax do, r falls to their maximum, and l and o, which have the range of fp32, are scaled up to it (r at most kReach below the row's
-// largest score: with weights of 2^15, values of 2^16 and 2^30 keys the sums stay under 2^105).  So a weight keeps its
-// precision unless it is less than 2^-17 of another of the same 32 or 64 keys, where it is off by 2^-28 of that one at most, or 2^-65 of
-// the row's largest.
+// largest score: with weights of 2^15, values of 2^16 and 2^30 keys the sums stay under 2^105).  So a weight is off by 2^-28 of
+// the largest of the same 32 or 64 keys at most, and has 11 bits or more from 2^-17 of that one on.
 #include <algorithm>
 #include <type_traits>
 
@@ -67,6 +67,12 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <class E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), typename E::Pair));
+}
+
+// What pack2 leaves of a and b, in 16 bits.
+template <class E>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t both) {
+  return pack2<E>(a - E::to_f32(both & 0xFFFF), b - E::to_f32(both >> 16));
 }
 
 constexpr float kFall = 8.f, kReach = 40.f;
@@ -311,15 +317,28 @@ __device__ __forceinline__ int thread_again() {
   return t;
 }
 
+// 16 bytes a lane from base + off to 1 KB of LDS at the wave's `dst`, lane by lane.  In assembly, so that the compiler does not put a
+// wait for every load into LDS before every read of it: what a read needs has arrived at the barrier before (arrive() below).  No
+// register is written but m0, which nothing else in this file uses.
+__device__ __forceinline__ void copy_to_lds(const char* base, uint32_t off, char* dst) {
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
+}
+// The same from a place of each lane's own.
+__device__ __forceinline__ void copy_to_lds(const uint16_t* from, char* dst) {
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+}
+
 // ------------------------------------------------------------------ 16 rows, four waves over the keys
 // For blocks of few rows.  Scores transposed, S^T = K Q^T: lane l holds query row l & 15 and keys 4 (l >> 4) + e of each of two
 // 16-key tiles, which, with those eight keys as the reduction's octet l >> 4, is the B operand of O^T = V^T P^T as it stands.  The A
 // operand needs eight keys of one dim per lane: a lane loads D / 16 neighbouring dims of its eight keys and pairs halves in
 // registers, so V needs no transpose and neither operand passes through LDS.
-// Bound: memory.  A wave has a round's 32 keys and values in flight, two workgroups a CU: one at head dim 256 (300 registers
-// instead of 256) takes 130 us instead of 120 for 64 sequences of up to 8192 keys, 572 MB (4.8 TB/s); streaming loads 132,
-// the rounds' places looked up eight rounds ahead 137.  One row behind 131072 keys, 268 MB: 43.5 us.  Few keys: latency,
-// 8 us for a row behind 4000.
+// Bound: memory.  A wave has a round's 32 keys and values in flight, two workgroups a CU: 64 sequences of up to 8192 keys, 572 MB, 124 us
+// (4.6 TB/s).  One workgroup a CU, with the registers of two: 10 us more; streaming loads 12, the rounds' places looked up eight rounds
+// ahead 17.  At head dim 256 the queries wait in LDS: in registers 16 of them went through memory in every round, 135 us.  One row behind
+// 131072 keys, 268 MB, both kernels: 62.7 us.  Few keys: latency.
 constexpr int kSmallRows = 16, kSmallUnit = 128;  // keys a round of the four waves
 template <int D>
 constexpr int kSmallPitch = D + 4;
@@ -341,11 +360,17 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
   const int n = visible_keys(w.keys, w.tokens, tok1, causal);      // keys that some row sees
   const int k0 = w.chunk * w.c * kSmallUnit, k1 = chunk_end(k0, w.c, kSmallUnit, n);
 
-  u32x4 q[KS];
-  {
+  // At head dim 256 the queries wait in the wave's area of LDS, which it needs for its sums at the end only.
+  constexpr bool kHeld = D == 256;
+  char* const area = wave == 0 ? areas[0] : wave == 1 ? areas[1] : wave == 2 ? areas[2] : areas[3];
+  u32x4 q[kHeld ? 1 : KS];
+  if (!kHeld || k0 + 32 * wave < k1) {  // a wave without keys leaves its area alone
     const uint16_t* qr = p.query + (w.start + tok) * p.query_token + head * p.query_head + 8 * kq;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (kHeld) copy_to_lds(qr + 32 * s, area + 1024 * s);
+      else q[s] = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+    }
   }
   const uint16_t* keys = side.keys + kvh * side.key_head;
   const uint16_t* vals = side.values + kvh * side.value_head;
@@ -371,15 +396,25 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
         for (int h = 0; h < VL; ++h) vf[4 * b + i][h] = *reinterpret_cast<const u32x4*>(vr + 8 * h);
       }
     }
+    uint32_t held_at = 16 * lane;
+    if constexpr (kHeld) {
+      if (j0 < k0 + kSmallUnit) wait_vmem();  // the wave's first round: the queries have arrived
+      asm volatile("" : "+v"(held_at)::"memory");
+    }
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      u32x4 qs;
+      if constexpr (kHeld) qs = *reinterpret_cast<const u32x4*>(area + held_at + 1024 * s);
+      else qs = q[s];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) acc[b] = E::mfma16(kf[b][s], qs, acc[b]);
+    }
     float s8[8];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) acc = E::mfma16(kf[b][s], q[s], acc);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s8[4 * b + e] = j0 + 16 * b + 4 * kq + e < visible ? acc[e] : -__builtin_inff();
-    }
+      for (int e = 0; e < 4; ++e) s8[4 * b + e] = j0 + 16 * b + 4 * kq + e < visible ? acc[b][e] : -__builtin_inff();
     float mc = fmaxf(fmaxf(fmaxf(s8[0], s8[1]), fmaxf(s8[2], s8[3])), fmaxf(fmaxf(s8[4], s8[5]), fmaxf(s8[6], s8[7])));
     mc = fmaxf(mc, __shfl_xor(mc, 16, 64));
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
@@ -403,9 +438,12 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     sum += __shfl_xor(sum, 32, 64);
     l = l * corr + sum;
     m = mn;
-    u32x4 pf;
+    u32x4 pf, pr;  // the weights' two parts
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pf[i] = pack2<E>(s8[2 * i], s8[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      pf[i] = pack2<E>(s8[2 * i], s8[2 * i + 1]);
+      pr[i] = rest2<E>(s8[2 * i], s8[2 * i + 1], pf[i]);
+    }
     const auto value = [&](int c, int i) {
       return __builtin_amdgcn_perm(vf[2 * i + 1][c >> 3][(c >> 1) & 3], vf[2 * i][c >> 3][(c >> 1) & 3],
                                    c & 1 ? 0x07060302u : 0x05040100u);
@@ -418,7 +456,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
         u32x4 a;
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = value(c, i);
-        o[c] = E::mfma16(a, pf, o[c]);
+        o[c] = E::mfma16(a, pr, E::mfma16(a, pf, o[c]));
       }
     } else {
       // Some row masks some of these keys: its weights there are 0, but 0 times an infinite or NaN value is not.  A column of the
@@ -438,7 +476,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
           u32x4 a;
 #pragma unroll
           for (int i = 0; i < 4; ++i) a[i] = value(c, i) & keep[i];
-          const f32x4 t = E::mfma16(a, pf, o[c]);
+          const f32x4 t = E::mfma16(a, pr, E::mfma16(a, pf, o[c]));
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[c][e] = mine ? t[e] : o[c][e];
         }
@@ -455,7 +493,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
   const auto factor = [&](float mw, float M) { return __builtin_amdgcn_exp2f(mw - reference(M)); };
   const float M = fmaxf(fmaxf(mx[0][lr], mx[1][lr]), fmaxf(mx[2][lr], mx[3][lr]));
   const float f = factor(m, M);
-  float* const mine = reinterpret_cast<float*>(wave == 0 ? areas[0] : wave == 1 ? areas[1] : wave == 2 ? areas[2] : areas[3]) + lr * kPitch;
+  float* const mine = reinterpret_cast<float*>(area) + lr * kPitch;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -499,11 +537,11 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // keys 8 (e / 4) + 4 (l >> 5) + e % 4 of a 32-key block (e: element of the 32x32 result), whose elements 8 s to 8 s + 7 are, as a
 // reduction's octet l >> 5, the B operand of O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's
 // operand needs eight keys of a dim: two transposing LDS reads of four keys each.
-// Bound: matrix instructions and LDS reads, which take about as long (a wave reads every key and value for its 32 rows; 64 rows a
-// wave would halve the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of
-// 256: 242 us, 995 TFLOP/s (a large library product 1305); prompts of 442 to 2222 tokens, 32 heads of 128: 131 us,
-// 658, of which a workgroup's start and end take a quarter at 13 steps on average.  Started cold, a launch spends about 14 us
-// before and behind its steps, most of it fetching code that runs once.
+// Bound: matrix instructions, behind them LDS reads (a wave reads every key and value for its 32 rows; 64 rows a wave would halve
+// the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of 256: 322 to 328 us, 733 to
+// 747 TFLOP/s of the formulas, 1.1 PFLOP/s of matrix instructions with the weights' second parts (a large library product 1.3); prompts
+// of 442 to 2222 tokens, 32 heads of 128: 160 to 163 us.  Started cold, a launch spends about 14 us before and behind its
+// steps, most of it fetching code that runs once.
 // The rows' reference moves only when a score exceeds it by kRise (weights reach 2^kRise, their relative precision is the same): the
 // accumulators are rescaled a few times a row instead of at every step.
 // A run of n matrix instructions that take one operand each from LDS: use(i, read(i)) for all i, each read kAhead instructions ahead of
@@ -527,13 +565,6 @@ __device__ __forceinline__ void feed(const Read& read, const Use& use) {
 __device__ __forceinline__ uint2 read_turned(const char* p) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
-}
-// 16 bytes a lane from base + off to 1 KB of LDS at the wave's `dst`, lane by lane.  In assembly, so that the compiler does not put a
-// wait for every load into LDS before every read of it: what a read needs has arrived at the barrier before (arrive() below).  No
-// register is written but m0, which nothing else in this file uses.
-__device__ __forceinline__ void copy_to_lds(const char* base, uint32_t off, char* dst) {
-  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
 }
 constexpr int kLargeRows = 128, kLargeUnit = 64, kLargeLeast = 4;
 template <int D>
@@ -771,16 +802,15 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
       m = to;
     }
     const float ref = reference(m) - E::kLargeBias;
-    u32x4 pf[4];
     float sum[2] = {0.f, 0.f};
     const auto weigh = [&](int e) {  // elements e and e + 1 of the step's 32
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][e & 15], p.scale_log2, -ref));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][(e & 15) + 1], p.scale_log2, -ref));
+      float x = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][e & 15], p.scale_log2, -ref));
+      float y = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][(e & 15) + 1], p.scale_log2, -ref));
+      asm volatile("" : "+v"(x), "+v"(y));  // made here, between the matrix instructions, not where they are used
       sum[0] += x;
       sum[1] += y;
-      uint32_t both = pack2<E>(x, y);
-      asm volatile("" : "+v"(both));  // made here, between the matrix instructions, not where it is used
-      pf[e >> 3][(e & 7) >> 1] = both;
+      now[e >> 4][e & 15] = x;
+      now[e >> 4][(e & 15) + 1] = y;
     };
     clear(next);
     constexpr int kPairK = KS / 8, kPairV = NC / 4;  // matrix instructions a pair of elements
@@ -811,6 +841,16 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
     if constexpr (!inner) {
       if (key0 + 64 > least) clean(held, key0);
     }
+    u32x4 pf, pr;  // the two parts of the weights of 16 keys
+    const auto split = [&](int part) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 8 * part + 2 * i;
+        const float x = now[e >> 4][e & 15], y = now[e >> 4][(e & 15) + 1];
+        pf[i] = pack2<E>(x, y);
+        pr[i] = rest2<E>(x, y, pf[i]);
+      }
+    };
     feed<4 * NC, kAhead>(
         [&](int k) {
           const char* at = held + ((vr ^ (64 * (k % NC))) + k / NC * 32 * D);
@@ -818,7 +858,9 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
           return u32x4{a.x, a.y, b.x, b.y};
         },
         [&](int k, u32x4 v) {
-          o[k % NC] = E::mfma32(v, pf[k / NC], o[k % NC]);
+          if (k % NC == 0) split(k / NC);
+          o[k % NC] = E::mfma32(v, pf, o[k % NC]);
+          o[k % NC] = E::mfma32(v, pr, o[k % NC]);
           if (k % kPairV == 0) {
             const int e = k / kPairV * 2;
             mc = fmaxf(fmaxf(mc, next[e >> 4][e & 15]), next[e >> 4][(e & 15) + 1]);
@@ -924,9 +966,9 @@ __global__ __launch_bounds__(256, kFrontLarge && D == 256 ? 1 : 2) void paged_pa
   static_assert(kArea >= kSmallArea<D>, "either fits");
   constexpr int kOwnRows = kOwnLarge ? kLargeRows : kSmallRows, kOwnUnit = kOwnLarge ? kLargeUnit : kSmallUnit;
   constexpr int kFrontRows = kFrontLarge ? kLargeRows : kSmallRows, kFrontUnit = kFrontLarge ? kLargeUnit : kSmallUnit;
-  // Time of a unit of own keys, and of a row tile's start and end, in units of the prefix: a 128-row step takes about 1.8 us and
-  // its kernel's start and end 14, a 16-row round 3 us or, when memory is the limit, 6, its start and end 8.  Measured from 1.2
-  // to 4 and 1 to 8: 64 sequences behind 8192 shared keys 37.5 to 40.8 us (38.9 here), 256 behind 32768 200 to 219 (200).
+  // Time of a unit of own keys, and of a row tile's start and end, in units of the prefix: a 128-row step takes about 2 us and its
+  // kernel's start and end 14, a 16-row round 3 us or, when memory is the limit, 6, its start and end 8.  kUnitCost from 1.5 to
+  // 4: 64 sequences behind 8192 shared keys 42.0 to 46.3 us (43.9 here), 256 behind 32768 254.7 to 258 (255).
   constexpr float kUnitCost = kOwnLarge == kFrontLarge ? 1.f : 3.f, kStartCost = kOwnLarge ? 8.f : kFrontLarge ? 4.5f : 2.f;
   __shared__ __align__(16) char s0[kArea], s1[kArea], s2[kArea], s3[kArea];
   __shared__ float mx[4][16], ls[4][16];
@@ -1068,9 +1110,9 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void paged_merge_k
 
 // Rows of a side's tiles, by the rows a sequence has on average: up to 20 take the kernel of 16 rows, whose waves share the
 // keys out; more, which would be two such tiles or several, take the one of 128, whose waves share the keys' way through LDS.  16 and
-// 128 rows, us: 64 sequences behind 4096 keys, 16 rows each 106 and 105, 24 rows 164 and 106, 32 rows 167 and 108; 8 sequences,
-// 16 rows 24 and 25, 24 rows 32 and 26, 128 rows at most 32 and 28.5; of unlike blocks, 64 of 18 rows on average 75 and 90, 8 of
-// 21 25 and 23, 64 of 31 115 and 93; 16 sequences of 24 rows behind 1000 keys 17 and 21; one row 13 and 18.
+// 128 rows, us: 64 sequences behind 4096 keys, 16 rows each 109 and 108, 24 rows 163 and 110, 32 rows 164 and 111; 8 sequences,
+// 16 rows 25 and 27, 24 rows 33 and 29, 75 rows on average 35 and 31; of unlike blocks, 64 of 18 rows on average 79 and 99, 8 of
+// 21 27 and 25, 64 of 31 121 and 102; 16 sequences of 24 rows behind 1000 keys 19 and 23; one row 14 and 20.
 int paged_tile_rows(int64_t tokens, int64_t sequences, int64_t group) {
   const int64_t blocks = std::max<int64_t>(1, std::min(tokens, sequences));
   return tokens * group > 20 * blocks ? kLargeRows : kSmallRows;

@@ -87,3 +87,34 @@ def test_sinks_that_come_and_go(pkg, device, shape, tokens):
         keys[(*at, 0)], values[at] = 8.0 + i / 4, 0.0
     batch.cache = batch.cache._replace(keys=keys.to(device), values=values.to(device))
     attend_checked(pkg, batch, None, 2 * pu.UNIT[FP16])
+
+
+def exact_to_the_rounding(got, want, limit, dtype):
+    """``want``, 64 bits, is off ``got`` by the output's rounding and ``limit`` before it; and over all elements no further than the
+    rounding alone is, but 1%: independent errors add as squares, so what comes before it is at most a seventh of the rounding."""
+    got = got.double().cpu()
+    over = (got - want).abs() - limit - pu.UNIT[dtype] * (want.abs() + limit) - pu.TINY[dtype]
+    assert float(over.max()) <= 0, float(over.max())
+    alone = (want.to(dtype).double() - want).square().sum().sqrt()
+    assert float((got - want).square().sum().sqrt()) <= 1.01 * float(alone), float((got - want).square().sum().sqrt() / alone)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [MODEL, WIDE])
+@pytest.mark.parametrize("spans,front", [([(1, 1500)] * 3, 0), ([(1, 20_000)], 0), ([(16, 900), (3, 77)], 0), ([(700, 2900), (90, 90)], 0),
+                                         ([(1, 300)] * 8, 900), ([(16, 400)] * 3, 2000), ([(130, 200)], 500)])
+def test_weights_are_as_exact_as_the_sums(pkg, device, spans, front, shape, causal, dtype):
+    """N(0, 1) rows.  A weight is held in two parts, each off by half a step: UNIT^2 of it is left out; in fp16 also up to
+    2^-25 where the second part is as small as that, which for 64 keys whose largest weighs 2^3 at least is 2^-22 of it (|v| < 8)."""
+    batch = pu.Batch(pkg, device, spans, page=64, dtype=dtype, seed=5, **shape)
+    prefix = pu.Batch(pkg, device, [(0, front)], page=64, dtype=dtype, seed=6, **shape) if front else None
+    scale = batch.dim ** -0.5
+    if prefix is None:
+        got = pkg.ops.paged_attention(batch.q, batch.cache, batch.s, scale=scale, causal=causal)
+    else:
+        got = pkg.ops.shared_prefix_attention(batch.q, prefix.cache, batch.cache, batch.s, scale=scale, causal=causal)
+    want, size, most, keys = pu.expected_wide(batch, scale, causal, device, prefix)
+    weight = (batch.dim + 6) * 2.0 ** -24 * scale * most + 2.0 ** -22 + pu.UNIT[dtype] ** 2
+    limit = (2 * weight + 2 * (keys + 16) * 2.0 ** -24) * size + (2.0 ** -22 * 8 if dtype == FP16 else 0.0)
+    exact_to_the_rounding(got, want, limit, dtype)
