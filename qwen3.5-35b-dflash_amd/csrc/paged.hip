@@ -515,8 +515,9 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     const int rr = w.tile * 16 + row, tk = divide(rr, p.by_group), hd = kvh * p.group + rr - tk * p.group;
     const int64_t out = static_cast<int64_t>(w.start + tk) * p.heads + hd;
     if (w.partial >= 0) {
-      v *= unbiased(E::kSmallBias);
-      sum *= unbiased(E::kSmallBias);
+      constexpr float by = unbiased(E::kSmallBias);
+      v *= by;
+      sum *= by;
       *reinterpret_cast<f32x4*>((on_front ? p.prefix_part : p.part) + (held + row) * D + c) = v;
       if (c == 0) {
         (on_front ? p.prefix_ml : p.ml)[held + row] = make_float2(Mr, sum);
