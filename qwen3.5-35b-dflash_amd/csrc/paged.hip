@@ -978,13 +978,8 @@ __global__ __launch_bounds__(256, kFrontLarge && D == 256 ? 1 : 2) void paged_pa
   int keys;
   SeqSpan last{0, 0, 0};
   const Work front = front_work(p, kFrontRows, kFrontUnit, &keys), own = own_work(p, kOwnRows, kOwnUnit, &last);
-  const float own_cost = static_cast<float>(own.units) * kUnitCost + static_cast<float>(own.tiles) * kStartCost;
-  const float places = static_cast<float>(p.slots), tiles = static_cast<float>(own.tiles * p.kv);
-  float for_own = places * own_cost / (own_cost + static_cast<float>(front.units) + 1.f);
-  if (for_own < tiles) for_own = tiles / rintf(tiles / for_own);  // as many row tiles to each place
-  for_own = fminf(fmaxf(for_own, 1.f), places - 1.f);
-  const float above = 1.000001f;  // more than the quotients' roundings take off
-  const int c0 = uniform(chunk_units(front.units, p.kv, above / (places - for_own), kFrontLarge ? kLargeLeast : 1));
+  const float for_own = own_places(own.units, own.tiles, front.units, p.kv, p.slots, kUnitCost, kStartCost);
+  const int c0 = uniform(front_chunk(front.units, p.kv, p.slots, for_own, kFrontLarge ? kLargeLeast : 1));
   const int chunks = uniform(tile_chunks(seq_units(keys, kFrontUnit), c0)), shares = front.tiles * chunks;
   Share w;
   if (id < shares) {
@@ -995,7 +990,7 @@ __global__ __launch_bounds__(256, kFrontLarge && D == 256 ? 1 : 2) void paged_pa
       return;
     }
   } else {
-    const int c1 = uniform(chunk_units(own.units, p.kv, above / for_own, kOwnLarge ? kLargeLeast : 1));
+    const int c1 = uniform(own_chunk(own.units, p.kv, for_own, kOwnLarge ? kLargeLeast : 1));
     if (!own_share(p, id - shares, kOwnRows, kOwnUnit, c1, last, &w)) return;
     if constexpr (kOwnLarge) large_share<D, E, false>(p, w, kvh, s0, s1, s2, s3, odd);
   }

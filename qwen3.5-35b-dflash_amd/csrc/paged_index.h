@@ -8,6 +8,7 @@
 // head, which bounds the grid without knowing a length on the host.
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 
 #if defined(__HIPCC__)
@@ -57,6 +58,23 @@ DFLASH_HD int chunk_units(double total, int kv, double per_slot, int least) {
   const int up = c < 1e9 ? static_cast<int>(c) + 1 : 1000000001;
   return up < least ? least : up;
 }
+// A prefix that all sequences share and their own keys, in one launch: of `slots` places the own keys get for_own, in [1, slots - 1]
+// whatever the work is, by what the two sides' units take (kUnitCost, kStartCost a row tile, in units of the prefix), and the
+// prefix the others.  Each side's chunks are cut for its places: c >= units * kv / places on either side, so together
+// there are at most slots / kv + tiles of both, as many as the grid has.
+DFLASH_HD float own_places(double own_units, int own_tiles, double front_units, int kv, int slots, float unit_cost, float start_cost) {
+  const float own_cost = static_cast<float>(own_units) * unit_cost + static_cast<float>(own_tiles) * start_cost;
+  const float places = static_cast<float>(slots), tiles = static_cast<float>(own_tiles * kv);
+  float for_own = places * own_cost / (own_cost + static_cast<float>(front_units) + 1.f);
+  if (for_own < tiles) for_own = tiles / rintf(tiles / for_own);  // as many row tiles to each place
+  return fminf(fmaxf(for_own, 1.f), places - 1.f);
+}
+constexpr float kAbove = 1.000001f;  // more than the quotients' roundings take off
+DFLASH_HD int front_chunk(double units, int kv, int slots, float for_own, int least) {
+  return chunk_units(units, kv, kAbove / (static_cast<float>(slots) - for_own), least);
+}
+DFLASH_HD int own_chunk(double units, int kv, float for_own, int least) { return chunk_units(units, kv, kAbove / for_own, least); }
+
 // Chunks a tile: one at least, which writes the rows of a sequence without keys.
 DFLASH_HD int tile_chunks(int units, int c) {
   const int k = static_cast<int>(static_cast<uint32_t>(units + c - 1) / static_cast<uint32_t>(c));
