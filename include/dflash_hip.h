@@ -353,9 +353,13 @@ typedef struct dflash_rows {
  *   y_i = n_i cos(a_i) - n_{i+h} sin(a_i), y_{i+h} = n_{i+h} cos(a_i) + n_i sin(a_i)  for i < h = rotary_dim / 2,
  *   a_i = position * inv_freq_i (inv_freq fp32 [h]; NULL: y = n); position: positions[token] (int32 [tokens]) or, NULL, the
  *   token's row in its sequence.
- * in fp32 with one rounding; angles are exact to fp32 at any position.  K rows are y, V rows the value as it is, and
- * query_out [tokens][heads][head_dim] the queries' y (query NULL, heads 0: none).  No two sequences may hold the
- * same page where a block's rows go.  Constraints: rotary_dim % 16 == 0, <= head_dim; tokens * (heads + 2 kv_heads) <= 2^24.
+ * in fp32 with one rounding.  K rows are y, V rows the value as it is, and query_out [tokens][heads][head_dim] the queries' y
+ * (query NULL, heads 0: none).  Where a block's rows go, no two sequences may hold the same page, nor one sequence twice,
+ * and keys and values share no memory (the same address is refused).
+ * Angles are reduced in 64 bits: exact to fp32 at any position.  dflash_attention_mixer forms them in fp32, off by up to half a
+ * step of the angle (4e-3 rad at position 100000), and keys that it left in a cache keep that: queries turned here meet them
+ * as exactly as they were turned, no more.
+ * Constraints: rotary_dim % 16 == 0, <= head_dim; tokens * (heads + 2 kv_heads) <= 2^24.
  */
 int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, const dflash_rows* value,
                         const int32_t* starts, int64_t tokens, const dflash_rows* query, int64_t heads,
@@ -366,14 +370,16 @@ int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, co
  * Attention of a batch of blocks over a paged cache (the math of FusedOps.attention,
  * model/qwen35_moe_dflash/fused/ops.py:25-123, per sequence): out[token][head] = sum_j softmax_j(scale q.k_j) v_j.
  * Tokens [starts[b], starts[b + 1]) are the last of sequence b's lengths[b] rows; causal: token i of them sees the rows up to
- * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums; weights
- * as the sum of two 16-bit parts (2^-16 of a weight at most is left out in bf16, 2^-22 in fp16).  A row that sees no key gives zeros; rows of tokens in no sequence are not
- * written.  Masked keys and values count for nothing, NaN and infinities among them.
+ * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums; a
+ * weight meets its value as the sum of two 16-bit parts (off by at most 2^-16 of itself in bf16; 2^-22 in fp16, or 2^-28 of
+ * the largest of 64 keys around).  A row that sees no key gives zeros; rows of tokens in no sequence are not written.  Masked
+ * keys and values count for nothing, NaN and infinities among them.
  * prefix (NULL: none): a cache of one sequence that every sequence of the batch continues.  Its rows are visible to all
  * tokens, before the sequence's own, and are read once for the whole batch.  Same kv_heads, head_dim and dtype; pages of
  * its own kind, of the same pool or another.
  * out [tokens][heads][head_dim], the query's dtype.  Constraints: heads <= 1024, heads % kv_heads == 0, tokens * heads <=
- * 2^22, sequences <= 2^20, 0 < scale <= 2e38.  The workspace depends on the sizes alone, not on the lengths.
+ * 2^22, sequences <= 2^20, 0 < scale <= 2e38 (scaled scores times log2 e have to stay in fp32's range).  The workspace
+ * depends on the sizes alone, not on the lengths.
  */
 size_t dflash_paged_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                               int64_t sequences, int has_prefix);

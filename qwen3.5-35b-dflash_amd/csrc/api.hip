@@ -1188,6 +1188,8 @@ int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, co
       if (int r = check_rows(query, "paged append query")) return r;
       if (!query_out || !aligned16(query_out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: query_out is NULL or misaligned");
     }
+    if (cache->keys == cache->values)
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "paged append: keys and values are the same memory, where a token has two rows to write");
     dflash::AppendParams p{};
     p.side = paged_side(cache);
     p.keys = static_cast<uint16_t*>(cache->keys);

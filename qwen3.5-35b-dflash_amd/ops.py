@@ -418,8 +418,8 @@ def paged_append(cache: PagedKV, key: torch.Tensor, value: torch.Tensor, starts:
     tokens past ``starts[B]`` are left out.  On the way ``key`` (and ``query`` ``[tokens, heads, head dim]``, whose result is
     returned) gets its RMS norm (``q_norm``, ``k_norm`` fp32 ``[head dim]``, applied as weight + 1) and the rotation of its
     first ``2 * len(inv_freq)`` features (half-split pairs) at ``positions`` (int32 ``[tokens]``; None: the row in the
-    sequence).  fp32 inside, one rounding.  ``key``, ``value`` and ``query`` may be views of one projection's rows.  No two
-    sequences may hold the same page where rows of the block go.  A table entry that is no page leaves its rows out.
+    sequence).  fp32 inside, one rounding.  ``key``, ``value`` and ``query`` may be views of one projection's rows.  Where rows
+    of the block go, no two sequences may hold the same page, nor one twice, and keys and values share no memory.  A table entry that is no page leaves its rows out.
     """
     if _plain(key) and (host := _lib.host()):
         done = host.paged_append(cache, key, value, starts, query, inv_freq, positions, q_norm, k_norm, eps)
