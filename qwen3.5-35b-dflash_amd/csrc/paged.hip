@@ -108,7 +108,7 @@ __device__ __forceinline__ PageAt page_at(const PagedSide& s, const int32_t* tab
 // made once for all its heads: 64-bit products and reduction by 2 pi (positions reach 2^31, where a 32-bit angle is off by
 // more than a turn), then fp32 functions of the remainder.
 // Bound: memory, behind it the angles' latency, which the first heads' loads cover: 15005 tokens of 48 rows at head dim 128, 218 MB,
-// 52.5 us (4.15 TB/s; a large copy 4.64); few tokens: the launch and the chain starts - table - store, 5.1 us for one.
+// 52.5 us (4.15 TB/s; a copy of 1 GB 5.16); few tokens: the launch and the chain starts - table - store, 5.1 us for one.
 template <int D, class E>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int L = D / 8, kHeads = 256 / L;
@@ -539,9 +539,9 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // reduction's octet l >> 5, the B operand of O^T = V^T P^T for keys 16 s of the block.  So a probability never leaves its lane.  V^T's
 // operand needs eight keys of a dim: two transposing LDS reads of four keys each.
 // Bound: matrix instructions, behind them LDS reads (a wave reads every key and value for its 32 rows; 64 rows a wave would halve
-// the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of 256: 322 to 328 us, 733 to
-// 747 TFLOP/s of the formulas, 1.1 PFLOP/s of matrix instructions with the weights' second parts (a large library product 1.3); prompts
-// of 442 to 2222 tokens, 32 heads of 128: 160 to 163 us.  Started cold, a launch spends about 14 us before and behind its
+// the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of 256: 313 to 328 us, 733 to
+// 767 TFLOP/s of the formulas, 1.1 PFLOP/s of matrix instructions with the weights' second parts (a large library product 1.3); prompts
+// of 442 to 2222 tokens, 32 heads of 128: 157 to 163 us.  Started cold, a launch spends about 14 us before and behind its
 // steps, most of it fetching code that runs once.
 // The rows' reference moves only when a score exceeds it by kRise (weights reach 2^kRise, their relative precision is the same): the
 // accumulators are rescaled a few times a row instead of at every step.
