@@ -14,13 +14,16 @@
 // values from N(0, 1)).  With one part it would be 2.0e-3 to 2.3e-3 and 2.6e-4; the second costs matrix instructions, a third of those of
 // the 128-row kernel: 322 instead of 237 us for its largest case below, 124 instead of 121 for decode of 64 sequences.
 //
-// The reference.  A probability is held as 2^(s_j log2 e - r + bias) with a reference r of its row, in units of log2; partial results
-// keep the r that their l and o belong to, and merge by it whatever it is.  In bf16, which has the range of fp32, r is a maximum and bias 0.
-// fp16 has its precision from 2^-14 to 2^16 only.  There the bias puts the largest weight at 2^15 at most, and r follows the keys
-// down as well as up: where all of a step's keys weigh less than 2^-kFall of it, as those behind one key that takes nearly all of the
-// softmax do, r falls to their maximum, and l and o, which have the range of fp32, are scaled up to it (r at most kReach below the row's
-// largest score: with weights of 2^15, values of 2^16 and 2^30 keys the sums stay under 2^105).  So a weight is off by 2^-28 of
-// the largest of the same 32 or 64 keys at most, and has 11 bits or more from 2^-17 of that one on.
+// The reference.  A probability is held as 2^(t_j - r), t_j = s_j log2 e in fp32, with a reference r of its row; partial results keep the
+// r that their l and o belong to, and merge by it whatever it is.  Both roundings of t_j - r are those of one product and one difference,
+// so that the largest score keeps the largest weight at any magnitude: with an fma the rounding of the row's maximum, which is more
+// than a binade from 2^24 on, would be part of every weight.  In bf16, which has the range of fp32, r is a maximum.
+// fp16 has its precision from 2^-14 to 2^16 only.  There r is lower, so that the largest weight is 2^kSmallBias or 2^kLargeBias and at
+// most 2^15.9, and it follows the keys down as well as up: where all of a step's keys weigh less than 2^-kFall of the reference's, as
+// those behind one key that takes nearly all of the softmax do, r falls to what their maximum asks for, and l and o, which have
+// the range of fp32, are scaled up to it (at most kReach below the highest so far: with weights of 2^16, values of 2^16 and 2^30 keys
+// the sums stay under 2^102).  So a weight is off by 2^-28 of the largest of the same 32 or 64 keys at most, and has 11 bits
+// or more from 2^-17 of that one on.
 #include <algorithm>
 #include <type_traits>
 
@@ -76,8 +79,18 @@ __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t both) {
 }
 
 constexpr float kFall = 8.f, kReach = 40.f;
-// 2^-bias, which takes the bias out of the sums that partial results keep.
-constexpr float unbiased(int bias) { return bias ? 0.5f * unbiased(bias - 1) : 1.f; }
+// A score in units of log2: a product of its own, never fused with the difference that follows.
+__device__ __forceinline__ float scaled(float score, float scale_log2) {
+#pragma clang fp contract(off)
+  return score * scale_log2;
+}
+// The reference whose largest weight is about 2^bias: t - bias, or t where that would round to less than t - (bias + 0.9).
+template <int bias>
+__device__ __forceinline__ float reference_of(float t) {
+  if constexpr (bias == 0) return t;
+  const float r = t - bias;
+  return t - r < bias + 0.9f ? r : t;
+}
 // The number that is subtracted: a row that has seen no key keeps weights of 0 (the exponent is -inf).
 __device__ __forceinline__ float reference(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
@@ -377,7 +390,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
   f32x4 o[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -__builtin_inff(), l = 0.f, peak = -__builtin_inff();  // the row's reference, sum of weights and largest score
+  float m = -__builtin_inff(), l = 0.f, peak = -__builtin_inff();  // the row's reference, sum of weights, highest reference
 
   for (int j0 = k0 + 32 * wave; j0 < k1; j0 += kSmallUnit) {
     u32x4 kf[2][KS], vf[8][VL];
@@ -418,12 +431,12 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     float mc = fmaxf(fmaxf(fmaxf(s8[0], s8[1]), fmaxf(s8[2], s8[3])), fmaxf(fmaxf(s8[4], s8[5]), fmaxf(s8[6], s8[7])));
     mc = fmaxf(mc, __shfl_xor(mc, 16, 64));
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
-    const float top = mc * p.scale_log2;
-    float mn = fmaxf(m, top);
+    const float want = reference_of<E::kSmallBias>(scaled(mc, p.scale_log2));
+    float mn = fmaxf(m, want);
     if constexpr (E::kNarrow) {
-      peak = fmaxf(peak, top);
-      const bool fall = (m - top > kFall) & (top > -__builtin_inff());
-      mn = fall ? fmaxf(top, peak - kReach) : mn;
+      peak = fmaxf(peak, want);
+      const bool fall = (m - want > kFall) & (want > -__builtin_inff());
+      mn = fall ? fmaxf(want, peak - kReach) : mn;
     }
     // a NaN score, which the maximum skips, makes l and o NaN, and so they stay
     const float ref = reference(mn);
@@ -431,7 +444,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s8[i], p.scale_log2, E::kSmallBias - ref));
+      s8[i] = __builtin_amdgcn_exp2f(scaled(s8[i], p.scale_log2) - ref);
       sum += s8[i];
     }
     sum += __shfl_xor(sum, 16, 64);
@@ -515,9 +528,6 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
     const int rr = w.tile * 16 + row, tk = divide(rr, p.by_group), hd = kvh * p.group + rr - tk * p.group;
     const int64_t out = static_cast<int64_t>(w.start + tk) * p.heads + hd;
     if (w.partial >= 0) {
-      constexpr float by = unbiased(E::kSmallBias);
-      v *= by;
-      sum *= by;
       *reinterpret_cast<f32x4*>((on_front ? p.prefix_part : p.part) + (held + row) * D + c) = v;
       if (c == 0) {
         (on_front ? p.prefix_ml : p.ml)[held + row] = make_float2(Mr, sum);
@@ -678,7 +688,7 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[c][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;  // reference of the row's weights, and the sum of this lane's weights
-  float peak = -__builtin_inff();        // the row's largest score so far, where the reference may fall
+  float peak = -__builtin_inff();        // the highest reference that its scores asked for, where it may fall
 
   // Step i multiplies the next step's keys with the queries, then its own weights with its values: the exponentials of its scores
   // stand between the matrix instructions of the one, the maximum of the next scores between those of the other.  Each half ends
@@ -784,13 +794,13 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
     asm volatile("" : "+v"(kr), "+v"(vr));  // no two dozen registers of places kept over the steps
     mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
     // a NaN score, which the maximum skips, makes l and o NaN, and so they stay
-    const float top = mc * p.scale_log2;
-    bool move = top - m > E::kRise;  // the first key's too, from -inf; not where both are
-    float to = top;
+    const float top = scaled(mc, p.scale_log2);
+    float to = reference_of<E::kLargeBias>(top);
+    bool move = top - m > E::kRise + E::kLargeBias;  // the first key's too, from -inf; not where both are
     if constexpr (E::kNarrow) {
-      peak = fmaxf(peak, top);
-      move |= (m - top > kFall) & (top > -__builtin_inff()) & (m > peak - kReach);
-      to = fmaxf(top, peak - kReach);
+      peak = fmaxf(peak, to);
+      move |= (m - to > kFall) & (to > -__builtin_inff()) & (m > peak - kReach);
+      to = fmaxf(to, peak - kReach);
     }
     if (__any(move)) {
       if (!move) to = m;
@@ -802,11 +812,11 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
         for (int e = 0; e < 16; ++e) o[c][e] *= move ? corr : 1.f;
       m = to;
     }
-    const float ref = reference(m) - E::kLargeBias;
+    const float ref = reference(m);
     float sum[2] = {0.f, 0.f};
     const auto weigh = [&](int e) {  // elements e and e + 1 of the step's 32
-      float x = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][e & 15], p.scale_log2, -ref));
-      float y = __builtin_amdgcn_exp2f(__builtin_fmaf(now[e >> 4][(e & 15) + 1], p.scale_log2, -ref));
+      float x = __builtin_amdgcn_exp2f(scaled(now[e >> 4][e & 15], p.scale_log2) - ref);
+      float y = __builtin_amdgcn_exp2f(scaled(now[e >> 4][(e & 15) + 1], p.scale_log2) - ref);
       asm volatile("" : "+v"(x), "+v"(y));  // made here, between the matrix instructions, not where they are used
       sum[0] += x;
       sum[1] += y;
@@ -914,14 +924,13 @@ __device__ __forceinline__ void large_share(const PagedParams& p, const Share& w
   const int64_t out = static_cast<int64_t>(w.start + at_token) * p.heads + at_head;
   if (w.partial >= 0) {
     const int64_t held = (static_cast<int64_t>(w.partial + w.chunk) * p.kv + kvh) * kLargeRows + mine;
-    constexpr float by = unbiased(E::kLargeBias);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>((kPrefix ? p.prefix_part : p.part) + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e] * by, o[c][e + 1] * by, o[c][e + 2] * by, o[c][e + 3] * by};
+        *reinterpret_cast<f32x4*>((kPrefix ? p.prefix_part : p.part) + held * D + 32 * c + 2 * e + 4 * part) = f32x4{o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
     if (part == 0) {
-      (kPrefix ? p.prefix_ml : p.ml)[held] = make_float2(m, l * by);
+      (kPrefix ? p.prefix_ml : p.ml)[held] = make_float2(m, l);
       if (w.chunk == 0) (kPrefix ? p.prefix_info : p.info)[out] = make_int2(static_cast<int>(held), w.chunks);
     }
   } else {

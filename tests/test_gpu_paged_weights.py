@@ -118,3 +118,31 @@ def test_weights_are_as_exact_as_the_sums(pkg, device, spans, front, shape, caus
     weight = (batch.dim + 6) * 2.0 ** -24 * scale * most + 2.0 ** -22 + pu.UNIT[dtype] ** 2
     limit = (2 * weight + 2 * (keys + 16) * 2.0 ** -24) * size + (2.0 ** -22 * 8 if dtype == FP16 else 0.0)
     exact_to_the_rounding(got, want, limit, dtype)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("scale", [2.0 ** 10, 2.0 ** 12, 2.0 ** 40])
+@pytest.mark.parametrize("spans,shape,front", [([(1, 5000), (1, 333)], SMALL, 0), ([(1, 700)] * 20, MODEL, 0), ([(33, 3001)], SMALL, 0),
+                                               ([(40, 900)] * 3, MODEL, 0), ([(1, 400)] * 8, WIDE, 900), ([(16, 300)] * 3, MODEL, 700)])
+def test_scores_of_many_millions_choose_their_largest_keys(pkg, device, spans, shape, front, scale, dtype):
+    """Scores past 2^25, where a step of fp32 is more than a binade of the weights: keys differ by more than 1000 or not at all, so a
+    row is the mean of the values at its largest score, whichever way the reference was rounded."""
+    gen = torch.Generator().manual_seed(8)
+
+    def steep(batch):
+        keys = batch.host["keys"]
+        keys[..., 0] = torch.where(torch.isnan(keys[..., 0]), keys[..., 0], (32.0 * torch.randint(-2000, 2000, keys.shape[:3], generator=gen)).to(dtype))
+        batch.cache = batch.cache._replace(keys=keys.to(device))
+        return batch
+
+    batch = steep(sink_batch(pkg, device, spans, None, 0.0, 1.0, dtype, shape, 7))
+    prefix = steep(sink_batch(pkg, device, [(0, front)], None, 0.0, 1.0, dtype, shape, 8)) if front else None
+    if prefix is None:
+        got = pkg.ops.paged_attention(batch.q, batch.cache, batch.s, scale=scale)
+    else:
+        got = pkg.ops.shared_prefix_attention(batch.q, prefix.cache, batch.cache, batch.s, scale=scale)
+    want, size, _, keys = pu.expected_wide(batch, scale, True, device, prefix)
+    # equal weights of equal keys: the roundings of the sums, the parts and the output are left
+    limit = (2 * pu.UNIT[dtype] ** 2 + 2 * (keys + 16) * 2.0 ** -24) * size
+    over = (got.double().cpu() - want).abs() - limit - pu.UNIT[dtype] * (want.abs() + limit)
+    assert torch.isfinite(got).all() and float(over.max()) <= 0, float(over.max())
