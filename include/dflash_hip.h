@@ -373,7 +373,8 @@ int dflash_paged_append(const dflash_paged_kv* cache, const dflash_rows* key, co
  * its own, else every row of its sequence.  heads / kv_heads query heads share a KV head.  fp32 scores and sums; a
  * weight meets its value as the sum of two 16-bit parts (off by at most 2^-16 of itself in bf16; 2^-22 in fp16, or 2^-28 of
  * the largest of 64 keys around).  A row that sees no key gives zeros; rows of tokens in no sequence are not written.  Masked
- * keys and values count for nothing, NaN and infinities among them.
+ * keys and values count for nothing, NaN and infinities among them; a value that is NaN or infinite leaves its feature NaN or
+ * infinite in the rows that see it.
  * prefix (NULL: none): a cache of one sequence that every sequence of the batch continues.  Its rows are visible to all
  * tokens, before the sequence's own, and are read once for the whole batch.  Same kv_heads, head_dim and dtype; pages of
  * its own kind, of the same pool or another.

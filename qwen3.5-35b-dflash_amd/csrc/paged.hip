@@ -551,7 +551,7 @@ __device__ __forceinline__ void small_share(const PagedParams& p, const Share& w
 // Bound: matrix instructions, behind them LDS reads (a wave reads every key and value for its 32 rows; 64 rows a wave would halve
 // the reads but need more than its 512 registers at head dim 256).  2048 tokens behind 6144 keys, 16 heads of 256: 313 to 328 us, 733 to
 // 767 TFLOP/s of the formulas, 1.1 PFLOP/s of matrix instructions with the weights' second parts (a large library product 1.3); prompts
-// of 442 to 2222 tokens, 32 heads of 128: 157 to 163 us.  Started cold, a launch spends about 14 us before and behind its
+// of 442 to 2222 tokens, 32 heads of 128: 157 to 165 us.  Started cold, a launch spends about 14 us before and behind its
 // steps, most of it fetching code that runs once.
 // The rows' reference moves only when a score exceeds it by kRise (weights reach 2^kRise, their relative precision is the same): the
 // accumulators are rescaled a few times a row instead of at every step.
