@@ -504,7 +504,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKV, starts: torch.Tensor, *
     Tokens ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) are the last of sequence ``b``'s ``lengths[b]`` rows
     (``paged_append`` wrote theirs); ``causal``: each sees the rows up to its own, else all of its sequence.  fp32 scores
     and sums.  A token that sees no row gives zeros; tokens past ``starts[B]`` are not written (``out``: a tensor to write
-    into, whose other rows stay as they are).
+    into, the query itself if need be, whose other rows stay as they are).
     """
     return _paged_attention("paged_attention", query, None, cache, starts, scale, causal, out, workspace)
 
