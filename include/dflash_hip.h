@@ -389,6 +389,101 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The states of a GDN layer for many sequences: a pool of slots, each a conv history [channels][3] (the last three rows
+ * of the convolution's input, oldest first) and a recurrent state fp32 [value_heads][head_dim][head_dim] (key feature, value
+ * feature).  Slot s lies at s * history_stride and s * recurrent_stride elements.  Sequence b has slot slots[b]; one
+ * outside [0, pool_slots) is no slot: its sequence starts from zeros and leaves no state.  Where states are written, no two
+ * sequences may have the same slot.
+ * A call's tokens [starts[b], starts[b + 1]) are the next ones of sequence b; starts: int32 [sequences + 1], ascending from 0 to
+ * at most `tokens`; tokens in no sequence are left out and their rows of the output not written.  counts int32
+ * [sequences] or NULL: the state is left as after the first counts[b] of them (NULL: all); with none the slot stays as
+ * it is.  fresh uint8 [sequences] or NULL: not 0, the state before the block is taken as zeros whatever the slot holds.
+ * slots, starts, counts and fresh are read on the device when the call runs: a captured call follows their later values.
+ * Constraints: dtype BF16 or F16; channels % 8 == 0, <= 2^16; head_dim 64 or 128; history_stride % 8 == 0, recurrent_stride
+ * % 4 == 0; sequences * value_heads <= 2^22, tokens <= 2^20.
+ */
+typedef struct dflash_state_pool {
+  void* history;
+  float* recurrent;
+  const int32_t* slots;
+  int64_t sequences, pool_slots, history_stride, recurrent_stride;
+  int64_t channels, value_heads, head_dim;
+  int32_t dtype; /* enum dflash_dtype, of the histories and of every 16-bit row */
+} dflash_state_pool;
+
+/*
+ * Causal depthwise convolution with SiLU (FusedOps.conv_state_update and causal_conv1d,
+ * model/qwen35_moe_dflash/fused/ops.py:36-53, for a batch): out[t][c] = silu(sum_j weight[c][j] X[t - 3 + j][c]), fp32 inside, X the
+ * rows of x with the history before them.  x: rows of `channels`, token_stride apart (head_stride not used); weight
+ * [channels][4]; out [tokens][channels].  Uses history only (recurrent may be NULL).
+ */
+int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const void* weight, const int32_t* starts,
+                    const int32_t* counts, const uint8_t* fresh, int64_t tokens, void* out, void* stream);
+
+/*
+ * The gated delta rule (FusedOps.chunk_gated_delta_rule, model/qwen35_moe_dflash/fused/ops.py:54-71, for a batch).  Per value head h of
+ * key head h / (value_heads / key_heads), from the sequence's state S on:
+ *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  out = S^T q
+ * q = query * scale and k = key, both over sqrt(sum of squares + 1e-6) where `normalise` is not 0.  With a_log and dt_bias
+ * (fp32 [value_heads], both or neither) g = -exp(a_log) softplus(decay + dt_bias) and beta = sigmoid(beta), else decay and beta
+ * are g and beta themselves: [tokens][value_heads] of gates_dtype, decay_stride and beta_stride elements a row.
+ * query and key [tokens][key_heads][head_dim], value and out [tokens][value_heads][head_dim]; fp32 inside, the state's products
+ * as exact as fp32.  Uses recurrent only (history may be NULL).
+ * longest: tokens of the longest block where the caller knows it, else 0.  It chooses the kernels, never the result.
+ */
+typedef struct dflash_rule {
+  dflash_rows query, key, value;
+  const void* decay;
+  const void* beta;
+  int64_t decay_stride, beta_stride;
+  const float* a_log;
+  const float* dt_bias;
+  int64_t key_heads;
+  float scale;
+  int32_t normalise;
+  int32_t gates_dtype;
+} dflash_rule;
+size_t dflash_gdn_rule_workspace_bytes(int64_t tokens, int64_t key_heads, int64_t value_heads, int64_t head_dim, int64_t sequences,
+                                       int64_t longest);
+int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, const int32_t* starts, const int32_t* counts,
+                    const uint8_t* fresh, int64_t tokens, int64_t longest, void* out, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/*
+ * Conv histories and recurrent states after the first counts[b] (required) tokens of blocks that dflash_gdn_conv (rows x) and
+ * dflash_gdn_rule took with counts of 0: what commits the accepted part of every block.  rule->query is not used.
+ */
+int dflash_gdn_advance(const dflash_state_pool* pool, const dflash_rows* x, const dflash_rule* rule, const int32_t* starts,
+                       const int32_t* counts, const uint8_t* fresh, int64_t tokens, void* stream);
+
+/*
+ * Check of drafted tokens by the target's probabilities from given random numbers (the greedy check is
+ * FusedTargetSession.verify, model/qwen35_moe_dflash/fused/session.py:316-341).  Sequence b has rows [starts[b], starts[b + 1]) of
+ * logits (starts int32 [sequences + 1]); row r predicts the token behind it, drafted[r] (int32 [rows]) is the drafter's choice for
+ * it, the last row's is not read.  p, q: softmax of target and draft logits over temperature[b] (fp32; NULL: 1).
+ *   accepted[b]: rows before the first r with not uniforms[r] * q(drafted[r]) < p(drafted[r]), at most all but the last;
+ *   token[b]: drawn from max(p - q, 0) of that row with uniforms[r + 1], after the last row from its p with its own uniform: the
+ *   first token at which the running sum exceeds uniform * sum (where rounding leaves none, the last that can be drawn).
+ * draft NULL: each drafted token was chosen outright (q is 1 there).  A temperature that is not above 0: p is 1 at the first
+ * largest logit and the drafter's choice counts as outright.  A drafted token outside the vocabulary is never accepted.  Where
+ * max(p - q, 0) is zero everywhere the token is drawn from p; where p is too (no logit above -infinity), and in a sequence
+ * without rows, token is -1.  NaN logits count as -infinity, +infinity as the largest fp32 number.  Sums and the weights of the
+ * rows that tokens are drawn from are 64 bits; the result does not depend on how the work is split.
+ * Logits of dtype BF16, F16 or F32, rows of `vocab`, target_stride and draft_stride elements apart.
+ * Constraints: vocab <= 2^24, rows <= 2^20, sequences <= 2^20.
+ */
+typedef struct dflash_logits {
+  const void* target;
+  const void* draft;
+  int64_t target_stride, draft_stride, rows, vocab;
+  int32_t dtype;
+} dflash_logits;
+size_t dflash_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab, int64_t sequences, int has_draft);
+int dflash_verify_drafts(const dflash_logits* logits, const int32_t* drafted, const int32_t* starts, int64_t sequences,
+                         const float* uniforms, const float* temperature, int32_t* accepted, int32_t* token, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
  * Measurement mode (no counterpart in the reference; for benchmarks and
  * profilers that time one kernel of the layer on its own): while a stage is
  * set, dflash_moe_w4a16 and dflash_moe_experts_w4a16 validate their arguments

@@ -126,6 +126,61 @@ class RowsDesc(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
+class PoolDesc(ctypes.Structure):
+    """``struct dflash_state_pool``."""
+
+    _fields_ = [
+        ("history", ctypes.c_void_p),
+        ("recurrent", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("sequences", ctypes.c_int64),
+        ("pool_slots", ctypes.c_int64),
+        ("history_stride", ctypes.c_int64),
+        ("recurrent_stride", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("value_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class RuleDesc(ctypes.Structure):
+    """``struct dflash_rule``."""
+
+    _fields_ = [
+        ("query", RowsDesc),
+        ("key", RowsDesc),
+        ("value", RowsDesc),
+        ("decay", ctypes.c_void_p),
+        ("beta", ctypes.c_void_p),
+        ("decay_stride", ctypes.c_int64),
+        ("beta_stride", ctypes.c_int64),
+        ("a_log", ctypes.c_void_p),
+        ("dt_bias", ctypes.c_void_p),
+        ("key_heads", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("normalise", ctypes.c_int32),
+        ("gates_dtype", ctypes.c_int32),
+    ]
+
+
+class LogitsDesc(ctypes.Structure):
+    """``struct dflash_logits``."""
+
+    _fields_ = [
+        ("target", ctypes.c_void_p),
+        ("draft", ctypes.c_void_p),
+        ("target_stride", ctypes.c_int64),
+        ("draft_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+_POOLP = ctypes.POINTER(PoolDesc)
+_RULEP = ctypes.POINTER(RuleDesc)
+_LOGITSP = ctypes.POINTER(LogitsDesc)
 _PAGEDP = ctypes.POINTER(PagedDesc)
 _ROWSP = ctypes.POINTER(RowsDesc)
 _GDNP = ctypes.POINTER(GdnDesc)
@@ -163,6 +218,12 @@ SIGNATURES = {
     "dflash_paged_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, ctypes.c_int]),
     "dflash_paged_attention": (ctypes.c_int, [_PAGEDP, _PAGEDP, _ROWSP, _P, _I64, _I64, ctypes.c_float, ctypes.c_int, _P,
                                               _P, _SZ, _P]),
+    "dflash_gdn_conv": (ctypes.c_int, [_POOLP, _ROWSP, _P, _P, _P, _P, _I64, _P, _P]),
+    "dflash_gdn_rule_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "dflash_gdn_rule": (ctypes.c_int, [_POOLP, _RULEP, _P, _P, _P, _I64, _I64, _P, _P, _SZ, _P]),
+    "dflash_gdn_advance": (ctypes.c_int, [_POOLP, _ROWSP, _RULEP, _P, _P, _P, _I64, _P]),
+    "dflash_verify_drafts_workspace_bytes": (_SZ, [_I64, _I64, _I64, ctypes.c_int]),
+    "dflash_verify_drafts": (ctypes.c_int, [_LOGITSP, _P, _P, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
     "dflash_set_split_down": (ctypes.c_int, [ctypes.c_int]),
     "dflash_set_tile_pieces": (ctypes.c_int, [ctypes.c_int]),
     "dflash_moe_split_down": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int32,

@@ -23,7 +23,8 @@ LIBRARY = PACKAGE_DIR / "libdflash_hip.so"
 TIMELINE_LIBRARY = PACKAGE_DIR / "libdflash_hip_timeline.so"
 SOURCES = ("csrc/api.hip", "csrc/route.hip", "csrc/w4_gemm.hip", "csrc/w4_stream.hip",
            "csrc/w4_tile.hip", "csrc/w4_verify.hip", "csrc/w4_small.hip", "csrc/w4_linear.hip",
-           "csrc/repack.hip", "csrc/gdn.hip", "csrc/attention.hip", "csrc/paged.hip")
+           "csrc/repack.hip", "csrc/gdn.hip", "csrc/attention.hip", "csrc/paged.hip", "csrc/gdn_batch.hip",
+           "csrc/drafts.hip")
 HOST_SOURCE = "csrc/host.cpp"
 HOST_LIBRARY = PACKAGE_DIR / "dflash_host.so"
 ARCH = "gfx950"

@@ -1289,6 +1289,262 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
   }
 }
 
+namespace {
+// ---------------------------------------------------------------- batches of sequences: states and drafts
+int check_pool(const dflash_state_pool* c, const char* name, bool history, bool recurrent) {
+  const auto bad = [&](const char* what) { return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
+  if (!c) return bad("the state pool is NULL");
+  if (c->dtype != DFLASH_DTYPE_BF16 && c->dtype != DFLASH_DTYPE_F16)
+    return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": dtype must be BF16 or F16");
+  if (c->sequences < 0 || c->sequences > (1 << 20) || c->pool_slots < 0 || c->pool_slots > 0x7FFFFFFF)
+    return bad("sequences or slots out of range");
+  if (c->sequences > 0 && !c->slots) return bad("slots is NULL");
+  if (history) {
+    if (c->channels <= 0 || c->channels > (1 << 16) || c->channels % 8)
+      return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": channels must be a multiple of 8, at most 2^16");
+    if (c->pool_slots > 0 && (!c->history || !aligned16(c->history))) return bad("history NULL or not 16-byte aligned");
+    if (c->history_stride < 0 || c->history_stride % 8) return bad("history_stride must be a multiple of 8");
+  }
+  if (recurrent) {
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": head_dim must be 64 or 128");
+    if (c->value_heads < 1 || c->value_heads > 1024 || c->sequences * c->value_heads > (1 << 22))
+      return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": value_heads must be in [1, 1024], sequences * value_heads at most 2^22");
+    if (c->pool_slots > 0 && (!c->recurrent || !aligned16(c->recurrent))) return bad("recurrent NULL or not 16-byte aligned");
+    if (c->recurrent_stride < 0 || c->recurrent_stride % 4) return bad("recurrent_stride must be a multiple of 4");
+  }
+  return DFLASH_OK;
+}
+
+int check_block(const char* name, const int32_t* starts, int64_t tokens) {
+  if (tokens < 0 || tokens > (1 << 20)) return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": tokens must be in [0, 2^20]");
+  if (!starts) return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string(name) + ": starts is NULL");
+  return DFLASH_OK;
+}
+
+dflash::PoolParams pool_params(const dflash_state_pool* c, const int32_t* starts, const int32_t* counts, const uint8_t* fresh,
+                               int64_t tokens) {
+  dflash::PoolParams p{};
+  p.history = static_cast<uint16_t*>(c->history);
+  p.recurrent = c->recurrent;
+  p.history_stride = c->history_stride;
+  p.recurrent_stride = c->recurrent_stride;
+  p.pool_slots = static_cast<int>(c->pool_slots);
+  p.B = static_cast<int>(c->sequences);
+  p.T = static_cast<int>(tokens);
+  p.slots = c->slots;
+  p.starts = starts;
+  p.counts = counts;
+  p.fresh = fresh;
+  return p;
+}
+
+int check_rule(const dflash_rule* r, const dflash_state_pool* c, const char* name, bool query) {
+  const auto bad = [&](const char* what) { return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
+  if (!r) return bad("the rule's rows are NULL");
+  if (r->key_heads < 1 || c->value_heads % r->key_heads) return bad("value_heads must be a multiple of key_heads");
+  if (query)
+    if (int e = check_rows(&r->query, (std::string(name) + " query").c_str())) return e;
+  if (int e = check_rows(&r->key, (std::string(name) + " key").c_str())) return e;
+  if (int e = check_rows(&r->value, (std::string(name) + " value").c_str())) return e;
+  if (!r->decay || !r->beta) return bad("decay or beta is NULL");
+  if (r->gates_dtype != DFLASH_DTYPE_BF16 && r->gates_dtype != DFLASH_DTYPE_F16 && r->gates_dtype != DFLASH_DTYPE_F32)
+    return bad("unknown gates_dtype");
+  const uintptr_t size = r->gates_dtype == DFLASH_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(r->decay) % size || reinterpret_cast<uintptr_t>(r->beta) % size) return bad("decay or beta misaligned");
+  if (r->decay_stride < 0 || r->beta_stride < 0) return bad("negative strides of decay or beta");
+  if (!r->a_log != !r->dt_bias) return bad("a_log and dt_bias go together");
+  if (!(r->scale >= -3.0e38f && r->scale <= 3.0e38f)) return bad("scale must be finite");
+  return DFLASH_OK;
+}
+
+dflash::RuleParams rule_params(const dflash_rule* r, const dflash_state_pool* c, const dflash::PoolParams& pool) {
+  dflash::RuleParams p{};
+  p.pool = pool;
+  p.query = static_cast<const uint16_t*>(r->query.data);
+  p.query_token = r->query.token_stride;
+  p.query_head = r->query.head_stride;
+  p.key = static_cast<const uint16_t*>(r->key.data);
+  p.key_token = r->key.token_stride;
+  p.key_head = r->key.head_stride;
+  p.value = static_cast<const uint16_t*>(r->value.data);
+  p.value_token = r->value.token_stride;
+  p.value_head = r->value.head_stride;
+  p.decay = r->decay;
+  p.beta = r->beta;
+  p.decay_stride = r->decay_stride;
+  p.beta_stride = r->beta_stride;
+  p.gates_dtype = r->gates_dtype;
+  p.a_log = r->a_log;
+  p.dt_bias = r->dt_bias;
+  p.Hv = static_cast<int>(c->value_heads);
+  p.rep = static_cast<int>(c->value_heads / r->key_heads);
+  p.normalise = r->normalise != 0;
+  p.scale = r->scale;
+  return p;
+}
+
+int conv_params(const dflash_state_pool* pool, const dflash_rows* x, const char* name, const dflash::PoolParams& params,
+                dflash::ConvParams* p) {
+  if (int e = check_rows(x, name)) return e;
+  p->pool = params;
+  p->x = static_cast<const uint16_t*>(x->data);
+  p->x_stride = x->token_stride;
+  p->channels = static_cast<int>(pool->channels);
+  return DFLASH_OK;
+}
+
+// Parts that the rows of logits are cut into: about kDraftGroups workgroups in the first pass, and as many for the rows that tokens
+// are drawn from, of 2048 tokens at least.
+constexpr int64_t kDraftGroups = 4096;
+struct DraftLayout {
+  int64_t splits, split_octets, parts, part_octets;
+  size_t stats, choice, norms, part, total;
+};
+bool draft_shape_ok(int64_t rows, int64_t vocab, int64_t sequences) {
+  return rows >= 0 && rows <= (1 << 20) && vocab >= 1 && vocab <= (1 << 24) && sequences >= 0 && sequences <= (1 << 20);
+}
+DraftLayout draft_layout(int64_t rows, int64_t vocab, int64_t B, bool draft) {
+  DraftLayout L;
+  const int64_t octets = (vocab + 14) / 8;  // a row may begin up to seven tokens behind a 16-byte boundary
+  const auto cut = [&](int64_t count, int64_t* parts, int64_t* each) {
+    const int64_t want = std::max<int64_t>(1, kDraftGroups / std::max<int64_t>(1, count));
+    *each = std::max<int64_t>(256, (octets + want - 1) / want);
+    *parts = (octets + *each - 1) / *each;
+  };
+  cut(rows * (draft ? 2 : 1), &L.splits, &L.split_octets);
+  cut(B * 4, &L.parts, &L.part_octets);
+  Carver c;
+  L.stats = c.take(sizeof(dflash::DraftStats) * (draft ? 2 : 1) * static_cast<size_t>(rows * L.splits));
+  L.choice = c.take(sizeof(dflash::DraftChoice) * static_cast<size_t>(B));
+  L.norms = c.take(sizeof(double) * 2 * static_cast<size_t>(B * L.parts));
+  L.part = c.take(sizeof(dflash::DraftPart) * static_cast<size_t>(B * L.parts));
+  L.total = c.off;
+  return L;
+}
+}  // namespace
+
+int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const void* weight, const int32_t* starts,
+                    const int32_t* counts, const uint8_t* fresh, int64_t tokens, void* out, void* stream) {
+  try {
+    if (int r = check_pool(pool, "gdn conv", true, false)) return r;
+    if (tokens == 0 || pool->sequences == 0) return DFLASH_OK;
+    if (int r = check_block("gdn conv", starts, tokens)) return r;
+    dflash::ConvParams p{};
+    if (int r = conv_params(pool, x, "gdn conv x", pool_params(pool, starts, counts, fresh, tokens), &p)) return r;
+    if (!weight || !aligned16(weight) || !out || !aligned16(out))
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: weight or out is NULL or not 16-byte aligned");
+    if (out == x->data) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: out cannot be x, whose rows are read after a row is written");
+    p.weight = static_cast<const uint16_t*>(weight);
+    p.out = static_cast<uint16_t*>(out);
+    dflash::launch_gdn_conv(pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
+    return launch_status("gdn conv");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
+size_t dflash_gdn_rule_workspace_bytes(int64_t tokens, int64_t key_heads, int64_t value_heads, int64_t head_dim, int64_t sequences,
+                                       int64_t longest) {
+  (void)tokens, (void)key_heads, (void)value_heads, (void)head_dim, (void)sequences, (void)longest;
+  return 0;
+}
+
+int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, const int32_t* starts, const int32_t* counts,
+                    const uint8_t* fresh, int64_t tokens, int64_t longest, void* out, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  try {
+    if (int r = check_pool(pool, "gdn rule", false, true)) return r;
+    if (tokens == 0 || pool->sequences == 0) return DFLASH_OK;
+    if (int r = check_block("gdn rule", starts, tokens)) return r;
+    if (int r = check_rule(rule, pool, "gdn rule", true)) return r;
+    if (longest < 0) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: longest must not be negative");
+    if (!out || !aligned16(out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out is NULL or not 16-byte aligned");
+    (void)workspace, (void)workspace_bytes;
+    dflash::RuleParams p = rule_params(rule, pool, pool_params(pool, starts, counts, fresh, tokens));
+    p.out = static_cast<uint16_t*>(out);
+    dflash::launch_gdn_rule(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
+    return launch_status("gdn rule");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
+int dflash_gdn_advance(const dflash_state_pool* pool, const dflash_rows* x, const dflash_rule* rule, const int32_t* starts,
+                       const int32_t* counts, const uint8_t* fresh, int64_t tokens, void* stream) {
+  try {
+    if (int r = check_pool(pool, "gdn advance", true, true)) return r;
+    if (tokens == 0 || pool->sequences == 0) return DFLASH_OK;
+    if (int r = check_block("gdn advance", starts, tokens)) return r;
+    if (!counts) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn advance: counts is NULL");
+    if (int r = check_rule(rule, pool, "gdn advance", false)) return r;
+    const dflash::PoolParams params = pool_params(pool, starts, counts, fresh, tokens);
+    dflash::ConvParams c{};
+    if (int r = conv_params(pool, x, "gdn advance x", params, &c)) return r;
+    dflash::launch_gdn_advance(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, rule_params(rule, pool, params),
+                               c, static_cast<hipStream_t>(stream));
+    return launch_status("gdn advance");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
+size_t dflash_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab, int64_t sequences, int has_draft) {
+  if (!draft_shape_ok(rows, vocab, sequences)) return 0;
+  return draft_layout(rows, vocab, sequences, has_draft != 0).total;
+}
+
+int dflash_verify_drafts(const dflash_logits* logits, const int32_t* drafted, const int32_t* starts, int64_t sequences,
+                         const float* uniforms, const float* temperature, int32_t* accepted, int32_t* token, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  try {
+    const auto bad = [](const char* what) { return fail(DFLASH_ERR_INVALID_ARGUMENT, std::string("verify drafts: ") + what); };
+    if (!logits) return bad("logits is NULL");
+    const int64_t rows = logits->rows, V = logits->vocab;
+    if (!draft_shape_ok(rows, V, sequences))
+      return fail(DFLASH_ERR_UNSUPPORTED, "verify drafts: rows and sequences must be at most 2^20, vocab in [1, 2^24]");
+    if (logits->dtype != DFLASH_DTYPE_BF16 && logits->dtype != DFLASH_DTYPE_F16 && logits->dtype != DFLASH_DTYPE_F32)
+      return fail(DFLASH_ERR_UNSUPPORTED, "verify drafts: dtype must be BF16, F16 or F32");
+    if (sequences == 0) return DFLASH_OK;
+    const uintptr_t size = logits->dtype == DFLASH_DTYPE_F32 ? 4 : 2;
+    if (rows > 0 && (!logits->target || !drafted || !uniforms)) return bad("target, drafted or uniforms is NULL");
+    if (reinterpret_cast<uintptr_t>(logits->target) % size || reinterpret_cast<uintptr_t>(logits->draft) % size)
+      return bad("target or draft misaligned");
+    if (logits->target_stride < 0 || logits->draft_stride < 0) return bad("strides must not be negative");
+    if (!starts || !accepted || !token) return bad("starts, accepted or token is NULL");
+    const bool draft = logits->draft != nullptr;
+    const DraftLayout L = draft_layout(rows, V, sequences, draft);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < L.total)
+      return fail(DFLASH_ERR_WORKSPACE, "verify drafts workspace needs " + std::to_string(L.total) + " bytes");
+    dflash::DraftParams p{};
+    p.target = logits->target;
+    p.draft = logits->draft;
+    p.target_stride = logits->target_stride;
+    p.draft_stride = logits->draft_stride;
+    p.dtype = logits->dtype;
+    p.V = static_cast<int>(V);
+    p.B = static_cast<int>(sequences);
+    p.rows = static_cast<int>(rows);
+    p.drafted = drafted;
+    p.starts = starts;
+    p.uniforms = uniforms;
+    p.temperature = temperature;
+    p.accepted = accepted;
+    p.token = token;
+    p.splits = static_cast<int>(L.splits);
+    p.split_octets = static_cast<int>(L.split_octets);
+    p.parts = static_cast<int>(L.parts);
+    p.part_octets = static_cast<int>(L.part_octets);
+    p.stats = at<dflash::DraftStats>(workspace, L.stats);
+    p.choice = at<dflash::DraftChoice>(workspace, L.choice);
+    p.norms = at<double>(workspace, L.norms);
+    p.part = at<dflash::DraftPart>(workspace, L.part);
+    dflash::launch_verify_drafts(p, static_cast<hipStream_t>(stream));
+    return launch_status("verify drafts");
+  } catch (...) {
+    return fail(DFLASH_ERR_HIP, "unexpected host exception");
+  }
+}
+
 int dflash_router_logits(const void* hidden, int64_t tokens, int64_t hidden_size, const void* router_weight,
                          int64_t experts, float* logits, void* stream) {
   try {

@@ -409,4 +409,70 @@ int paged_slots(int tile_rows, int head_dim, int cus);
 void launch_paged_append(int head_dim, bool bf16, const AppendParams& p, hipStream_t stream);
 void launch_paged_attention(int head_dim, bool bf16, const PagedParams& p, hipStream_t stream);
 
+// Conv histories and recurrent states of a batch of sequences (gdn_batch.hip), strides in elements.
+struct PoolParams {
+  uint16_t* history;              // [pool_slots] slots of [channels][3]
+  float* recurrent;               // [pool_slots] slots of [Hv][dim][dim]
+  int64_t history_stride, recurrent_stride;
+  int pool_slots, B, T;
+  const int32_t* slots;           // [B]
+  const int32_t* starts;          // [B + 1]
+  const int32_t* counts;          // [B] or null: every token of the block
+  const uint8_t* fresh;           // [B] or null
+};
+struct ConvParams {
+  PoolParams pool;
+  const uint16_t* x;              // rows of `channels`, x_stride apart
+  int64_t x_stride;
+  const uint16_t* weight;         // [channels][4]
+  int channels;                   // a multiple of 8
+  uint16_t* out;                  // [T][channels]
+};
+struct RuleParams {
+  PoolParams pool;
+  const uint16_t *query, *key, *value;
+  int64_t query_token, query_head, key_token, key_head, value_token, value_head;
+  const void *decay, *beta;       // [T][Hv] by their row strides
+  int64_t decay_stride, beta_stride;
+  int gates_dtype;                // enum dflash_dtype
+  const float *a_log, *dt_bias;   // [Hv], or both null: decay and beta are the gates themselves
+  int Hv, rep;                    // value heads, of each key head
+  int normalise;
+  float scale;
+  uint16_t* out;                  // [T][Hv][dim]
+};
+void launch_gdn_conv(bool bf16, const ConvParams& p, hipStream_t stream);
+void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, hipStream_t stream);
+void launch_gdn_advance(int dim, bool bf16, const RuleParams& p, const ConvParams& c, hipStream_t stream);
+
+// Check of drafted tokens (drafts.hip).
+struct DraftStats {               // of one part of a row
+  float top;                      // largest logit
+  int32_t at;                     // where it stands first (rows at temperature 0)
+  double sum;                     // of exp((l - top) / temperature)
+};
+struct DraftChoice {              // of one sequence: the row that its token comes from
+  int32_t row, has_draft;         // row -1: none; has_draft: the drafter's distribution, or its one token, is taken off
+  float target_top, draft_top;
+};
+struct DraftPart {                // of one part of that row
+  double left, whole;             // sums of the weights that are left and of the target's own
+  int32_t last_left, last_whole;  // last tokens with such a weight, -1: none
+};
+struct DraftParams {
+  const void *target, *draft;     // [rows][V] by their strides; draft may be null
+  int64_t target_stride, draft_stride;
+  int dtype, V, B, rows;
+  const int32_t *drafted, *starts;
+  const float *uniforms, *temperature;
+  int32_t *accepted, *token;
+  int splits, split_octets;       // parts of a row in the first pass, and eights of tokens in one
+  int parts, part_octets;         // parts of the chosen rows
+  DraftStats* stats;              // [2][rows][splits]
+  DraftChoice* choice;            // [B]
+  double* norms;                  // [2][B][parts]
+  DraftPart* part;                // [B][parts]
+};
+void launch_verify_drafts(const DraftParams& p, hipStream_t stream);
+
 }  // namespace dflash

@@ -529,6 +529,276 @@ def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head
                                                                   int(has_prefix)))
 
 
+class StatePool(NamedTuple):
+    """The states of a GDN layer for ``B`` sequences (``dflash_state_pool`` in ``include/dflash_hip.h``): sequence ``b`` has slot
+    ``slots[b]`` of both pools; one that is no slot stands for a sequence that starts from zeros and leaves no state.
+    ``slots`` is read on the device when a call runs, so a captured call follows its later values."""
+
+    history: Optional[torch.Tensor]    # bf16 or fp16 [slots, channels, 3]: last rows of the convolution's input, oldest first
+    recurrent: Optional[torch.Tensor]  # fp32 [slots, value heads, head dim, head dim] (key feature, value feature)
+    slots: torch.Tensor                # int32 [B]
+
+
+_GATE_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16}
+
+
+def _slot_pool(t, name: str, dtypes, ndim: int, unit: int, device: torch.device) -> torch.Tensor:
+    """A pool whose slots the kernels read and write as they lie."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.ndim != ndim or t.device != device:
+        raise ValueError(f"{name} must be a pool of {' or '.join(map(str, dtypes))} slots with {ndim} dimensions on {device}")
+    inner = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size > 1 and stride != inner:
+            raise ValueError(f"{name} needs contiguous slots")
+        inner *= size
+    if t.data_ptr() % 16 or t.stride(0) % unit or (t.shape[0] > 1 and t.stride(0) < inner):
+        raise ValueError(f"{name} needs 16-byte aligned slots that do not overlap")
+    return t
+
+
+def _pool(pool: StatePool, name: str, dtype: Optional[torch.dtype], history: bool, recurrent: bool) -> tuple:
+    """The descriptor of a valid state pool, its device, and what has to outlive the call."""
+    if not isinstance(pool, StatePool):
+        raise ValueError(f"{name} takes a StatePool (history, recurrent, slots)")
+    device = _require_device(pool.slots, *(t for t, used in ((pool.history, history), (pool.recurrent, recurrent)) if used))
+    slots = pool.slots
+    if slots.ndim != 1:
+        raise ValueError("slots must be int32 [sequences]")
+    slots = _int32(slots, tuple(slots.shape), "slots", device)
+    desc = _lib.PoolDesc(slots=slots.data_ptr(), sequences=slots.shape[0])
+    counts = set()
+    if history:
+        h = _slot_pool(pool.history, "history", tuple(_PAGED_DTYPES), 3, 8, device)
+        if h.shape[2] != 3:
+            raise ValueError("history must be [slots, channels, 3]: the convolution has four taps")
+        if dtype is not None and h.dtype != dtype:
+            raise ValueError(f"history must be {dtype}, as the rows are")
+        dtype = h.dtype
+        desc.history, desc.history_stride, desc.channels = h.data_ptr(), h.stride(0), h.shape[1]
+        counts.add(h.shape[0])
+    if recurrent:
+        r = _slot_pool(pool.recurrent, "recurrent", (torch.float32,), 4, 4, device)
+        if r.shape[2] != r.shape[3]:
+            raise ValueError("recurrent must be [slots, value heads, head dim, head dim]")
+        desc.recurrent, desc.recurrent_stride, desc.value_heads, desc.head_dim = r.data_ptr(), r.stride(0), r.shape[1], r.shape[2]
+        counts.add(r.shape[0])
+    if len(counts) != 1:
+        raise ValueError("history and recurrent need as many slots")
+    desc.pool_slots = counts.pop()
+    if dtype not in _PAGED_DTYPES:
+        raise ValueError(f"{name} takes bfloat16 or float16 rows")
+    desc.dtype = _PAGED_DTYPES[dtype]
+    return desc, device, slots
+
+
+def _block_rows(t, name: str, dtype, device: torch.device, ndim: int, tokens: Optional[int], *last) -> torch.Tensor:
+    """``t`` as rows of a block that the kernels read: as it lies, or a contiguous copy."""
+    if (not isinstance(t, torch.Tensor) or t.ndim != ndim or t.dtype != dtype or t.device != device
+            or (tokens is not None and t.shape[0] != tokens) or any(a is not None and a != b for a, b in zip(last, t.shape[1:]))):
+        shape = ", ".join(str("..." if a is None else a) for a in last)
+        raise ValueError(f"{name} must be {dtype} [{'tokens' if tokens is None else tokens}, {shape}] on {device}")
+    return t if _aligned(t) else t.contiguous()
+
+
+def _flags(fresh, count: int, device: torch.device) -> Optional[torch.Tensor]:
+    if fresh is None:
+        return None
+    if (not isinstance(fresh, torch.Tensor) or fresh.dtype not in (torch.bool, torch.uint8) or tuple(fresh.shape) != (count,)
+            or fresh.device != device):
+        raise ValueError(f"fresh must be bool [{count}] on {device}")
+    return fresh.contiguous()
+
+
+def _block_ints(starts, counts, count: int, device: torch.device) -> tuple:
+    return (_int32(starts, (count + 1,), "starts", device),
+            None if counts is None else _int32(counts, (count,), "counts", device))
+
+
+def _rule(pool_desc, device, query, key, value, decay, beta, a_log, dt_bias, normalise, scale) -> tuple:
+    """The descriptor of valid rows of the delta rule, and what has to outlive the call."""
+    hv, dim = pool_desc.value_heads, pool_desc.head_dim
+    dtype = value.dtype
+    value = _block_rows(value, "value", dtype, device, 3, None, hv, dim)
+    tokens = value.shape[0]
+    key = _block_rows(key, "key", dtype, device, 3, tokens, None, dim)
+    hk = key.shape[1]
+    if hk < 1 or hv % hk:
+        raise ValueError("value heads must be a multiple of the key heads")
+    if query is not None:
+        query = _block_rows(query, "query", dtype, device, 3, tokens, hk, dim)
+    gates = []
+    for name, t in (("decay", decay), ("beta", beta)):
+        if (not isinstance(t, torch.Tensor) or t.dtype not in _GATE_DTYPES or t.dtype != decay.dtype or tuple(t.shape) != (tokens, hv)
+                or t.device != device):
+            raise ValueError(f"{name} must be float32, bfloat16 or float16 [{tokens}, {hv}] on {device}, decay and beta of one dtype")
+        gates.append(t if t.stride(1) == 1 or hv == 1 else t.contiguous())
+    decay, beta = gates
+    if (a_log is None) != (dt_bias is None):
+        raise ValueError("a_log and dt_bias go together")
+    vectors = []
+    for name, t in (("a_log", a_log), ("dt_bias", dt_bias)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != (hv,) or t.device != device):
+            raise ValueError(f"{name} must be float32 [{hv}] on {device}")
+        vectors.append(None if t is None else t.contiguous())
+    if type(normalise) is not bool or isinstance(scale, bool) or not isinstance(scale, (int, float, type(None))):
+        raise ValueError("normalise must be a bool and scale a number")
+    rows = lambda t: _lib.RowsDesc() if t is None else _lib.RowsDesc(t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
+    desc = _lib.RuleDesc(rows(query), rows(key), rows(value), decay.data_ptr(), beta.data_ptr(), decay.stride(0), beta.stride(0),
+                         *(None if v is None else v.data_ptr() for v in vectors), hk, dim ** -0.5 if scale is None else scale,
+                         int(normalise), _GATE_DTYPES[decay.dtype])
+    return desc, tokens, (query, key, value, decay, beta, *vectors)
+
+
+def gdn_conv(x: torch.Tensor, weight: torch.Tensor, pool: StatePool, starts: torch.Tensor, *, fresh: Optional[torch.Tensor] = None,
+             counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal depthwise convolution with SiLU of a batch of blocks: ``x`` and result ``[tokens, channels]``.
+
+    Tokens ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) continue sequence ``b`` behind the three rows that its slot of
+    ``pool.history`` holds (zeros where ``fresh[b]``); ``weight`` ``[channels, 1, 4]``, its last tap the token's own.  The slot
+    then holds the last rows after ``counts[b]`` of the tokens (int32 ``[B]``; None: all of them; 0: it stays as it is).  fp32 inside, one
+    rounding.  ``x`` may be a view of a projection's rows.  Tokens in no sequence are not written (``out``: a tensor to write into,
+    which shares no memory with ``x``).
+    """
+    if not isinstance(x, torch.Tensor):
+        raise ValueError("x must be a tensor [tokens, channels]")
+    desc, device, slots = _pool(pool, "gdn_conv", x.dtype, True, False)
+    x = _block_rows(x, "x", x.dtype, device, 2, None, desc.channels)
+    if (not isinstance(weight, torch.Tensor) or weight.dtype != x.dtype or weight.device != device
+            or tuple(weight.shape) != (desc.channels, 1, 4)):
+        raise ValueError(f"weight must be {x.dtype} [{desc.channels}, 1, 4] on {device}")
+    weight = weight if _as(weight, x.dtype, weight.shape, device) else weight.clone(memory_format=torch.contiguous_format)
+    starts, counts = _block_ints(starts, counts, desc.sequences, device)
+    flags = _flags(fresh, desc.sequences, device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    elif not _as(out, x.dtype, x.shape, device):
+        raise ValueError(f"out must be a contiguous {x.dtype} {list(x.shape)} tensor on {device}")
+    _untracked("gdn_conv", x, weight, pool.history, out)
+    with torch.cuda.device(device):
+        _lib.call("dflash_gdn_conv", ctypes.byref(desc), ctypes.byref(_lib.RowsDesc(x.data_ptr(), x.stride(0), 0)), _ptr(weight),
+                  _ptr(starts), _ptr(counts), _ptr(flags), x.shape[0], _ptr(out), _stream(device))
+    return out
+
+
+def gdn_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay: torch.Tensor, beta: torch.Tensor, pool: StatePool,
+             starts: torch.Tensor, *, a_log: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
+             normalise: bool = True, scale: Optional[float] = None, fresh: Optional[torch.Tensor] = None,
+             counts: Optional[torch.Tensor] = None, longest: Optional[int] = None, out: Optional[torch.Tensor] = None,
+             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gated delta rule of a batch of blocks over a pool of states: ``query``, ``key`` ``[tokens, key heads, head dim]``, ``value`` and
+    result ``[tokens, value heads, head dim]``.
+
+    Tokens ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) continue sequence ``b`` from the state in its slot of
+    ``pool.recurrent`` (zeros where ``fresh[b]``): ``S <- e^g S; u = beta (v - S^T k); S <- S + k u^T; o = S^T q``, ``q`` times ``scale``
+    (head dim ** -0.5), both over their L2 norms (``normalise``).  ``decay`` and ``beta`` ``[tokens, value heads]`` are ``g`` and
+    ``beta``, or with ``a_log`` and ``dt_bias`` (fp32 ``[value heads]``) a layer's projections: ``g = -exp(a_log) softplus(decay +
+    dt_bias)``, ``beta = sigmoid(beta)``.  The slot then holds the state after ``counts[b]`` tokens (int32 ``[B]``; None: all of them;
+    0: it stays as it is, as a verify block's does until :func:`gdn_advance`).  ``longest``: tokens of the longest block, if the caller
+    knows it, for the choice of the kernels.  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
+    tensor to write into, which shares no memory with the rows).
+    """
+    if not isinstance(value, torch.Tensor):
+        raise ValueError("value must be a tensor [tokens, value heads, head dim]")
+    if query is None:
+        raise ValueError("gdn_rule needs a query")
+    if longest is not None and (type(longest) is not int or longest < 0):
+        raise ValueError("longest must be an int, not negative")
+    desc, device, slots = _pool(pool, "gdn_rule", value.dtype, False, True)
+    rule, tokens, keep = _rule(desc, device, query, key, value, decay, beta, a_log, dt_bias, normalise, scale)
+    starts, counts = _block_ints(starts, counts, desc.sequences, device)
+    flags = _flags(fresh, desc.sequences, device)
+    shape = (tokens, desc.value_heads, desc.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=value.dtype, device=device)
+    elif not _as(out, value.dtype, shape, device):
+        raise ValueError(f"out must be a contiguous {value.dtype} {list(shape)} tensor on {device}")
+    _untracked("gdn_rule", query, key, value, decay, beta, a_log, dt_bias, pool.recurrent, out)
+    with torch.cuda.device(device):
+        ws = _workspace(gdn_rule_workspace_bytes(tokens, rule.key_heads, desc.value_heads, desc.head_dim, desc.sequences, longest or 0),
+                        device, workspace)
+        _lib.call("dflash_gdn_rule", ctypes.byref(desc), ctypes.byref(rule), _ptr(starts), _ptr(counts), _ptr(flags), tokens,
+                  longest or 0, _ptr(out), _ptr(ws), ws.numel(), _stream(device))
+    return out
+
+
+def gdn_rule_workspace_bytes(tokens: int, key_heads: int, value_heads: int, head_dim: int, sequences: int, longest: int = 0) -> int:
+    return int(_lib.load().dflash_gdn_rule_workspace_bytes(tokens, key_heads, value_heads, head_dim, sequences, longest))
+
+
+def gdn_advance(pool: StatePool, x: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay: torch.Tensor, beta: torch.Tensor,
+                starts: torch.Tensor, counts: torch.Tensor, *, a_log: Optional[torch.Tensor] = None,
+                dt_bias: Optional[torch.Tensor] = None, normalise: bool = True, fresh: Optional[torch.Tensor] = None) -> None:
+    """Histories and states after the first ``counts[b]`` tokens of blocks that :func:`gdn_conv` (its ``x``) and :func:`gdn_rule` took
+    without advancing them (``counts`` of 0): commits the accepted part of every sequence's block in one launch."""
+    if not isinstance(value, torch.Tensor):
+        raise ValueError("value must be a tensor [tokens, value heads, head dim]")
+    if counts is None:
+        raise ValueError("gdn_advance needs counts")
+    desc, device, slots = _pool(pool, "gdn_advance", value.dtype, True, True)
+    rule, tokens, keep = _rule(desc, device, None, key, value, decay, beta, a_log, dt_bias, normalise, None)
+    x = _block_rows(x, "x", value.dtype, device, 2, tokens, desc.channels)
+    starts, counts = _block_ints(starts, counts, desc.sequences, device)
+    flags = _flags(fresh, desc.sequences, device)
+    _untracked("gdn_advance", x, key, value, decay, beta, a_log, dt_bias, pool.history, pool.recurrent)
+    with torch.cuda.device(device):
+        _lib.call("dflash_gdn_advance", ctypes.byref(desc), ctypes.byref(_lib.RowsDesc(x.data_ptr(), x.stride(0), 0)),
+                  ctypes.byref(rule), _ptr(starts), _ptr(counts), _ptr(flags), tokens, _stream(device))
+
+
+class Verified(NamedTuple):
+    """Outputs of :func:`verify_drafts`."""
+
+    accepted: torch.Tensor   # int32 [B]: drafted tokens accepted
+    token: torch.Tensor      # int32 [B]: the token behind them, -1: none
+
+
+def verify_drafts(target: torch.Tensor, drafted: torch.Tensor, starts: torch.Tensor, uniforms: torch.Tensor, *,
+                  draft: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> Verified:
+    """Which drafted tokens the target's probabilities accept, and the token behind them, from given random numbers.
+
+    Rows ``[starts[b], starts[b + 1])`` (``starts`` int32 ``[B + 1]``) of the logits ``target`` ``[rows, vocab]`` are sequence ``b``'s; row ``r``
+    predicts the token behind it, ``drafted[r]`` (int32 ``[rows]``) is the drafter's choice for it, drawn from ``draft`` ``[rows, vocab]``
+    (None: chosen outright); the last row of a sequence has none.  ``temperature`` fp32 ``[B]`` (None: 1) divides both; 0 is greedy.
+    With the softmaxes ``p`` and ``q`` a token ``x`` is accepted iff ``uniforms[r] * q(x) < p(x)`` (fp32 ``[rows]`` in [0, 1)); the first that is not
+    is replaced by a draw from ``max(p - q, 0)`` with the next row's uniform, and all accepted are followed by a draw from the last
+    row's ``p`` with its own: the emitted tokens follow the target's distribution.  One row a sequence is plain sampling.  Logits bf16, fp16 or fp32; sums, and the weights that tokens are drawn
+    by, in 64 bits.
+    """
+    device = _require_device(target, drafted, starts, uniforms)
+    if target.ndim != 2 or target.dtype not in _GATE_DTYPES or target.shape[1] < 1:
+        raise ValueError("target must be bfloat16, float16 or float32 [rows, vocab]")
+    rows, vocab = target.shape
+    if draft is not None and (not isinstance(draft, torch.Tensor) or draft.dtype != target.dtype or draft.shape != target.shape
+                              or draft.device != device):
+        raise ValueError(f"draft must be {target.dtype} [{rows}, {vocab}] on {device}")
+    if starts.ndim != 1 or starts.shape[0] < 1:
+        raise ValueError("starts must be int32 [sequences + 1]")
+    count = starts.shape[0] - 1
+    starts = _int32(starts, (count + 1,), "starts", device)
+    drafted = _int32(drafted, (rows,), "drafted", device)
+    for name, t, n in (("uniforms", uniforms, rows), ("temperature", temperature, count)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != (n,) or t.device != device):
+            raise ValueError(f"{name} must be float32 [{n}] on {device}")
+    uniforms = uniforms.contiguous()
+    temperature = None if temperature is None else temperature.contiguous()
+    target, draft = (t if t is None or t.stride(1) == 1 else t.contiguous() for t in (target, draft))
+    _untracked("verify_drafts", target, draft, uniforms, temperature)
+    accepted = torch.empty((count,), dtype=torch.int32, device=device)
+    token = torch.empty((count,), dtype=torch.int32, device=device)
+    logits = _lib.LogitsDesc(target.data_ptr(), None if draft is None else draft.data_ptr(), target.stride(0),
+                             0 if draft is None else draft.stride(0), rows, vocab, _GATE_DTYPES[target.dtype])
+    with torch.cuda.device(device):
+        ws = _workspace(verify_drafts_workspace_bytes(rows, vocab, count, draft is not None), device, workspace)
+        _lib.call("dflash_verify_drafts", ctypes.byref(logits), _ptr(drafted), _ptr(starts), count, _ptr(uniforms), _ptr(temperature),
+                  _ptr(accepted), _ptr(token), _ptr(ws), ws.numel(), _stream(device))
+    return Verified(accepted, token)
+
+
+def verify_drafts_workspace_bytes(rows: int, vocab: int, sequences: int, has_draft: bool) -> int:
+    return int(_lib.load().dflash_verify_drafts_workspace_bytes(rows, vocab, sequences, int(has_draft)))
+
+
 def router_logits(hidden: torch.Tensor, router_weight: torch.Tensor) -> torch.Tensor:
     """fp32 ``[T, E]`` logits from bf16 ``hidden [..., H]`` and bf16 ``router_weight [E, H]``."""
     device = _require_device(hidden, router_weight)
