@@ -400,7 +400,7 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
  * it is.  fresh uint8 [sequences] or NULL: not 0, the state before the block is taken as zeros whatever the slot holds.
  * slots, starts, counts and fresh are read on the device when the call runs: a captured call follows their later values.
  * Constraints: dtype BF16 or F16; channels % 8 == 0, <= 2^16; head_dim 64 or 128; history_stride % 8 == 0, recurrent_stride
- * % 4 == 0; sequences * value_heads <= 2^22, tokens <= 2^20.
+ * % 4 == 0; sequences * value_heads <= 2^19, tokens <= 2^20, tokens * value_heads <= 2^28.
  */
 typedef struct dflash_state_pool {
   void* history;

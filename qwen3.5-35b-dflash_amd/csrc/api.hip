@@ -1307,8 +1307,8 @@ int check_pool(const dflash_state_pool* c, const char* name, bool history, bool 
   }
   if (recurrent) {
     if (c->head_dim != 64 && c->head_dim != 128) return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": head_dim must be 64 or 128");
-    if (c->value_heads < 1 || c->value_heads > 1024 || c->sequences * c->value_heads > (1 << 22))
-      return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": value_heads must be in [1, 1024], sequences * value_heads at most 2^22");
+    if (c->value_heads < 1 || c->value_heads > 1024 || c->sequences * c->value_heads > (1 << 19))
+      return fail(DFLASH_ERR_UNSUPPORTED, std::string(name) + ": value_heads must be in [1, 1024], sequences * value_heads at most 2^19");
     if (c->pool_slots > 0 && (!c->recurrent || !aligned16(c->recurrent))) return bad("recurrent NULL or not 16-byte aligned");
     if (c->recurrent_stride < 0 || c->recurrent_stride % 4) return bad("recurrent_stride must be a multiple of 4");
   }
@@ -1443,10 +1443,39 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
   }
 }
 
+namespace {
+// Blocks of more tokens than this go 64 at a time.
+constexpr int64_t kRuleSteps = 16;
+
+struct RuleLayout {
+  int64_t chunks;  // 0: token after token, without a workspace
+  size_t t, p, kt, scalars, total;
+};
+bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
+  return T >= 0 && T <= (1 << 20) && Hk > 0 && Hv > 0 && Hv <= 1024 && Hv % Hk == 0 && (D == 64 || D == 128) && B >= 0 && B <= (1 << 20) &&
+         B * Hv <= (1 << 19) && T * Hv <= (1 << 28) && longest >= 0;
+}
+RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
+  RuleLayout L{};
+  if (B == 0 || T == 0) return L;
+  if (longest == 0) longest = std::min(T, 2 * ((T + B - 1) / B));  // not known: as if none were twice the average
+  if (std::min(longest, T) <= kRuleSteps) return L;
+  L.chunks = T / dflash::kRuleChunk + std::min(T, B);
+  Carver c;
+  const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
+  L.t = c.take(each * 3 * part);
+  L.p = c.take(each * 2 * part);
+  L.kt = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
+  L.scalars = c.take(each * sizeof(dflash::ChunkScalars));
+  L.total = c.off;
+  return L;
+}
+}  // namespace
+
 size_t dflash_gdn_rule_workspace_bytes(int64_t tokens, int64_t key_heads, int64_t value_heads, int64_t head_dim, int64_t sequences,
                                        int64_t longest) {
-  (void)tokens, (void)key_heads, (void)value_heads, (void)head_dim, (void)sequences, (void)longest;
-  return 0;
+  if (!rule_shape_ok(tokens, key_heads, value_heads, head_dim, sequences, longest)) return 0;
+  return rule_layout(tokens, key_heads, value_heads, head_dim, sequences, longest).total;
 }
 
 int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, const int32_t* starts, const int32_t* counts,
@@ -1458,10 +1487,26 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
     if (int r = check_block("gdn rule", starts, tokens)) return r;
     if (int r = check_rule(rule, pool, "gdn rule", true)) return r;
     if (longest < 0) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: longest must not be negative");
+    if (tokens * pool->value_heads > (1 << 28)) return fail(DFLASH_ERR_UNSUPPORTED, "gdn rule: tokens * value_heads must be at most 2^28");
     if (!out || !aligned16(out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out is NULL or not 16-byte aligned");
-    (void)workspace, (void)workspace_bytes;
+    if (out == rule->query.data || out == rule->key.data || out == rule->value.data)
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out cannot be the query, key or value, which are read after it is written");
     dflash::RuleParams p = rule_params(rule, pool, pool_params(pool, starts, counts, fresh, tokens));
     p.out = static_cast<uint16_t*>(out);
+    const RuleLayout L = rule_layout(tokens, rule->key_heads, pool->value_heads, pool->head_dim, pool->sequences, longest);
+    if (L.chunks) {
+      if (!workspace || !aligned16(workspace) || workspace_bytes < L.total)
+        return fail(DFLASH_ERR_WORKSPACE, "gdn rule workspace needs " + std::to_string(L.total) + " bytes");
+      dflash::ChunkParams c{};
+      c.rule = p;
+      c.chunks = static_cast<int>(L.chunks);
+      c.t = at<uint16_t>(workspace, L.t);
+      c.p = at<uint16_t>(workspace, L.p);
+      c.kt = at<uint16_t>(workspace, L.kt);
+      c.scalars = at<dflash::ChunkScalars>(workspace, L.scalars);
+      dflash::launch_gdn_chunks(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, c, static_cast<hipStream_t>(stream));
+      return launch_status("gdn rule");
+    }
     dflash::launch_gdn_rule(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
     return launch_status("gdn rule");
   } catch (...) {

@@ -340,6 +340,529 @@ __global__ __launch_bounds__(256) void gdn_advance_kernel(RuleParams p, ConvPara
   store_history<kBf16>(c.pool, s, channel, h, c.x, c.x_stride);
 }
 
+// ------------------------------------------------------------------ the rule, 64 tokens at a time
+// With G the running sum of g in a chunk, r the keys' and q's norms' inverses (q's with the scale) and raw rows k, q, v:
+//   A_ts = beta_t r_t r_s e^{G_t - G_s} k_t.k_s (s < t),   T = (I + A)^-1 diag(beta),
+//   P_ts = rq_t r_s e^{G_t - G_s} q_t.k_s (s <= t),
+//   X = V - diag(e^G r) K S,   U = T X,   O = diag(e^G rq) Q S + P U,   S <- e^{G_64} S + K^T diag(e^{G_64 - G} r) U.
+// T and P do not depend on the state: gdn_chunk_kernel makes them for all chunks at once, and gdn_scan_kernel walks a
+// sequence's chunks with a 16-column slice of the state per workgroup.
+//
+// Precision: the products take 16-bit operands of the matrix cores and sum in fp32.  Raw rows are 16 bits as they are (fp16:
+// two bf16 parts, since states need bf16's range), norms and gates stand beside them as fp32 factors.  What meets them (S, X, U,
+// T) is cut into three bf16 parts, 24 bits, and of their products those above 2^-24 of the whole are taken; for what only an
+// output sees (Q S, P U) two parts, 2^-16, far under the half step that the output is rounded by.  So states come out as from
+// fp32 products, at 2/3 to 1/3 of the 16-bit rate instead of 1/16 of it.
+constexpr int kChunk = 64, kPitch = 68;     // tokens of a chunk; floats of an LDS row
+constexpr int kTriangle = 6;                // 16 x 32 fragments of a lower triangle of 64 x 64
+__device__ __forceinline__ int triangle(int block, int step) { return block < 2 ? block : 2 * block - 2 + step; }
+
+// Chunks of a sequence; and the sequence and chunk of an ordinal (a wave's lanes together), x = B: none; or with `of` >= 0 the
+// chunks of the sequences before that one.
+__device__ __forceinline__ int chunks_of(const PoolParams& p, int b) {
+  const int start = clampi(p.starts[b], 0, p.T);
+  return (clampi(p.starts[b + 1], start, p.T) - start + kChunk - 1) / kChunk;
+}
+__device__ __forceinline__ int2 chunk_place(const PoolParams& p, int ordinal) {
+  int base = 0;
+  for (int i = 0; i < p.B; i += 64) {
+    const int b = i + lane_id();
+    const int own = b < p.B ? chunks_of(p, b) : 0;
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane_id() >= o) sum += v;
+    }
+    const uint64_t over = __ballot(base + sum > ordinal);
+    if (over) {
+      const int lane = __ffsll(static_cast<unsigned long long>(over)) - 1;
+      return make_int2(__builtin_amdgcn_readfirstlane(i + lane),
+                       __builtin_amdgcn_readfirstlane(ordinal - base - (__shfl(sum, lane, 64) - __shfl(own, lane, 64))));
+    }
+    base += __shfl(sum, 63, 64);
+  }
+  return make_int2(p.B, 0);
+}
+__device__ __forceinline__ int chunks_before(const PoolParams& p, int b) {
+  int sum = 0;  // bounded: starts that do not ascend may count a token many times
+  for (int i = lane_id(); i < b; i += 64) sum = min(sum + chunks_of(p, i), 1 << 24);
+  return __builtin_amdgcn_readfirstlane(wave_sum_int(sum));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ f32x4 mfma_rows(uint4 a, uint4 b, f32x4 c) {
+  if constexpr (kBf16) return mfma16x16x32(a, b, c);
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// x as the sum of kParts bf16 numbers, each the rounding of what the ones before leave.
+template <int kParts, int kN>
+__device__ __forceinline__ void cut(const float (&x)[kN], uint32_t (&parts)[kParts][kN / 2]) {
+  float rest[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) rest[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      const uint32_t lo = f32_to_bf16(rest[2 * i]), hi = f32_to_bf16(rest[2 * i + 1]);
+      parts[p][i] = lo | hi << 16;
+      rest[2 * i] -= __uint_as_float(lo << 16);
+      rest[2 * i + 1] -= __uint_as_float(hi << 16);
+    }
+}
+// Eight 16-bit values as bf16 parts: bf16 as they are, fp16 (11 bits) as two.
+template <bool kBf16>
+__device__ __forceinline__ void row_parts(uint4 w, uint4 (&parts)[kBf16 ? 1 : 2]) {
+  if constexpr (kBf16) {
+    parts[0] = w;
+  } else {
+    float f[8];
+    unpack8<false>(w, f);
+    uint32_t c[2][4];
+    cut<2, 8>(f, c);
+    parts[0] = make_uint4(c[0][0], c[0][1], c[0][2], c[0][3]);
+    parts[1] = make_uint4(c[1][0], c[1][1], c[1][2], c[1][3]);
+  }
+}
+
+// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
+  const RuleParams& p = c.rule;
+  constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2;
+  __shared__ __align__(16) float am[kChunk][kPitch], pm[kChunk][kPitch], tm[kChunk][kPitch];
+  __shared__ double gsum[kChunk];
+  __shared__ float beta[kChunk], rk[kChunk], rq[kChunk];
+  static_assert(sizeof(uint16_t) * kChunk * (kDim + 8) <= sizeof(tm), "the keys fit where T will be");
+  uint16_t(*kraw)[kDim + 8] = reinterpret_cast<uint16_t(*)[kDim + 8]>(&tm[0][0]);
+  const int ordinal = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
+  const int2 place = chunk_place(p.pool, ordinal);
+  if (place.x == p.pool.B) return;
+  const Span s = span_of(p.pool, place.x);
+  const int t0 = s.start + place.y * kChunk, n = min(kChunk, s.start + s.tokens - t0);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, quarter = lane >> 4;
+  const int blocks = (n + 15) / 16;  // row blocks that hold tokens
+
+  uint4 kf[4][kSteps], qf[kSteps];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) {
+      const int r = 16 * j + lr;
+      kf[j][m] = make_uint4(0, 0, 0, 0);
+      if (j <= wave && r < n)
+        kf[j][m] = *reinterpret_cast<const uint4*>(p.key + (t0 + r) * p.key_token + khead * p.key_head + 32 * m + 8 * quarter);
+    }
+#pragma unroll
+  for (int m = 0; m < kSteps; ++m) {
+    const int r = 16 * wave + lr;
+    qf[m] = make_uint4(0, 0, 0, 0);
+    if (r < n) qf[m] = *reinterpret_cast<const uint4*>(p.query + (t0 + r) * p.query_token + khead * p.query_head + 32 * m + 8 * quarter);
+  }
+  if (wave == 0) {
+    float2 g = make_float2(0.f, 0.f);
+    if (lane < n) g = gates_of(p, t0 + lane, head);
+    // the running log decay in 64 bits, so that a decay e^{G_t - G_s} is as exact as its own exponent; bounded from below, so
+    // that what stands behind a decay of -infinity keeps its bits (e^-200 is 0 in fp32 all the same)
+    double sum = g.x < -200.0f ? -200.0f : g.x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    gsum[lane] = sum;
+    beta[lane] = g.y;
+  }
+  // norms of this wave's rows, and its keys for the transposed copy
+  float kk = 0.f, qq = 0.f;
+#pragma unroll
+  for (int m = 0; m < kSteps; ++m) {
+    float f[8];
+    uint4 own = kf[0][m];
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+      if (j == wave) own = kf[j][m];
+    unpack8<kBf16>(own, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kk += f[i] * f[i];
+    unpack8<kBf16>(qf[m], f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qq += f[i] * f[i];
+    *reinterpret_cast<uint4*>(&kraw[16 * wave + lr][32 * m + 8 * quarter]) = own;
+  }
+  kk += __shfl_xor(kk, 16, 64);
+  kk += __shfl_xor(kk, 32, 64);
+  qq += __shfl_xor(qq, 16, 64);
+  qq += __shfl_xor(qq, 32, 64);
+  if (quarter == 0) {
+    rk[16 * wave + lr] = p.normalise ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f;
+    rq[16 * wave + lr] = (p.normalise ? 1.0f / sqrtf(qq + 1e-6f) : 1.0f) * p.scale;
+  }
+  __syncthreads();
+
+  // A and P of this wave's rows
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > (wave | 1)) continue;  // never read
+    f32x4 a{0.f, 0.f, 0.f, 0.f}, q{0.f, 0.f, 0.f, 0.f};
+    if (j <= wave) {
+#pragma unroll
+      for (int m = 0; m < kSteps; ++m) {
+        uint4 own = kf[0][m];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+          if (i == wave) own = kf[i][m];
+        a = mfma_rows<kBf16>(own, kf[j][m], a);
+        q = mfma_rows<kBf16>(qf[m], kf[j][m], q);
+      }
+    }
+    const int col = 16 * j + lr;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * wave + 4 * quarter + e;
+      const float decay = col <= row ? expf(static_cast<float>(gsum[row] - gsum[col])) * rk[col] : 0.f;
+      am[row][col] = col < row ? beta[row] * rk[row] * decay * a[e] : 0.f;
+      pm[row][col] = col <= row ? rq[row] * decay * q[e] : 0.f;
+    }
+  }
+  // the keys transposed, once for the value heads that share them
+  const int64_t at = static_cast<int64_t>(ordinal) * p.Hv + head;
+  if (head % p.rep == 0) {
+    uint16_t* to = c.kt + (static_cast<int64_t>(ordinal) * (p.Hv / p.rep) + khead) * (kRowParts * kDim * kChunk);
+    for (int f = wave; f < kDim / 16 * 2; f += 4) {  // fragment: 16 features, 32 tokens
+      uint16_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = kraw[32 * (f & 1) + 8 * quarter + i][16 * (f >> 1) + lr];
+      uint4 parts[kRowParts];
+      row_parts<kBf16>(make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16), parts);
+#pragma unroll
+      for (int i = 0; i < kRowParts; ++i) *reinterpret_cast<uint4*>(to + (i * kDim * kChunk) + (f * 64 + lane) * 8) = parts[i];
+    }
+  }
+  __syncthreads();
+
+  // (I + A)^-1: the diagonal blocks by forward substitution, a column a lane; then block column w on wave w:
+  // T_ij = -T_ii sum_k A_ik T_kj.  A result's registers (rows 4 quarter + e) are the next product's B operand when the sum is
+  // taken in that order.
+  if (lane < 16) {
+    float x[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      float sum0 = t == lr ? 1.f : 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < t; ++i) {
+        const float a = am[16 * wave + t][16 * wave + i];
+        if (i & 1) sum1 -= a * x[i];
+        else sum0 -= a * x[i];
+      }
+      x[t] = sum0 + sum1;
+      tm[16 * wave + t][16 * wave + lr] = x[t];
+    }
+  }
+  __syncthreads();
+  {
+    f32x4 col[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j != wave) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) col[j][e] = tm[16 * j + 4 * quarter + e][16 * j + lr];
+#pragma unroll
+      for (int i = j + 1; i < 4; ++i) {
+        f32x4 sum{0.f, 0.f, 0.f, 0.f}, next{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = j; k < i; ++k) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(&am[16 * i + lr][16 * k + 4 * quarter]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum = mfma16x16x4f32(a[e], col[k][e], sum);
+        }
+        const f32x4 d = *reinterpret_cast<const f32x4*>(&tm[16 * i + lr][16 * i + 4 * quarter]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next = mfma16x16x4f32(d[e], -sum[e], next);
+        col[i] = next;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j != wave) continue;
+#pragma unroll
+      for (int i = j + 1; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tm[16 * i + 4 * quarter + e][16 * j + lr] = col[i][e];
+      if (!(j & 1)) continue;  // above the diagonal in the same fragment
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tm[16 * (j - 1) + 4 * quarter + e][16 * j + lr] = 0.f;
+    }
+  }
+  __syncthreads();
+
+  // as fragments of the scan
+  if (wave < blocks) {
+    const int row = 16 * wave + lr;
+    for (int m = 0; m <= wave / 2; ++m) {
+      const int col = 32 * m + 8 * quarter, f = triangle(wave, m);
+      float x[8], y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = tm[row][col + i] * beta[col + i];
+        y[i] = pm[row][col + i];
+      }
+      uint32_t tp[3][4], pp[2][4];
+      cut<3, 8>(x, tp);
+      cut<2, 8>(y, pp);
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        *reinterpret_cast<uint4*>(c.t + ((at * 3 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(tp[i][0], tp[i][1], tp[i][2], tp[i][3]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint4*>(c.p + ((at * 2 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(pp[i][0], pp[i][1], pp[i][2], pp[i][3]);
+    }
+  }
+  if (tid < kChunk) {
+    ChunkScalars* to = c.scalars + at;
+    const bool in = tid < n;
+    const float head_decay = expf(static_cast<float>(gsum[tid]));
+    to->key[tid] = in ? head_decay * rk[tid] : 0.f;
+    to->query[tid] = head_decay * rq[tid];
+    to->write[tid] = in ? expf(static_cast<float>(gsum[kChunk - 1] - gsum[tid])) * rk[tid] : 0.f;
+    to->norm[tid] = rk[tid];
+    to->total[tid] = gsum[tid];
+  }
+}
+
+// One workgroup per (sequence, value head, 16 columns of the state), the sequence's chunks in turn.  Waves 0 to 3 take X and U
+// of 16 tokens each, waves 4 to 7 the outputs of 16 tokens each, and every wave with 16 w < kDim rows 16 w .. 16 w + 15 of the state.
+// What one wave leaves for the others (S, X, U as bf16 parts in the order of a B operand) goes through LDS, three barriers a chunk;
+// what the chunk kernel left is loaded a chunk ahead, a fragment a load.
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
+  const RuleParams& p = c.rule;
+  constexpr int kSteps = kDim / 32, kTiles = kDim / 16, kSlices = kDim / 16, kRowParts = kBf16 ? 1 : 2;
+  __shared__ __align__(16) uint4 sp[3][kSteps * 64], xp[3][128], wp[3][128], up[2][128];
+  const int group = blockIdx.x / (8 * kSlices), rest = blockIdx.x % (8 * kSlices);
+  const int unit = group * 8 + rest % 8, slice = rest / 8;  // a head's slices on one XCD, which share all but V
+  if (unit >= p.pool.B * p.Hv) return;
+  const int b = unit / p.Hv, head = unit % p.Hv, khead = head / p.rep;
+  const Span s = span_of(p.pool, b);
+  if (s.tokens == 0) return;
+  const int base = chunks_before(p.pool, b), count = min((s.tokens + kChunk - 1) / kChunk, c.chunks - base);
+  if (count <= 0) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int lr = lane & 15, quarter = lane >> 4, block = wave & 3;
+  const bool solves = wave < 4, holds = wave < kTiles;
+  const int col = 16 * slice + lr;
+  float* state = p.pool.recurrent + s.slot * p.pool.recurrent_stride + (static_cast<int64_t>(head) * kDim + 16 * wave + 4 * quarter) * kDim + col;
+  f32x4 st{0.f, 0.f, 0.f, 0.f};
+  if (holds && !s.fresh)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st[e] = state[e * kDim];
+
+  struct Ops {
+    uint4 rows[kSteps];        // K (waves 0 to 3) or Q
+    uint4 mat[3][2];           // T or P
+    uint4 kt[kRowParts][2];
+    f32x4 row_scale, write;    // e^G r or e^G rq; e^{G_64 - G} r
+    uint16_t v[4];
+    float total;               // G of the chunk
+  };
+  auto load = [&](int i, Ops& o) {
+    const int64_t at = static_cast<int64_t>(base + i) * p.Hv + head;
+    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
+    if (16 * block < n) {
+      const int r = t0 + min(16 * block + lr, n - 1);
+      const uint16_t* rows = solves ? p.key + r * p.key_token + khead * p.key_head : p.query + r * p.query_token + khead * p.query_head;
+#pragma unroll
+      for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + 32 * m + 8 * quarter);
+#pragma unroll
+      for (int i3 = 0; i3 < 3; ++i3)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          if (m <= block / 2 && (solves || i3 < 2))
+            o.mat[i3][m] = *reinterpret_cast<const uint4*>(
+                (solves ? c.t + ((at * 3 + i3) * kTriangle + triangle(block, m)) * 512 : c.p + ((at * 2 + i3) * kTriangle + triangle(block, m)) * 512) +
+                lane * 8);
+      const ChunkScalars* f = c.scalars + at;
+      o.row_scale = *reinterpret_cast<const f32x4*>((solves ? f->key : f->query) + 16 * block + 4 * quarter);
+      if (solves) {
+        o.write = *reinterpret_cast<const f32x4*>(f->write + 16 * block + 4 * quarter);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + min(16 * block + 4 * quarter + e, n - 1);
+          o.v[e] = p.value[t * p.value_token + head * p.value_head + col];
+        }
+      }
+    }
+    o.total = static_cast<float>(c.scalars[at].total[kChunk - 1]);
+    if (holds) {
+      const uint16_t* kt = c.kt + (static_cast<int64_t>(base + i) * (p.Hv / p.rep) + khead) * (kRowParts * kDim * kChunk);
+#pragma unroll
+      for (int i3 = 0; i3 < kRowParts; ++i3)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) o.kt[i3][m] = *reinterpret_cast<const uint4*>(kt + i3 * kDim * kChunk + ((2 * wave + m) * 64 + lane) * 8);
+    }
+  };
+  // four values of rows 16 w + 4 quarter .. + 3, this lane's column, as half a B operand's eight
+  auto put = [&](uint4* to, int parts_stride, int parts, const uint32_t (*w)[2], int tile) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < parts)
+        reinterpret_cast<uint2*>(to + i * parts_stride + (2 * tile + (quarter >> 1)) * 16 + lr)[quarter & 1] = make_uint2(w[i][0], w[i][1]);
+  };
+  auto put_state = [&]() {
+    if (!holds) return;
+    const float x[4] = {st[0], st[1], st[2], st[3]};
+    uint32_t w[3][2];
+    cut<3, 4>(x, w);
+    put(&sp[0][0], kSteps * 64, 3, w, wave);
+  };
+  // e^total S + K^T diag(write) U from wp, for the rows that this wave holds
+  auto update = [&](const Ops& o, float total) {
+    const float keep = expf(total);
+    f32x4 sum = keep * st;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      uint4 u[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) u[i] = wp[i][m * 64 + lane];
+#pragma unroll
+      for (int i = 2; i >= 0; --i) {
+        sum = mfma16x16x32(o.kt[0][m], u[i], sum);
+        if (!kBf16 && i < 2) sum = mfma16x16x32(o.kt[kRowParts - 1][m], u[i], sum);
+      }
+    }
+    return sum;
+  };
+
+  auto step = [&](int i, const Ops& o, Ops& next) {
+    if (i + 1 < count) load(i + 1, next);
+    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
+    const bool active = 16 * block < n;
+    // the state before the chunk, where that is what is kept
+    if (holds && i > 0 && s.count == i * kChunk)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[e * kDim] = st[e];
+    lds_barrier();  // sp
+    f32x4 rows{0.f, 0.f, 0.f, 0.f};
+    if (active) {
+#pragma unroll
+      for (int m = 0; m < kSteps; ++m) {
+        uint4 r[kRowParts], x[3];
+        row_parts<kBf16>(o.rows[m], r);
+#pragma unroll
+        for (int i3 = 0; i3 < 3; ++i3)
+          if (i3 < 2 || solves) x[i3] = sp[i3][m * 64 + lane];
+        if (solves) rows = mfma16x16x32(r[0], x[2], rows);
+        if (!kBf16 && solves) rows = mfma16x16x32(r[kRowParts - 1], x[1], rows);
+        rows = mfma16x16x32(r[0], x[1], rows);
+        if (!kBf16) rows = mfma16x16x32(r[kRowParts - 1], x[0], rows);
+        rows = mfma16x16x32(r[0], x[0], rows);
+      }
+    }
+    if (solves) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (active)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = to_f32<kBf16>(o.v[e]) - o.row_scale[e] * rows[e];
+      uint32_t w[3][2];
+      cut<3, 4>(x, w);
+      put(&xp[0][0], 128, 3, w, block);
+    }
+    lds_barrier();  // xp
+    float u[4] = {0.f, 0.f, 0.f, 0.f};
+    if (solves) {
+      if (active) {
+        f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          if (m <= block / 2) {
+            uint4 x[3];
+#pragma unroll
+            for (int i3 = 0; i3 < 3; ++i3) x[i3] = xp[i3][m * 64 + lane];
+            sum = mfma16x16x32(o.mat[2][m], x[0], sum);
+            sum = mfma16x16x32(o.mat[1][m], x[1], sum);
+            sum = mfma16x16x32(o.mat[0][m], x[2], sum);
+            sum = mfma16x16x32(o.mat[1][m], x[0], sum);
+            sum = mfma16x16x32(o.mat[0][m], x[1], sum);
+            sum = mfma16x16x32(o.mat[0][m], x[0], sum);
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = sum[e];
+      }
+      uint32_t w[3][2], v[2][2];
+      const float scaled[4] = {active ? o.write[0] * u[0] : 0.f, active ? o.write[1] * u[1] : 0.f, active ? o.write[2] * u[2] : 0.f,
+                               active ? o.write[3] * u[3] : 0.f};
+      cut<3, 4>(scaled, w);
+      put(&wp[0][0], 128, 3, w, block);
+      cut<2, 4>(u, v);
+      put(&up[0][0], 128, 2, v, block);
+    }
+    lds_barrier();  // wp, up
+    const int part = s.count - i * kChunk;  // tokens of this chunk that the kept state has
+    f32x4 after = st;
+    if (holds) after = update(o, o.total);
+    if (!solves && active) {
+      f32x4 sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = o.row_scale[e] * rows[e];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        if (m <= block / 2) {
+          const uint4 x0 = up[0][m * 64 + lane], x1 = up[1][m * 64 + lane];
+          sum = mfma16x16x32(o.mat[1][m], x0, sum);
+          sum = mfma16x16x32(o.mat[0][m], x1, sum);
+          sum = mfma16x16x32(o.mat[0][m], x0, sum);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * block + 4 * quarter + e;
+        if (r < n) p.out[(static_cast<int64_t>(t0 + r) * p.Hv + head) * kDim + col] = from_f32<kBf16>(sum[e]);
+      }
+    }
+    if (part > 0 && part < n) {
+      // the kept state ends inside this chunk: U once more, with the decays up to its last token
+      const ChunkScalars* f = c.scalars + static_cast<int64_t>(base + i) * p.Hv + head;
+      const double end = f->total[part - 1];
+      lds_barrier();
+      if (solves) {
+        float scaled[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 16 * block + 4 * quarter + e;
+          scaled[e] = r < part ? u[e] * expf(static_cast<float>(end - f->total[r])) * f->norm[r] : 0.f;
+        }
+        uint32_t w[3][2];
+        cut<3, 4>(scaled, w);
+        put(&wp[0][0], 128, 3, w, block);
+      }
+      lds_barrier();
+      if (holds) {
+        const f32x4 kept = update(o, static_cast<float>(end));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) state[e * kDim] = kept[e];
+      }
+    }
+    st = after;
+    put_state();
+  };
+
+  Ops o0, o1;
+  load(0, o0);
+  put_state();
+#pragma unroll 1
+  for (int i = 0; i < count; i += 2) {
+    step(i, o0, o1);
+    if (i + 1 < count) step(i + 1, o1, o0);
+  }
+  if (holds && s.count == s.tokens && s.count > 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) state[e * kDim] = st[e];
+}
+
 }  // namespace
 
 void launch_gdn_conv(bool bf16, const ConvParams& p, hipStream_t stream) {
@@ -354,6 +877,18 @@ void launch_gdn_conv(bool bf16, const ConvParams& p, hipStream_t stream) {
     if (bf16) hipLaunchKernelGGL((gdn_conv_kernel<true, kRows>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((gdn_conv_kernel<false, kRows>), grid, dim3(256), 0, stream, p);
   }
+}
+
+template <bool kBf16, int kDim>
+void launch_chunks(const ChunkParams& c, hipStream_t stream) {
+  const RuleParams& p = c.rule;
+  hipLaunchKernelGGL((gdn_chunk_kernel<kBf16, kDim>), dim3(c.chunks * p.Hv), dim3(256), 0, stream, c);
+  hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim>), dim3((p.pool.B * p.Hv + 7) / 8 * 8 * (kDim / 16)), dim3(512), 0, stream, c);
+}
+
+void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t stream) {
+  if (dim == 128) bf16 ? launch_chunks<true, 128>(c, stream) : launch_chunks<false, 128>(c, stream);
+  else bf16 ? launch_chunks<true, 64>(c, stream) : launch_chunks<false, 64>(c, stream);
 }
 
 void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, hipStream_t stream) {

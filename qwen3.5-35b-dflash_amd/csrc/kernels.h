@@ -441,6 +441,22 @@ struct RuleParams {
   float scale;
   uint16_t* out;                  // [T][Hv][dim]
 };
+// Blocks of many tokens, 64 at a time: what a chunk's tokens need beside their rows, per (chunk, value head).
+constexpr int kRuleChunk = 64;
+struct ChunkScalars {
+  float key[kRuleChunk], query[kRuleChunk];  // e^G / |k|, e^G scale / |q|
+  float write[kRuleChunk], norm[kRuleChunk]; // e^{G_end - G} / |k|, 1 / |k|
+  double total[kRuleChunk];                  // G, the log decay summed up to the token
+};
+struct ChunkParams {
+  RuleParams rule;
+  int chunks;                     // at most: T / 64 + B
+  uint16_t* t;                    // [chunks][Hv][3 parts][6 fragments][64 lanes][8]
+  uint16_t* p;                    // [chunks][Hv][2 parts][6 fragments][64 lanes][8]
+  uint16_t* kt;                   // [chunks][key heads][1 (bf16) or 2 parts][dim / 16][2 fragments][64 lanes][8]
+  ChunkScalars* scalars;          // [chunks][Hv]
+};
+void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t stream);
 void launch_gdn_conv(bool bf16, const ConvParams& p, hipStream_t stream);
 void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, hipStream_t stream);
 void launch_gdn_advance(int dim, bool bf16, const RuleParams& p, const ConvParams& c, hipStream_t stream);

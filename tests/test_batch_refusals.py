@@ -65,7 +65,7 @@ def test_bad_histories_and_states(pkg):
         refused(lib, _conv, message, pool=_pool(lib, **change))
         refused(lib, _advance, message, pool=_pool(lib, **change))
     for change, message in [(dict(head_dim=96), "head_dim"), (dict(head_dim=256), "head_dim"), (dict(value_heads=0), "value_heads"),
-                            (dict(value_heads=1025), "value_heads"), (dict(sequences=1 << 20, value_heads=8), "2\\^22"),
+                            (dict(value_heads=1025), "value_heads"), (dict(sequences=1 << 19, value_heads=8), "2\\^19"),
                             (dict(recurrent=None), "recurrent"), (dict(recurrent=ADDRESS + 4), "recurrent"),
                             (dict(recurrent_stride=6), "multiple of 4"), (dict(recurrent_stride=-4), "multiple of 4")]:
         refused(lib, _delta, message, pool=_pool(lib, **change))
@@ -96,7 +96,8 @@ def test_rule_refusals(pkg):
         refused(lib, _advance, message, rule=_rule(lib, **change))
     for kw, message in [(dict(rule=0), "NULL"), (dict(rule=_rule(lib, query=_rows(lib, None))), "query"), (dict(starts=None), "starts"),
                         (dict(tokens=-1), "2\\^20"), (dict(tokens=1 << 62), "2\\^20"), (dict(longest=-1), "longest"), (dict(out=None), "out"),
-                        (dict(out=ADDRESS + 8), "out")]:
+                        (dict(out=ADDRESS + 8), "out"), (dict(out=ADDRESS), "out cannot be"), (dict(tokens=500, ws=None), "workspace"),
+                        (dict(tokens=500, ws=ADDRESS + 8), "workspace"), (dict(longest=17, tokens=17, size=100), "workspace"), (dict(tokens=1 << 20, pool=_pool(lib, value_heads=512)), "2\\^28")]:
         refused(lib, _delta, message, **kw)
     for kw, message in [(dict(rule=0), "NULL"), (dict(counts=None), "counts"), (dict(starts=None), "starts"),
                         (dict(x=_rows(lib, ADDRESS + 2)), "x"), (dict(tokens=1 << 21), "2\\^20")]:
