@@ -1449,7 +1449,7 @@ constexpr int64_t kRuleSteps = 16;
 
 struct RuleLayout {
   int64_t chunks;  // 0: token after token, without a workspace
-  size_t t, p, kt, scalars, total;
+  size_t rows, v, t, p, kt, scalars, total;
 };
 bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
   return T >= 0 && T <= (1 << 20) && Hk > 0 && Hv > 0 && Hv <= 1024 && Hv % Hk == 0 && (D == 64 || D == 128) && B >= 0 && B <= (1 << 20) &&
@@ -1463,6 +1463,8 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   L.chunks = T / dflash::kRuleChunk + std::min(T, B);
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
+  L.rows = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
+  L.v = c.take(each * 2 * D * dflash::kRuleChunk);
   L.t = c.take(each * 3 * part);
   L.p = c.take(each * 2 * part);
   L.kt = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
@@ -1500,6 +1502,9 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
       dflash::ChunkParams c{};
       c.rule = p;
       c.chunks = static_cast<int>(L.chunks);
+      c.cus = cu_count();
+      c.rows = at<uint16_t>(workspace, L.rows);
+      c.v = at<uint16_t>(workspace, L.v);
       c.t = at<uint16_t>(workspace, L.t);
       c.p = at<uint16_t>(workspace, L.p);
       c.kt = at<uint16_t>(workspace, L.kt);

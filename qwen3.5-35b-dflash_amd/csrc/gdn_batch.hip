@@ -407,10 +407,11 @@ __device__ __forceinline__ void cut(const float (&x)[kN], uint32_t (&parts)[kPar
   for (int p = 0; p < kParts; ++p)
 #pragma unroll
     for (int i = 0; i < kN / 2; ++i) {
-      const uint32_t lo = f32_to_bf16(rest[2 * i]), hi = f32_to_bf16(rest[2 * i + 1]);
-      parts[p][i] = lo | hi << 16;
-      rest[2 * i] -= __uint_as_float(lo << 16);
-      rest[2 * i + 1] -= __uint_as_float(hi << 16);
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      parts[p][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{rest[2 * i], rest[2 * i + 1]}, bf16x2));
+      rest[2 * i] -= __uint_as_float(parts[p][i] << 16);
+      rest[2 * i + 1] -= __uint_as_float(parts[p][i] & 0xFFFF0000u);
     }
 }
 // Eight 16-bit values as bf16 parts: bf16 as they are, fp16 (11 bits) as two.
@@ -428,16 +429,23 @@ __device__ __forceinline__ void row_parts(uint4 w, uint4 (&parts)[kBf16 ? 1 : 2]
   }
 }
 
-// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices.
+// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices.  Rows come in whole (256 bytes a
+// load of 16 lanes) and pass through LDS: what the scan reads eight times over, once a slice, it finds in the order of
+// its operands, 1 KB a load (rows read straight into operands cost a cache line a lane).
 template <bool kBf16, int kDim>
 __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
   const RuleParams& p = c.rule;
-  constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2;
-  __shared__ __align__(16) float am[kChunk][kPitch], pm[kChunk][kPitch], tm[kChunk][kPitch];
+  constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2, kRaw = kDim + 8;
+  union Shared {
+    uint16_t raw[kChunk][kRaw];
+    float f[kChunk][kPitch];
+  };
+  __shared__ __align__(16) Shared keys_t, query_p, value_a;  // first the rows, then T, P and A
   __shared__ double gsum[kChunk];
   __shared__ float beta[kChunk], rk[kChunk], rq[kChunk];
-  static_assert(sizeof(uint16_t) * kChunk * (kDim + 8) <= sizeof(tm), "the keys fit where T will be");
-  uint16_t(*kraw)[kDim + 8] = reinterpret_cast<uint16_t(*)[kDim + 8]>(&tm[0][0]);
+  auto& tm = keys_t.f;
+  auto& pm = query_p.f;
+  auto& am = value_a.f;
   const int ordinal = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
   const int2 place = chunk_place(p.pool, ordinal);
   if (place.x == p.pool.B) return;
@@ -446,101 +454,121 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lr = lane & 15, quarter = lane >> 4;
   const int blocks = (n + 15) / 16;  // row blocks that hold tokens
+  const int64_t at = static_cast<int64_t>(ordinal) * p.Hv + head;
 
-  uint4 kf[4][kSteps], qf[kSteps];
+  {
+    constexpr int kLanes = kDim / 8, kRows = 256 / kLanes;  // lanes a row, rows a pass
+    const int r0 = tid / kLanes, d = tid % kLanes * 8;
+    uint4 k[kChunk / kRows], q[kChunk / kRows], v[kChunk / kRows];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < kChunk / kRows; ++i) {
+      const int r = r0 + i * kRows;
+      const int64_t t = t0 + min(r, n - 1);
+      k[i] = *reinterpret_cast<const uint4*>(p.key + t * p.key_token + khead * p.key_head + d);
+      q[i] = *reinterpret_cast<const uint4*>(p.query + t * p.query_token + khead * p.query_head + d);
+      v[i] = *reinterpret_cast<const uint4*>(p.value + t * p.value_token + head * p.value_head + d);
+    }
+    if (wave == 0) {
+      float2 g = make_float2(0.f, 0.f);
+      if (lane < n) g = gates_of(p, t0 + lane, head);
+      // the running log decay in 64 bits, so that a decay e^{G_t - G_s} is as exact as its own exponent; bounded from below, so
+      // that what stands behind a decay of -infinity keeps its bits (e^-200 is 0 in fp32 all the same)
+      double sum = g.x < -200.0f ? -200.0f : g.x;
 #pragma unroll
-    for (int m = 0; m < kSteps; ++m) {
-      const int r = 16 * j + lr;
-      kf[j][m] = make_uint4(0, 0, 0, 0);
-      if (j <= wave && r < n)
-        kf[j][m] = *reinterpret_cast<const uint4*>(p.key + (t0 + r) * p.key_token + khead * p.key_head + 32 * m + 8 * quarter);
+      for (int o = 1; o < 64; o <<= 1) {
+        const double x = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += x;
+      }
+      gsum[lane] = sum;
+      beta[lane] = g.y;
     }
 #pragma unroll
-  for (int m = 0; m < kSteps; ++m) {
-    const int r = 16 * wave + lr;
-    qf[m] = make_uint4(0, 0, 0, 0);
-    if (r < n) qf[m] = *reinterpret_cast<const uint4*>(p.query + (t0 + r) * p.query_token + khead * p.query_head + 32 * m + 8 * quarter);
-  }
-  if (wave == 0) {
-    float2 g = make_float2(0.f, 0.f);
-    if (lane < n) g = gates_of(p, t0 + lane, head);
-    // the running log decay in 64 bits, so that a decay e^{G_t - G_s} is as exact as its own exponent; bounded from below, so
-    // that what stands behind a decay of -infinity keeps its bits (e^-200 is 0 in fp32 all the same)
-    double sum = g.x < -200.0f ? -200.0f : g.x;
+    for (int i = 0; i < kChunk / kRows; ++i) {
+      const int r = r0 + i * kRows;
+      if (r >= n) k[i] = q[i] = v[i] = make_uint4(0, 0, 0, 0);
+      float f[8], kk = 0.f, qq = 0.f;
+      unpack8<kBf16>(k[i], f);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double v = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += v;
+      for (int e = 0; e < 8; ++e) kk += f[e] * f[e];
+      unpack8<kBf16>(q[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qq += f[e] * f[e];
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) {
+        kk += __shfl_xor(kk, o, 64);
+        qq += __shfl_xor(qq, o, 64);
+      }
+      if (d == 0) {
+        rk[r] = p.normalise ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f;
+        rq[r] = (p.normalise ? 1.0f / sqrtf(qq + 1e-6f) : 1.0f) * p.scale;
+      }
+      *reinterpret_cast<uint4*>(&keys_t.raw[r][d]) = k[i];
+      *reinterpret_cast<uint4*>(&query_p.raw[r][d]) = q[i];
+      *reinterpret_cast<uint4*>(&value_a.raw[r][d]) = v[i];
     }
-    gsum[lane] = sum;
-    beta[lane] = g.y;
-  }
-  // norms of this wave's rows, and its keys for the transposed copy
-  float kk = 0.f, qq = 0.f;
-#pragma unroll
-  for (int m = 0; m < kSteps; ++m) {
-    float f[8];
-    uint4 own = kf[0][m];
-#pragma unroll
-    for (int j = 1; j < 4; ++j)
-      if (j == wave) own = kf[j][m];
-    unpack8<kBf16>(own, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) kk += f[i] * f[i];
-    unpack8<kBf16>(qf[m], f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qq += f[i] * f[i];
-    *reinterpret_cast<uint4*>(&kraw[16 * wave + lr][32 * m + 8 * quarter]) = own;
-  }
-  kk += __shfl_xor(kk, 16, 64);
-  kk += __shfl_xor(kk, 32, 64);
-  qq += __shfl_xor(qq, 16, 64);
-  qq += __shfl_xor(qq, 32, 64);
-  if (quarter == 0) {
-    rk[16 * wave + lr] = p.normalise ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f;
-    rq[16 * wave + lr] = (p.normalise ? 1.0f / sqrtf(qq + 1e-6f) : 1.0f) * p.scale;
   }
   __syncthreads();
 
-  // A and P of this wave's rows
+  // A and P of this wave's rows, without their factors
+  f32x4 a[4], q[4];
+  uint4 own_k[kSteps], own_q[kSteps];
+#pragma unroll
+  for (int m = 0; m < kSteps; ++m) {
+    own_k[m] = *reinterpret_cast<const uint4*>(&keys_t.raw[16 * wave + lr][32 * m + 8 * quarter]);
+    own_q[m] = *reinterpret_cast<const uint4*>(&query_p.raw[16 * wave + lr][32 * m + 8 * quarter]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    a[j] = q[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (j <= wave)
+#pragma unroll
+      for (int m = 0; m < kSteps; ++m) {
+        const uint4 k = *reinterpret_cast<const uint4*>(&keys_t.raw[16 * j + lr][32 * m + 8 * quarter]);
+        a[j] = mfma_rows<kBf16>(own_k[m], k, a[j]);
+        q[j] = mfma_rows<kBf16>(own_q[m], k, q[j]);
+      }
+  }
+  // the rows as operands: keys and queries, and the keys transposed, once for the value heads that share them
+  if (head % p.rep == 0) {
+    uint16_t* to = c.rows + (static_cast<int64_t>(ordinal) * (p.Hv / p.rep) + khead) * (2 * kDim * kChunk) + lane * 8;
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) {
+      *reinterpret_cast<uint4*>(to + (wave * kSteps + m) * 512) = own_k[m];
+      *reinterpret_cast<uint4*>(to + kDim * kChunk + (wave * kSteps + m) * 512) = own_q[m];
+    }
+    to = c.kt + (static_cast<int64_t>(ordinal) * (p.Hv / p.rep) + khead) * (kRowParts * kDim * kChunk) + lane * 8;
+    for (int f = wave; f < kDim / 16 * 2; f += 4) {  // fragment: 16 features, 32 tokens
+      uint16_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = keys_t.raw[32 * (f & 1) + 8 * quarter + i][16 * (f >> 1) + lr];
+      uint4 parts[kRowParts];
+      row_parts<kBf16>(make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16), parts);
+#pragma unroll
+      for (int i = 0; i < kRowParts; ++i) *reinterpret_cast<uint4*>(to + i * kDim * kChunk + f * 512) = parts[i];
+    }
+  }
+  {
+    // the values in the order of a result: rows 4 quarter + e of a row block, column lr of a slice
+    uint16_t* to = c.v + at * (kDim * kChunk) + lane * 4;
+#pragma unroll
+    for (int i = 0; i < kDim / 16; ++i) {
+      uint16_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = value_a.raw[16 * wave + 4 * quarter + e][16 * i + lr];
+      *reinterpret_cast<uint2*>(to + (i * 4 + wave) * 256) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    }
+  }
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (j > (wave | 1)) continue;  // never read
-    f32x4 a{0.f, 0.f, 0.f, 0.f}, q{0.f, 0.f, 0.f, 0.f};
-    if (j <= wave) {
-#pragma unroll
-      for (int m = 0; m < kSteps; ++m) {
-        uint4 own = kf[0][m];
-#pragma unroll
-        for (int i = 1; i < 4; ++i)
-          if (i == wave) own = kf[i][m];
-        a = mfma_rows<kBf16>(own, kf[j][m], a);
-        q = mfma_rows<kBf16>(qf[m], kf[j][m], q);
-      }
-    }
     const int col = 16 * j + lr;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = 16 * wave + 4 * quarter + e;
-      const float decay = col <= row ? expf(static_cast<float>(gsum[row] - gsum[col])) * rk[col] : 0.f;
-      am[row][col] = col < row ? beta[row] * rk[row] * decay * a[e] : 0.f;
-      pm[row][col] = col <= row ? rq[row] * decay * q[e] : 0.f;
-    }
-  }
-  // the keys transposed, once for the value heads that share them
-  const int64_t at = static_cast<int64_t>(ordinal) * p.Hv + head;
-  if (head % p.rep == 0) {
-    uint16_t* to = c.kt + (static_cast<int64_t>(ordinal) * (p.Hv / p.rep) + khead) * (kRowParts * kDim * kChunk);
-    for (int f = wave; f < kDim / 16 * 2; f += 4) {  // fragment: 16 features, 32 tokens
-      uint16_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = kraw[32 * (f & 1) + 8 * quarter + i][16 * (f >> 1) + lr];
-      uint4 parts[kRowParts];
-      row_parts<kBf16>(make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16), parts);
-#pragma unroll
-      for (int i = 0; i < kRowParts; ++i) *reinterpret_cast<uint4*>(to + (i * kDim * kChunk) + (f * 64 + lane) * 8) = parts[i];
+      const float decay = col <= row ? __expf(static_cast<float>(gsum[row] - gsum[col])) * rk[col] : 0.f;
+      am[row][col] = col < row ? beta[row] * rk[row] * decay * a[j][e] : 0.f;
+      pm[row][col] = col <= row ? rq[row] * decay * q[j][e] : 0.f;
     }
   }
   __syncthreads();
@@ -555,53 +583,44 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
       float sum0 = t == lr ? 1.f : 0.f, sum1 = 0.f;
 #pragma unroll
       for (int i = 0; i < t; ++i) {
-        const float a = am[16 * wave + t][16 * wave + i];
-        if (i & 1) sum1 -= a * x[i];
-        else sum0 -= a * x[i];
+        const float f = am[16 * wave + t][16 * wave + i];
+        if (i & 1) sum1 -= f * x[i];
+        else sum0 -= f * x[i];
       }
       x[t] = sum0 + sum1;
       tm[16 * wave + t][16 * wave + lr] = x[t];
     }
   }
   __syncthreads();
-  {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j != wave) continue;
     f32x4 col[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j != wave) continue;
+    for (int e = 0; e < 4; ++e) col[j][e] = tm[16 * j + 4 * quarter + e][16 * j + lr];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) col[j][e] = tm[16 * j + 4 * quarter + e][16 * j + lr];
+    for (int i = j + 1; i < 4; ++i) {
+      f32x4 sum{0.f, 0.f, 0.f, 0.f}, next{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = j + 1; i < 4; ++i) {
-        f32x4 sum{0.f, 0.f, 0.f, 0.f}, next{0.f, 0.f, 0.f, 0.f};
+      for (int k = j; k < i; ++k) {
+        const f32x4 f = *reinterpret_cast<const f32x4*>(&am[16 * i + lr][16 * k + 4 * quarter]);
 #pragma unroll
-        for (int k = j; k < i; ++k) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(&am[16 * i + lr][16 * k + 4 * quarter]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum = mfma16x16x4f32(a[e], col[k][e], sum);
-        }
-        const f32x4 d = *reinterpret_cast<const f32x4*>(&tm[16 * i + lr][16 * i + 4 * quarter]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) next = mfma16x16x4f32(d[e], -sum[e], next);
-        col[i] = next;
+        for (int e = 0; e < 4; ++e) sum = mfma16x16x4f32(f[e], col[k][e], sum);
       }
+      const f32x4 d = *reinterpret_cast<const f32x4*>(&tm[16 * i + lr][16 * i + 4 * quarter]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) next = mfma16x16x4f32(d[e], -sum[e], next);
+      col[i] = next;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tm[16 * i + 4 * quarter + e][16 * j + lr] = next[e];
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j != wave) continue;
-#pragma unroll
-      for (int i = j + 1; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) tm[16 * i + 4 * quarter + e][16 * j + lr] = col[i][e];
-      if (!(j & 1)) continue;  // above the diagonal in the same fragment
+    if (j & 1)  // above the diagonal in the same fragment
 #pragma unroll
       for (int e = 0; e < 4; ++e) tm[16 * (j - 1) + 4 * quarter + e][16 * j + lr] = 0.f;
-    }
   }
   __syncthreads();
 
-  // as fragments of the scan
+  // T and P as operands
   if (wave < blocks) {
     const int row = 16 * wave + lr;
     for (int m = 0; m <= wave / 2; ++m) {
@@ -632,235 +651,351 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
     to->write[tid] = in ? expf(static_cast<float>(gsum[kChunk - 1] - gsum[tid])) * rk[tid] : 0.f;
     to->norm[tid] = rk[tid];
     to->total[tid] = gsum[tid];
+    if (tid == 0) to->keep = expf(static_cast<float>(gsum[kChunk - 1]));
   }
 }
 
-// One workgroup per (sequence, value head, 16 columns of the state), the sequence's chunks in turn.  Waves 0 to 3 take X and U
-// of 16 tokens each, waves 4 to 7 the outputs of 16 tokens each, and every wave with 16 w < kDim rows 16 w .. 16 w + 15 of the state.
-// What one wave leaves for the others (S, X, U as bf16 parts in the order of a B operand) goes through LDS, three barriers a chunk;
-// what the chunk kernel left is loaded a chunk ahead, a fragment a load.
-template <bool kBf16, int kDim>
-__global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
+// What the waves of gdn_scan_kernel leave for one another: S, X, U times its writes' decays, and U (of this chunk and the one before),
+// as bf16 parts in the order of a B operand, per 16 columns.
+template <int kDim, int kTiles>
+struct ScanShared {
+  uint4 state[kTiles][3][kDim * 2], x[kTiles][3][128], write[kTiles][3][128], u[2][kTiles][2][128];
+};
+// Four values of rows 16 tile + 4 quarter .. + 3 and a lane's column: half of a B operand's eight, per part.
+template <int kParts>
+__device__ __forceinline__ void put_parts(uint4* to, int part_stride, const float (&x)[4], int tile) {
+  const int lane = lane_id(), lr = lane & 15, quarter = lane >> 4;
+  uint32_t w[kParts][2];
+  cut<kParts, 4>(x, w);
+#pragma unroll
+  for (int i = 0; i < kParts; ++i)
+    reinterpret_cast<uint2*>(to + i * part_stride + (2 * tile + (quarter >> 1)) * 16 + lr)[quarter & 1] = make_uint2(w[i][0], w[i][1]);
+}
+
+// The chunk's place in a walk over a sequence.
+struct ScanWalk {
+  int base, count, head, slice;
+};
+
+// Waves 0 to 3 of gdn_scan_kernel: X and U of 16 tokens.  In both kinds of waves loads stand in no branch but a first one (indices
+// are bounded instead) and nothing is computed from them before they are needed, so that those of the two chunks ahead stay in flight.
+template <bool kBf16, int kDim, int kTiles>
+__device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, const ScanWalk& w, int block, ScanShared<kDim, kTiles>& lds) {
   const RuleParams& p = c.rule;
-  constexpr int kSteps = kDim / 32, kTiles = kDim / 16, kSlices = kDim / 16, kRowParts = kBf16 ? 1 : 2;
-  __shared__ __align__(16) uint4 sp[3][kSteps * 64], xp[3][128], wp[3][128], up[2][128];
-  const int group = blockIdx.x / (8 * kSlices), rest = blockIdx.x % (8 * kSlices);
-  const int unit = group * 8 + rest % 8, slice = rest / 8;  // a head's slices on one XCD, which share all but V
-  if (unit >= p.pool.B * p.Hv) return;
-  const int b = unit / p.Hv, head = unit % p.Hv, khead = head / p.rep;
-  const Span s = span_of(p.pool, b);
-  if (s.tokens == 0) return;
-  const int base = chunks_before(p.pool, b), count = min((s.tokens + kChunk - 1) / kChunk, c.chunks - base);
-  if (count <= 0) return;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int lr = lane & 15, quarter = lane >> 4, block = wave & 3;
-  const bool solves = wave < 4, holds = wave < kTiles;
-  const int col = 16 * slice + lr;
-  float* state = p.pool.recurrent + s.slot * p.pool.recurrent_stride + (static_cast<int64_t>(head) * kDim + 16 * wave + 4 * quarter) * kDim + col;
-  f32x4 st{0.f, 0.f, 0.f, 0.f};
-  if (holds && !s.fresh)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) st[e] = state[e * kDim];
-
+  constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2;
+  const int lane = lane_id(), quarter = lane >> 4, khead = w.head / p.rep, last = w.count - 1;
   struct Ops {
-    uint4 rows[kSteps];        // K (waves 0 to 3) or Q
-    uint4 mat[3][2];           // T or P
-    uint4 kt[kRowParts][2];
-    f32x4 row_scale, write;    // e^G r or e^G rq; e^{G_64 - G} r
-    uint16_t v[4];
-    float total;               // G of the chunk
+    uint4 rows[kSteps], mat[3][2];  // K, T
+    f32x4 scale, write;             // e^G r, e^{G_64 - G} r
+    uint2 v[kTiles];
   };
-  auto load = [&](int i, Ops& o) {
-    const int64_t at = static_cast<int64_t>(base + i) * p.Hv + head;
-    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
-    if (16 * block < n) {
-      const int r = t0 + min(16 * block + lr, n - 1);
-      const uint16_t* rows = solves ? p.key + r * p.key_token + khead * p.key_head : p.query + r * p.query_token + khead * p.query_head;
+  const auto load = [&](int i, Ops& o) {
+    const int64_t at = static_cast<int64_t>(w.base + i) * p.Hv + w.head;
+    const uint16_t* mat = c.t + at * (3 * kTriangle * 512) + triangle(block, 0) * 512 + lane * 8;
+    if (block > 1)
 #pragma unroll
-      for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + 32 * m + 8 * quarter);
+      for (int i3 = 0; i3 < 3; ++i3) o.mat[i3][1] = *reinterpret_cast<const uint4*>(mat + (i3 * kTriangle + 1) * 512);
 #pragma unroll
-      for (int i3 = 0; i3 < 3; ++i3)
+    for (int i3 = 0; i3 < 3; ++i3) o.mat[i3][0] = *reinterpret_cast<const uint4*>(mat + i3 * kTriangle * 512);
+    const uint16_t* rows = c.rows + (static_cast<int64_t>(w.base + i) * (p.Hv / p.rep) + khead) * (2 * kDim * kChunk) + block * (kSteps * 512) + lane * 8;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-          if (m <= block / 2 && (solves || i3 < 2))
-            o.mat[i3][m] = *reinterpret_cast<const uint4*>(
-                (solves ? c.t + ((at * 3 + i3) * kTriangle + triangle(block, m)) * 512 : c.p + ((at * 2 + i3) * kTriangle + triangle(block, m)) * 512) +
-                lane * 8);
-      const ChunkScalars* f = c.scalars + at;
-      o.row_scale = *reinterpret_cast<const f32x4*>((solves ? f->key : f->query) + 16 * block + 4 * quarter);
-      if (solves) {
-        o.write = *reinterpret_cast<const f32x4*>(f->write + 16 * block + 4 * quarter);
+    for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + m * 512);
+    const ChunkScalars* f = c.scalars + at;
+    o.scale = *reinterpret_cast<const f32x4*>(f->key + 16 * block + 4 * quarter);
+    o.write = *reinterpret_cast<const f32x4*>(f->write + 16 * block + 4 * quarter);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = t0 + min(16 * block + 4 * quarter + e, n - 1);
-          o.v[e] = p.value[t * p.value_token + head * p.value_head + col];
-        }
-      }
-    }
-    o.total = static_cast<float>(c.scalars[at].total[kChunk - 1]);
-    if (holds) {
-      const uint16_t* kt = c.kt + (static_cast<int64_t>(base + i) * (p.Hv / p.rep) + khead) * (kRowParts * kDim * kChunk);
-#pragma unroll
-      for (int i3 = 0; i3 < kRowParts; ++i3)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) o.kt[i3][m] = *reinterpret_cast<const uint4*>(kt + i3 * kDim * kChunk + ((2 * wave + m) * 64 + lane) * 8);
-    }
+    for (int x = 0; x < kTiles; ++x)
+      o.v[x] = *reinterpret_cast<const uint2*>(c.v + at * (kDim * kChunk) + ((kTiles * w.slice + x) * 4 + block) * 256 + lane * 4);
   };
-  // four values of rows 16 w + 4 quarter .. + 3, this lane's column, as half a B operand's eight
-  auto put = [&](uint4* to, int parts_stride, int parts, const uint32_t (*w)[2], int tile) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < parts)
-        reinterpret_cast<uint2*>(to + i * parts_stride + (2 * tile + (quarter >> 1)) * 16 + lr)[quarter & 1] = make_uint2(w[i][0], w[i][1]);
-  };
-  auto put_state = [&]() {
-    if (!holds) return;
-    const float x[4] = {st[0], st[1], st[2], st[3]};
-    uint32_t w[3][2];
-    cut<3, 4>(x, w);
-    put(&sp[0][0], kSteps * 64, 3, w, wave);
-  };
-  // e^total S + K^T diag(write) U from wp, for the rows that this wave holds
-  auto update = [&](const Ops& o, float total) {
-    const float keep = expf(total);
-    f32x4 sum = keep * st;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      uint4 u[3];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) u[i] = wp[i][m * 64 + lane];
-#pragma unroll
-      for (int i = 2; i >= 0; --i) {
-        sum = mfma16x16x32(o.kt[0][m], u[i], sum);
-        if (!kBf16 && i < 2) sum = mfma16x16x32(o.kt[kRowParts - 1][m], u[i], sum);
-      }
-    }
-    return sum;
-  };
-
-  auto step = [&](int i, const Ops& o, Ops& next) {
-    if (i + 1 < count) load(i + 1, next);
-    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
+  const auto step = [&](int i, Ops& o) {
+    const int n = min(kChunk, s.tokens - i * kChunk);
     const bool active = 16 * block < n;
-    // the state before the chunk, where that is what is kept
-    if (holds && i > 0 && s.count == i * kChunk)
+    lds_barrier();  // the state's parts are there
 #pragma unroll
-      for (int e = 0; e < 4; ++e) state[e * kDim] = st[e];
-    lds_barrier();  // sp
-    f32x4 rows{0.f, 0.f, 0.f, 0.f};
-    if (active) {
-#pragma unroll
-      for (int m = 0; m < kSteps; ++m) {
-        uint4 r[kRowParts], x[3];
-        row_parts<kBf16>(o.rows[m], r);
-#pragma unroll
-        for (int i3 = 0; i3 < 3; ++i3)
-          if (i3 < 2 || solves) x[i3] = sp[i3][m * 64 + lane];
-        if (solves) rows = mfma16x16x32(r[0], x[2], rows);
-        if (!kBf16 && solves) rows = mfma16x16x32(r[kRowParts - 1], x[1], rows);
-        rows = mfma16x16x32(r[0], x[1], rows);
-        if (!kBf16) rows = mfma16x16x32(r[kRowParts - 1], x[0], rows);
-        rows = mfma16x16x32(r[0], x[0], rows);
-      }
-    }
-    if (solves) {
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (active)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = to_f32<kBf16>(o.v[e]) - o.row_scale[e] * rows[e];
-      uint32_t w[3][2];
-      cut<3, 4>(x, w);
-      put(&xp[0][0], 128, 3, w, block);
-    }
-    lds_barrier();  // xp
-    float u[4] = {0.f, 0.f, 0.f, 0.f};
-    if (solves) {
+    for (int x = 0; x < kTiles; ++x) {
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
       if (active) {
-        f32x4 sum{0.f, 0.f, 0.f, 0.f};
+        f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+          uint4 r[kRowParts], st[3];
+          row_parts<kBf16>(o.rows[m], r);
+#pragma unroll
+          for (int i3 = 0; i3 < 3; ++i3) st[i3] = lds.state[x][i3][m * 64 + lane];
+#pragma unroll
+          for (int i3 = 2; i3 >= 0; --i3) {
+            if (!kBf16 && i3 < 2) sum[m & 1] = mfma16x16x32(r[kRowParts - 1], st[i3], sum[m & 1]);
+            sum[m & 1] = mfma16x16x32(r[0], st[i3], sum[m & 1]);
+          }
+        }
+        const uint16_t v[4] = {static_cast<uint16_t>(o.v[x].x), static_cast<uint16_t>(o.v[x].x >> 16), static_cast<uint16_t>(o.v[x].y),
+                               static_cast<uint16_t>(o.v[x].y >> 16)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = to_f32<kBf16>(v[e]) - o.scale[e] * (sum[0][e] + sum[1][e]);
+      }
+      put_parts<3>(lds.x[x][0], 128, f, block);
+    }
+    lds_barrier();  // X is there
+    float u[kTiles][4];
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) {
+      float scaled[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[x][e] = 0.f;
+      if (active) {
+        f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int m = 0; m < 2; ++m)
           if (m <= block / 2) {
-            uint4 x[3];
+            uint4 f[3];
 #pragma unroll
-            for (int i3 = 0; i3 < 3; ++i3) x[i3] = xp[i3][m * 64 + lane];
-            sum = mfma16x16x32(o.mat[2][m], x[0], sum);
-            sum = mfma16x16x32(o.mat[1][m], x[1], sum);
-            sum = mfma16x16x32(o.mat[0][m], x[2], sum);
-            sum = mfma16x16x32(o.mat[1][m], x[0], sum);
-            sum = mfma16x16x32(o.mat[0][m], x[1], sum);
-            sum = mfma16x16x32(o.mat[0][m], x[0], sum);
+            for (int i3 = 0; i3 < 3; ++i3) f[i3] = lds.x[x][i3][m * 64 + lane];
+            sum[0] = mfma16x16x32(o.mat[2][m], f[0], sum[0]);
+            sum[1] = mfma16x16x32(o.mat[1][m], f[1], sum[1]);
+            sum[0] = mfma16x16x32(o.mat[0][m], f[2], sum[0]);
+            sum[1] = mfma16x16x32(o.mat[1][m], f[0], sum[1]);
+            sum[0] = mfma16x16x32(o.mat[0][m], f[1], sum[0]);
+            sum[1] = mfma16x16x32(o.mat[0][m], f[0], sum[1]);
           }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = sum[e];
+        for (int e = 0; e < 4; ++e) {
+          u[x][e] = sum[0][e] + sum[1][e];
+          scaled[e] = o.write[e] * u[x][e];
+        }
       }
-      uint32_t w[3][2], v[2][2];
-      const float scaled[4] = {active ? o.write[0] * u[0] : 0.f, active ? o.write[1] * u[1] : 0.f, active ? o.write[2] * u[2] : 0.f,
-                               active ? o.write[3] * u[3] : 0.f};
-      cut<3, 4>(scaled, w);
-      put(&wp[0][0], 128, 3, w, block);
-      cut<2, 4>(u, v);
-      put(&up[0][0], 128, 2, v, block);
+      put_parts<3>(lds.write[x][0], 128, scaled, block);
     }
-    lds_barrier();  // wp, up
-    const int part = s.count - i * kChunk;  // tokens of this chunk that the kept state has
-    f32x4 after = st;
-    if (holds) after = update(o, o.total);
-    if (!solves && active) {
-      f32x4 sum;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = o.row_scale[e] * rows[e];
+    for (int x = 0; x < kTiles; ++x) put_parts<2>(lds.u[i & 1][x][0], 128, u[x], block);
+    lds_barrier();  // U is there
+    const int part = s.count - i * kChunk;
+    if (part > 0 && part < n) {
+      // the kept state ends inside this chunk: U once more, with the decays up to its last token
+      const ChunkScalars* f = c.scalars + static_cast<int64_t>(w.base + i) * p.Hv + w.head;
+      const double end = f->total[part - 1];
+      float factor[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * block + 4 * quarter + e;
+        factor[e] = r < part ? expf(static_cast<float>(end - f->total[r])) * f->norm[r] : 0.f;
+      }
+      lds_barrier();  // the whole chunk's is taken
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        const float scaled[4] = {factor[0] * u[x][0], factor[1] * u[x][1], factor[2] * u[x][2], factor[3] * u[x][3]};
+        put_parts<3>(lds.write[x][0], 128, scaled, block);
+      }
+      lds_barrier();
+    }
+    load(min(i + 2, last), o);
+  };
+  Ops o0, o1;
+  load(0, o0);
+  load(min(1, last), o1);
+  wait_vmem();  // so that the loop, whose registers these loads may have passed through, starts with none in flight
+#pragma unroll 1
+  for (int i = 0; i <= last; i += 2) {
+    step(i, o0);
+    if (i < last) step(i + 1, o1);
+  }
+}
+
+// Waves 4 to 7: the outputs of 16 tokens and a quarter of the state's rows.  Q S follows the state at once; P U, which nobody waits
+// for, a chunk later, while the others solve.
+template <bool kBf16, int kDim, int kTiles>
+__device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s, const ScanWalk& w, int block, ScanShared<kDim, kTiles>& lds) {
+  const RuleParams& p = c.rule;
+  constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2, kHeld = kDim / 64;  // 16-row tiles of the state
+  const int lane = lane_id(), lr = lane & 15, quarter = lane >> 4, khead = w.head / p.rep, last = w.count - 1;
+  const int col = 16 * kTiles * w.slice + lr;
+  float* state = p.pool.recurrent + s.slot * p.pool.recurrent_stride +
+                 (static_cast<int64_t>(w.head) * kDim + 16 * kHeld * block + 4 * quarter) * kDim + col;
+  f32x4 st[kHeld][kTiles];
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) st[h][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!s.fresh)
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[h][x][e] = state[(16 * h + e) * kDim + 16 * x];
+  const auto keep_state = [&](const f32x4 (&from)[kHeld][kTiles]) {
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) state[(16 * h + e) * kDim + 16 * x] = from[h][x][e];
+  };
+  const auto put_state = [&]() {
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        const float f[4] = {st[h][x][0], st[h][x][1], st[h][x][2], st[h][x][3]};
+        put_parts<3>(lds.state[x][0], kDim * 2, f, kHeld * block + h);
+      }
+  };
+
+  struct Ops {
+    uint4 rows[kSteps], kt[kRowParts][kHeld][2];             // Q, the keys transposed
+    f32x4 scale;                                             // e^G rq
+    float keep;                                              // e^G of the chunk
+  };
+  const auto load = [&](int i, Ops& o) {
+    const int64_t at = static_cast<int64_t>(w.base + i) * p.Hv + w.head;
+    const int64_t shared = static_cast<int64_t>(w.base + i) * (p.Hv / p.rep) + khead;
+    const uint16_t* rows = c.rows + shared * (2 * kDim * kChunk) + kDim * kChunk + block * (kSteps * 512) + lane * 8;
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + m * 512);
+    const ChunkScalars* f = c.scalars + at;
+    o.scale = *reinterpret_cast<const f32x4*>(f->query + 16 * block + 4 * quarter);
+    o.keep = f->keep;
+    const uint16_t* kt = c.kt + shared * (kRowParts * kDim * kChunk) + block * (kHeld * 1024) + lane * 8;
+#pragma unroll
+    for (int i3 = 0; i3 < kRowParts; ++i3)
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) o.kt[i3][h][m] = *reinterpret_cast<const uint4*>(kt + i3 * kDim * kChunk + (2 * h + m) * 512);
+  };
+  uint4 mat[2][2];  // P of the chunk before
+  const auto load_mat = [&](int i) {
+    const uint16_t* from = c.p + (static_cast<int64_t>(w.base + i) * p.Hv + w.head) * (2 * kTriangle * 512) + triangle(block, 0) * 512 + lane * 8;
+    if (block > 1)
+#pragma unroll
+      for (int i3 = 0; i3 < 2; ++i3) mat[i3][1] = *reinterpret_cast<const uint4*>(from + (i3 * kTriangle + 1) * 512);
+#pragma unroll
+    for (int i3 = 0; i3 < 2; ++i3) mat[i3][0] = *reinterpret_cast<const uint4*>(from + i3 * kTriangle * 512);
+  };
+  // keep S + K^T (the writes in LDS)
+  const auto update = [&](const Ops& o, float keep, f32x4 (&sum)[kHeld][kTiles]) {
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) {
+      uint4 u[2][3];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) u[m][i] = lds.write[x][i][m * 64 + lane];
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) sum[h][x] = keep * st[h][x];
+#pragma unroll
+      for (int i = 2; i >= 0; --i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int h = 0; h < kHeld; ++h) {
+            if (!kBf16 && i < 2) sum[h][x] = mfma16x16x32(o.kt[kRowParts - 1][h][m], u[m][i], sum[h][x]);
+            sum[h][x] = mfma16x16x32(o.kt[0][h][m], u[m][i], sum[h][x]);
+          }
+    }
+  };
+  f32x4 seen[kTiles];  // e^G rq Q S of the chunk whose P U is still to come
+  const auto write_out = [&](int i) {
+    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
+    if (16 * block >= n) return;
+#pragma unroll
+    for (int x = 0; x < kTiles; ++x) {
+      f32x4 sum = seen[x];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         if (m <= block / 2) {
-          const uint4 x0 = up[0][m * 64 + lane], x1 = up[1][m * 64 + lane];
-          sum = mfma16x16x32(o.mat[1][m], x0, sum);
-          sum = mfma16x16x32(o.mat[0][m], x1, sum);
-          sum = mfma16x16x32(o.mat[0][m], x0, sum);
+          const uint4 x0 = lds.u[i & 1][x][0][m * 64 + lane], x1 = lds.u[i & 1][x][1][m * 64 + lane];
+          sum = mfma16x16x32(mat[1][m], x0, sum);
+          sum = mfma16x16x32(mat[0][m], x1, sum);
+          sum = mfma16x16x32(mat[0][m], x0, sum);
         }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 16 * block + 4 * quarter + e;
-        if (r < n) p.out[(static_cast<int64_t>(t0 + r) * p.Hv + head) * kDim + col] = from_f32<kBf16>(sum[e]);
+        if (r < n) p.out[(static_cast<int64_t>(t0 + r) * p.Hv + w.head) * kDim + col + 16 * x] = from_f32<kBf16>(sum[e]);
       }
     }
-    if (part > 0 && part < n) {
-      // the kept state ends inside this chunk: U once more, with the decays up to its last token
-      const ChunkScalars* f = c.scalars + static_cast<int64_t>(base + i) * p.Hv + head;
-      const double end = f->total[part - 1];
-      lds_barrier();
-      if (solves) {
-        float scaled[4];
+  };
+
+  const auto step = [&](int i, const Ops& o, Ops& next) {
+    const int n = min(kChunk, s.tokens - i * kChunk);
+    const bool active = 16 * block < n;
+    lds_barrier();  // the state's parts are there
+    f32x4 rows[kTiles];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 16 * block + 4 * quarter + e;
-          scaled[e] = r < part ? u[e] * expf(static_cast<float>(end - f->total[r])) * f->norm[r] : 0.f;
+    for (int x = 0; x < kTiles; ++x) rows[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (active)
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+          uint4 r[kRowParts];
+          row_parts<kBf16>(o.rows[m], r);
+          const uint4 f0 = lds.state[x][0][m * 64 + lane], f1 = lds.state[x][1][m * 64 + lane];
+          rows[x] = mfma16x16x32(r[0], f1, rows[x]);
+          if (!kBf16) rows[x] = mfma16x16x32(r[kRowParts - 1], f0, rows[x]);
+          rows[x] = mfma16x16x32(r[0], f0, rows[x]);
         }
-        uint32_t w[3][2];
-        cut<3, 4>(scaled, w);
-        put(&wp[0][0], 128, 3, w, block);
-      }
-      lds_barrier();
-      if (holds) {
-        const f32x4 kept = update(o, static_cast<float>(end));
+    if (i > 0 && s.count == i * kChunk) keep_state(st);  // the kept state ends where this chunk begins
+    lds_barrier();                                       // X is there
+    if (i > 0) write_out(i - 1);
+    load_mat(i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) state[e * kDim] = kept[e];
-      }
+    for (int x = 0; x < kTiles; ++x) seen[x] = o.scale * rows[x];
+    load(min(i + 1, last), next);
+    lds_barrier();  // U is there
+    f32x4 after[kHeld][kTiles];
+    update(o, o.keep, after);
+    const int part = s.count - i * kChunk;
+    if (part > 0 && part < n) {
+      const double end = c.scalars[static_cast<int64_t>(w.base + i) * p.Hv + w.head].total[part - 1];
+      lds_barrier();
+      lds_barrier();
+      f32x4 kept[kHeld][kTiles];
+      update(o, expf(static_cast<float>(end)), kept);
+      keep_state(kept);
     }
-    st = after;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) st[h][x] = after[h][x];
     put_state();
   };
 
   Ops o0, o1;
   load(0, o0);
   put_state();
+  wait_vmem();
 #pragma unroll 1
-  for (int i = 0; i < count; i += 2) {
+  for (int i = 0; i <= last; i += 2) {
     step(i, o0, o1);
-    if (i + 1 < count) step(i + 1, o1, o0);
+    if (i < last) step(i + 1, o1, o0);
   }
-  if (holds && s.count == s.tokens && s.count > 0)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) state[e * kDim] = st[e];
+  write_out(last);
+  if (s.count == s.tokens && s.count > 0) keep_state(st);
+}
+
+// One workgroup per (sequence, value head, 16 kTiles columns of the state), the sequence's chunks in turn.  Three barriers a chunk:
+// S, then X, then U are there.
+template <bool kBf16, int kDim, int kTiles>
+__global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
+  const RuleParams& p = c.rule;
+  constexpr int kSlices = kDim / (16 * kTiles);
+  __shared__ __align__(16) ScanShared<kDim, kTiles> lds;
+  const int group = blockIdx.x / (8 * kSlices), rest = blockIdx.x % (8 * kSlices);
+  const int unit = group * 8 + rest % 8;  // a head's slices on one XCD, which share all but V
+  if (unit >= p.pool.B * p.Hv) return;
+  const int b = unit / p.Hv;
+  const Span s = span_of(p.pool, b);
+  if (s.tokens == 0) return;
+  ScanWalk w;
+  w.base = chunks_before(p.pool, b);
+  w.count = min((s.tokens + kChunk - 1) / kChunk, c.chunks - w.base);
+  w.head = unit % p.Hv;
+  w.slice = rest / 8;
+  if (w.count <= 0) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave < 4) scan_solve<kBf16, kDim, kTiles>(c, s, w, wave, lds);
+  else scan_output<kBf16, kDim, kTiles>(c, s, w, wave - 4, lds);
 }
 
 }  // namespace
@@ -883,7 +1018,12 @@ template <bool kBf16, int kDim>
 void launch_chunks(const ChunkParams& c, hipStream_t stream) {
   const RuleParams& p = c.rule;
   hipLaunchKernelGGL((gdn_chunk_kernel<kBf16, kDim>), dim3(c.chunks * p.Hv), dim3(256), 0, stream, c);
-  hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim>), dim3((p.pool.B * p.Hv + 7) / 8 * 8 * (kDim / 16)), dim3(512), 0, stream, c);
+  const int units = (p.pool.B * p.Hv + 7) / 8 * 8;
+  // 32 columns a workgroup read half as much a column; 16 give every CU one where heads are few
+  if (units * (kDim / 32) >= c.cus)
+    hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 2>), dim3(units * (kDim / 32)), dim3(512), 0, stream, c);
+  else
+    hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 1>), dim3(units * (kDim / 16)), dim3(512), 0, stream, c);
 }
 
 void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t stream) {

@@ -447,10 +447,14 @@ struct ChunkScalars {
   float key[kRuleChunk], query[kRuleChunk];  // e^G / |k|, e^G scale / |q|
   float write[kRuleChunk], norm[kRuleChunk]; // e^{G_end - G} / |k|, 1 / |k|
   double total[kRuleChunk];                  // G, the log decay summed up to the token
+  float keep, unused[3];                     // e^G of the whole chunk
 };
 struct ChunkParams {
   RuleParams rule;
   int chunks;                     // at most: T / 64 + B
+  int cus;
+  uint16_t* rows;                 // [chunks][key heads][keys, queries][4 row blocks][dim / 32][64 lanes][8]
+  uint16_t* v;                    // [chunks][Hv][dim / 16][4 row blocks][64 lanes][4]
   uint16_t* t;                    // [chunks][Hv][3 parts][6 fragments][64 lanes][8]
   uint16_t* p;                    // [chunks][Hv][2 parts][6 fragments][64 lanes][8]
   uint16_t* kt;                   // [chunks][key heads][1 (bf16) or 2 parts][dim / 16][2 fragments][64 lanes][8]
