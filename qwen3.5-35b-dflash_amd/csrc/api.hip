@@ -1394,8 +1394,8 @@ int conv_params(const dflash_state_pool* pool, const dflash_rows* x, const char*
 }
 
 // Parts that the rows of logits are cut into: about kDraftGroups workgroups in the first pass, and as many for the rows that tokens
-// are drawn from, of 2048 tokens at least.
-constexpr int64_t kDraftGroups = 4096;
+// are drawn from, of 2048 tokens at least; of these at most kDraftParts, a thread each of the workgroup that joins them.
+constexpr int64_t kDraftGroups = 4096, kDraftParts = 256;
 struct DraftLayout {
   int64_t splits, split_octets, parts, part_octets;
   size_t stats, choice, norms, part, total;
@@ -1406,13 +1406,13 @@ bool draft_shape_ok(int64_t rows, int64_t vocab, int64_t sequences) {
 DraftLayout draft_layout(int64_t rows, int64_t vocab, int64_t B, bool draft) {
   DraftLayout L;
   const int64_t octets = (vocab + 14) / 8;  // a row may begin up to seven tokens behind a 16-byte boundary
-  const auto cut = [&](int64_t count, int64_t* parts, int64_t* each) {
-    const int64_t want = std::max<int64_t>(1, kDraftGroups / std::max<int64_t>(1, count));
+  const auto cut = [&](int64_t count, int64_t most, int64_t* parts, int64_t* each) {
+    const int64_t want = std::min(most, std::max<int64_t>(1, kDraftGroups / std::max<int64_t>(1, count)));
     *each = std::max<int64_t>(256, (octets + want - 1) / want);
     *parts = (octets + *each - 1) / *each;
   };
-  cut(rows * (draft ? 2 : 1), &L.splits, &L.split_octets);
-  cut(B * 4, &L.parts, &L.part_octets);
+  cut(rows * (draft ? 2 : 1), kDraftGroups, &L.splits, &L.split_octets);
+  cut(B, kDraftParts, &L.parts, &L.part_octets);
   Carver c;
   L.stats = c.take(sizeof(dflash::DraftStats) * (draft ? 2 : 1) * static_cast<size_t>(rows * L.splits));
   L.choice = c.take(sizeof(dflash::DraftChoice) * static_cast<size_t>(B));

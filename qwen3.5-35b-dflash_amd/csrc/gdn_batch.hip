@@ -935,13 +935,13 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
           if (!kBf16) rows[x] = mfma16x16x32(r[kRowParts - 1], f0, rows[x]);
           rows[x] = mfma16x16x32(r[0], f0, rows[x]);
         }
+    load(min(i + 1, last), next);
     if (i > 0 && s.count == i * kChunk) keep_state(st);  // the kept state ends where this chunk begins
     lds_barrier();                                       // X is there
     if (i > 0) write_out(i - 1);
     load_mat(i);
 #pragma unroll
     for (int x = 0; x < kTiles; ++x) seen[x] = o.scale * rows[x];
-    load(min(i + 1, last), next);
     lds_barrier();  // U is there
     f32x4 after[kHeld][kTiles];
     update(o, o.keep, after);

@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 
 #include "../../include/dflash_hip.h"
 
@@ -26,6 +27,7 @@ namespace {
 PyTypeObject* g_packed_type = nullptr;
 PyTypeObject* g_shared_type = nullptr;
 PyTypeObject* g_paged_type = nullptr;
+PyTypeObject* g_pool_type = nullptr;
 PyObject* g_check = nullptr;
 
 struct Entries {
@@ -44,6 +46,12 @@ struct Entries {
   decltype(&dflash_paged_append) paged_append;
   decltype(&dflash_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
   decltype(&dflash_paged_attention) paged_attention;
+  decltype(&dflash_gdn_conv) gdn_conv;
+  decltype(&dflash_gdn_rule_workspace_bytes) gdn_rule_workspace_bytes;
+  decltype(&dflash_gdn_rule) gdn_rule;
+  decltype(&dflash_gdn_advance) gdn_advance;
+  decltype(&dflash_verify_drafts_workspace_bytes) verify_drafts_workspace_bytes;
+  decltype(&dflash_verify_drafts) verify_drafts;
 } g_entry;
 
 // _lib.check of a nonzero status: raises DflashError with the library's message
@@ -585,10 +593,313 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(PackedW4, SharedExpert, PagedKV, _lib.check, address of an entry by name)
+int dtype_of(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat ? DFLASH_DTYPE_F32 : t.scalar_type() == at::kHalf ? DFLASH_DTYPE_F16 : DFLASH_DTYPE_BF16;
+}
+bool is_gate(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+
+// A pool whose slots the kernels take as they lie (ops._slot_pool).
+bool slot_pool(const at::Tensor& t, int64_t ndim, int64_t unit, at::Device device) {
+  if (t.dim() != ndim || t.device() != device || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.stride(0) % unit || tracked(t)) return false;
+  int64_t inner = 1;
+  for (int64_t i = ndim - 1; i > 0; --i) {
+    if (t.size(i) > 1 && t.stride(i) != inner) return false;
+    inner *= t.size(i);
+  }
+  return t.size(0) <= 1 || t.stride(0) >= inner;
+}
+
+// The descriptor of a valid StatePool of `dtype` rows on the current device (ops._pool).
+bool state_pool(PyObject* o, at::ScalarType dtype, bool history, bool recurrent, at::Device device, dflash_state_pool* d) {
+  if (Py_TYPE(o) != g_pool_type || device.index() != c10::hip::current_device()) return false;
+  const at::Tensor* slots = tensor(PyTuple_GET_ITEM(o, 2));
+  if (!slots || slots->dim() != 1 || slots->scalar_type() != at::kInt || slots->device() != device || !slots->is_contiguous() ||
+      (dtype != at::kBFloat16 && dtype != at::kHalf))
+    return false;
+  *d = dflash_state_pool{};
+  d->slots = static_cast<const int32_t*>(slots->data_ptr());
+  d->sequences = slots->size(0);
+  d->pool_slots = -1;
+  d->dtype = dtype == at::kHalf ? DFLASH_DTYPE_F16 : DFLASH_DTYPE_BF16;
+  if (history) {
+    const at::Tensor* h = tensor(PyTuple_GET_ITEM(o, 0));
+    if (!h || h->scalar_type() != dtype || !slot_pool(*h, 3, 8, device) || h->size(2) != 3) return false;
+    d->history = h->data_ptr();
+    d->history_stride = h->stride(0);
+    d->channels = h->size(1);
+    d->pool_slots = h->size(0);
+  }
+  if (recurrent) {
+    const at::Tensor* r = tensor(PyTuple_GET_ITEM(o, 1));
+    if (!r || r->scalar_type() != at::kFloat || !slot_pool(*r, 4, 4, device) || r->size(2) != r->size(3) ||
+        (history && r->size(0) != d->pool_slots))
+      return false;
+    d->recurrent = static_cast<float*>(r->data_ptr());
+    d->recurrent_stride = r->stride(0);
+    d->value_heads = r->size(1);
+    d->head_dim = r->size(2);
+    d->pool_slots = r->size(0);
+  }
+  return true;
+}
+
+// Rows of a block as they lie (ops._block_rows); `size` -1: any.
+const at::Tensor* block_rows(PyObject* o, at::ScalarType dtype, at::Device device, at::IntArrayRef sizes) {
+  const at::Tensor* t = tensor(o);
+  if (!t || t->dim() != static_cast<int64_t>(sizes.size()) || t->scalar_type() != dtype || t->device() != device || !rows_aligned(*t) ||
+      tracked(*t))
+    return nullptr;
+  for (size_t i = 0; i < sizes.size(); ++i)
+    if (sizes[i] >= 0 && t->size(i) != sizes[i]) return nullptr;
+  return t;
+}
+
+// starts, counts and fresh of a block: false where ops.py has to look.
+struct BlockArgs {
+  const int32_t *starts, *counts = nullptr;
+  const uint8_t* fresh = nullptr;
+};
+bool block_args(PyObject* starts, PyObject* counts, PyObject* fresh, int64_t sequences, at::Device device, BlockArgs* out) {
+  const at::Tensor* t = ints(starts, {sequences + 1}, device);
+  if (!t) return false;
+  out->starts = static_cast<const int32_t*>(t->data_ptr());
+  if (counts != Py_None) {
+    if (!(t = ints(counts, {sequences}, device))) return false;
+    out->counts = static_cast<const int32_t*>(t->data_ptr());
+  }
+  if (fresh != Py_None) {
+    t = tensor(fresh);
+    if (!t || (t->scalar_type() != at::kBool && t->scalar_type() != at::kByte) || t->dim() != 1 || t->size(0) != sequences ||
+        t->device() != device || !t->is_contiguous())
+      return false;
+    out->fresh = static_cast<const uint8_t*>(t->data_ptr());
+  }
+  return true;
+}
+
+// ops._rule: the rows (a[0] the query or null, then key, value, decay, beta) and a_log, dt_bias, normalise, scale (null: without).
+bool rule_args(PyObject* query, PyObject* const* a, PyObject* a_log, PyObject* dt_bias, PyObject* normalise, PyObject* scale,
+               const dflash_state_pool& pool, at::ScalarType dtype, at::Device device, dflash_rule* r, int64_t* tokens) {
+  const int64_t hv = pool.value_heads, dim = pool.head_dim;
+  const at::Tensor* value = block_rows(a[1], dtype, device, {-1, hv, dim});
+  if (!value) return false;
+  *tokens = value->size(0);
+  const at::Tensor* key = block_rows(a[0], dtype, device, {*tokens, -1, dim});
+  if (!key || key->size(1) < 1 || hv % key->size(1)) return false;
+  *r = dflash_rule{};
+  if (query) {
+    const at::Tensor* q = block_rows(query, dtype, device, {*tokens, key->size(1), dim});
+    if (!q) return false;
+    r->query = dflash_rows{q->data_ptr(), q->stride(0), q->stride(1)};
+  }
+  r->key = dflash_rows{key->data_ptr(), key->stride(0), key->stride(1)};
+  r->value = dflash_rows{value->data_ptr(), value->stride(0), value->stride(1)};
+  const at::Tensor *decay = tensor(a[2]), *beta = tensor(a[3]);
+  for (const at::Tensor* t : {decay, beta})
+    if (!t || !is_gate(*t) || t->scalar_type() != decay->scalar_type() || t->dim() != 2 || t->size(0) != *tokens || t->size(1) != hv ||
+        t->device() != device || (t->stride(1) != 1 && hv != 1) || tracked(*t))
+      return false;
+  r->decay = decay->data_ptr();
+  r->beta = beta->data_ptr();
+  r->decay_stride = decay->stride(0);
+  r->beta_stride = beta->stride(0);
+  r->gates_dtype = dtype_of(*decay);
+  if ((a_log == Py_None) != (dt_bias == Py_None)) return false;
+  if (a_log != Py_None) {
+    const float* v[2];
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor* t = tensor(i ? dt_bias : a_log);
+      if (!t || t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != hv || t->device() != device || !t->is_contiguous() ||
+          tracked(*t))
+        return false;
+      v[i] = static_cast<const float*>(t->data_ptr());
+    }
+    r->a_log = v[0];
+    r->dt_bias = v[1];
+  }
+  if (!PyBool_Check(normalise) || (scale && scale != Py_None && !PyFloat_CheckExact(scale))) return false;
+  r->normalise = normalise == Py_True;
+  r->scale = scale && scale != Py_None ? static_cast<float>(PyFloat_AS_DOUBLE(scale)) : static_cast<float>(std::pow(static_cast<double>(std::max<int64_t>(dim, 1)), -0.5));
+  r->key_heads = key->size(1);
+  return true;
+}
+
+// A new output, or the caller's; false: one that ops.py has to look at.
+bool output_of(PyObject* o, at::IntArrayRef shape, at::ScalarType dtype, at::Device device, at::Tensor* out) {
+  if (o == Py_None) {
+    *out = make(shape, dtype, device);
+    return true;
+  }
+  const at::Tensor* given = exactly(o, dtype, shape, device);
+  if (!given || tracked(*given)) return false;
+  *out = *given;
+  return true;
+}
+PyObject* given_or(PyObject* o, at::Tensor&& out) {
+  if (o == Py_None) return THPVariable_Wrap(std::move(out));
+  Py_INCREF(o);
+  return o;
+}
+
+// gdn_conv(x, weight, pool, starts, fresh, counts, out)
+PyObject* gdn_conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 7)) return nullptr;
+  const at::Tensor* x = plain_state() ? tensor(a[0]) : nullptr;
+  if (!x) Py_RETURN_NONE;
+  const at::Device device = x->device();
+  const at::ScalarType dtype = x->scalar_type();
+  dflash_state_pool pool;
+  BlockArgs block;
+  if (!state_pool(a[2], dtype, true, false, device, &pool) || !block_rows(a[0], dtype, device, {-1, pool.channels})) Py_RETURN_NONE;
+  const at::Tensor* weight = exactly(a[1], dtype, {pool.channels, 1, 4}, device);
+  if (!weight || tracked(*weight) || !block_args(a[3], a[5], a[4], pool.sequences, device, &block)) Py_RETURN_NONE;
+  at::Tensor out;
+  if (!output_of(a[6], x->sizes(), dtype, device, &out)) Py_RETURN_NONE;
+  const dflash_rows rows{x->data_ptr(), x->stride(0), 0};
+  const int64_t tokens = x->size(0);
+  void* st = stream_of(device);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.gdn_conv(&pool, &rows, weight->data_ptr(), block.starts, block.counts, block.fresh, tokens, out.data_ptr(), st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_gdn_conv", status);
+  return given_or(a[6], std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// gdn_rule(query, key, value, decay, beta, pool, starts, a_log, dt_bias, normalise, scale, fresh, counts, longest, out, workspace)
+PyObject* gdn_rule(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 16)) return nullptr;
+  const at::Tensor* value = plain_state() ? tensor(a[2]) : nullptr;
+  if (!value) Py_RETURN_NONE;
+  const at::Device device = value->device();
+  const at::ScalarType dtype = value->scalar_type();
+  dflash_state_pool pool;
+  dflash_rule rule;
+  BlockArgs block;
+  int64_t tokens, longest = 0;
+  if (a[13] != Py_None) {
+    if (!PyLong_CheckExact(a[13])) Py_RETURN_NONE;
+    longest = PyLong_AsLongLong(a[13]);
+    if (longest < 0) {  // -1 with an error set, too: out of range
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+  }
+  if (!state_pool(a[5], dtype, false, true, device, &pool) ||
+      !rule_args(a[0], a + 1, a[7], a[8], a[9], a[10], pool, dtype, device, &rule, &tokens) ||
+      !block_args(a[6], a[12], a[11], pool.sequences, device, &block))
+    Py_RETURN_NONE;
+  at::Tensor out, ws;
+  if (!output_of(a[14], value->sizes(), dtype, device, &out)) Py_RETURN_NONE;
+  const size_t need = g_entry.gdn_rule_workspace_bytes(tokens, rule.key_heads, pool.value_heads, pool.head_dim, pool.sequences, longest);
+  if ((need || a[15] != Py_None) && !workspace_of(a[15], need, device, &ws)) Py_RETURN_NONE;
+  void* st = stream_of(device);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.gdn_rule(&pool, &rule, block.starts, block.counts, block.fresh, tokens, longest, out.data_ptr(),
+                            ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_gdn_rule", status);
+  return given_or(a[14], std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// gdn_advance(pool, x, key, value, decay, beta, starts, counts, a_log, dt_bias, normalise, fresh): True
+PyObject* gdn_advance(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 12)) return nullptr;
+  const at::Tensor* value = plain_state() ? tensor(a[3]) : nullptr;
+  if (!value || a[7] == Py_None) Py_RETURN_NONE;
+  const at::Device device = value->device();
+  const at::ScalarType dtype = value->scalar_type();
+  dflash_state_pool pool;
+  dflash_rule rule;
+  BlockArgs block;
+  int64_t tokens;
+  if (!state_pool(a[0], dtype, true, true, device, &pool) ||
+      !rule_args(nullptr, a + 2, a[8], a[9], a[10], nullptr, pool, dtype, device, &rule, &tokens) ||
+      !block_args(a[6], a[7], a[11], pool.sequences, device, &block))
+    Py_RETURN_NONE;
+  const at::Tensor* x = block_rows(a[1], dtype, device, {tokens, pool.channels});
+  if (!x) Py_RETURN_NONE;
+  const dflash_rows rows{x->data_ptr(), x->stride(0), 0};
+  void* st = stream_of(device);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.gdn_advance(&pool, &rows, &rule, block.starts, block.counts, block.fresh, tokens, st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_gdn_advance", status);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(target, drafted, starts, uniforms, draft, temperature, workspace): (accepted, token)
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!want(n, 7)) return nullptr;
+  const at::Tensor* target = plain_state() ? tensor(a[0]) : nullptr;
+  if (!target || target->dim() != 2 || !is_gate(*target) || target->size(1) < 1 || target->stride(1) != 1 || tracked(*target) ||
+      target->device().index() != c10::hip::current_device())
+    Py_RETURN_NONE;
+  const at::Device device = target->device();
+  const int64_t rows = target->size(0), vocab = target->size(1);
+  const at::Tensor* starts = tensor(a[2]);
+  if (!starts || starts->dim() != 1 || starts->size(0) < 1) Py_RETURN_NONE;
+  const int64_t count = starts->size(0) - 1;
+  const auto floats = [&](PyObject* o, int64_t size) -> const at::Tensor* {
+    const at::Tensor* t = tensor(o);
+    return t && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == size && t->device() == device && t->is_contiguous() && !tracked(*t)
+               ? t
+               : nullptr;
+  };
+  const at::Tensor *drafted = ints(a[1], {rows}, device), *uniforms = floats(a[3], rows), *draft = nullptr, *temperature = nullptr;
+  if (!drafted || !uniforms || !ints(a[2], {count + 1}, device)) Py_RETURN_NONE;
+  if (a[4] != Py_None) {
+    draft = tensor(a[4]);
+    if (!draft || draft->scalar_type() != target->scalar_type() || draft->sizes() != target->sizes() || draft->device() != device ||
+        draft->stride(1) != 1 || tracked(*draft))
+      Py_RETURN_NONE;
+  }
+  if (a[5] != Py_None && !(temperature = floats(a[5], count))) Py_RETURN_NONE;
+  at::Tensor ws, accepted, token;
+  if (!workspace_of(a[6], g_entry.verify_drafts_workspace_bytes(rows, vocab, count, draft != nullptr), device, &ws)) Py_RETURN_NONE;
+  accepted = make({count}, at::kInt, device);
+  token = make({count}, at::kInt, device);
+  dflash_logits logits{};
+  logits.target = target->data_ptr();
+  logits.draft = draft ? draft->data_ptr() : nullptr;
+  logits.target_stride = target->stride(0);
+  logits.draft_stride = draft ? draft->stride(0) : 0;
+  logits.rows = rows;
+  logits.vocab = vocab;
+  logits.dtype = dtype_of(*target);
+  const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  const auto f32 = [](const at::Tensor* t) { return t ? static_cast<const float*>(t->data_ptr()) : nullptr; };
+  void* st = stream_of(device);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_entry.verify_drafts(&logits, i32(*drafted), i32(*starts), count, f32(uniforms), f32(temperature), i32(accepted), i32(token),
+                                 ws.data_ptr(), ws.numel(), st);
+  Py_END_ALLOW_THREADS
+  if (status) return refused("dflash_verify_drafts", status);
+  PyObject* r = PyTuple_New(2);
+  if (r) {
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(accepted)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(token)));
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(PackedW4, SharedExpert, PagedKV, StatePool, _lib.check, address of an entry by name)
 PyObject* bind(PyObject*, PyObject* args) {
-  PyObject *packed, *shared, *cache, *check, *find;
-  if (!PyArg_ParseTuple(args, "O!O!O!OO", &PyType_Type, &packed, &PyType_Type, &shared, &PyType_Type, &cache, &check, &find))
+  PyObject *packed, *shared, *cache, *pool, *check, *find;
+  if (!PyArg_ParseTuple(args, "O!O!O!O!OO", &PyType_Type, &packed, &PyType_Type, &shared, &PyType_Type, &cache, &PyType_Type, &pool, &check, &find))
     return nullptr;
   bool ok = true;
   const auto get = [&](const char* name, auto& fn) {
@@ -613,6 +924,12 @@ PyObject* bind(PyObject*, PyObject* args) {
   get("dflash_paged_append", g_entry.paged_append);
   get("dflash_paged_attention_workspace_bytes", g_entry.paged_attention_workspace_bytes);
   get("dflash_paged_attention", g_entry.paged_attention);
+  get("dflash_gdn_conv", g_entry.gdn_conv);
+  get("dflash_gdn_rule_workspace_bytes", g_entry.gdn_rule_workspace_bytes);
+  get("dflash_gdn_rule", g_entry.gdn_rule);
+  get("dflash_gdn_advance", g_entry.gdn_advance);
+  get("dflash_verify_drafts_workspace_bytes", g_entry.verify_drafts_workspace_bytes);
+  get("dflash_verify_drafts", g_entry.verify_drafts);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "bind: an entry has no address");
     return nullptr;
@@ -620,17 +937,19 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_INCREF(packed);
   Py_INCREF(shared);
   Py_INCREF(cache);
+  Py_INCREF(pool);
   Py_INCREF(check);
   g_check = check;
   g_packed_type = reinterpret_cast<PyTypeObject*>(packed);
   g_shared_type = reinterpret_cast<PyTypeObject*>(shared);
   g_paged_type = reinterpret_cast<PyTypeObject*>(cache);
+  g_pool_type = reinterpret_cast<PyTypeObject*>(pool);
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(linear), FAST(moe), FAST(gdn), FAST(attention), FAST(commit), FAST(rms_norm),
-                         FAST(paged_append), FAST(paged_attention),
+                         FAST(paged_append), FAST(paged_attention), FAST(gdn_conv), FAST(gdn_rule), FAST(gdn_advance), FAST(verify_drafts),
                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dflash_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -659,6 +659,10 @@ def gdn_conv(x: torch.Tensor, weight: torch.Tensor, pool: StatePool, starts: tor
     rounding.  ``x`` may be a view of a projection's rows.  Tokens in no sequence are not written (``out``: a tensor to write into,
     which shares no memory with ``x``).
     """
+    if _plain(x) and (host := _lib.host()):
+        done = host.gdn_conv(x, weight, pool, starts, fresh, counts, out)
+        if done is not None:
+            return done
     if not isinstance(x, torch.Tensor):
         raise ValueError("x must be a tensor [tokens, channels]")
     desc, device, slots = _pool(pool, "gdn_conv", x.dtype, True, False)
@@ -697,6 +701,11 @@ def gdn_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay:
     knows it, for the choice of the kernels.  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
     tensor to write into, which shares no memory with the rows).
     """
+    if _plain(value) and query is not None and (host := _lib.host()):
+        done = host.gdn_rule(query, key, value, decay, beta, pool, starts, a_log, dt_bias, normalise, scale, fresh, counts, longest, out,
+                             workspace)
+        if done is not None:
+            return done
     if not isinstance(value, torch.Tensor):
         raise ValueError("value must be a tensor [tokens, value heads, head dim]")
     if query is None:
@@ -730,6 +739,9 @@ def gdn_advance(pool: StatePool, x: torch.Tensor, key: torch.Tensor, value: torc
                 dt_bias: Optional[torch.Tensor] = None, normalise: bool = True, fresh: Optional[torch.Tensor] = None) -> None:
     """Histories and states after the first ``counts[b]`` tokens of blocks that :func:`gdn_conv` (its ``x``) and :func:`gdn_rule` took
     without advancing them (``counts`` of 0): commits the accepted part of every sequence's block in one launch."""
+    if _plain(value) and (host := _lib.host()):
+        if host.gdn_advance(pool, x, key, value, decay, beta, starts, counts, a_log, dt_bias, normalise, fresh) is not None:
+            return
     if not isinstance(value, torch.Tensor):
         raise ValueError("value must be a tensor [tokens, value heads, head dim]")
     if counts is None:
@@ -765,6 +777,10 @@ def verify_drafts(target: torch.Tensor, drafted: torch.Tensor, starts: torch.Ten
     row's ``p`` with its own: the emitted tokens follow the target's distribution.  One row a sequence is plain sampling.  Logits bf16, fp16 or fp32; sums, and the weights that tokens are drawn
     by, in 64 bits.
     """
+    if _plain(target) and (host := _lib.host()):
+        done = host.verify_drafts(target, drafted, starts, uniforms, draft, temperature, workspace)
+        if done is not None:
+            return Verified(*done)
     device = _require_device(target, drafted, starts, uniforms)
     if target.ndim != 2 or target.dtype not in _GATE_DTYPES or target.shape[1] < 1:
         raise ValueError("target must be bfloat16, float16 or float32 [rows, vocab]")
