@@ -1393,12 +1393,12 @@ int conv_params(const dflash_state_pool* pool, const dflash_rows* x, const char*
   return DFLASH_OK;
 }
 
-// Parts that the rows of logits are cut into: about kDraftGroups workgroups in the first pass, and as many for the rows that tokens
-// are drawn from, of 2048 tokens at least; of these at most kDraftParts, a thread each of the workgroup that joins them.
+// Parts that the rows of logits are cut into.  In the first pass a workgroup each, about kDraftGroups of them, of 2048 tokens at
+// least.  Of the rows that tokens are drawn from a wave each, at most kDraftParts, which one workgroup joins, a thread a part.
 constexpr int64_t kDraftGroups = 4096, kDraftParts = 256;
 struct DraftLayout {
   int64_t splits, split_octets, parts, part_octets;
-  size_t stats, choice, norms, part, total;
+  size_t stats, choice, norms, ratio, left, total;
 };
 bool draft_shape_ok(int64_t rows, int64_t vocab, int64_t sequences) {
   return rows >= 0 && rows <= (1 << 20) && vocab >= 1 && vocab <= (1 << 24) && sequences >= 0 && sequences <= (1 << 20);
@@ -1406,18 +1406,19 @@ bool draft_shape_ok(int64_t rows, int64_t vocab, int64_t sequences) {
 DraftLayout draft_layout(int64_t rows, int64_t vocab, int64_t B, bool draft) {
   DraftLayout L;
   const int64_t octets = (vocab + 14) / 8;  // a row may begin up to seven tokens behind a 16-byte boundary
-  const auto cut = [&](int64_t count, int64_t most, int64_t* parts, int64_t* each) {
-    const int64_t want = std::min(most, std::max<int64_t>(1, kDraftGroups / std::max<int64_t>(1, count)));
-    *each = std::max<int64_t>(256, (octets + want - 1) / want);
+  const auto cut = [&](int64_t want, int64_t least, int64_t* parts, int64_t* each) {
+    *each = std::max(least, (octets + want - 1) / want);
     *parts = (octets + *each - 1) / *each;
   };
-  cut(rows * (draft ? 2 : 1), kDraftGroups, &L.splits, &L.split_octets);
-  cut(B, kDraftParts, &L.parts, &L.part_octets);
+  cut(std::max<int64_t>(1, kDraftGroups / std::max<int64_t>(1, rows * (draft ? 2 : 1))), 256, &L.splits, &L.split_octets);
+  cut(std::min(kDraftParts, std::max<int64_t>(4, 4 * kDraftGroups / std::max<int64_t>(1, B))), 64, &L.parts, &L.part_octets);
+  L.parts = (L.parts + 3) / 4 * 4;
   Carver c;
   L.stats = c.take(sizeof(dflash::DraftStats) * (draft ? 2 : 1) * static_cast<size_t>(rows * L.splits));
   L.choice = c.take(sizeof(dflash::DraftChoice) * static_cast<size_t>(B));
-  L.norms = c.take(sizeof(double) * 2 * static_cast<size_t>(B * L.parts));
-  L.part = c.take(sizeof(dflash::DraftPart) * static_cast<size_t>(B * L.parts));
+  L.norms = c.take(sizeof(double) * 2 * static_cast<size_t>(B * L.parts / 4));
+  L.ratio = c.take(sizeof(double) * static_cast<size_t>(B));
+  L.left = c.take(sizeof(double) * static_cast<size_t>(B * L.parts));
   L.total = c.off;
   return L;
 }
@@ -1587,7 +1588,8 @@ int dflash_verify_drafts(const dflash_logits* logits, const int32_t* drafted, co
     p.stats = at<dflash::DraftStats>(workspace, L.stats);
     p.choice = at<dflash::DraftChoice>(workspace, L.choice);
     p.norms = at<double>(workspace, L.norms);
-    p.part = at<dflash::DraftPart>(workspace, L.part);
+    p.ratio = at<double>(workspace, L.ratio);
+    p.left = at<double>(workspace, L.left);
     dflash::launch_verify_drafts(p, static_cast<hipStream_t>(stream));
     return launch_status("verify drafts");
   } catch (...) {

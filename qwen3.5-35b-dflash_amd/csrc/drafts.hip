@@ -237,6 +237,8 @@ constexpr int kChooseWaves = 16;
 template <int kType>
 __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftParams p) {
   __shared__ int stop;
+  __shared__ DraftChoice choices[kChooseWaves];
+  __shared__ int largest[kChooseWaves];
   const int b = blockIdx.x, wave = threadIdx.x >> 6;
   const int start = clampi(p.starts[b], 0, p.rows), n = clampi(p.starts[b + 1], start, p.rows) - start;
   const float t = temperature_of(p, b);
@@ -250,159 +252,143 @@ __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftPa
   }
   if (threadIdx.x == 0) stop = n - 1;
   __syncthreads();
-  for (int i0 = 0; i0 < n - 1; i0 += kChooseWaves) {
+  int i0 = 0;
+  for (;; i0 += kChooseWaves) {
     const int i = i0 + wave, row = start + i;
-    if (i < n - 1) {
-      const int x = p.drafted[row];
+    if (i < n) {
+      const bool drafted = i < n - 1, ask = drafted && p.draft && t > 0.0f;
+      const int x = drafted ? p.drafted[row] : -1;
       const bool inside = x >= 0 && x < p.V;
       const Whole target = joined(p, 0, row, t);
-      bool accepted;
-      if (t == 0.0f) {
+      Whole draft{kNone, kNowhere, 0.0};
+      if (ask) draft = joined(p, 1, row, t);
+      bool accepted = false;
+      if (drafted && t == 0.0f) {
         accepted = inside && x == target.at && p.uniforms[row] < 1.0f;
-      } else {
+      } else if (drafted) {
         const double scale = scale_of(t);
         const auto chance = [&](const void* data, int64_t stride, const Whole& r) {
           return inside && r.sum > 0.0 ? weight(Row<kType>(data, stride, row, p.V).at(x), r.top, scale) / r.sum : 0.0;
         };
         const double px = chance(p.target, p.target_stride, target);
-        const double qx = p.draft ? chance(p.draft, p.draft_stride, joined(p, 1, row, t)) : 1.0;
+        const double qx = ask ? chance(p.draft, p.draft_stride, draft) : 1.0;
         accepted = static_cast<double>(p.uniforms[row]) * qx < px;
       }
-      if (!accepted && lane_id() == 0) atomicMin(&stop, i);
+      if (lane_id() == 0) {
+        choices[wave] = DraftChoice{row, drafted, target.top, draft.top};
+        largest[wave] = target.at;
+        if (!accepted) atomicMin(&stop, i);
+      }
     }
     __syncthreads();
-    if (stop < i0 + kChooseWaves) break;
+    if (stop < i0 + kChooseWaves) break;  // at the last row at the latest
   }
-  __syncthreads();
-  const int row = start + stop;
-  if (wave == 0) {
-    const Whole target = joined(p, 0, row, t);
-    const bool rejected = stop < n - 1;
-    float draft_top = kNone;
-    if (rejected && p.draft && t > 0.0f) draft_top = joined(p, 1, row, t).top;
-    if (lane_id() == 0) {
-      p.accepted[b] = stop;
-      DraftChoice c;
-      c.row = row;
-      c.has_draft = rejected;
-      c.target_top = target.top;
-      c.draft_top = draft_top;
-      if (t == 0.0f) {
-        // the largest logit's first token; none where every logit is -infinity
-        p.token[b] = target.at == kNowhere ? -1 : target.at;
-        c.row = -1;
-      }
-      p.choice[b] = c;
+  if (threadIdx.x == 0) {
+    DraftChoice c = choices[stop - i0];
+    p.accepted[b] = stop;
+    if (t == 0.0f) {
+      // the largest logit's first token; none where every logit is -infinity
+      const int at = largest[stop - i0];
+      p.token[b] = at == kNowhere ? -1 : at;
+      c.row = -1;
     }
+    p.choice[b] = c;
   }
 }
 
 // ------------------------------------------------------------------ the rows that tokens are drawn from
-// Their norms in 64 bits, a part a workgroup; y: target or drafter.
+// Their norms in 64 bits, four parts a workgroup; y: target or drafter.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_norm_kernel(DraftParams p) {
   __shared__ double sums[4];
-  const int part = blockIdx.x % p.parts, b = blockIdx.x / p.parts, side = blockIdx.y, tid = threadIdx.x;
+  const int groups = p.parts / 4, group = blockIdx.x % groups, b = blockIdx.x / groups, side = blockIdx.y, tid = threadIdx.x;
   const DraftChoice c = p.choice[b];
   if (c.row < 0 || !c.has_draft) return;
   const double scale = scale_of(temperature_of(p, b));
   const Row<kType> data(side ? p.draft : p.target, side ? p.draft_stride : p.target_stride, c.row, p.V);
   const float top = side ? c.draft_top : c.target_top;
+  const int last = min(4 * (group + 1) * p.part_octets, data.eights());
   double sum = 0.0;
-  for (int o = part * p.part_octets + tid; o < min((part + 1) * p.part_octets, data.eights()); o += 256) {
+  for (int o = 4 * group * p.part_octets + tid; o < last; o += 256) {
     float f[8];
     data.eight(data.first(o), f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += weight(f[i], top, scale);
   }
   sum = wave_sum64(sum);
-  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  if (lane_id() == 0) sums[tid >> 6] = sum;
   __syncthreads();
-  if (tid == 0) p.norms[(static_cast<int64_t>(side) * p.B + b) * p.parts + part] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if (tid == 0) p.norms[(static_cast<int64_t>(side) * p.B + b) * groups + group] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-// What a chosen row's tokens weigh: w_j = p_j - q_j where that is above zero.
+// What a chosen row's tokens weigh, in units of its largest logit's weight: e_j - f_j norm(e) / norm(f) where that is above zero, e
+// and f the target's and the drafter's weights.
 template <int kType>
 struct Residual {
   Row<kType> target, draft;
   float target_top, draft_top;
-  double scale, by_target, by_draft;  // 1 / norm, 0 where the row has nothing
-  bool both;                          // the drafter's distribution is taken off
-  int one;                            // the token that the drafter chose outright, -1: none
+  double scale, ratio;  // norm(e) / norm(f), 0 where the drafter's row has nothing
+  bool both;            // the drafter's distribution is taken off
+  int one;              // the token that the drafter chose outright, -1: none
 
-  __device__ static double norm(const DraftParams& p, int side, int b) {
-    const double* n = p.norms + (static_cast<int64_t>(side) * p.B + b) * p.parts;
-    double sum = 0.0;
-    for (int i = lane_id(); i < p.parts; i += 64) sum += n[i];
-    return wave_sum64(sum);
-  }
   __device__ Residual(const DraftParams& p, int b, const DraftChoice& c)
       : target(p.target, p.target_stride, c.row, p.V), draft(p.draft ? p.draft : p.target, p.draft ? p.draft_stride : p.target_stride, c.row, p.V),
-        target_top(c.target_top), draft_top(c.draft_top), scale(scale_of(temperature_of(p, b))), by_target(1.0), by_draft(0.0),
-        both(c.has_draft && p.draft), one(c.has_draft && !p.draft ? p.drafted[c.row] : -1) {
-    if (both) {
-      const double a = norm(p, 0, b), d = norm(p, 1, b);
-      by_target = a > 0.0 ? 1.0 / a : 0.0;
-      by_draft = d > 0.0 ? 1.0 / d : 0.0;
+        target_top(c.target_top), draft_top(c.draft_top), scale(scale_of(temperature_of(p, b))), ratio(0.0), both(c.has_draft && p.draft),
+        one(c.has_draft && !p.draft ? p.drafted[c.row] : -1) {}
+  // The ratio from the parts of the norms (a wave's lanes together)
+  __device__ void find_ratio(const DraftParams& p, int b) {
+    const int groups = p.parts / 4;  // at most 64
+    const double* n = p.norms + static_cast<int64_t>(b) * groups;
+    const int i = min(lane_id(), groups - 1);
+    double e = n[i], f = n[static_cast<int64_t>(p.B) * groups + i];
+    if (lane_id() >= groups) e = f = 0.0;
+    for (int o = 1; o < 64; o <<= 1) {
+      e += __shfl_xor(e, o, 64);
+      f += __shfl_xor(f, o, 64);
     }
+    ratio = f > 0.0 ? e / f : 0.0;
   }
-  // Weights of tokens [j, j + 8): the target's own and what is left of them.
-  __device__ void eight(int64_t j, double (&whole)[8], double (&left)[8]) const {
+  // Weight of one token: what is left of the target's, or its own.
+  __device__ double one_of(float f, float g, int j, bool use_left) const {
+    const double own = weight(f, target_top, scale);
+    if (!use_left) return own;
+    if (both) return fmax(fma(-ratio, weight(g, draft_top, scale), own), 0.0);
+    return j == one ? 0.0 : own;
+  }
+  // Sum of what is left of a wave's eights o, o + 64, ... before `last`, by lanes.
+  __device__ double sum(int o, int last) const {
     float f[8], g[8];
-    target.eight(j, f);
-    if (both) draft.eight(j, g);
+    double s[2] = {0.0, 0.0};
+    if (both) {
+      for (; o < last; o += 64) {
+        target.eight(target.first(o), f);
+        draft.eight(target.first(o), g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      whole[i] = weight(f[i], target_top, scale) * by_target;
-      left[i] = j + i == one ? 0.0 : whole[i];
-      if (both) left[i] = fmax(whole[i] - weight(g[i], draft_top, scale) * by_draft, 0.0);
+        for (int i = 0; i < 8; ++i) s[i & 1] += fmax(fma(-ratio, weight(g[i], draft_top, scale), weight(f[i], target_top, scale)), 0.0);
+      }
+    } else {
+      for (; o < last; o += 64) {
+        const int j = target.first(o);
+        target.eight(j, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i & 1] += j + i == one ? 0.0 : weight(f[i], target_top, scale);
+      }
     }
+    return s[0] + s[1];
   }
 };
 
+// Sums of what is left, a part a wave.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_parts_kernel(DraftParams p) {
-  __shared__ double sums[2][4];
-  __shared__ int lasts[2][4];
-  const int part = blockIdx.x % p.parts, b = blockIdx.x / p.parts, tid = threadIdx.x;
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), part = unit % p.parts, b = unit / p.parts;
   const DraftChoice c = p.choice[b];
   if (c.row < 0) return;
-  const Residual<kType> r(p, b, c);
-  double sl = 0.0, sw = 0.0;
-  int ll = -1, lw = -1;
-  for (int o = part * p.part_octets + tid; o < min((part + 1) * p.part_octets, r.target.eights()); o += 256) {
-    double whole[8], left[8];
-    const int j = r.target.first(o);
-    r.eight(j, whole, left);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sl += left[i];
-      sw += whole[i];
-      if (left[i] > 0.0) ll = j + i;
-      if (whole[i] > 0.0) lw = j + i;
-    }
-  }
-  sl = wave_sum64(sl);
-  sw = wave_sum64(sw);
-  for (int o = 1; o < 64; o <<= 1) {
-    ll = max(ll, __shfl_xor(ll, o, 64));
-    lw = max(lw, __shfl_xor(lw, o, 64));
-  }
-  if ((tid & 63) == 0) {
-    sums[0][tid >> 6] = sl;
-    sums[1][tid >> 6] = sw;
-    lasts[0][tid >> 6] = ll;
-    lasts[1][tid >> 6] = lw;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    DraftPart d;
-    d.left = (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]);
-    d.whole = (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]);
-    d.last_left = max(max(lasts[0][0], lasts[0][1]), max(lasts[0][2], lasts[0][3]));
-    d.last_whole = max(max(lasts[1][0], lasts[1][1]), max(lasts[1][2], lasts[1][3]));
-    p.part[static_cast<int64_t>(b) * p.parts + part] = d;
-  }
+  Residual<kType> r(p, b, c);
+  if (r.both) r.find_ratio(p, b);
+  if (part == 0 && lane_id() == 0) p.ratio[b] = r.ratio;
+  const double sum = wave_sum64(r.sum(part * p.part_octets + lane_id(), min((part + 1) * p.part_octets, r.target.eights())));
+  if (lane_id() == 0) p.left[static_cast<int64_t>(b) * p.parts + part] = sum;
 }
 
 // Running sum over a workgroup's 256 threads, a thread's own included, from `base` on; `waves`: its four waves' sums.
@@ -420,73 +406,86 @@ __device__ __forceinline__ double running_sum(double own, double base, double* w
   return base + sum;
 }
 
-// One workgroup a sequence: the part in which the running sum passes u times the whole, then the token in it.
+// One workgroup a sequence: the part in which the running sum passes u times the whole, then the token in it.  Where nothing is
+// left (the drafter's distribution is the target's, to the roundings) the same with the target's own weights, over the whole row.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_token_kernel(DraftParams p) {
-  __shared__ double waves[4];
-  __shared__ double totals[2][4];
-  __shared__ double base;
-  __shared__ int lasts[4], found, chosen;
-  const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
+  __shared__ double waves[4], base;
+  __shared__ int found, last, chosen;
+  __shared__ float logits[2][8][256];
+  const int b = blockIdx.x, tid = threadIdx.x;
   const DraftChoice c = p.choice[b];
   if (c.row < 0) return;
-  const DraftPart* parts = p.part + static_cast<int64_t>(b) * p.parts;  // at most 256
-  DraftPart own{0.0, 0.0, -1, -1};
-  if (tid < p.parts) own = parts[tid];
-  const double left = wave_sum64(own.left), whole = wave_sum64(own.whole);
-  if ((tid & 63) == 0) {
-    totals[0][wave] = left;
-    totals[1][wave] = whole;
-  }
-  if (tid == 0) chosen = kNowhere;
-  __syncthreads();
-  const double all_left = (totals[0][0] + totals[0][1]) + (totals[0][2] + totals[0][3]);
-  const bool use_left = all_left > 0.0;
-  const double total = use_left ? all_left : (totals[1][0] + totals[1][1]) + (totals[1][2] + totals[1][3]);
-  const double mine = use_left ? own.left : own.whole;
-  int last = use_left ? own.last_left : own.last_whole;
-  const int own_last = last;
-  for (int o = 1; o < 64; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
-  if ((tid & 63) == 0) lasts[wave] = last;
-  const double goal = static_cast<double>(p.uniforms[c.has_draft ? c.row + 1 : c.row]) * total;
-  const double run = running_sum(mine, 0.0, waves);
-  if (run > goal) atomicMin(&chosen, tid);
-  __syncthreads();
-  if (tid == chosen) {
-    found = own_last;  // where rounding hides the place
-    base = run - mine;
-  }
-  if (chosen == kNowhere && tid == 0) found = max(max(lasts[0], lasts[1]), max(lasts[2], lasts[3]));
-  __syncthreads();
-  if (chosen != kNowhere) {
-    const Residual<kType> r(p, b, c);
-    const int end = min((chosen + 1) * p.part_octets, r.target.eights());
-    const int each = (p.part_octets + 255) / 256, first = chosen * p.part_octets + tid * each;
-    double sum = 0.0;
-    for (int o = first; o < min(first + each, end); ++o) {
-      double w[8], l[8];
-      r.eight(r.target.first(o), w, l);
+  Residual<kType> r(p, b, c);
+  r.ratio = p.ratio[b];
+  const double u = static_cast<double>(p.uniforms[c.has_draft ? c.row + 1 : c.row]);
+  // Walks over eights [from, to), 2048 tokens at a time, eight neighbours a thread, from the sum `before` on: the first token at
+  // which the sum exceeds `goal` into `found`, the last that weighs anything into `last`; returns the sum at the end.  The
+  // weights are made in loops that stay loops: straight code would run once, and fetching it takes longer than running it.
+  const auto walk = [&](int from, int to, double before, double goal, bool use_left) {
+    for (int o0 = from; o0 < to; o0 += 256) {
+      const int o = o0 + tid, j = r.target.first(o);
+      double sum = 0.0;
+      int held = -1;
+      if (o < to) {
+        float f[8];
+        r.target.eight(j, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += use_left ? l[i] : w[i];
-    }
-    const double until = running_sum(sum, base, waves);
-    if (until > goal) {
-      double at = until - sum;
-      for (int o = first; o < min(first + each, end); ++o) {
-        double w[8], l[8];
-        const int j = r.target.first(o);
-        r.eight(j, w, l);
+        for (int i = 0; i < 8; ++i) logits[0][i][tid] = f[i];
+        if (r.both) {
+          r.draft.eight(j, f);
 #pragma unroll
+          for (int i = 0; i < 8; ++i) logits[1][i][tid] = f[i];
+        }
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
-          const double v = use_left ? l[i] : w[i];
-          at += v;
-          if (at > goal && v > 0.0) atomicMin(&found, j + i);
+          const double v = r.one_of(logits[0][i][tid], logits[1][i][tid], j + i, use_left);
+          sum += v;
+          if (v > 0.0) held = j + i;
         }
       }
+      const double until = running_sum(sum, before, waves);
+      if (held >= 0) atomicMax(&last, held);
+      if (until > goal && held >= 0) {
+        double at = until - sum;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const double v = r.one_of(logits[0][i][tid], logits[1][i][tid], j + i, use_left);
+          at += v;
+          if ((at > goal && v > 0.0) || j + i == held) {  // its last one where rounding hides the place
+            atomicMin(&found, j + i);
+            break;
+          }
+        }
+      }
+      before += (waves[0] + waves[1]) + (waves[2] + waves[3]);
+      if (before > goal) break;
     }
     __syncthreads();
+    return before;
+  };
+  const int eights = r.target.eights();
+  const double mine = tid < p.parts ? p.left[static_cast<int64_t>(b) * p.parts + tid] : 0.0;  // at most 256 parts
+  if (tid == 0) {
+    found = kNowhere;
+    chosen = kNowhere;
+    last = -1;
   }
-  if (tid == 0) p.token[b] = found;
+  const double run = running_sum(mine, 0.0, waves);
+  const double total = (waves[0] + waves[1]) + (waves[2] + waves[3]);
+  if (total > 0.0) {
+    const double goal = u * total;
+    if (run > goal && mine > 0.0) atomicMin(&chosen, tid);
+    __syncthreads();
+    if (tid == chosen) base = run - mine;
+    __syncthreads();
+    if (chosen != kNowhere) walk(chosen * p.part_octets, min((chosen + 1) * p.part_octets, eights), base, goal, true);
+    if (found == kNowhere) walk(0, eights, 0.0, INFINITY, true);  // no sum exceeds it (a random number of one or above)
+  } else {
+    const double whole = walk(0, eights, 0.0, INFINITY, false);
+    if (whole > 0.0) walk(0, eights, 0.0, u * whole, false);
+  }
+  if (tid == 0) p.token[b] = found != kNowhere ? found : last;
 }
 
 template <int kType>
@@ -495,8 +494,8 @@ void launch(const DraftParams& p, hipStream_t stream) {
   if (p.rows) hipLaunchKernelGGL(draft_stats_kernel<kType>, dim3(p.rows * p.splits, sides), dim3(256), 0, stream, p);
   hipLaunchKernelGGL(draft_choose_kernel<kType>, dim3(p.B), dim3(64 * kChooseWaves), 0, stream, p);
   if (!p.rows) return;
-  if (p.draft) hipLaunchKernelGGL(draft_norm_kernel<kType>, dim3(p.B * p.parts, 2), dim3(256), 0, stream, p);
-  hipLaunchKernelGGL(draft_parts_kernel<kType>, dim3(p.B * p.parts), dim3(256), 0, stream, p);
+  if (p.draft) hipLaunchKernelGGL(draft_norm_kernel<kType>, dim3(p.B * p.parts / 4, 2), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(draft_parts_kernel<kType>, dim3(p.B * p.parts / 4), dim3(256), 0, stream, p);
   hipLaunchKernelGGL(draft_token_kernel<kType>, dim3(p.B), dim3(256), 0, stream, p);
 }
 

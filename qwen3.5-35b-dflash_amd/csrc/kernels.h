@@ -475,10 +475,6 @@ struct DraftChoice {              // of one sequence: the row that its token com
   int32_t row, has_draft;         // row -1: none; has_draft: the drafter's distribution, or its one token, is taken off
   float target_top, draft_top;
 };
-struct DraftPart {                // of one part of that row
-  double left, whole;             // sums of the weights that are left and of the target's own
-  int32_t last_left, last_whole;  // last tokens with such a weight, -1: none
-};
 struct DraftParams {
   const void *target, *draft;     // [rows][V] by their strides; draft may be null
   int64_t target_stride, draft_stride;
@@ -487,11 +483,12 @@ struct DraftParams {
   const float *uniforms, *temperature;
   int32_t *accepted, *token;
   int splits, split_octets;       // parts of a row in the first pass, and eights of tokens in one
-  int parts, part_octets;         // parts of the chosen rows
+  int parts, part_octets;         // parts of the chosen rows, a multiple of 4, at most 256
   DraftStats* stats;              // [2][rows][splits]
   DraftChoice* choice;            // [B]
-  double* norms;                  // [2][B][parts]
-  DraftPart* part;                // [B][parts]
+  double* norms;                  // [2][B][parts / 4]
+  double* ratio;                  // [B]: of the norms
+  double* left;                   // [B][parts]: sums of what is left
 };
 void launch_verify_drafts(const DraftParams& p, hipStream_t stream);
 
