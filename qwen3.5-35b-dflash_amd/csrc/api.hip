@@ -1446,10 +1446,11 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
 
 namespace {
 // Blocks of more tokens than this go 64 at a time.
-constexpr int64_t kRuleSteps = 16;
+constexpr int64_t kRuleSteps = 32;
 
 struct RuleLayout {
-  int64_t chunks;  // 0: token after token, without a workspace
+  int64_t longest;  // tokens of the longest block, as far as the host knows
+  int64_t chunks;   // 0: blocks of up to kRuleSteps tokens, without a workspace
   size_t rows, v, t, p, kt, scalars, total;
 };
 bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
@@ -1460,7 +1461,8 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   RuleLayout L{};
   if (B == 0 || T == 0) return L;
   if (longest == 0) longest = std::min(T, 2 * ((T + B - 1) / B));  // not known: as if none were twice the average
-  if (std::min(longest, T) <= kRuleSteps) return L;
+  L.longest = std::min(longest, T);
+  if (L.longest <= kRuleSteps) return L;
   L.chunks = T / dflash::kRuleChunk + std::min(T, B);
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
@@ -1513,7 +1515,8 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
       dflash::launch_gdn_chunks(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, c, static_cast<hipStream_t>(stream));
       return launch_status("gdn rule");
     }
-    dflash::launch_gdn_rule(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
+    dflash::launch_gdn_rule(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, p, L.longest,
+                            static_cast<hipStream_t>(stream));
     return launch_status("gdn rule");
   } catch (...) {
     return fail(DFLASH_ERR_HIP, "unexpected host exception");

@@ -36,15 +36,17 @@ struct Span {
   int count;                // tokens that the state advances by, 0: it stays
   bool fresh;               // the state before the block is zeros
 };
+// b is the same in every lane, and so is what stands in memory for it.
 __device__ __forceinline__ Span span_of(const PoolParams& p, int b) {
+  const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   Span s;
-  s.start = clampi(p.starts[b], 0, p.T);
-  s.tokens = clampi(p.starts[b + 1], s.start, p.T) - s.start;
-  s.slot = p.slots[b];
+  s.start = clampi(one(p.starts[b]), 0, p.T);
+  s.tokens = clampi(one(p.starts[b + 1]), s.start, p.T) - s.start;
+  s.slot = one(p.slots[b]);
   if (s.slot < 0 || s.slot >= p.pool_slots) s.slot = -1;
-  s.count = p.counts ? clampi(p.counts[b], 0, s.tokens) : s.tokens;
+  s.count = p.counts ? clampi(one(p.counts[b]), 0, s.tokens) : s.tokens;
   if (s.slot < 0) s.count = 0;
-  s.fresh = s.slot < 0 || (p.fresh && p.fresh[b]);
+  s.fresh = s.slot < 0 || (p.fresh && one(p.fresh[b]));
   return s;
 }
 
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void gdn_conv_kernel(ConvParams p) {
   }
 }
 
-// ------------------------------------------------------------------ the rule, token after token
+// ------------------------------------------------------------------ the rule over short blocks
 __device__ __forceinline__ float gate_value(const void* data, int dtype, int64_t i) {
   if (dtype == 1) return static_cast<const float*>(data)[i];
   const uint16_t v = static_cast<const uint16_t*>(data)[i];
@@ -191,148 +193,464 @@ __device__ __forceinline__ float2 gates_of(const RuleParams& p, int64_t token, i
   return make_float2(g, b);
 }
 
-// One workgroup per (sequence, value head), its state in registers: wave w holds columns [w D/4, (w + 1) D/4), a lane four
-// columns of kPer rows, so a column's two products with the state (S^T k, S^T q) are sums over kGroups lanes of one wave
-// and no token needs a barrier.  A slight decay is applied as S + (e^g - 1) S, one fma: e^g itself is off by half a step near 1,
-// which a head that remembers thousands of tokens would sum up wherever its decay is a constant.  o = S_new^T q = e^g S_old^T q + u (k.q) takes both products from the old state.
-constexpr float kStrong = 2.0f;  // no value of e^g - 1 for g <= 0: the decay is applied as e^g S
+// x as the sum of kParts bf16 numbers, each the rounding of what the ones before leave.
+template <int kParts, int kN>
+__device__ __forceinline__ void cut(const float (&x)[kN], uint32_t (&parts)[kParts][kN / 2]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  float rest[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) rest[i] = x[i];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      parts[p][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{rest[2 * i], rest[2 * i + 1]}, bf16x2));
+      rest[2 * i] -= __uint_as_float(parts[p][i] << 16);
+      rest[2 * i + 1] -= __uint_as_float(parts[p][i] & 0xFFFF0000u);
+    }
+}
+// Eight 16-bit values as bf16 parts: bf16 as they are, fp16 (11 bits) as two.
+template <bool kBf16>
+__device__ __forceinline__ void row_parts(uint4 w, uint4 (&parts)[kBf16 ? 1 : 2]) {
+  if constexpr (kBf16) {
+    parts[0] = w;
+  } else {
+    float f[8];
+    unpack8<false>(w, f);
+    uint32_t c[2][4];
+    cut<2, 8>(f, c);
+    parts[0] = make_uint4(c[0][0], c[0][1], c[0][2], c[0][3]);
+    parts[1] = make_uint4(c[1][0], c[1][1], c[1][2], c[1][3]);
+  }
+}
+template <bool kBf16>
+__device__ __forceinline__ f32x4 mfma_rows(uint4 a, uint4 b, f32x4 c) {
+  if constexpr (kBf16) return mfma16x16x32(a, b, c);
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16x16x16(uint2 a, uint2 b, f32x4 c) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
 
-template <bool kBf16, int kDim, bool kOut>
-__device__ __forceinline__ void rule_steps(const RuleParams& p, int b, int head, float* lds) {
-  constexpr int kCols = kDim / 16, kGroups = 64 / kCols, kQuads = kDim / (4 * kGroups), kBlock = 16;
-  float(*ks)[kDim] = reinterpret_cast<float(*)[kDim]>(lds);
-  float(*qs)[kDim] = ks + kBlock;
-  float(*vs)[kDim] = qs + (kOut ? kBlock : 0);
-  float(*scalars)[4] = reinterpret_cast<float(*)[4]>(vs + kBlock);  // e^g, beta, k.q, e^g - 1 or kStrong
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+__device__ __forceinline__ float2 buf_load8(buf_rsrc r, int lane_offset, int offset) {
+  return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, 0));
+}
+__device__ __forceinline__ void buf_store8(buf_rsrc r, int lane_offset, int offset, float2 v) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, lane_offset, offset, 0);
+}
+
+__device__ __forceinline__ void buf_store16(buf_rsrc r, int lane_offset, int offset, f32x4 v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, lane_offset, offset, 0);
+}
+
+// Sum over groups of 8 or 16 neighbouring lanes, and over the four 16-lane rows of a wave: no LDS trip.
+template <int kLanes>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f32<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += dpp_f32<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += dpp_f32<0x141>(v);  // row_half_mirror
+  if constexpr (kLanes == 16) v += dpp_f32<0x140>(v);  // row_mirror
+  return v;
+}
+__device__ __forceinline__ float rows_sum(float v) {
+  auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// ------------------------------------------------------------------ the rule, token after token
+// For blocks of a token or two, where reading and writing the state is all (a token's arithmetic takes as long whatever the block
+// is).  One workgroup per (sequence, value head), its state in registers: wave w holds columns [w D/4, (w + 1) D/4), a lane four
+// columns of kQuads x 4 rows, so a column's products with the state (S^T k, S^T q) are sums over kGroups lanes of one wave, and
+// so are the norms: no LDS and no barrier, and between the sequence's place and the last store one round trip to memory.
+// o = S_new^T q = e^g S_old^T q + u (k.q) takes both products from the old state.  64 sequences 54 us (5.0 TB/s), one 6 us, its latency.
+template <int kGroups>
+__device__ __forceinline__ float groups_sum(float v) {
+  if constexpr (kGroups == 16) v += dpp_f32<0x124>(v);  // row_ror:4
+  return rows_sum(v + dpp_f32<0x128>(v));               // row_ror:8
+}
+
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
+  constexpr int kCols = kDim / 16, kGroups = 64 / kCols, kQuads = kDim / (4 * kGroups);
+  const int b = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = wave * (kDim / 4) + 4 * (lane % kCols), group = lane / kCols;
   const Span s = span_of(p.pool, b);
-  const int limit = kOut ? s.tokens : s.count;
-  if (limit == 0) return;
-  float* place = p.pool.recurrent + s.slot * p.pool.recurrent_stride + static_cast<int64_t>(head) * kDim * kDim + col;
+  if (s.tokens == 0) return;
+  const buf_rsrc place = make_rsrc(p.pool.recurrent + max(s.slot, 0) * p.pool.recurrent_stride + static_cast<int64_t>(head) * kDim * kDim,
+                                   s.slot < 0 ? 0 : kDim * kDim * 4);
+  const int at = (4 * group * kDim + col) * 4;
+  const auto row_place = [](int j, int e) { return (4 * kGroups * j + e) * kDim * 4; };
+  struct Token {
+    uint2 k[kQuads], q[kQuads], v;
+    float2 gates;
+  };
+  const auto load = [&](int i) {
+    Token o;
+    const int64_t t = s.start + i;
+    const uint16_t* k = p.key + t * p.key_token + khead * p.key_head + 4 * group;
+    const uint16_t* q = p.query + t * p.query_token + khead * p.query_head + 4 * group;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) {
+      o.k[j] = *reinterpret_cast<const uint2*>(k + 4 * kGroups * j);
+      o.q[j] = *reinterpret_cast<const uint2*>(q + 4 * kGroups * j);
+    }
+    o.v = *reinterpret_cast<const uint2*>(p.value + t * p.value_token + head * p.value_head + col);
+    o.gates = gates_of(p, t, head);
+    return o;
+  };
+  const auto four = [](uint2 w) {
+    return f32x4{to_f32<kBf16>(static_cast<uint16_t>(w.x)), to_f32<kBf16>(static_cast<uint16_t>(w.x >> 16)),
+                 to_f32<kBf16>(static_cast<uint16_t>(w.y)), to_f32<kBf16>(static_cast<uint16_t>(w.y >> 16))};
+  };
   f32x4 state[kQuads][4];  // rows 4 kGroups j + 4 group + e
+  if (s.fresh) {
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j)
+    for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      state[j][e] = s.fresh ? f32x4{0.f, 0.f, 0.f, 0.f}
-                            : *reinterpret_cast<const f32x4*>(place + (4 * kGroups * j + 4 * group + e) * kDim);
-  const int khead = head / p.rep;
-  for (int t0 = 0; t0 < limit; t0 += kBlock) {
-    const int n = min(kBlock, limit - t0);
-    if (t0) __syncthreads();
-    for (int i = wave; i < n; i += 4) {
-      const int64_t t = s.start + t0 + i;
-      constexpr int kEach = kDim / 64;
-      float k[kEach], q[kEach], kk = 0.f, qq = 0.f, kq = 0.f;
+      for (int e = 0; e < 4; ++e) state[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  } else {
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int d = lane * kEach + e;
-        k[e] = to_f32<kBf16>(p.key[t * p.key_token + khead * p.key_head + d]);
-        if constexpr (kOut) q[e] = to_f32<kBf16>(p.query[t * p.query_token + khead * p.query_head + d]);
-        vs[i][d] = to_f32<kBf16>(p.value[t * p.value_token + head * p.value_head + d]);
-        kk += k[e] * k[e];
-        if constexpr (kOut) {
-          qq += q[e] * q[e];
-          kq += q[e] * k[e];
-        }
-      }
-      float rk = 1.f, rq = p.scale;
-      if (p.normalise) {
-        rk = 1.0f / sqrtf(wave_sum(kk) + 1e-6f);
-        if constexpr (kOut) rq *= 1.0f / sqrtf(wave_sum(qq) + 1e-6f);
-      }
-      if constexpr (kOut) kq = wave_sum(kq) * rk * rq;
+    for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        ks[i][lane * kEach + e] = k[e] * rk;
-        if constexpr (kOut) qs[i][lane * kEach + e] = q[e] * rq;
-      }
-      const float2 g = gates_of(p, t, head);
-      if (lane == 0) {
-        scalars[i][0] = expf(g.x);
-        scalars[i][1] = g.y;
-        scalars[i][2] = kq;
-        scalars[i][3] = g.x > -0.5f ? expm1f(g.x) : kStrong;
+      for (int e = 0; e < 4; ++e) state[j][e] = __builtin_bit_cast(f32x4, buf_load16(place, at, row_place(j, e)));
+  }
+  Token token = load(0);
+#pragma unroll 1
+  for (int i = 0;; ++i) {
+    f32x4 k[kQuads], kd{0.f, 0.f, 0.f, 0.f}, qd{0.f, 0.f, 0.f, 0.f};
+    float kk = 0.f, qq = 0.f, kq = 0.f;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) {
+      k[j] = four(token.k[j]);
+      const f32x4 q = four(token.q[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kk += k[j][e] * k[j][e];
+        qq += q[e] * q[e];
+        kq += k[j][e] * q[e];
+        kd += state[j][e] * k[j][e];
+        qd += state[j][e] * q[e];
       }
     }
-    __syncthreads();
-    for (int i = 0; i < n; ++i) {
-      f32x4 k[kQuads], q[kQuads], kd{0.f, 0.f, 0.f, 0.f}, qd{0.f, 0.f, 0.f, 0.f};
+    kk = groups_sum<kGroups>(kk);
+    qq = groups_sum<kGroups>(qq);
+    kq = groups_sum<kGroups>(kq);
 #pragma unroll
-      for (int j = 0; j < kQuads; ++j) {
-        k[j] = *reinterpret_cast<const f32x4*>(&ks[i][4 * kGroups * j + 4 * group]);
-        if constexpr (kOut) q[j] = *reinterpret_cast<const f32x4*>(&qs[i][4 * kGroups * j + 4 * group]);
-      }
+    for (int x = 0; x < 4; ++x) {
+      kd[x] = groups_sum<kGroups>(kd[x]);
+      qd[x] = groups_sum<kGroups>(qd[x]);
+    }
+    const float rk = p.normalise ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f, rq = (p.normalise ? 1.0f / sqrtf(qq + 1e-6f) : 1.0f) * p.scale;
+    const float g = token.gates.x, decay = expf(g);
+    const f32x4 u = token.gates.y * (four(token.v) - (decay * rk) * kd);
+    if (group == 0) {
+      const f32x4 o = (decay * rq) * qd + (kq * rk * rq) * u;
+      ushort4 w;
+      w.x = from_f32<kBf16>(o[0]);
+      w.y = from_f32<kBf16>(o[1]);
+      w.z = from_f32<kBf16>(o[2]);
+      w.w = from_f32<kBf16>(o[3]);
+      *reinterpret_cast<ushort4*>(p.out + (static_cast<int64_t>(s.start + i) * p.Hv + head) * kDim + col) = w;
+    }
+    const bool last = i + 1 == s.tokens;
+    if (last && s.count != s.tokens) break;  // nobody sees the state behind the last token
+    if (!last) token = load(i + 1);
+    // a slight decay as S + (e^g - 1) S: e^g itself is off by half a step near 1, which a head that remembers thousands of tokens
+    // would sum up wherever its decay is a constant
+    const bool slight = g > -0.5f;
+    const float fade = slight ? expm1f(g) : decay, rest = slight ? 1.0f : 0.0f;
+    const f32x4 write = rk * u;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[j][e] = (fade * state[j][e] + rest * state[j][e]) + k[j][e] * write;
+    if (i + 1 == s.count)
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          kd += state[j][e] * k[j][e];
-          if constexpr (kOut) qd += state[j][e] * q[j][e];
-        }
-#pragma unroll
-      for (int o = kCols; o < 64; o <<= 1)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          kd[c] += __shfl_xor(kd[c], o, 64);
-          if constexpr (kOut) qd[c] += __shfl_xor(qd[c], o, 64);
-        }
-      const float decay = scalars[i][0], beta = scalars[i][1];
-      const f32x4 v = *reinterpret_cast<const f32x4*>(&vs[i][col]);
-      const f32x4 u = beta * (v - decay * kd);
-      if constexpr (kOut) {
-        if (group == 0) {
-          const f32x4 o = decay * qd + scalars[i][2] * u;
-          ushort4 r;
-          r.x = from_f32<kBf16>(o[0]);
-          r.y = from_f32<kBf16>(o[1]);
-          r.z = from_f32<kBf16>(o[2]);
-          r.w = from_f32<kBf16>(o[3]);
-          *reinterpret_cast<ushort4*>(p.out + (static_cast<int64_t>(s.start + t0 + i) * p.Hv + head) * kDim + col) = r;
-        }
-      }
-      const float fade = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scalars[i][3])));
-      if (fade != kStrong) {
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) state[j][e] = (fade * state[j][e] + state[j][e]) + k[j][e] * u;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) state[j][e] = decay * state[j][e] + k[j][e] * u;
-      }
-      if (t0 + i + 1 == s.count)
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4*>(place + (4 * kGroups * j + 4 * group + e) * kDim) = state[j][e];
-    }
+        for (int e = 0; e < 4; ++e) buf_store16(place, at, row_place(j, e), state[j][e]);
+    if (last) break;
   }
 }
 
-constexpr int rule_lds(int dim, bool out) { return 16 * ((out ? 3 : 2) * dim + 4); }
+// ------------------------------------------------------------------ the rule, 16 tokens at a time
+// A workgroup holds one head's state of one sequence in registers, 32 columns a wave: register (i, x, e) of lane l is row
+// 16 i + 4 (l >> 4) + e, column 2 (l & 15) + x, which is the layout of a matrix instruction's result (the columns of tile x are
+// every other one, so that a lane loads two neighbours) and, when the sum over rows is taken in that order, of a B operand.  So
+// the state takes part in products without leaving its registers.  Sub-blocks of up to 16 tokens with the formulas of a chunk (below):
+//   X = V - diag(e^G r) K S,  U = T X,  O = diag(e^G rq) Q S + P U,  S <- e^G S + K^T diag(e^{G_end - G} r) U.
+template <bool kBf16, int kDim>
+struct BlockShared {
+  uint16_t k[16][kDim + 8], q[16][kDim + 8];
+  float a[16][20], t[16][20], p[16][20];
+  double total[16];           // G
+  float gate[16], beta[16], rk[16], rq[16], key[16], query[16], write[16], keep[16];
+};
+
+template <bool kBf16, int kDim, bool kOut>
+__device__ __forceinline__ void rule_block(const RuleParams& p, int b, int head, BlockShared<kBf16, kDim>& lds) {
+  constexpr int kTiles = kDim / 16, kWaves = kDim / 32, kLanes = kDim / 8, kRowParts = kBf16 ? 1 : 2;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, quarter = lane >> 4;
+  const int col = 32 * wave + 2 * lr, khead = head / p.rep;
+  const Span s = span_of(p.pool, b);
+  const int limit = kOut ? s.tokens : s.count;
+  if (limit == 0) return;
+  // through a buffer, whose rows are uniform offsets: a lane's own 32 addresses would take 64 registers (no slot: nothing is read or written)
+  const buf_rsrc place = make_rsrc(p.pool.recurrent + max(s.slot, 0) * p.pool.recurrent_stride + static_cast<int64_t>(head) * kDim * kDim,
+                                   s.slot < 0 ? 0 : kDim * kDim * 4);
+  const int at = (4 * quarter * kDim + col) * 4;
+  const auto row_place = [](int i, int e) { return (16 * i + e) * kDim * 4; };
+  float st[kTiles][4][2];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = s.fresh ? make_float2(0.f, 0.f) : buf_load8(place, at, row_place(i, e));
+      st[i][e][0] = v.x;
+      st[i][e][1] = v.y;
+    }
+#pragma unroll 1
+  for (int b0 = 0; b0 < limit; b0 += 16) {
+    const int n = min(16, limit - b0), t0 = s.start + b0;
+    if (b0) __syncthreads();
+    {
+      const int r = tid / kLanes, d = tid % kLanes * 8;  // a row each group of lanes
+      const int64_t t = t0 + min(r, n - 1);
+      uint4 k = *reinterpret_cast<const uint4*>(p.key + t * p.key_token + khead * p.key_head + d), q = make_uint4(0, 0, 0, 0);
+      if constexpr (kOut) q = *reinterpret_cast<const uint4*>(p.query + t * p.query_token + khead * p.query_head + d);
+      if (r >= n) k = q = make_uint4(0, 0, 0, 0);
+      if (wave == kWaves - 1 && lane < 16) {
+        float2 g = make_float2(0.f, 0.f);
+        if (lane < n) g = gates_of(p, t0 + lane, head);
+        lds.gate[lane] = g.x < -200.0f ? -200.0f : g.x;  // e^-200 is 0 in fp32, and what stands behind it keeps its bits
+        lds.beta[lane] = g.y;
+      }
+      float f[8], h[8], kk = 0.f, qq = 0.f;
+      unpack8<kBf16>(k, f);
+      unpack8<kBf16>(q, h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        kk += f[e] * f[e];
+        qq += h[e] * h[e];
+      }
+      kk = group_sum<kLanes>(kk);
+      const float rk = p.normalise ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f;
+      float rq = p.scale;
+      if constexpr (kOut) {
+        qq = group_sum<kLanes>(qq);
+        if (p.normalise) rq *= 1.0f / sqrtf(qq + 1e-6f);
+      }
+      if (d == 0) {
+        lds.rk[r] = rk;
+        lds.rq[r] = rq;
+      }
+      *reinterpret_cast<uint4*>(&lds.k[r][d]) = k;
+      if constexpr (kOut) *reinterpret_cast<uint4*>(&lds.q[r][d]) = q;
+    }
+    uint32_t v[4];  // two columns of tokens 4 quarter + e
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = *reinterpret_cast<const uint32_t*>(p.value + (t0 + min(4 * quarter + e, n - 1)) * p.value_token + head * p.value_head + col);
+    __syncthreads();
+
+    // K S and Q S, 32 rows of the state an instruction
+    f32x4 ks[2], qs[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) ks[x] = qs[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // first what the others wait for: A on wave 0, P on the next
+    if (wave < (kOut ? 2 : 1)) {
+      f32x4 d{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int m = 0; m < kDim / 32; ++m) {
+        const uint4 other = *reinterpret_cast<const uint4*>(&lds.k[lr][32 * m + 8 * quarter]);
+        const uint4 own = wave ? *reinterpret_cast<const uint4*>(&lds.q[lr][32 * m + 8 * quarter]) : other;
+        d = mfma_rows<kBf16>(own, other, d);
+      }
+      // the running log decay in 64 bits, so that a decay e^{G_t - G_s} is as exact as its own exponent
+      double sum = 0.0, here = 0.0, rows[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sum += static_cast<double>(lds.gate[i]);
+        if (i == lr) here = sum;
+        if (i >> 2 == quarter) rows[i & 3] = sum;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = 4 * quarter + e;
+        const float decay = lr <= t ? __expf(static_cast<float>(rows[e] - here)) * lds.rk[lr] : 0.f;
+        if (wave) lds.p[t][lr] = lds.rq[t] * decay * d[e];
+        else lds.a[t][lr] = lr < t ? lds.beta[t] * lds.rk[t] * decay * d[e] : 0.f;
+      }
+      if (wave == 0) {
+        if (lane < 16) {
+          const float decay = expf(static_cast<float>(here));
+          lds.key[lr] = decay * lds.rk[lr];
+          lds.query[lr] = decay * lds.rq[lr];
+          lds.write[lr] = expf(static_cast<float>(sum - here)) * lds.rk[lr];
+          lds.total[lr] = here;
+          lds.keep[lr] = decay;
+        }
+        // (I + A)^-1 diag(beta) by forward substitution, a column a lane (one wave wrote A and reads it)
+        __builtin_amdgcn_wave_barrier();
+        if (lane < 16) {
+          float x[16];
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            float s0 = t == lr ? lds.beta[lr] : 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < t; ++i) {
+              const float f = lds.a[t][i];
+              if (i & 1) s1 -= f * x[i];
+              else s0 -= f * x[i];
+            }
+            x[t] = s0 + s1;
+            lds.t[t][lr] = x[t];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < kDim / 32; ++m) {
+      uint4 k[kRowParts], q[kRowParts];
+      const auto rows = [&](const uint16_t(&from)[16][kDim + 8], uint4(&to)[kRowParts]) {
+        const uint2 lo = *reinterpret_cast<const uint2*>(&from[lr][32 * m + 4 * quarter]);
+        const uint2 hi = *reinterpret_cast<const uint2*>(&from[lr][32 * m + 16 + 4 * quarter]);
+        row_parts<kBf16>(make_uint4(lo.x, lo.y, hi.x, hi.y), to);
+      };
+      rows(lds.k, k);
+      if constexpr (kOut) rows(lds.q, q);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f[8] = {st[2 * m][0][x],     st[2 * m][1][x],     st[2 * m][2][x],     st[2 * m][3][x],
+                            st[2 * m + 1][0][x], st[2 * m + 1][1][x], st[2 * m + 1][2][x], st[2 * m + 1][3][x]};
+        uint32_t c[3][4];
+        cut<3, 8>(f, c);
+#pragma unroll
+        for (int i = 2; i >= 0; --i) {
+          const uint4 part = make_uint4(c[i][0], c[i][1], c[i][2], c[i][3]);
+          if (!kBf16 && i < 2) ks[x] = mfma16x16x32(k[kRowParts - 1], part, ks[x]);
+          ks[x] = mfma16x16x32(k[0], part, ks[x]);
+          if constexpr (kOut)
+            if (i < 2) {
+              if (!kBf16 && i < 1) qs[x] = mfma16x16x32(q[kRowParts - 1], part, qs[x]);
+              qs[x] = mfma16x16x32(q[0], part, qs[x]);
+            }
+        }
+      }
+    }
+    __syncthreads();
+    const f32x4 key = *reinterpret_cast<const f32x4*>(&lds.key[4 * quarter]), t = *reinterpret_cast<const f32x4*>(&lds.t[lr][4 * quarter]);
+    f32x4 u[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      u[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        u[x] = mfma16x16x4f32(t[e], to_f32<kBf16>(static_cast<uint16_t>(v[e] >> 16 * x)) - key[e] * ks[x][e], u[x]);
+    }
+    if constexpr (kOut) {
+      const f32x4 query = *reinterpret_cast<const f32x4*>(&lds.query[4 * quarter]), w = *reinterpret_cast<const f32x4*>(&lds.p[lr][4 * quarter]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        qs[x] *= query;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qs[x] = mfma16x16x4f32(w[e], u[x][e], qs[x]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * quarter + e < n)
+          *reinterpret_cast<uint32_t*>(p.out + (static_cast<int64_t>(t0 + 4 * quarter + e) * p.Hv + head) * kDim + col) =
+              from_f32<kBf16>(qs[0][e]) | static_cast<uint32_t>(from_f32<kBf16>(qs[1][e])) << 16;
+    }
+    // the state after the first `part` tokens, into the pool or as the one that goes on
+    const auto after = [&](int part, bool keep_it) {
+      f32x4 write = *reinterpret_cast<const f32x4*>(&lds.write[4 * quarter]);
+      if (part < n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * quarter + e;
+          write[e] = r < part ? expf(static_cast<float>(lds.total[part - 1] - lds.total[r])) * lds.rk[r] : 0.f;
+        }
+      const float keep = lds.keep[part - 1];
+      uint2 w[2][3];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f[4] = {write[0] * u[x][0], write[1] * u[x][1], write[2] * u[x][2], write[3] * u[x][3]};
+        uint32_t c[3][2];
+        cut<3, 4>(f, c);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) w[x][i] = make_uint2(c[i][0], c[i][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        uint16_t r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = lds.k[4 * quarter + e][16 * i + lr];
+        uint2 k[kRowParts];
+        if constexpr (kBf16) {
+          k[0] = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+        } else {
+          const float f[4] = {to_f32<false>(r[0]), to_f32<false>(r[1]), to_f32<false>(r[2]), to_f32<false>(r[3])};
+          uint32_t c[2][2];
+          cut<2, 4>(f, c);
+          k[0] = make_uint2(c[0][0], c[0][1]);
+          k[1] = make_uint2(c[1][0], c[1][1]);
+        }
+        f32x4 sum[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[x][e] = keep * st[i][e][x];
+#pragma unroll
+          for (int j = 2; j >= 0; --j) {
+            if (!kBf16 && j < 2) sum[x] = mfma16x16x16(k[kRowParts - 1], w[x][j], sum[x]);
+            sum[x] = mfma16x16x16(k[0], w[x][j], sum[x]);
+          }
+        }
+        if (keep_it) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) buf_store8(place, at, row_place(i, e), make_float2(sum[0][e], sum[1][e]));
+        } else {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[i][e][x] = sum[x][e];
+        }
+      }
+    };
+    const int part = s.count - b0;
+    if (part > 0 && (part <= n || b0 + 16 >= limit)) after(min(part, n), true);
+    if (b0 + 16 >= limit) return;
+    after(n, false);
+  }
+}
 
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256) void gdn_rule_kernel(RuleParams p) {
-  __shared__ __align__(16) float lds[rule_lds(kDim, true)];
-  rule_steps<kBf16, kDim, true>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
+__global__ __launch_bounds__(2 * kDim, 3) void gdn_rule_kernel(RuleParams p) {
+  __shared__ __align__(16) BlockShared<kBf16, kDim> lds;
+  rule_block<kBf16, kDim, true>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
 }
 
 // States and conv histories after the part of the block that counts, one launch for both: the first B * Hv workgroups
 // take the states, the others the histories.
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256) void gdn_advance_kernel(RuleParams p, ConvParams c) {
-  __shared__ __align__(16) float lds[rule_lds(kDim, false)];
+__global__ __launch_bounds__(2 * kDim, 3) void gdn_advance_kernel(RuleParams p, ConvParams c) {
+  __shared__ __align__(16) BlockShared<kBf16, kDim> lds;
   const int states = p.pool.B * p.Hv;
   if (static_cast<int>(blockIdx.x) < states) {
-    rule_steps<kBf16, kDim, false>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
+    rule_block<kBf16, kDim, false>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
     return;
   }
-  const int across = (c.channels + 2047) / 2048, i = blockIdx.x - states;
-  const int channel = (i % across * 256 + threadIdx.x) * 8;
+  const int across = (c.channels + 16 * kDim - 1) / (16 * kDim), i = blockIdx.x - states;
+  const int channel = (i % across * 2 * kDim + threadIdx.x) * 8;
   if (channel >= c.channels) return;
   const Span s = span_of(c.pool, i / across);
   if (s.count == 0) return;
@@ -388,45 +706,6 @@ __device__ __forceinline__ int chunks_before(const PoolParams& p, int b) {
   int sum = 0;  // bounded: starts that do not ascend may count a token many times
   for (int i = lane_id(); i < b; i += 64) sum = min(sum + chunks_of(p, i), 1 << 24);
   return __builtin_amdgcn_readfirstlane(wave_sum_int(sum));
-}
-
-template <bool kBf16>
-__device__ __forceinline__ f32x4 mfma_rows(uint4 a, uint4 b, f32x4 c) {
-  if constexpr (kBf16) return mfma16x16x32(a, b, c);
-  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// x as the sum of kParts bf16 numbers, each the rounding of what the ones before leave.
-template <int kParts, int kN>
-__device__ __forceinline__ void cut(const float (&x)[kN], uint32_t (&parts)[kParts][kN / 2]) {
-  float rest[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) rest[i] = x[i];
-#pragma unroll
-  for (int p = 0; p < kParts; ++p)
-#pragma unroll
-    for (int i = 0; i < kN / 2; ++i) {
-      typedef float f32x2 __attribute__((ext_vector_type(2)));
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      parts[p][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{rest[2 * i], rest[2 * i + 1]}, bf16x2));
-      rest[2 * i] -= __uint_as_float(parts[p][i] << 16);
-      rest[2 * i + 1] -= __uint_as_float(parts[p][i] & 0xFFFF0000u);
-    }
-}
-// Eight 16-bit values as bf16 parts: bf16 as they are, fp16 (11 bits) as two.
-template <bool kBf16>
-__device__ __forceinline__ void row_parts(uint4 w, uint4 (&parts)[kBf16 ? 1 : 2]) {
-  if constexpr (kBf16) {
-    parts[0] = w;
-  } else {
-    float f[8];
-    unpack8<false>(w, f);
-    uint32_t c[2][4];
-    cut<2, 8>(f, c);
-    parts[0] = make_uint4(c[0][0], c[0][1], c[0][2], c[0][3]);
-    parts[1] = make_uint4(c[1][0], c[1][1], c[1][2], c[1][3]);
-  }
 }
 
 // One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices.  Rows come in whole (256 bytes a
@@ -1031,26 +1310,26 @@ void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t str
   else bf16 ? launch_chunks<true, 64>(c, stream) : launch_chunks<false, 64>(c, stream);
 }
 
-void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, hipStream_t stream) {
-  const dim3 grid(p.pool.B * p.Hv);
-  if (dim == 128) {
-    if (bf16) hipLaunchKernelGGL((gdn_rule_kernel<true, 128>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((gdn_rule_kernel<false, 128>), grid, dim3(256), 0, stream, p);
-  } else {
-    if (bf16) hipLaunchKernelGGL((gdn_rule_kernel<true, 64>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((gdn_rule_kernel<false, 64>), grid, dim3(256), 0, stream, p);
-  }
+constexpr int64_t kTokenSteps = 2;  // blocks of so many tokens go token after token
+template <bool kBf16, int kDim>
+void launch_rule(const RuleParams& p, int64_t longest, hipStream_t stream) {
+  if (longest <= kTokenSteps) hipLaunchKernelGGL((gdn_token_kernel<kBf16, kDim>), dim3(p.pool.B * p.Hv), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((gdn_rule_kernel<kBf16, kDim>), dim3(p.pool.B * p.Hv), dim3(2 * kDim), 0, stream, p);
+}
+template <bool kBf16, int kDim>
+void launch_advance(const RuleParams& p, const ConvParams& c, hipStream_t stream) {
+  const int across = (c.channels + 16 * kDim - 1) / (16 * kDim);
+  hipLaunchKernelGGL((gdn_advance_kernel<kBf16, kDim>), dim3(p.pool.B * (p.Hv + across)), dim3(2 * kDim), 0, stream, p, c);
+}
+
+void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, int64_t longest, hipStream_t stream) {
+  if (dim == 128) bf16 ? launch_rule<true, 128>(p, longest, stream) : launch_rule<false, 128>(p, longest, stream);
+  else bf16 ? launch_rule<true, 64>(p, longest, stream) : launch_rule<false, 64>(p, longest, stream);
 }
 
 void launch_gdn_advance(int dim, bool bf16, const RuleParams& p, const ConvParams& c, hipStream_t stream) {
-  const dim3 grid(p.pool.B * p.Hv + p.pool.B * ((c.channels + 2047) / 2048));
-  if (dim == 128) {
-    if (bf16) hipLaunchKernelGGL((gdn_advance_kernel<true, 128>), grid, dim3(256), 0, stream, p, c);
-    else hipLaunchKernelGGL((gdn_advance_kernel<false, 128>), grid, dim3(256), 0, stream, p, c);
-  } else {
-    if (bf16) hipLaunchKernelGGL((gdn_advance_kernel<true, 64>), grid, dim3(256), 0, stream, p, c);
-    else hipLaunchKernelGGL((gdn_advance_kernel<false, 64>), grid, dim3(256), 0, stream, p, c);
-  }
+  if (dim == 128) bf16 ? launch_advance<true, 128>(p, c, stream) : launch_advance<false, 128>(p, c, stream);
+  else bf16 ? launch_advance<true, 64>(p, c, stream) : launch_advance<false, 64>(p, c, stream);
 }
 
 }  // namespace dflash

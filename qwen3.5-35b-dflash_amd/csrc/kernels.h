@@ -462,7 +462,8 @@ struct ChunkParams {
 };
 void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t stream);
 void launch_gdn_conv(bool bf16, const ConvParams& p, hipStream_t stream);
-void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, hipStream_t stream);
+// `longest`: tokens of the longest block, as far as the host knows; blocks of any length are right
+void launch_gdn_rule(int dim, bool bf16, const RuleParams& p, int64_t longest, hipStream_t stream);
 void launch_gdn_advance(int dim, bool bf16, const RuleParams& p, const ConvParams& c, hipStream_t stream);
 
 // Check of drafted tokens (drafts.hip).

@@ -97,7 +97,7 @@ def test_rule_refusals(pkg):
     for kw, message in [(dict(rule=0), "NULL"), (dict(rule=_rule(lib, query=_rows(lib, None))), "query"), (dict(starts=None), "starts"),
                         (dict(tokens=-1), "2\\^20"), (dict(tokens=1 << 62), "2\\^20"), (dict(longest=-1), "longest"), (dict(out=None), "out"),
                         (dict(out=ADDRESS + 8), "out"), (dict(out=ADDRESS), "out cannot be"), (dict(tokens=500, ws=None), "workspace"),
-                        (dict(tokens=500, ws=ADDRESS + 8), "workspace"), (dict(longest=17, tokens=17, size=100), "workspace"), (dict(tokens=1 << 20, pool=_pool(lib, value_heads=512)), "2\\^28")]:
+                        (dict(tokens=500, ws=ADDRESS + 8), "workspace"), (dict(longest=33, tokens=33, size=100), "workspace"), (dict(tokens=1 << 20, pool=_pool(lib, value_heads=512)), "2\\^28")]:
         refused(lib, _delta, message, **kw)
     for kw, message in [(dict(rule=0), "NULL"), (dict(counts=None), "counts"), (dict(starts=None), "starts"),
                         (dict(x=_rows(lib, ADDRESS + 2)), "x"), (dict(tokens=1 << 21), "2\\^20")]:

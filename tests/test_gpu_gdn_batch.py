@@ -57,7 +57,7 @@ def test_conv_of_many_tokens(pkg, device):
     layer.check_conv(layer.conv())
 
 
-@pytest.mark.parametrize("longest", [None, 1, 200])
+@pytest.mark.parametrize("longest", [None, 1, 16, 200])
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("spans", SPANS.values(), ids=SPANS.keys())
 def test_rule(pkg, device, spans, shape, longest):
@@ -68,7 +68,7 @@ def test_rule(pkg, device, spans, shape, longest):
     assert (out[layer.tokens:] == 7.0).all()
 
 
-@pytest.mark.parametrize("longest", [1, 200])
+@pytest.mark.parametrize("longest", [1, 16, 200])
 @pytest.mark.parametrize("counts", [[0] * 6, [1, 20, 64, 65, 128, 129], [70, 16, 63, 1, 127, 400], [-1, 36, 0, 2, 191, 300]])
 @pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, FP16)])
 def test_rule_counts(pkg, device, counts, dim, dtype, longest):
@@ -77,7 +77,7 @@ def test_rule_counts(pkg, device, counts, dim, dtype, longest):
     layer.check_rule(layer.rule(longest=longest))
 
 
-@pytest.mark.parametrize("longest", [1, 200])
+@pytest.mark.parametrize("longest", [1, 16, 200])
 @pytest.mark.parametrize("kind", [torch.float32, BF16, FP16])
 def test_rule_gates_given(pkg, device, kind, longest):
     """Gates as they are, from hardly any decay to states that vanish within a token."""
@@ -86,7 +86,7 @@ def test_rule_gates_given(pkg, device, kind, longest):
         layer.check_rule(layer.rule(longest=longest), f"decay {scale}")
 
 
-@pytest.mark.parametrize("longest", [1, 200])
+@pytest.mark.parametrize("longest", [1, 16, 200])
 def test_rule_without_norm(pkg, device, longest):
     layer = Layer(pkg, device, [5, 100, 64], seed=3)
     for t in (layer.key, layer.d["key"]):    # of norm about one, as the bound asks: a power of two takes nothing off
@@ -94,7 +94,7 @@ def test_rule_without_norm(pkg, device, longest):
     layer.check_rule(layer.rule(normalise=False, scale=0.5, longest=longest), normalise=False, scale=0.5)
 
 
-@pytest.mark.parametrize("longest", [1, 200])
+@pytest.mark.parametrize("longest", [1, 16, 200])
 def test_rule_repeated_keys(pkg, device, longest):
     """One key in every token: the chunk's system is as far from the identity as it gets."""
     layer = Layer(pkg, device, [200, 64], raw_gates=False, decay_scale=0.001, seed=8)
@@ -105,7 +105,7 @@ def test_rule_repeated_keys(pkg, device, longest):
 
 def test_rule_gates_at_their_ends(pkg, device):
     """Decays of zero and -infinity, writes of zero and one; a key of zeros."""
-    for longest in (1, 200):
+    for longest in (1, 16, 200):
         layer = Layer(pkg, device, [80, 5], raw_gates=False, seed=4)
         for t in (layer.decay, layer.d["decay"]):
             t[3], t[10], t[70], t[82] = float("-inf"), 0.0, float("-inf"), float("-inf")
@@ -144,7 +144,7 @@ def test_advance_is_what_the_forward_leaves(pkg, device):
     kept.check_state(want, bound)
 
 
-@pytest.mark.parametrize("longest", [1, 500])
+@pytest.mark.parametrize("longest", [1, 16, 500])
 def test_repeats_bit_for_bit(pkg, device, longest):
     spans = [1, 16, 200, 65, 0, 3]
     a, b = (Layer(pkg, device, spans, seed=6, key_heads=4, value_heads=8) for _ in range(2))
