@@ -1451,7 +1451,7 @@ constexpr int64_t kRuleSteps = 32;
 struct RuleLayout {
   int64_t longest;  // tokens of the longest block, as far as the host knows
   int64_t chunks;   // 0: blocks of up to kRuleSteps tokens, without a workspace
-  size_t rows, v, t, p, kt, scalars, total;
+  size_t rows, t, p, kt, scalars, total;
 };
 bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
   return T >= 0 && T <= (1 << 20) && Hk > 0 && Hv > 0 && Hv <= 1024 && Hv % Hk == 0 && (D == 64 || D == 128) && B >= 0 && B <= (1 << 20) &&
@@ -1467,8 +1467,7 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
   L.rows = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
-  L.v = c.take(each * 2 * D * dflash::kRuleChunk);
-  L.t = c.take(each * 3 * part);
+  L.t = c.take(each * 2 * part);
   L.p = c.take(each * 2 * part);
   L.kt = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
   L.scalars = c.take(each * sizeof(dflash::ChunkScalars));
@@ -1507,8 +1506,7 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
       c.chunks = static_cast<int>(L.chunks);
       c.cus = cu_count();
       c.rows = at<uint16_t>(workspace, L.rows);
-      c.v = at<uint16_t>(workspace, L.v);
-      c.t = at<uint16_t>(workspace, L.t);
+      c.t = at<float>(workspace, L.t);
       c.p = at<uint16_t>(workspace, L.p);
       c.kt = at<uint16_t>(workspace, L.kt);
       c.scalars = at<dflash::ChunkScalars>(workspace, L.scalars);

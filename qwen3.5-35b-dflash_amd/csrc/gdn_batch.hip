@@ -719,12 +719,12 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
     uint16_t raw[kChunk][kRaw];
     float f[kChunk][kPitch];
   };
-  __shared__ __align__(16) Shared keys_t, query_p, value_a;  // first the rows, then T, P and A
+  __shared__ __align__(16) Shared keys_t, query_p;  // first the rows, then T and P
+  __shared__ __align__(16) float am[kChunk][kPitch];
   __shared__ double gsum[kChunk];
   __shared__ float beta[kChunk], rk[kChunk], rq[kChunk];
   auto& tm = keys_t.f;
   auto& pm = query_p.f;
-  auto& am = value_a.f;
   const int ordinal = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
   const int2 place = chunk_place(p.pool, ordinal);
   if (place.x == p.pool.B) return;
@@ -738,14 +738,13 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
   {
     constexpr int kLanes = kDim / 8, kRows = 256 / kLanes;  // lanes a row, rows a pass
     const int r0 = tid / kLanes, d = tid % kLanes * 8;
-    uint4 k[kChunk / kRows], q[kChunk / kRows], v[kChunk / kRows];
+    uint4 k[kChunk / kRows], q[kChunk / kRows];
 #pragma unroll
     for (int i = 0; i < kChunk / kRows; ++i) {
       const int r = r0 + i * kRows;
       const int64_t t = t0 + min(r, n - 1);
       k[i] = *reinterpret_cast<const uint4*>(p.key + t * p.key_token + khead * p.key_head + d);
       q[i] = *reinterpret_cast<const uint4*>(p.query + t * p.query_token + khead * p.query_head + d);
-      v[i] = *reinterpret_cast<const uint4*>(p.value + t * p.value_token + head * p.value_head + d);
     }
     if (wave == 0) {
       float2 g = make_float2(0.f, 0.f);
@@ -764,7 +763,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
 #pragma unroll
     for (int i = 0; i < kChunk / kRows; ++i) {
       const int r = r0 + i * kRows;
-      if (r >= n) k[i] = q[i] = v[i] = make_uint4(0, 0, 0, 0);
+      if (r >= n) k[i] = q[i] = make_uint4(0, 0, 0, 0);
       float f[8], kk = 0.f, qq = 0.f;
       unpack8<kBf16>(k[i], f);
 #pragma unroll
@@ -783,7 +782,6 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
       }
       *reinterpret_cast<uint4*>(&keys_t.raw[r][d]) = k[i];
       *reinterpret_cast<uint4*>(&query_p.raw[r][d]) = q[i];
-      *reinterpret_cast<uint4*>(&value_a.raw[r][d]) = v[i];
     }
   }
   __syncthreads();
@@ -824,17 +822,6 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
       row_parts<kBf16>(make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16), parts);
 #pragma unroll
       for (int i = 0; i < kRowParts; ++i) *reinterpret_cast<uint4*>(to + i * kDim * kChunk + f * 512) = parts[i];
-    }
-  }
-  {
-    // the values in the order of a result: rows 4 quarter + e of a row block, column lr of a slice
-    uint16_t* to = c.v + at * (kDim * kChunk) + lane * 4;
-#pragma unroll
-    for (int i = 0; i < kDim / 16; ++i) {
-      uint16_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = value_a.raw[16 * wave + 4 * quarter + e][16 * i + lr];
-      *reinterpret_cast<uint2*>(to + (i * 4 + wave) * 256) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
     }
   }
   __syncthreads();
@@ -910,12 +897,11 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
         x[i] = tm[row][col + i] * beta[col + i];
         y[i] = pm[row][col + i];
       }
-      uint32_t tp[3][4], pp[2][4];
-      cut<3, 8>(x, tp);
+      uint32_t pp[2][4];
       cut<2, 8>(y, pp);
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        *reinterpret_cast<uint4*>(c.t + ((at * 3 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(tp[i][0], tp[i][1], tp[i][2], tp[i][3]);
+      float* t = c.t + (at * kTriangle + f) * 512 + lane * 4;
+      *reinterpret_cast<float4*>(t) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(t + 256) = make_float4(x[4], x[5], x[6], x[7]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         *reinterpret_cast<uint4*>(c.p + ((at * 2 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(pp[i][0], pp[i][1], pp[i][2], pp[i][3]);
@@ -955,6 +941,11 @@ __device__ __forceinline__ void put_parts(uint4* to, int part_stride, const floa
 struct ScanWalk {
   int base, count, head, slice;
 };
+// Column of tile x and lane column lr: with two tiles every other one, so that a lane's two are neighbours.
+template <int kTiles>
+__device__ __forceinline__ int scan_column(const ScanWalk& w, int lr) {
+  return kTiles * (16 * w.slice + lr);
+}
 
 // Waves 0 to 3 of gdn_scan_kernel: X and U of 16 tokens.  In both kinds of waves loads stand in no branch but a first one (indices
 // are bounded instead) and nothing is computed from them before they are needed, so that those of the two chunks ahead stay in flight.
@@ -963,30 +954,47 @@ __device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, 
   const RuleParams& p = c.rule;
   constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2;
   const int lane = lane_id(), quarter = lane >> 4, khead = w.head / p.rep, last = w.count - 1;
+  const int col = scan_column<kTiles>(w, lane & 15);
   struct Ops {
-    uint4 rows[kSteps], mat[3][2];  // K, T
-    f32x4 scale, write;             // e^G r, e^{G_64 - G} r
-    uint2 v[kTiles];
+    uint4 rows[kSteps];  // K
+    float4 mat[2][2];    // T
+    f32x4 scale, write;  // e^G r, e^{G_64 - G} r
+    uint32_t v[4];       // V: a row's kTiles columns
   };
   const auto load = [&](int i, Ops& o) {
     const int64_t at = static_cast<int64_t>(w.base + i) * p.Hv + w.head;
-    const uint16_t* mat = c.t + at * (3 * kTriangle * 512) + triangle(block, 0) * 512 + lane * 8;
+    const float* mat = c.t + (at * kTriangle + triangle(block, 0)) * 512 + lane * 4;
     if (block > 1)
 #pragma unroll
-      for (int i3 = 0; i3 < 3; ++i3) o.mat[i3][1] = *reinterpret_cast<const uint4*>(mat + (i3 * kTriangle + 1) * 512);
+      for (int h = 0; h < 2; ++h) o.mat[1][h] = *reinterpret_cast<const float4*>(mat + 512 + 256 * h);
 #pragma unroll
-    for (int i3 = 0; i3 < 3; ++i3) o.mat[i3][0] = *reinterpret_cast<const uint4*>(mat + i3 * kTriangle * 512);
+    for (int h = 0; h < 2; ++h) o.mat[0][h] = *reinterpret_cast<const float4*>(mat + 256 * h);
     const uint16_t* rows = c.rows + (static_cast<int64_t>(w.base + i) * (p.Hv / p.rep) + khead) * (2 * kDim * kChunk) + block * (kSteps * 512) + lane * 8;
 #pragma unroll
     for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + m * 512);
     const ChunkScalars* f = c.scalars + at;
     o.scale = *reinterpret_cast<const f32x4*>(f->key + 16 * block + 4 * quarter);
     o.write = *reinterpret_cast<const f32x4*>(f->write + 16 * block + 4 * quarter);
+    const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
 #pragma unroll
-    for (int x = 0; x < kTiles; ++x)
-      o.v[x] = *reinterpret_cast<const uint2*>(c.v + at * (kDim * kChunk) + ((kTiles * w.slice + x) * 4 + block) * 256 + lane * 4);
+    for (int e = 0; e < 4; ++e) {
+      const uint16_t* v = p.value + (t0 + min(16 * block + 4 * quarter + e, n - 1)) * p.value_token + w.head * p.value_head + col;
+      if constexpr (kTiles == 2) o.v[e] = *reinterpret_cast<const uint32_t*>(v);
+      else o.v[e] = *v;
+    }
   };
-  const auto step = [&](int i, Ops& o) {
+  uint4 mat[3][2];  // T of the chunk at hand, in parts
+  const auto cut_mat = [&](const Ops& o) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float f[8] = {o.mat[m][0].x, o.mat[m][0].y, o.mat[m][0].z, o.mat[m][0].w, o.mat[m][1].x, o.mat[m][1].y, o.mat[m][1].z, o.mat[m][1].w};
+      uint32_t parts[3][4];
+      cut<3, 8>(f, parts);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) mat[i][m] = make_uint4(parts[i][0], parts[i][1], parts[i][2], parts[i][3]);
+    }
+  };
+  const auto step = [&](int i, Ops& o, const Ops& next) {
     const int n = min(kChunk, s.tokens - i * kChunk);
     const bool active = 16 * block < n;
     lds_barrier();  // the state's parts are there
@@ -1007,10 +1015,8 @@ __device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, 
             sum[m & 1] = mfma16x16x32(r[0], st[i3], sum[m & 1]);
           }
         }
-        const uint16_t v[4] = {static_cast<uint16_t>(o.v[x].x), static_cast<uint16_t>(o.v[x].x >> 16), static_cast<uint16_t>(o.v[x].y),
-                               static_cast<uint16_t>(o.v[x].y >> 16)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = to_f32<kBf16>(v[e]) - o.scale[e] * (sum[0][e] + sum[1][e]);
+        for (int e = 0; e < 4; ++e) f[e] = to_f32<kBf16>(static_cast<uint16_t>(o.v[e] >> 16 * x)) - o.scale[e] * (sum[0][e] + sum[1][e]);
       }
       put_parts<3>(lds.x[x][0], 128, f, block);
     }
@@ -1029,12 +1035,12 @@ __device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, 
             uint4 f[3];
 #pragma unroll
             for (int i3 = 0; i3 < 3; ++i3) f[i3] = lds.x[x][i3][m * 64 + lane];
-            sum[0] = mfma16x16x32(o.mat[2][m], f[0], sum[0]);
-            sum[1] = mfma16x16x32(o.mat[1][m], f[1], sum[1]);
-            sum[0] = mfma16x16x32(o.mat[0][m], f[2], sum[0]);
-            sum[1] = mfma16x16x32(o.mat[1][m], f[0], sum[1]);
-            sum[0] = mfma16x16x32(o.mat[0][m], f[1], sum[0]);
-            sum[1] = mfma16x16x32(o.mat[0][m], f[0], sum[1]);
+            sum[0] = mfma16x16x32(mat[2][m], f[0], sum[0]);
+            sum[1] = mfma16x16x32(mat[1][m], f[1], sum[1]);
+            sum[0] = mfma16x16x32(mat[0][m], f[2], sum[0]);
+            sum[1] = mfma16x16x32(mat[1][m], f[0], sum[1]);
+            sum[0] = mfma16x16x32(mat[0][m], f[1], sum[0]);
+            sum[1] = mfma16x16x32(mat[0][m], f[0], sum[1]);
           }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1067,15 +1073,17 @@ __device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, 
       lds_barrier();
     }
     load(min(i + 2, last), o);
+    cut_mat(next);
   };
   Ops o0, o1;
   load(0, o0);
   load(min(1, last), o1);
   wait_vmem();  // so that the loop, whose registers these loads may have passed through, starts with none in flight
+  cut_mat(o0);
 #pragma unroll 1
   for (int i = 0; i <= last; i += 2) {
-    step(i, o0);
-    if (i < last) step(i + 1, o1);
+    step(i, o0, o1);
+    if (i < last) step(i + 1, o1, o0);
   }
 }
 
@@ -1086,7 +1094,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
   const RuleParams& p = c.rule;
   constexpr int kSteps = kDim / 32, kRowParts = kBf16 ? 1 : 2, kHeld = kDim / 64;  // 16-row tiles of the state
   const int lane = lane_id(), lr = lane & 15, quarter = lane >> 4, khead = w.head / p.rep, last = w.count - 1;
-  const int col = 16 * kTiles * w.slice + lr;
+  const int col = scan_column<kTiles>(w, lr);
   float* state = p.pool.recurrent + s.slot * p.pool.recurrent_stride +
                  (static_cast<int64_t>(w.head) * kDim + 16 * kHeld * block + 4 * quarter) * kDim + col;
   f32x4 st[kHeld][kTiles];
@@ -1094,20 +1102,26 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
   for (int h = 0; h < kHeld; ++h)
 #pragma unroll
     for (int x = 0; x < kTiles; ++x) st[h][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  typedef float Columns __attribute__((ext_vector_type(kTiles)));
   if (!s.fresh)
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
 #pragma unroll
-      for (int x = 0; x < kTiles; ++x)
+      for (int e = 0; e < 4; ++e) {
+        const Columns v = *reinterpret_cast<const Columns*>(state + (16 * h + e) * kDim);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st[h][x][e] = state[(16 * h + e) * kDim + 16 * x];
+        for (int x = 0; x < kTiles; ++x) st[h][x][e] = v[x];
+      }
   const auto keep_state = [&](const f32x4 (&from)[kHeld][kTiles]) {
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
 #pragma unroll
-      for (int x = 0; x < kTiles; ++x)
+      for (int e = 0; e < 4; ++e) {
+        Columns v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) state[(16 * h + e) * kDim + 16 * x] = from[h][x][e];
+        for (int x = 0; x < kTiles; ++x) v[x] = from[h][x][e];
+        *reinterpret_cast<Columns*>(state + (16 * h + e) * kDim) = v;
+      }
   };
   const auto put_state = [&]() {
 #pragma unroll
@@ -1176,21 +1190,26 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
   const auto write_out = [&](int i) {
     const int t0 = s.start + i * kChunk, n = min(kChunk, s.tokens - i * kChunk);
     if (16 * block >= n) return;
+    f32x4 sum[kTiles];
 #pragma unroll
     for (int x = 0; x < kTiles; ++x) {
-      f32x4 sum = seen[x];
+      sum[x] = seen[x];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         if (m <= block / 2) {
           const uint4 x0 = lds.u[i & 1][x][0][m * 64 + lane], x1 = lds.u[i & 1][x][1][m * 64 + lane];
-          sum = mfma16x16x32(mat[1][m], x0, sum);
-          sum = mfma16x16x32(mat[0][m], x1, sum);
-          sum = mfma16x16x32(mat[0][m], x0, sum);
+          sum[x] = mfma16x16x32(mat[1][m], x0, sum[x]);
+          sum[x] = mfma16x16x32(mat[0][m], x1, sum[x]);
+          sum[x] = mfma16x16x32(mat[0][m], x0, sum[x]);
         }
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * block + 4 * quarter + e;
-        if (r < n) p.out[(static_cast<int64_t>(t0 + r) * p.Hv + w.head) * kDim + col + 16 * x] = from_f32<kBf16>(sum[e]);
+    for (int e = 0; e < 4; ++e) {
+      const int r = 16 * block + 4 * quarter + e;
+      uint16_t* to = p.out + (static_cast<int64_t>(t0 + r) * p.Hv + w.head) * kDim + col;
+      if (r < n) {
+        if constexpr (kTiles == 2) *reinterpret_cast<uint32_t*>(to) = from_f32<kBf16>(sum[0][e]) | static_cast<uint32_t>(from_f32<kBf16>(sum[1][e])) << 16;
+        else *to = from_f32<kBf16>(sum[0][e]);
       }
     }
   };
