@@ -1445,12 +1445,19 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
 }
 
 namespace {
-// Blocks of more tokens than this go 64 at a time.
-constexpr int64_t kRuleSteps = 32;
+// Whether blocks go 64 tokens at a time.  Sixteen at a time a workgroup walks its sequence in 5.7 us a step, and all of them together
+// take 0.83 ns a token and head of 128; 64 at a time a step is 1.7 us and the whole 1.1 ns, 9 us dearer to start (head dim 64: half a
+// token).  Measured us, 16 and 64 at a time: 1 block of 24 tokens 19 and 19, of 64 30 and 19; 8 of 64 37 and 40, of 128 60 and 54; 16 of
+// 256 130 and 148; 64 of 256 433 and 582; at head dim 64 8 of 64 23 and 17, 32 of 64 31 and 34.
+bool chunks_pay(int64_t longest, int64_t T, int64_t Hv, int64_t D) {
+  if (longest <= 16) return false;
+  const double l = static_cast<double>(longest), all = static_cast<double>(T) * static_cast<double>(Hv) * static_cast<double>(D) / 128;
+  return std::max(356.0 * l, 0.83 * all) > 9000.0 + std::max(27.0 * l, 1.1 * all);
+}
 
 struct RuleLayout {
   int64_t longest;  // tokens of the longest block, as far as the host knows
-  int64_t chunks;   // 0: blocks of up to kRuleSteps tokens, without a workspace
+  int64_t chunks;   // 0: not 64 tokens at a time, and without a workspace
   size_t rows, t, p, kt, scalars, total;
 };
 bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
@@ -1462,7 +1469,7 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   if (B == 0 || T == 0) return L;
   if (longest == 0) longest = std::min(T, 2 * ((T + B - 1) / B));  // not known: as if none were twice the average
   L.longest = std::min(longest, T);
-  if (L.longest <= kRuleSteps) return L;
+  if (!chunks_pay(L.longest, T, Hv, D)) return L;
   L.chunks = T / dflash::kRuleChunk + std::min(T, B);
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
