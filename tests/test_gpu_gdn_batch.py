@@ -167,3 +167,17 @@ def test_blocks_in_pieces(pkg, device):
                                          starts, a_log=d["a_log"], dt_bias=d["dt_bias"], fresh=torch.tensor([fresh] * 2, device=device))
         assert float(((got.double().cpu() - want[0]).abs() - want[1]).max()) <= 0
         layer.check_state(want[2], want[3], str(cut))
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (128, FP16), (64, BF16), (64, FP16)])
+def test_rule_of_prompts_with_many_heads(pkg, device, dim, dtype):
+    """Sequences and heads enough that a workgroup takes 32 columns of the state; blocks that end at every place of a chunk, empty and
+    fresh ones among them, counts inside."""
+    spans = [70, 1, 130, 0, 64, 200, 33, 129] * (1 if dim == 128 else 2)
+    for counts in (None, [min(n, 65) - b % 3 for b, n in enumerate(spans)]):
+        layer = Layer(pkg, device, spans, key_heads=4, value_heads=8, dim=dim, dtype=dtype, seed=11, spare=2, missing=(2,), fresh=(0, 5),
+                      counts=counts)
+        out = filled(layer, layer.hv, dim)
+        layer.rule(out, longest=200)
+        layer.check_rule(out)
+        assert (out[layer.tokens:] == 7.0).all()
