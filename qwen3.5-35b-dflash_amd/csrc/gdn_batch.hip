@@ -4,6 +4,8 @@
 // S <- e^g S; u = beta (v - S^T k); S <- S + k u^T; o = S^T q).  Tokens [starts[b], starts[b + 1]) of the block are sequence
 // b's; its conv history and state are slot slots[b] of the pool.  All three are read on the device, and whatever they
 // hold leads to no address outside the block or the pool.
+//
+// Times stand for heads of 128 (16 of keys, 32 of values) where nothing else is said.
 #include "kernels.h"
 
 namespace dflash {
@@ -130,7 +132,7 @@ __device__ __forceinline__ uint4 conv8(const float (&r0)[8], const float (&r1)[8
 
 // A workgroup per kRows tokens and 2048 channels, a thread eight neighbouring channels.  A block's first three rows read the
 // history that the same thread replaces, so they go with the first of them, whichever tile they fall into.  Bound by memory: tiles
-// inside one sequence have all their rows in flight at once.
+// inside one sequence have all their rows in flight at once.  8869 tokens of five prompts, 8192 channels: 56 us, 5.2 TB/s; a token 3.3.
 template <bool kBf16, int kRows>
 __global__ __launch_bounds__(256) void gdn_conv_kernel(ConvParams p) {
   const int t0 = blockIdx.x * kRows, channel = (blockIdx.y * 256 + threadIdx.x) * 8;
@@ -301,7 +303,8 @@ __device__ __forceinline__ float rows_sum(float v) {
 // is).  One workgroup per (sequence, value head), its state in registers: wave w holds columns [w D/4, (w + 1) D/4), a lane four
 // columns of kQuads x 4 rows, so a column's products with the state (S^T k, S^T q) are sums over kGroups lanes of one wave, and
 // so are the norms: no LDS and no barrier, and between the sequence's place and the last store one round trip to memory.
-// o = S_new^T q = e^g S_old^T q + u (k.q) takes both products from the old state.  64 sequences 54 us (5.0 TB/s), one 6 us, its latency.
+// o = S_new^T q = e^g S_old^T q + u (k.q) takes both products from the old state.  64 sequences 57 us (4.7 TB/s; 45 where the last-level
+// cache still holds their states from the call before), one 6 us, its latency.
 template <int kGroups>
 __device__ __forceinline__ float groups_sum(float v) {
   if constexpr (kGroups == 16) v += dpp_f32<0x124>(v);  // row_ror:4
@@ -419,6 +422,9 @@ __global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
 // every other one, so that a lane loads two neighbours) and, when the sum over rows is taken in that order, of a B operand.  So
 // the state takes part in products without leaving its registers.  Sub-blocks of up to 16 tokens with the formulas of a chunk (below):
 //   X = V - diag(e^G r) K S,  U = T X,  O = diag(e^G rq) Q S + P U,  S <- e^G S + K^T diag(e^{G_end - G} r) U.
+// 32 sequences of up to 16 tokens 34 us with the state left alone (74 MB: memory takes 14; the rest is the sub-block's chain of
+// K K^T, the substitution, two products and the output, 5.7 us behind the load of the state, in 1.3 rounds of three workgroups a CU),
+// 40 us as gdn_advance, which writes it (139 MB).
 template <bool kBf16, int kDim>
 struct BlockShared {
   uint16_t k[16][kDim + 8], q[16][kDim + 8];
@@ -740,7 +746,8 @@ __device__ __forceinline__ int chunks_before(const PoolParams& p, int b) {
   return __builtin_amdgcn_readfirstlane(wave_sum_int(sum));
 }
 
-// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices.  Rows come in whole (256 bytes a
+// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices: 2048 of them 48 us for 4096 tokens of one
+// sequence, a chain of seven steps with barriers between, two workgroups a CU.  Rows come in whole (256 bytes a
 // load of 16 lanes) and pass through LDS: what the scan reads eight times over, once a slice, it finds in the order of
 // its operands, 1 KB a load (rows read straight into operands cost a cache line a lane).
 template <bool kBf16, int kDim>
@@ -1305,7 +1312,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 }
 
 // One workgroup per (sequence, value head, 16 kTiles columns of the state), the sequence's chunks in turn.  Three barriers a chunk:
-// S, then X, then U are there.
+// S, then X, then U are there.  Bound by that chain: 1.75 us a chunk, 112 us for 4096 tokens of one sequence.
 template <bool kBf16, int kDim, int kTiles>
 __global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
   const RuleParams& p = c.rule;
@@ -1351,8 +1358,11 @@ void launch_chunks(const ChunkParams& c, hipStream_t stream) {
   const RuleParams& p = c.rule;
   hipLaunchKernelGGL((gdn_chunk_kernel<kBf16, kDim>), dim3(c.chunks * p.Hv), dim3(256), 0, stream, c);
   const int units = (p.pool.B * p.Hv + 7) / 8 * 8;
-  // 32 columns a workgroup read half as much a column; 16 give every CU one where heads are few
-  if (units * (kDim / 32) >= c.cus)
+  // A CU runs a workgroup about as fast as several would share it.  With 32 columns one reads half as much a column and takes 1.5 to 1.7 times as long as with 16: it
+  // pays where that saves rounds of the card.  us, 16 and 32 columns, by sequences of 1024 tokens: one 50 and 60, two 90 and 75, four 160 and
+  // 135; head dim 64, 16 heads, of 512 tokens: six 36 and 35, twelve 58 and 63.
+  const auto rounds = [&](int columns) { return (units * (kDim / columns) + c.cus - 1) / c.cus; };
+  if (5 * rounds(32) <= 3 * rounds(16))
     hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 2>), dim3(units * (kDim / 32)), dim3(512), 0, stream, c);
   else
     hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 1>), dim3(units * (kDim / 16)), dim3(512), 0, stream, c);
@@ -1363,7 +1373,10 @@ void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t str
   else bf16 ? launch_chunks<true, 64>(c, stream) : launch_chunks<false, 64>(c, stream);
 }
 
-constexpr int64_t kTokenSteps = 2;  // blocks of so many tokens go token after token
+// Blocks of up to so many tokens go token after token.  us, that way and 16 at a time: 64 sequences of one token 45 and 66, of two 49 and
+// 66, of three 57 and 70, of four both 66; 32 of four 41 and 42; one of one 6.7 and 7.5, of four 12.0 and 12.6; head dim 64, 32 of two 7.9 and 11.0, of four
+// 11.9 and 11.0.
+constexpr int64_t kTokenSteps = 3;
 template <bool kBf16, int kDim>
 void launch_rule(const RuleParams& p, int64_t longest, hipStream_t stream) {
   if (longest <= kTokenSteps) hipLaunchKernelGGL((gdn_token_kernel<kBf16, kDim>), dim3(p.pool.B * p.Hv), dim3(256), 0, stream, p);

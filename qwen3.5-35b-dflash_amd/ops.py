@@ -699,7 +699,7 @@ def gdn_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay:
     dt_bias)``, ``beta = sigmoid(beta)``.  The slot then holds the state after ``counts[b]`` tokens (int32 ``[B]``; None: all of them;
     0: it stays as it is, as a verify block's does until :func:`gdn_advance`).  ``longest``: tokens of the longest block, if the caller
     knows it, for the choice of the kernels.  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
-    tensor to write into, which shares no memory with the rows).
+    tensor to write into, which shares no memory with the rows).  A NaN or infinity in a token may reach all outputs of its block and head.
     """
     if _plain(value) and query is not None and (host := _lib.host()):
         done = host.gdn_rule(query, key, value, decay, beta, pool, starts, a_log, dt_bias, normalise, scale, fresh, counts, longest, out,
@@ -774,8 +774,8 @@ def verify_drafts(target: torch.Tensor, drafted: torch.Tensor, starts: torch.Ten
     (None: chosen outright); the last row of a sequence has none.  ``temperature`` fp32 ``[B]`` (None: 1) divides both; 0 is greedy.
     With the softmaxes ``p`` and ``q`` a token ``x`` is accepted iff ``uniforms[r] * q(x) < p(x)`` (fp32 ``[rows]`` in [0, 1)); the first that is not
     is replaced by a draw from ``max(p - q, 0)`` with the next row's uniform, and all accepted are followed by a draw from the last
-    row's ``p`` with its own: the emitted tokens follow the target's distribution.  One row a sequence is plain sampling.  Logits bf16, fp16 or fp32; sums, and the weights that tokens are drawn
-    by, in 64 bits.
+    row's ``p`` with its own: the emitted tokens follow the target's distribution.  One row a sequence is plain sampling.  Logits bf16,
+    fp16 or fp32, NaN as -infinity; sums, and the weights that tokens are drawn by, in 64 bits.
     """
     if _plain(target) and (host := _lib.host()):
         done = host.verify_drafts(target, drafted, starts, uniforms, draft, temperature, workspace)
