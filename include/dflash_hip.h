@@ -431,7 +431,8 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
  * are g and beta themselves: [tokens][value_heads] of gates_dtype, decay_stride and beta_stride elements a row.
  * query and key [tokens][key_heads][head_dim], value and out [tokens][value_heads][head_dim]; fp32 inside, the state's products
  * as exact as fp32.  Uses recurrent only (history may be NULL).
- * longest: tokens of the longest block where the caller knows it, else 0.  It chooses the kernels, never the result.
+ * longest: tokens of the longest block where the caller knows it, else 0.  It chooses the kernels and with them the order of roundings,
+ * nothing else: blocks of any length are right with any of it.
  */
 typedef struct dflash_rule {
   dflash_rows query, key, value;

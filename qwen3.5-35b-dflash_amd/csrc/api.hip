@@ -1455,9 +1455,11 @@ bool chunks_pay(int64_t longest, int64_t T, int64_t Hv, int64_t D) {
   return std::max(356.0 * l, 0.83 * all) > 9000.0 + std::max(27.0 * l, 1.1 * all);
 }
 
+constexpr int64_t kShortBlock = 32;
 struct RuleLayout {
   int64_t longest;  // tokens of the longest block, as far as the host knows
   int64_t chunks;   // 0: not 64 tokens at a time, and without a workspace
+  int64_t least, sequences;  // tokens of a block that goes 64 at a time at least, how many there are at most
   size_t rows, t, p, kt, scalars, total;
 };
 bool rule_shape_ok(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, int64_t longest) {
@@ -1470,7 +1472,13 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   if (longest == 0) longest = std::min(T, 2 * ((T + B - 1) / B));  // not known: as if none were twice the average
   L.longest = std::min(longest, T);
   if (!chunks_pay(L.longest, T, Hv, D)) return L;
-  L.chunks = T / dflash::kRuleChunk + std::min(T, B);
+  // Short blocks beside long ones go their own way, in a launch of their own: a workgroup of the scan takes as long for a token as for 64.
+  // us with that launch and without, heads of 128: 1024 tokens and 63 blocks of one 115 and 247, three of one 55 and 58, one 57 and 56; four
+  // prompts 94 and 92; 16 heads of 64, 1024 tokens and 15 of one 52 and 43.
+  L.least = B * Hv * D * D <= 3 << 19 ? 1 : kShortBlock + 1;
+  L.sequences = std::min(T / L.least, B);
+  if (L.sequences == 0) return L;
+  L.chunks = T / dflash::kRuleChunk + L.sequences;
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
   L.rows = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
@@ -1510,6 +1518,9 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
         return fail(DFLASH_ERR_WORKSPACE, "gdn rule workspace needs " + std::to_string(L.total) + " bytes");
       dflash::ChunkParams c{};
       c.rule = p;
+      c.least = static_cast<int>(L.least);
+      c.sequences = static_cast<int>(L.sequences);
+      c.typical = static_cast<int>(std::clamp<int64_t>((tokens + L.longest / 2) / L.longest, 1, L.sequences));
       c.chunks = static_cast<int>(L.chunks);
       c.cus = cu_count();
       c.rows = at<uint16_t>(workspace, L.rows);

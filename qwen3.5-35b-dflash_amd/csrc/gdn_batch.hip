@@ -312,13 +312,10 @@ __device__ __forceinline__ float groups_sum(float v) {
 }
 
 template <bool kBf16, int kDim>
-__global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
+__device__ __forceinline__ void rule_tokens(const RuleParams& p, const Span& s, int head) {
   constexpr int kCols = kDim / 16, kGroups = 64 / kCols, kQuads = kDim / (4 * kGroups);
-  const int b = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int khead = head / p.rep, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = wave * (kDim / 4) + 4 * (lane % kCols), group = lane / kCols;
-  const Span s = span_of(p.pool, b);
-  if (s.tokens == 0) return;
   const buf_rsrc place = make_rsrc(p.pool.recurrent + max(s.slot, 0) * p.pool.recurrent_stride + static_cast<int64_t>(head) * kDim * kDim,
                                    s.slot < 0 ? 0 : kDim * kDim * 4);
   const int at = (4 * group * kDim + col) * 4;
@@ -415,6 +412,16 @@ __global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
     if (last) break;
   }
 }
+template <bool kBf16, int kDim>
+__global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
+  const Span s = span_of(p.pool, blockIdx.x / p.Hv);
+  if (s.tokens > 0) rule_tokens<kBf16, kDim>(p, s, blockIdx.x % p.Hv);
+}
+
+// Blocks of up to so many tokens go token after token.  us, that way and 16 at a time: 64 sequences of one token 45 and 66, of two 49 and
+// 66, of three 57 and 70, of four both 66; 32 of four 41 and 42; one of one 6.7 and 7.5, of four 12.0 and 12.6; head dim 64, 32 of two 7.9 and
+// 11.0, of four 11.9 and 11.0.
+constexpr int kTokenSteps = 3;
 
 // ------------------------------------------------------------------ the rule, 16 tokens at a time
 // A workgroup holds one head's state of one sequence in registers, 32 columns a wave: register (i, x, e) of lane l is row
@@ -434,11 +441,10 @@ struct BlockShared {
 };
 
 template <bool kBf16, int kDim, bool kOut>
-__device__ __forceinline__ void rule_block(const RuleParams& p, int b, int head, BlockShared<kBf16, kDim>& lds) {
+__device__ __forceinline__ void rule_block(const RuleParams& p, const Span& s, int head, BlockShared<kBf16, kDim>& lds) {
   constexpr int kTiles = kDim / 16, kWaves = kDim / 32, kLanes = kDim / 8, kRowParts = kBf16 ? 1 : 2;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, quarter = lane >> 4;
   const int col = 32 * wave + 2 * lr, khead = head / p.rep;
-  const Span s = span_of(p.pool, b);
   const int limit = kOut ? s.tokens : s.count;
   if (limit == 0) return;
   // through a buffer, whose rows are uniform offsets: a lane's own 32 addresses would take 64 registers (no slot: nothing is read or written)
@@ -674,7 +680,15 @@ __device__ __forceinline__ void rule_block(const RuleParams& p, int b, int head,
 template <bool kBf16, int kDim>
 __global__ __launch_bounds__(2 * kDim, 3) void gdn_rule_kernel(RuleParams p) {
   __shared__ __align__(16) BlockShared<kBf16, kDim> lds;
-  rule_block<kBf16, kDim, true>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
+  const Span s = span_of(p.pool, blockIdx.x / p.Hv);
+  if (p.most && s.tokens > p.most) return;
+  if constexpr (kDim == 128) {  // four waves, as that way is cut
+    if (s.tokens <= kTokenSteps) {
+      if (s.tokens > 0) rule_tokens<kBf16, kDim>(p, s, blockIdx.x % p.Hv);
+      return;
+    }
+  }
+  rule_block<kBf16, kDim, true>(p, s, blockIdx.x % p.Hv, lds);
 }
 
 // States and conv histories after the part of the block that counts, one launch for both: the first B * Hv workgroups
@@ -684,7 +698,7 @@ __global__ __launch_bounds__(2 * kDim, 3) void gdn_advance_kernel(RuleParams p, 
   __shared__ __align__(16) BlockShared<kBf16, kDim> lds;
   const int states = p.pool.B * p.Hv;
   if (static_cast<int>(blockIdx.x) < states) {
-    rule_block<kBf16, kDim, false>(p, blockIdx.x / p.Hv, blockIdx.x % p.Hv, lds);
+    rule_block<kBf16, kDim, false>(p, span_of(p.pool, blockIdx.x / p.Hv), blockIdx.x % p.Hv, lds);
     return;
   }
   const int across = (c.channels + 16 * kDim - 1) / (16 * kDim), i = blockIdx.x - states;
@@ -713,17 +727,17 @@ constexpr int kChunk = 64, kPitch = 68;     // tokens of a chunk; floats of an L
 constexpr int kTriangle = 6;                // 16 x 32 fragments of a lower triangle of 64 x 64
 __device__ __forceinline__ int triangle(int block, int step) { return block < 2 ? block : 2 * block - 2 + step; }
 
-// Chunks of a sequence; and the sequence and chunk of an ordinal (a wave's lanes together), x = B: none; or with `of` >= 0 the
-// chunks of the sequences before that one.
-__device__ __forceinline__ int chunks_of(const PoolParams& p, int b) {
-  const int start = clampi(p.starts[b], 0, p.T);
-  return (clampi(p.starts[b + 1], start, p.T) - start + kChunk - 1) / kChunk;
+// Chunks of a sequence, none of one with fewer than `least` tokens; and the sequence and chunk of an ordinal (a wave's lanes together),
+// x = B: none.
+__device__ __forceinline__ int chunks_of(const PoolParams& p, int least, int b) {
+  const int start = clampi(p.starts[b], 0, p.T), tokens = clampi(p.starts[b + 1], start, p.T) - start;
+  return tokens < least ? 0 : (tokens + kChunk - 1) / kChunk;
 }
-__device__ __forceinline__ int2 chunk_place(const PoolParams& p, int ordinal) {
+__device__ __forceinline__ int2 chunk_place(const PoolParams& p, int least, int ordinal) {
   int base = 0;
   for (int i = 0; i < p.B; i += 64) {
     const int b = i + lane_id();
-    const int own = b < p.B ? chunks_of(p, b) : 0;
+    const int own = b < p.B ? chunks_of(p, least, b) : 0;
     int sum = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -740,10 +754,24 @@ __device__ __forceinline__ int2 chunk_place(const PoolParams& p, int ordinal) {
   }
   return make_int2(p.B, 0);
 }
-__device__ __forceinline__ int chunks_before(const PoolParams& p, int b) {
-  int sum = 0;  // bounded: starts that do not ascend may count a token many times
-  for (int i = lane_id(); i < b; i += 64) sum = min(sum + chunks_of(p, i), 1 << 24);
-  return __builtin_amdgcn_readfirstlane(wave_sum_int(sum));
+// The sequence with chunks that `ordinal` of them stand before, and the chunks before its own; x = B: none.
+__device__ __forceinline__ int2 sequence_place(const PoolParams& p, int least, int ordinal) {
+  int seen = 0, base = 0;
+  for (int i = 0; i < p.B; i += 64) {
+    const int lane = lane_id(), b = i + lane;
+    const int own = b < p.B ? chunks_of(p, least, b) : 0;
+    const uint64_t held = __ballot(own > 0);
+    const int n = __popcll(held);
+    if (seen + n > ordinal) {
+      const uint64_t at = __ballot(own > 0 && __popcll(held & ((uint64_t{1} << lane) - 1)) == ordinal - seen);
+      const int hit = __ffsll(static_cast<unsigned long long>(at)) - 1;
+      const int before = wave_sum_int(lane < hit ? own : 0);
+      return make_int2(__builtin_amdgcn_readfirstlane(i + hit), __builtin_amdgcn_readfirstlane(base + before));
+    }
+    seen += n;
+    base = min(base + wave_sum_int(own), 1 << 24);  // bounded: starts that do not ascend may count a token many times
+  }
+  return make_int2(p.B, 0);
 }
 
 // One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices: 2048 of them 48 us for 4096 tokens of one
@@ -765,7 +793,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
   auto& tm = keys_t.f;
   auto& pm = query_p.f;
   const int ordinal = blockIdx.x / p.Hv, head = blockIdx.x % p.Hv, khead = head / p.rep;
-  const int2 place = chunk_place(p.pool, ordinal);
+  const int2 place = chunk_place(p.pool, c.least, ordinal);
   if (place.x == p.pool.B) return;
   const Span s = span_of(p.pool, place.x);
   const int t0 = s.start + place.y * kChunk, n = min(kChunk, s.start + s.tokens - t0);
@@ -1320,12 +1348,12 @@ __global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
   __shared__ __align__(16) ScanShared<kDim, kTiles> lds;
   const int group = blockIdx.x / (8 * kSlices), rest = blockIdx.x % (8 * kSlices);
   const int unit = group * 8 + rest % 8;  // a head's slices on one XCD, which share all but V
-  if (unit >= p.pool.B * p.Hv) return;
-  const int b = unit / p.Hv;
-  const Span s = span_of(p.pool, b);
-  if (s.tokens == 0) return;
+  if (unit >= c.sequences * p.Hv) return;
+  const int2 place = sequence_place(p.pool, c.least, unit / p.Hv);
+  if (place.x == p.pool.B) return;
+  const Span s = span_of(p.pool, place.x);
   ScanWalk w;
-  w.base = chunks_before(p.pool, b);
+  w.base = place.y;
   w.count = min((s.tokens + kChunk - 1) / kChunk, c.chunks - w.base);
   w.head = unit % p.Hv;
   w.slice = rest / 8;
@@ -1357,15 +1385,20 @@ template <bool kBf16, int kDim>
 void launch_chunks(const ChunkParams& c, hipStream_t stream) {
   const RuleParams& p = c.rule;
   hipLaunchKernelGGL((gdn_chunk_kernel<kBf16, kDim>), dim3(c.chunks * p.Hv), dim3(256), 0, stream, c);
-  const int units = (p.pool.B * p.Hv + 7) / 8 * 8;
+  const int units = (c.sequences * p.Hv + 7) / 8 * 8, typical = c.typical * p.Hv;
   // A CU runs a workgroup about as fast as several would share it.  With 32 columns one reads half as much a column and takes 1.5 to 1.7 times as long as with 16: it
   // pays where that saves rounds of the card.  us, 16 and 32 columns, by sequences of 1024 tokens: one 50 and 60, two 90 and 75, four 160 and
   // 135; head dim 64, 16 heads, of 512 tokens: six 36 and 35, twelve 58 and 63.
-  const auto rounds = [&](int columns) { return (units * (kDim / columns) + c.cus - 1) / c.cus; };
+  const auto rounds = [&](int columns) { return (typical * (kDim / columns) + c.cus - 1) / c.cus; };
   if (5 * rounds(32) <= 3 * rounds(16))
     hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 2>), dim3(units * (kDim / 32)), dim3(512), 0, stream, c);
   else
     hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 1>), dim3(units * (kDim / 16)), dim3(512), 0, stream, c);
+  if (c.least > 1) {
+    RuleParams rest = p;
+    rest.most = c.least - 1;
+    hipLaunchKernelGGL((gdn_rule_kernel<kBf16, kDim>), dim3(p.pool.B * p.Hv), dim3(2 * kDim), 0, stream, rest);
+  }
 }
 
 void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t stream) {
@@ -1373,10 +1406,6 @@ void launch_gdn_chunks(int dim, bool bf16, const ChunkParams& c, hipStream_t str
   else bf16 ? launch_chunks<true, 64>(c, stream) : launch_chunks<false, 64>(c, stream);
 }
 
-// Blocks of up to so many tokens go token after token.  us, that way and 16 at a time: 64 sequences of one token 45 and 66, of two 49 and
-// 66, of three 57 and 70, of four both 66; 32 of four 41 and 42; one of one 6.7 and 7.5, of four 12.0 and 12.6; head dim 64, 32 of two 7.9 and 11.0, of four
-// 11.9 and 11.0.
-constexpr int64_t kTokenSteps = 3;
 template <bool kBf16, int kDim>
 void launch_rule(const RuleParams& p, int64_t longest, hipStream_t stream) {
   if (longest <= kTokenSteps) hipLaunchKernelGGL((gdn_token_kernel<kBf16, kDim>), dim3(p.pool.B * p.Hv), dim3(256), 0, stream, p);

@@ -439,6 +439,7 @@ struct RuleParams {
   int Hv, rep;                    // value heads, of each key head
   int normalise;
   float scale;
+  int most;                       // blocks of more tokens are left to another launch; 0: none are
   uint16_t* out;                  // [T][Hv][dim]
 };
 // Blocks of many tokens, 64 at a time: what a chunk's tokens need beside their rows, per (chunk, value head).
@@ -451,7 +452,9 @@ struct ChunkScalars {
 };
 struct ChunkParams {
   RuleParams rule;
-  int chunks;                     // at most: T / 64 + B
+  int least;                      // blocks of fewer tokens are left to another launch
+  int sequences, typical;         // with at least so many tokens: at most; about
+  int chunks;                     // at most: T / 64 + sequences
   int cus;
   uint16_t* rows;                 // [chunks][key heads][keys, queries][4 row blocks][dim / 32][64 lanes][8]
   float* t;                       // [chunks][Hv][6 fragments][2 halves][64 lanes][4]

@@ -168,6 +168,21 @@ def test_starts_that_are_no_such_thing_stay_inside(pkg, device, longest):
     assert same_bits(d["recurrent"][3:].cpu(), held[0].cpu()) and same_bits(d["history"][3:].cpu(), held[1].cpu())
 
 
+def test_starts_of_many_sequences_that_are_no_such_thing_stay_inside(pkg, device):
+    """The same of a batch whose long and short blocks have launches of their own: more long blocks than the tokens could hold."""
+    layer = Layer(pkg, device, [20] * 30, seed=3, counts=[0] * 30)
+    d, heads = layer.d, torch.full((664, 4, 128), 3.0, dtype=BF16, device=device)
+    size = pkg.ops.gdn_rule_workspace_bytes(600, 2, 4, 128, 30, 300)
+    assert size > 0
+    room = torch.full((size + (1 << 20),), 0x5A, dtype=torch.uint8, device=device)
+    before = d["recurrent"].clone()
+    for bad in ([0, 600] * 15 + [0], [0] + [600, 0] * 15, [0] + [40, 600] * 15, list(range(600, -20, -20)), [1 << 30] * 31, [-(1 << 31), 1 << 30] * 15 + [5]):
+        d["starts"].copy_(torch.tensor(bad, dtype=torch.int32))
+        layer.rule(heads[:600], longest=300, workspace=room[:size])
+    torch.cuda.synchronize()
+    assert (heads[600:] == 3).all() and (room[size:] == 0x5A).all() and same_bits(before.cpu(), d["recurrent"].cpu())
+
+
 def test_rows_of_drafts_that_are_no_such_thing_stay_inside(pkg, device):
     _, dev = drafts(device, [5, 4, 7], vocab=3001)
     size = pkg.ops.verify_drafts_workspace_bytes(16, 3001, 3, True)

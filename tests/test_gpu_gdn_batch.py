@@ -169,15 +169,40 @@ def test_blocks_in_pieces(pkg, device):
         layer.check_state(want[2], want[3], str(cut))
 
 
+@pytest.mark.parametrize("longest", [60, 200])
 @pytest.mark.parametrize("dim,dtype", [(128, BF16), (128, FP16), (64, BF16), (64, FP16)])
-def test_rule_of_prompts_with_many_heads(pkg, device, dim, dtype):
-    """Sequences and heads enough that a workgroup takes 32 columns of the state; blocks that end at every place of a chunk, empty and
-    fresh ones among them, counts inside."""
+def test_rule_of_prompts_with_many_heads(pkg, device, dim, dtype, longest):
+    """Sequences and heads enough that a workgroup takes 32 columns of the state (at 60, which says that all are about alike); blocks that
+    end at every place of a chunk, empty and fresh ones among them, counts inside."""
     spans = [70, 1, 130, 0, 64, 200, 33, 129] * (1 if dim == 128 else 2)
     for counts in (None, [min(n, 65) - b % 3 for b, n in enumerate(spans)]):
         layer = Layer(pkg, device, spans, key_heads=4, value_heads=8, dim=dim, dtype=dtype, seed=11, spare=2, missing=(2,), fresh=(0, 5),
                       counts=counts)
         out = filled(layer, layer.hv, dim)
-        layer.rule(out, longest=200)
+        layer.rule(out, longest=longest)
         layer.check_rule(out)
         assert (out[layer.tokens:] == 7.0).all()
+
+
+@pytest.mark.parametrize("longest", [None, 1, 16, 250])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (128, FP16), (64, BF16), (64, FP16)])
+def test_rule_of_long_and_short_blocks(pkg, device, dim, dtype, longest):
+    """Prompts among verify blocks and single tokens, whose launches share the batch: every sequence in exactly one of them."""
+    spans = [1, 2, 200, 0, 3, 33, 32, 16, 70, 1, 34, 31, 1, 5, 250, 0, 4, 17, 64, 65, 1, 1, 12, 40, 1, 2] * (1 if dim == 128 else 3)
+    for counts in (None, [(n * 3) // 4 + b % 2 for b, n in enumerate(spans)], [0] * len(spans)):
+        layer = Layer(pkg, device, spans, value_heads=6, dim=dim, dtype=dtype, seed=12, spare=2, missing=(1, 8), fresh=(0, 2, 6, 20), counts=counts)
+        out = filled(layer, layer.hv, dim)
+        layer.rule(out, longest=longest)
+        layer.check_rule(out)
+        assert (out[layer.tokens:] == 7.0).all()
+
+
+def test_rule_of_many_sequences(pkg, device):
+    """More sequences than are searched at a time, prompts at the search's ends."""
+    spans = [1] * 200
+    for b, n in ((0, 40), (63, 70), (64, 65), (127, 33), (130, 130), (199, 99)):
+        spans[b] = n
+    layer = Layer(pkg, device, spans, value_heads=2, seed=13, fresh=(63, 199), missing=(64,))
+    layer.check_rule(layer.rule(longest=130))
+    layer.d["starts"][:] = 0   # every block empty
+    assert layer.rule(longest=130).shape == (layer.total, 2, 128)
