@@ -1357,6 +1357,14 @@ int check_rule(const dflash_rule* r, const dflash_state_pool* c, const char* nam
   return DFLASH_OK;
 }
 
+// Whether any byte of 16-bit rows [tokens][heads][size] lies in what a contiguous output of `out_size` values spans.
+bool rows_meet(const dflash_rows& r, int64_t tokens, int64_t heads, int64_t size, const void* out, int64_t out_size) {
+  typedef unsigned __int128 wide;
+  const wide from = reinterpret_cast<uintptr_t>(r.data), to = reinterpret_cast<uintptr_t>(out);
+  const wide end = from + 2 * (static_cast<wide>(tokens - 1) * r.token_stride + static_cast<wide>(heads - 1) * r.head_stride + size);
+  return from < to + 2 * static_cast<wide>(out_size) && to < end;
+}
+
 dflash::RuleParams rule_params(const dflash_rule* r, const dflash_state_pool* c, const dflash::PoolParams& pool) {
   dflash::RuleParams p{};
   p.pool = pool;
@@ -1434,7 +1442,8 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
     if (int r = conv_params(pool, x, "gdn conv x", pool_params(pool, starts, counts, fresh, tokens), &p)) return r;
     if (!weight || !aligned16(weight) || !out || !aligned16(out))
       return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: weight or out is NULL or not 16-byte aligned");
-    if (out == x->data) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: out cannot be x, whose rows are read after a row is written");
+    if (rows_meet(*x, tokens, 1, pool->channels, out, tokens * pool->channels))
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: out cannot be x or overlap it, whose rows are read after a row is written");
     p.weight = static_cast<const uint16_t*>(weight);
     p.out = static_cast<uint16_t*>(out);
     dflash::launch_gdn_conv(pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
@@ -1508,8 +1517,11 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
     if (longest < 0) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: longest must not be negative");
     if (tokens * pool->value_heads > (1 << 28)) return fail(DFLASH_ERR_UNSUPPORTED, "gdn rule: tokens * value_heads must be at most 2^28");
     if (!out || !aligned16(out)) return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out is NULL or not 16-byte aligned");
-    if (out == rule->query.data || out == rule->key.data || out == rule->value.data)
-      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out cannot be the query, key or value, which are read after it is written");
+    const int64_t outputs = tokens * pool->value_heads * pool->head_dim;
+    if (rows_meet(rule->query, tokens, rule->key_heads, pool->head_dim, out, outputs) ||
+        rows_meet(rule->key, tokens, rule->key_heads, pool->head_dim, out, outputs) ||
+        rows_meet(rule->value, tokens, pool->value_heads, pool->head_dim, out, outputs))
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out cannot be or overlap the query, key or value, which are read after it is written");
     dflash::RuleParams p = rule_params(rule, pool, pool_params(pool, starts, counts, fresh, tokens));
     p.out = static_cast<uint16_t*>(out);
     const RuleLayout L = rule_layout(tokens, rule->key_heads, pool->value_heads, pool->head_dim, pool->sequences, longest);
@@ -1550,6 +1562,8 @@ int dflash_gdn_advance(const dflash_state_pool* pool, const dflash_rows* x, cons
     const dflash::PoolParams params = pool_params(pool, starts, counts, fresh, tokens);
     dflash::ConvParams c{};
     if (int r = conv_params(pool, x, "gdn advance x", params, &c)) return r;
+    if (pool->sequences * (pool->value_heads + pool->channels / (16 * pool->head_dim) + 1) > (1 << 24))
+      return fail(DFLASH_ERR_UNSUPPORTED, "gdn advance: too many sequences, value heads and channels for a launch");
     dflash::launch_gdn_advance(static_cast<int>(pool->head_dim), pool->dtype == DFLASH_DTYPE_BF16, rule_params(rule, pool, params),
                                c, static_cast<hipStream_t>(stream));
     return launch_status("gdn advance");

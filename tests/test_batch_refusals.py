@@ -78,6 +78,7 @@ def test_conv_refusals(pkg):
                         (dict(x=_rows(lib, token_stride=508)), "multiples of 8"), (dict(x=_rows(lib, token_stride=-512)), "multiples of 8"),
                         (dict(weight=None), "weight"), (dict(weight=ADDRESS + 8), "weight"), (dict(out=None), "out"),
                         (dict(out=ADDRESS + 8), "out"), (dict(out=ADDRESS), "out cannot be x"), (dict(starts=None), "starts"),
+                        (dict(out=ADDRESS + 2 * 512 * 3 - 16), "overlap"), (dict(out=ADDRESS - 2 * 512 * 3 + 16), "overlap"),
                         (dict(tokens=-1), "2\\^20"), (dict(tokens=(1 << 20) + 1), "2\\^20"), (dict(tokens=1 << 62), "2\\^20")]:
         refused(lib, _conv, message, **kw)
     _conv(lib, tokens=0)                                         # nothing to do
@@ -97,11 +98,15 @@ def test_rule_refusals(pkg):
     for kw, message in [(dict(rule=0), "NULL"), (dict(rule=_rule(lib, query=_rows(lib, None))), "query"), (dict(starts=None), "starts"),
                         (dict(tokens=-1), "2\\^20"), (dict(tokens=1 << 62), "2\\^20"), (dict(longest=-1), "longest"), (dict(out=None), "out"),
                         (dict(out=ADDRESS + 8), "out"), (dict(out=ADDRESS), "out cannot be"), (dict(tokens=500, ws=None), "workspace"),
+                        (dict(rule=_rule(lib, value=_rows(lib, 2 * ADDRESS - 2 * (2 * 512 + 256) + 16))), "overlap"),
+                        (dict(rule=_rule(lib, query=_rows(lib, 2 * ADDRESS + 2 * 3 * 256 - 16))), "overlap"),
                         (dict(tokens=500, ws=ADDRESS + 8), "workspace"), (dict(longest=33, tokens=33, size=100), "workspace"), (dict(tokens=1 << 20, pool=_pool(lib, value_heads=512)), "2\\^28")]:
         refused(lib, _delta, message, **kw)
     for kw, message in [(dict(rule=0), "NULL"), (dict(counts=None), "counts"), (dict(starts=None), "starts"),
                         (dict(x=_rows(lib, ADDRESS + 2)), "x"), (dict(tokens=1 << 21), "2\\^20")]:
         refused(lib, _advance, message, **kw)
+    refused(lib, _advance, "too many", pool=_pool(lib, sequences=1 << 19, value_heads=1, channels=1 << 16, history_stride=3 << 16),
+            rule=_rule(lib, key_heads=1), x=_rows(lib, token_stride=1 << 16))
     _delta(lib, tokens=0)
     _delta(lib, pool=_pool(lib, sequences=0))
     _advance(lib, tokens=0)
