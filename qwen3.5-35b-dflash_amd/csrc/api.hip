@@ -1486,7 +1486,7 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   // prompts 94 and 92; 16 heads of 64, 1024 tokens and 15 of one 52 and 43.
   L.least = B * Hv * D * D <= 3 << 19 ? 1 : kShortBlock + 1;
   L.sequences = std::min(T / L.least, B);
-  if (L.sequences == 0) return L;
+  if (L.sequences == 0 || L.longest < L.least) return L;
   L.chunks = T / dflash::kRuleChunk + L.sequences;
   Carver c;
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;

@@ -698,7 +698,7 @@ def gdn_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay:
     ``beta``, or with ``a_log`` and ``dt_bias`` (fp32 ``[value heads]``) a layer's projections: ``g = -exp(a_log) softplus(decay +
     dt_bias)``, ``beta = sigmoid(beta)``.  The slot then holds the state after ``counts[b]`` tokens (int32 ``[B]``; None: all of them;
     0: it stays as it is, as a verify block's does until :func:`gdn_advance`).  ``longest``: tokens of the longest block, if the caller
-    knows it, for the choice of the kernels.  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
+    knows it, for the choice of the kernels (else as if none were twice the average).  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
     tensor to write into, which shares no memory with the rows).  A NaN or infinity in a token may reach all outputs of its block and head.
     """
     if _plain(value) and query is not None and (host := _lib.host()):
