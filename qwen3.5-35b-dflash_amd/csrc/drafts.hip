@@ -150,11 +150,14 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   const auto take = [&](int o, const float (&f)[8]) {
     float m = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
     if (t == 0.0f) {
-      if (m > top || (at == kNowhere && m == top)) {
-        top = m;
+      if (m >= top) {
+        int place = kNowhere;
 #pragma unroll
         for (int i = 7; i >= 0; --i)
-          if (f[i] == m) at = data.first(o) + i;
+          if (f[i] == m) place = data.first(o) + i;
+        // by places, not by the order of visits: a row's first eight, where it is not whole, is seen last
+        if (m > top || place < at) at = place;
+        top = m;
       }
       return;
     }
