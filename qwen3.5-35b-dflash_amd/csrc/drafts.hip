@@ -494,8 +494,10 @@ __global__ __launch_bounds__(256) void draft_token_kernel(DraftParams p) {
     __syncthreads();
     if (tid == chosen) base = run - mine;
     __syncthreads();
+    // Added up token by token the part's end may come out a rounding lower than its sum, and not above the goal: then the part's last
+    // token is the one, and `last` holds it.  Where no part's sum exceeds the goal (a random number of one or above) it is the row's.
     if (chosen != kNowhere) walk(chosen * p.part_octets, min((chosen + 1) * p.part_octets, eights), base, goal, true);
-    if (found == kNowhere) walk(0, eights, 0.0, INFINITY, true);  // no sum exceeds it (a random number of one or above)
+    else walk(0, eights, 0.0, INFINITY, true);
   } else {
     const double whole = walk(0, eights, 0.0, INFINITY, false);
     if (whole > 0.0) walk(0, eights, 0.0, u * whole, false);
