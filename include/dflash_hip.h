@@ -470,8 +470,9 @@ int dflash_gdn_advance(const dflash_state_pool* pool, const dflash_rows* x, cons
  * draft NULL: each drafted token was chosen outright (q is 1 there).  A temperature that is not above 0: p is 1 at the first
  * largest logit and the drafter's choice counts as outright.  A drafted token outside the vocabulary is never accepted.  Where
  * max(p - q, 0) is zero everywhere the token is drawn from p; where p is too (no logit above -infinity), and in a sequence
- * without rows, token is -1.  NaN logits count as -infinity, +infinity as the largest fp32 number.  Sums and the weights of the
- * rows that tokens are drawn from are 64 bits; the result does not depend on how the work is split.
+ * without rows, token is -1.  NaN logits count as -infinity, +infinity as the largest fp32 number.  What decides is held in 64
+ * bits, weights and sums: a row is accepted or not whatever other rows the call has, and a draw depends on how the work is split only
+ * where its number lies within such roundings (1e-13 of the sum) of the border between two tokens.
  * Logits of dtype BF16, F16 or F32, rows of `vocab`, target_stride and draft_stride elements apart.
  * Constraints: vocab <= 2^24, rows <= 2^20, sequences <= 2^20.
  */

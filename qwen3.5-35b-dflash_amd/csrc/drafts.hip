@@ -7,9 +7,10 @@
 // row behind (r + 1, which tests nothing then) or of the last row itself.  So the tokens follow the target's distribution
 // whatever the drafter's is.
 //
-// A whole number hangs on a comparison, so what is compared carries 64 bits: the sums, and in the rows that tokens are drawn
-// from each weight, since one of 2.5e5 running sums lies within 1e-7 of a given number once in forty times.  The
-// acceptance test compares one number a row; its sums add 32-bit exponentials in 64 bits.
+// A whole number hangs on a comparison, so what decides carries 64 bits, weights and sums.  In the rows that tokens are drawn
+// from that is every weight, since one of 2.5e5 running sums lies within 1e-7 of a given number once in forty times.  The
+// acceptance test compares one number a row: sums of 32-bit exponentials tell on which side it is, but once in 3e4 rows or so, and
+// those rows are summed again.  So what is accepted depends on the row alone, not on how the rows of a call are cut.
 //
 // Logits that are NaN count as -infinity, +infinity as the largest fp32 number.  A row without a logit above -infinity has no
 // token to give.
@@ -130,7 +131,11 @@ __device__ __forceinline__ double wave_sum64(double v) {
 
 // ------------------------------------------------------------------ every row
 // Largest logit and sum of exponentials of one part of one row; y: target or drafter.  One pass: a thread keeps the largest logit
-// it has seen and the sum relative to it.  Bound by memory: 478 MB of logits (513 rows and their drafter's, 248 320 tokens in bf16) 83 us,
+// it has seen and the sum relative to `base`, which follows in steps of a factor of 2^16 at least, so that a row which rises all along
+// does not round the sum again and again.  The exponentials have 32 bits, eight are added in 32 and those sums in 64.  How far a
+// row's sum is off: an exponential of z = (l - base) c by the three roundings of z, 2.1 |z| 2^-24, and two of its own, the sum of eight by
+// four; |z| is at most 32 (16 and `base`'s own rounding) or what the weight 2^-y of the token says, so up to y = 40 that is
+// (6 + 2.1 * 40) 2^-24 < 2^-17, and all the tokens that weigh less add nothing to it.  Bound by memory: 478 MB of logits (513 rows and their drafter's, 248 320 tokens in bf16) 83 us,
 // 5.8 TB/s with what the last-level cache holds.
 template <int kType>
 __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
@@ -144,9 +149,10 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   if (side && (t == 0.0f || row + 1 == p.starts[b + 1])) return;
   const Row<kType> data(side ? p.draft : p.target, side ? p.draft_stride : p.target_stride, row, p.V);
   const int first = split * p.split_octets, last = min(first + p.split_octets, data.eights()), tid = threadIdx.x;
-  float top = kNone, sum = 0.f;
+  float top = kNone, base = kNone;
+  double sum = 0.0;
   int at = kNowhere;
-  const float c = t > 0.0f ? static_cast<float>(scale_of(t)) : 0.0f;
+  const float c = t > 0.0f ? static_cast<float>(scale_of(t)) : 0.0f, ahead = t > 0.0f ? 16.0f / c : 0.0f;
   const auto take = [&](int o, const float (&f)[8]) {
     float m = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
     if (t == 0.0f) {
@@ -161,14 +167,15 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
       }
       return;
     }
-    if (m > top) {
-      sum *= exp2f((top - m) * c);
-      top = m;
+    top = fmaxf(top, m);
+    if (m > base + ahead) {
+      sum *= static_cast<double>(exp2f((base - m) * c));
+      base = m;
     }
     float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i & 1] += __builtin_amdgcn_exp2f((f[i] - top) * c);
-    sum += s[0] + s[1];
+    for (int i = 0; i < 8; ++i) s[i & 1] += __builtin_amdgcn_exp2f((f[i] - base) * c);
+    sum += static_cast<double>(s[0] + s[1]);
   };
   // the eights inside the row, four loads in flight; its ends
   const int inner0 = max(first, data.ahead ? 1 : 0), inner1 = min(last, (p.V + data.ahead) / 8);
@@ -211,7 +218,7 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   if ((tid & 63) == 0) bests[tid >> 6] = best;
   __syncthreads();
   best = better(better(bests[0], bests[1]), better(bests[2], bests[3]));
-  const double s = wave_sum64(static_cast<double>(sum) * static_cast<double>(exp2f((top - best.top) * c)));
+  const double s = t > 0.0f ? wave_sum64(sum * weight(base, best.top, scale_of(t))) : 0.0;
   if ((tid & 63) == 0) sums[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) {
@@ -244,14 +251,17 @@ __device__ __forceinline__ Whole joined(const DraftParams& p, int side, int row,
 }
 
 // One workgroup a sequence, a wave a row: how many drafted tokens are accepted, and the row that the next one is drawn from.
-// Greedy sequences are done here.  A chain of dependent loads, 5.7 us for one sequence, 6.7 for 64; with a wave for each of 16 rows, since
-// four waves take their rows in turn.
+// Greedy sequences are done here.  A chain of dependent loads, 5.7 us for one block of 16 rows, 6.7 for 64; with a wave for each of 16 rows,
+// since four waves take their rows in turn.  A row whose test the sums of 32-bit exponentials leave open is summed again in 64 bits by the
+// whole workgroup, in an order of the tokens' places alone (50 us for a row of 248 320 tokens, the drafter's as long).
 constexpr int kChooseWaves = 16;
+constexpr double kDoubt = 0x1p-15;  // both sides' sums are off by less than 2^-17
+enum Outcome : int { kAccepted, kRejected, kOpen };
 template <int kType>
 __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftParams p) {
-  __shared__ int stop;
   __shared__ DraftChoice choices[kChooseWaves];
-  __shared__ int largest[kChooseWaves];
+  __shared__ int largest[kChooseWaves], outcomes[kChooseWaves];
+  __shared__ double sums[2][kChooseWaves];
   const int b = blockIdx.x, wave = threadIdx.x >> 6;
   const int start = clampi(p.starts[b], 0, p.rows), n = clampi(p.starts[b + 1], start, p.rows) - start;
   const float t = temperature_of(p, b);
@@ -263,38 +273,67 @@ __global__ __launch_bounds__(64 * kChooseWaves) void draft_choose_kernel(DraftPa
     }
     return;
   }
-  if (threadIdx.x == 0) stop = n - 1;
-  __syncthreads();
-  int i0 = 0;
+  const double scale = t > 0.0f ? scale_of(t) : 0.0;
+  // whether u q(x) < p(x), where the sums of the row's weights are known
+  const auto test = [&](int row, int x, float target_top, double target_sum, bool ask, float draft_top, double draft_sum) {
+    const auto chance = [&](const void* data, int64_t stride, float top, double sum) {
+      return x >= 0 && x < p.V && sum > 0.0 ? weight(Row<kType>(data, stride, row, p.V).at(x), top, scale) / sum : 0.0;
+    };
+    const double px = chance(p.target, p.target_stride, target_top, target_sum);
+    const double qx = (ask ? chance(p.draft, p.draft_stride, draft_top, draft_sum) : 1.0) * static_cast<double>(p.uniforms[row]);
+    return fabs(px - qx) < kDoubt * fmax(px, qx) ? make_int2(qx < px, kOpen) : make_int2(qx < px, qx < px ? kAccepted : kRejected);
+  };
+  int i0 = 0, stop = -1;
   for (;; i0 += kChooseWaves) {
     const int i = i0 + wave, row = start + i;
     if (i < n) {
       const bool drafted = i < n - 1, ask = drafted && p.draft && t > 0.0f;
-      const int x = drafted ? p.drafted[row] : -1;
-      const bool inside = x >= 0 && x < p.V;
       const Whole target = joined(p, 0, row, t);
       Whole draft{kNone, kNowhere, 0.0};
       if (ask) draft = joined(p, 1, row, t);
-      bool accepted = false;
-      if (drafted && t == 0.0f) {
-        accepted = inside && x == target.at && p.uniforms[row] < 1.0f;
-      } else if (drafted) {
-        const double scale = scale_of(t);
-        const auto chance = [&](const void* data, int64_t stride, const Whole& r) {
-          return inside && r.sum > 0.0 ? weight(Row<kType>(data, stride, row, p.V).at(x), r.top, scale) / r.sum : 0.0;
-        };
-        const double px = chance(p.target, p.target_stride, target);
-        const double qx = ask ? chance(p.draft, p.draft_stride, draft) : 1.0;
-        accepted = static_cast<double>(p.uniforms[row]) * qx < px;
+      int outcome = kRejected;
+      if (drafted) {
+        const int x = p.drafted[row];
+        if (t == 0.0f) outcome = x >= 0 && x < p.V && x == target.at && p.uniforms[row] < 1.0f ? kAccepted : kRejected;
+        else outcome = test(row, x, target.top, target.sum, ask, draft.top, draft.sum).y;
       }
       if (lane_id() == 0) {
         choices[wave] = DraftChoice{row, drafted, target.top, draft.top};
         largest[wave] = target.at;
-        if (!accepted) atomicMin(&stop, i);
+        outcomes[wave] = outcome;
       }
     }
     __syncthreads();
-    if (stop < i0 + kChooseWaves) break;  // at the last row at the latest
+    const int own = lane_id() < min(kChooseWaves, n - i0) ? outcomes[lane_id()] : kAccepted;
+    for (uint64_t held = __ballot(own != kAccepted); held; held &= held - 1) {  // the same in all waves
+      const int w = __ffsll(static_cast<unsigned long long>(held)) - 1;
+      const DraftChoice c = choices[w];
+      bool accepted = false;
+      if (__shfl(own, w, 64) == kOpen) {
+        for (int side = 0; side < (p.draft ? 2 : 1); ++side) {
+          const Row<kType> data(side ? p.draft : p.target, side ? p.draft_stride : p.target_stride, c.row, p.V);
+          double sum = 0.0;
+#pragma unroll 4
+          for (int j = threadIdx.x; j < p.V; j += 64 * kChooseWaves) sum += weight(data.at(j), side ? c.draft_top : c.target_top, scale);
+          sum = wave_sum64(sum);
+          if (lane_id() == 0) sums[side][wave] = sum;
+        }
+        __syncthreads();
+        double whole[2] = {0.0, 0.0};
+        for (int k = 0; k < kChooseWaves; ++k) {
+          whole[0] += sums[0][k];
+          if (p.draft) whole[1] += sums[1][k];
+        }
+        accepted = test(c.row, p.drafted[c.row], c.target_top, whole[0], p.draft != nullptr, c.draft_top, whole[1]).x;
+        __syncthreads();
+      }
+      if (!accepted) {  // at the last row at the latest
+        stop = i0 + w;
+        break;
+      }
+    }
+    if (stop >= 0) break;
+    __syncthreads();
   }
   if (threadIdx.x == 0) {
     DraftChoice c = choices[stop - i0];

@@ -775,7 +775,7 @@ def verify_drafts(target: torch.Tensor, drafted: torch.Tensor, starts: torch.Ten
     With the softmaxes ``p`` and ``q`` a token ``x`` is accepted iff ``uniforms[r] * q(x) < p(x)`` (fp32 ``[rows]`` in [0, 1)); the first that is not
     is replaced by a draw from ``max(p - q, 0)`` with the next row's uniform, and all accepted are followed by a draw from the last
     row's ``p`` with its own: the emitted tokens follow the target's distribution.  One row a sequence is plain sampling.  Logits bf16,
-    fp16 or fp32, NaN as -infinity; sums, and the weights that tokens are drawn by, in 64 bits.
+    fp16 or fp32, NaN as -infinity; weights and sums that a token or its acceptance hangs on have 64 bits.
     """
     if _plain(target) and (host := _lib.host()):
         done = host.verify_drafts(target, drafted, starts, uniforms, draft, temperature, workspace)

@@ -1,11 +1,72 @@
-"""GPU: draws of ``verify_drafts`` next to their limits."""
+"""GPU: acceptance tests and draws of ``verify_drafts`` next to their limits, which sums of 64 bits decide, alone or among others."""
 import math
 
 import pytest
 import torch
 
+from batch_util import chances
+from test_gpu_verify_drafts import check, make
+
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def at_the_limit(c, seed):
+    """Every row's random number is one of the two fp32 numbers next to p(x) / q(x), or to p(x) where the token was chosen outright."""
+    gen = torch.Generator().manual_seed(seed)
+    starts, rows = c["starts"].tolist(), c["target"].shape[0]
+    for b in range(len(starts) - 1):
+        t = 1.0 if c["temperature"] is None else float(c["temperature"][b])
+        for r in range(starts[b], starts[b + 1] - 1):
+            limit = float(chances(c["target"][r], t)[int(c["drafted"][r])])
+            if c["draft"] is not None:
+                limit /= float(chances(c["draft"][r], t)[int(c["drafted"][r])])
+            near = torch.tensor(limit, dtype=torch.float32)
+            other = torch.nextafter(near, torch.tensor(0.0 if float(near) > limit else math.inf))
+            c["uniforms"][r] = near if torch.rand((), generator=gen) < 0.5 else other
+    return c
+
+
+def rows_of(c, b):
+    lo, hi = int(c["starts"][b]), int(c["starts"][b + 1])
+    return {k: None if v is None else v[lo:hi].clone() for k, v in c.items() if k not in ("starts", "temperature")} | {
+        "starts": torch.tensor([0, hi - lo], dtype=torch.int32), "temperature": None if c["temperature"] is None else c["temperature"][b:b + 1]}
+
+
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("vocab,dtype", [(509, FP16), (32_001, BF16), (32_001, FP32), (100_277, FP32)])
+def test_acceptance_at_its_limit(pkg, device, vocab, dtype, one):
+    """Off by a step of fp32 at most, so that sums have to tell 6e-8 of them apart: all sequences in a call, and single ones alone."""
+    spans = [2, 3, 2, 4] * 10
+    c = make(spans, vocab, dtype, 5, noise=0.3, one=one, temperature=0.6 + 0.02 * torch.arange(40.0))
+    c["target"] = c["target"] * 0.2 if vocab == 509 else c["target"]
+    check(pkg, device, at_the_limit(c, 1))
+    for b in range(0, 40, 5):
+        check(pkg, device, rows_of(c, b), f"sequence {b}")
+
+
+@pytest.mark.parametrize("order", [1, -1])
+def test_acceptance_of_sorted_rows(pkg, device, order):
+    """Logits that rise or fall all along: a running maximum that moves with every token, or never."""
+    vocab, spans = 248_320, [2, 2, 3]
+    c = make(spans, vocab, FP32, 6, one=True)
+    line = torch.linspace(-6.0, 1.0, vocab)
+    for r in range(sum(spans)):
+        c["target"][r] = line if order > 0 else line.flip(0)
+        c["target"][r] += 1e-3 * r
+        c["drafted"][r] = vocab // 2 + r
+    check(pkg, device, at_the_limit(c, 2))
+
+
+def test_numbers_exactly_at_the_limit(pkg, device):
+    """p is a power of two and the random number the same: not below it, so not accepted; q of one half beside it."""
+    for vocab in (1024, 65_536):
+        for dtype in (BF16, FP16, FP32):
+            c = make([2, 2], vocab, dtype, 0, one=True)
+            c["target"][:] = 1.5
+            c["uniforms"][:] = torch.tensor([1.0 / vocab, 0.25, (1.0 - 2.0 ** -24) / vocab, 0.25])
+            dev = {k: None if v is None else v.to(device) for k, v in c.items()}
+            assert pkg.ops.verify_drafts(**dev).accepted.tolist() == [0, 1], (vocab, dtype)
 
 
 def test_a_part_whose_end_the_sum_hides(pkg, device):
