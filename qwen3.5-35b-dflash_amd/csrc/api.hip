@@ -1492,7 +1492,7 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   const size_t each = static_cast<size_t>(L.chunks * Hv), part = 6 * 64 * 16;
   L.rows = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
   L.t = c.take(each * 2 * part);
-  L.p = c.take(each * 2 * part);
+  L.p = c.take(each * 3 * part);
   L.kt = c.take(static_cast<size_t>(L.chunks * Hk) * 2 * 2 * D * dflash::kRuleChunk);
   L.scalars = c.take(each * sizeof(dflash::ChunkScalars));
   L.total = c.off;

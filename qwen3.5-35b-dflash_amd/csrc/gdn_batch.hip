@@ -582,11 +582,10 @@ __device__ __forceinline__ void rule_block(const RuleParams& p, const Span& s, i
           const uint4 part = make_uint4(c[i][0], c[i][1], c[i][2], c[i][3]);
           if (!kBf16 && i < 2) ks[x] = mfma16x16x32(k[kRowParts - 1], part, ks[x]);
           ks[x] = mfma16x16x32(k[0], part, ks[x]);
-          if constexpr (kOut)
-            if (i < 2) {
-              if (!kBf16 && i < 1) qs[x] = mfma16x16x32(q[kRowParts - 1], part, qs[x]);
-              qs[x] = mfma16x16x32(q[0], part, qs[x]);
-            }
+          if constexpr (kOut) {
+            if (!kBf16 && i < 2) qs[x] = mfma16x16x32(q[kRowParts - 1], part, qs[x]);
+            qs[x] = mfma16x16x32(q[0], part, qs[x]);
+          }
         }
       }
     }
@@ -720,9 +719,9 @@ __global__ __launch_bounds__(2 * kDim, 3) void gdn_advance_kernel(RuleParams p, 
 //
 // Precision: the products take 16-bit operands of the matrix cores and sum in fp32.  Raw rows are 16 bits as they are (fp16:
 // two bf16 parts, since states need bf16's range), norms and gates stand beside them as fp32 factors.  What meets them (S, X, U,
-// T) is cut into three bf16 parts, 24 bits, and of their products those above 2^-24 of the whole are taken; for what only an
-// output sees (Q S, P U) two parts, 2^-16, far under the half step that the output is rounded by.  So states come out as from
-// fp32 products, at 2/3 to 1/3 of the 16-bit rate instead of 1/16 of it.
+// T, P) is cut into three bf16 parts, 24 bits, and of their products those above 2^-24 of the whole are taken.  So states and outputs
+// come out as from fp32 products, at 1/3 to 1/6 of the 16-bit rate instead of 1/16 of it.  (Two parts for what only an output sees
+// would be exact enough for the output's own rounding, but not where its terms cancel: a prompt of 4096 tokens took 147 us so, 158 now.)
 constexpr int kChunk = 64, kPitch = 68;     // tokens of a chunk; floats of an LDS row
 constexpr int kTriangle = 6;                // 16 x 32 fragments of a lower triangle of 64 x 64
 __device__ __forceinline__ int triangle(int block, int step) { return block < 2 ? block : 2 * block - 2 + step; }
@@ -964,14 +963,14 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
         x[i] = tm[row][col + i] * beta[col + i];
         y[i] = pm[row][col + i];
       }
-      uint32_t pp[2][4];
-      cut<2, 8>(y, pp);
+      uint32_t pp[3][4];
+      cut<3, 8>(y, pp);
       float* t = c.t + (at * kTriangle + f) * 512 + lane * 4;
       *reinterpret_cast<float4*>(t) = make_float4(x[0], x[1], x[2], x[3]);
       *reinterpret_cast<float4*>(t + 256) = make_float4(x[4], x[5], x[6], x[7]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<uint4*>(c.p + ((at * 2 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(pp[i][0], pp[i][1], pp[i][2], pp[i][3]);
+      for (int i = 0; i < 3; ++i)
+        *reinterpret_cast<uint4*>(c.p + ((at * 3 + i) * kTriangle + f) * 512 + lane * 8) = make_uint4(pp[i][0], pp[i][1], pp[i][2], pp[i][3]);
     }
   }
   if (tid < kChunk) {
@@ -991,7 +990,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
 // as bf16 parts in the order of a B operand, per 16 columns.
 template <int kDim, int kTiles>
 struct ScanShared {
-  uint4 state[kTiles][3][kDim * 2], x[kTiles][3][128], write[kTiles][3][128], u[2][kTiles][2][128];
+  uint4 state[kTiles][3][kDim * 2], x[kTiles][3][128], write[kTiles][3][128], u[2][kTiles][3][128];
 };
 // Four values of rows 16 tile + 4 quarter .. + 3 and a lane's column: half of a B operand's eight, per part.
 template <int kParts>
@@ -1118,7 +1117,7 @@ __device__ __forceinline__ void scan_solve(const ChunkParams& c, const Span& s, 
       put_parts<3>(lds.write[x][0], 128, scaled, block);
     }
 #pragma unroll
-    for (int x = 0; x < kTiles; ++x) put_parts<2>(lds.u[i & 1][x][0], 128, u[x], block);
+    for (int x = 0; x < kTiles; ++x) put_parts<3>(lds.u[i & 1][x][0], 128, u[x], block);
     lds_barrier();  // U is there
     const int part = s.count - i * kChunk;
     if (part > 0 && part < n) {
@@ -1222,14 +1221,14 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 #pragma unroll
         for (int m = 0; m < 2; ++m) o.kt[i3][h][m] = *reinterpret_cast<const uint4*>(kt + i3 * kDim * kChunk + (2 * h + m) * 512);
   };
-  uint4 mat[2][2];  // P of the chunk before
+  uint4 mat[3][2];  // P of the chunk before, in parts
   const auto load_mat = [&](int i) {
-    const uint16_t* from = c.p + (static_cast<int64_t>(w.base + i) * p.Hv + w.head) * (2 * kTriangle * 512) + triangle(block, 0) * 512 + lane * 8;
+    const uint16_t* from = c.p + (static_cast<int64_t>(w.base + i) * p.Hv + w.head) * (3 * kTriangle * 512) + triangle(block, 0) * 512 + lane * 8;
     if (block > 1)
 #pragma unroll
-      for (int i3 = 0; i3 < 2; ++i3) mat[i3][1] = *reinterpret_cast<const uint4*>(from + (i3 * kTriangle + 1) * 512);
+      for (int i3 = 0; i3 < 3; ++i3) mat[i3][1] = *reinterpret_cast<const uint4*>(from + (i3 * kTriangle + 1) * 512);
 #pragma unroll
-    for (int i3 = 0; i3 < 2; ++i3) mat[i3][0] = *reinterpret_cast<const uint4*>(from + i3 * kTriangle * 512);
+    for (int i3 = 0; i3 < 3; ++i3) mat[i3][0] = *reinterpret_cast<const uint4*>(from + i3 * kTriangle * 512);
   };
   // keep S + K^T (the writes in LDS)
   const auto update = [&](const Ops& o, float keep, f32x4 (&sum)[kHeld][kTiles]) {
@@ -1264,10 +1263,15 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         if (m <= block / 2) {
-          const uint4 x0 = lds.u[i & 1][x][0][m * 64 + lane], x1 = lds.u[i & 1][x][1][m * 64 + lane];
-          sum[x] = mfma16x16x32(mat[1][m], x0, sum[x]);
-          sum[x] = mfma16x16x32(mat[0][m], x1, sum[x]);
-          sum[x] = mfma16x16x32(mat[0][m], x0, sum[x]);
+          uint4 f[3];
+#pragma unroll
+          for (int i3 = 0; i3 < 3; ++i3) f[i3] = lds.u[i & 1][x][i3][m * 64 + lane];
+          sum[x] = mfma16x16x32(mat[2][m], f[0], sum[x]);
+          sum[x] = mfma16x16x32(mat[1][m], f[1], sum[x]);
+          sum[x] = mfma16x16x32(mat[0][m], f[2], sum[x]);
+          sum[x] = mfma16x16x32(mat[1][m], f[0], sum[x]);
+          sum[x] = mfma16x16x32(mat[0][m], f[1], sum[x]);
+          sum[x] = mfma16x16x32(mat[0][m], f[0], sum[x]);
         }
     }
 #pragma unroll
@@ -1295,10 +1299,12 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
         for (int m = 0; m < kSteps; ++m) {
           uint4 r[kRowParts];
           row_parts<kBf16>(o.rows[m], r);
-          const uint4 f0 = lds.state[x][0][m * 64 + lane], f1 = lds.state[x][1][m * 64 + lane];
-          rows[x] = mfma16x16x32(r[0], f1, rows[x]);
-          if (!kBf16) rows[x] = mfma16x16x32(r[kRowParts - 1], f0, rows[x]);
-          rows[x] = mfma16x16x32(r[0], f0, rows[x]);
+#pragma unroll
+          for (int i3 = 2; i3 >= 0; --i3) {
+            const uint4 f = lds.state[x][i3][m * 64 + lane];
+            if (!kBf16 && i3 < 2) rows[x] = mfma16x16x32(r[kRowParts - 1], f, rows[x]);
+            rows[x] = mfma16x16x32(r[0], f, rows[x]);
+          }
         }
     load(min(i + 1, last), next);
     if (i > 0 && s.count == i * kChunk) keep_state(st);  // the kept state ends where this chunk begins

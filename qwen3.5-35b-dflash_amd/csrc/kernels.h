@@ -458,7 +458,7 @@ struct ChunkParams {
   int cus;
   uint16_t* rows;                 // [chunks][key heads][keys, queries][4 row blocks][dim / 32][64 lanes][8]
   float* t;                       // [chunks][Hv][6 fragments][2 halves][64 lanes][4]
-  uint16_t* p;                    // [chunks][Hv][2 parts][6 fragments][64 lanes][8]
+  uint16_t* p;                    // [chunks][Hv][3 parts][6 fragments][64 lanes][8]
   uint16_t* kt;                   // [chunks][key heads][1 (bf16) or 2 parts][dim / 16][2 fragments][64 lanes][8]
   ChunkScalars* scalars;          // [chunks][Hv]
 };
