@@ -227,6 +227,13 @@ __device__ __forceinline__ float2 gates_of(const RuleParams& p, int64_t token, i
   return make_float2(g, b);
 }
 
+// A state's decay by e^g as S <- by S + rest S.  A slight one is S + (e^g - 1) S: e^g itself is off by half a step near 1, which a head
+// that remembers thousands of tokens would sum up wherever its decay is a constant, call after call (a steady state's norm by 1e-4).
+struct Fade {
+  float by, rest;
+};
+__device__ __forceinline__ Fade fade_of(float g) { return g > -0.5f ? Fade{expm1f(g), 1.0f} : Fade{expf(g), 0.0f}; }
+
 // x as the sum of kParts bf16 numbers, each the rounding of what the ones before leave.
 template <int kParts, int kN>
 __device__ __forceinline__ void cut(const float (&x)[kN], uint32_t (&parts)[kParts][kN / 2]) {
@@ -395,15 +402,12 @@ __device__ __forceinline__ void rule_tokens(const RuleParams& p, const Span& s, 
     const bool last = i + 1 == s.tokens;
     if (last && s.count != s.tokens) break;  // nobody sees the state behind the last token
     if (!last) token = load(i + 1);
-    // a slight decay as S + (e^g - 1) S: e^g itself is off by half a step near 1, which a head that remembers thousands of tokens
-    // would sum up wherever its decay is a constant
-    const bool slight = g > -0.5f;
-    const float fade = slight ? expm1f(g) : decay, rest = slight ? 1.0f : 0.0f;
+    const Fade fade = fade_of(g);
     const f32x4 write = rk * u;
 #pragma unroll
     for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) state[j][e] = (fade * state[j][e] + rest * state[j][e]) + k[j][e] * write;
+      for (int e = 0; e < 4; ++e) state[j][e] = (fade.by * state[j][e] + fade.rest * state[j][e]) + k[j][e] * write;
     if (i + 1 == s.count)
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
@@ -437,7 +441,8 @@ struct BlockShared {
   uint16_t k[16][kDim + 8], q[16][kDim + 8];
   float a[16][20], t[16][20], p[16][20];
   double total[16];           // G
-  float gate[16], beta[16], rk[16], rq[16], key[16], query[16], write[16], keep[16];
+  float gate[16], beta[16], rk[16], rq[16], key[16], query[16], write[16];
+  Fade fade[16];              // by e^G
 };
 
 template <bool kBf16, int kDim, bool kOut>
@@ -540,7 +545,7 @@ __device__ __forceinline__ void rule_block(const RuleParams& p, const Span& s, i
           lds.query[lr] = decay * lds.rq[lr];
           lds.write[lr] = expf(static_cast<float>(sum - here)) * lds.rk[lr];
           lds.total[lr] = here;
-          lds.keep[lr] = decay;
+          lds.fade[lr] = fade_of(static_cast<float>(here));
         }
         // (I + A)^-1 diag(beta) by forward substitution, a column a lane (one wave wrote A and reads it)
         __builtin_amdgcn_wave_barrier();
@@ -622,7 +627,7 @@ __device__ __forceinline__ void rule_block(const RuleParams& p, const Span& s, i
           const int r = 4 * quarter + e;
           write[e] = r < part ? expf(static_cast<float>(lds.total[part - 1] - lds.total[r])) * lds.rk[r] : 0.f;
         }
-      const float keep = lds.keep[part - 1];
+      const Fade fade = lds.fade[part - 1];
       uint2 w[2][3];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -651,7 +656,7 @@ __device__ __forceinline__ void rule_block(const RuleParams& p, const Span& s, i
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum[x][e] = keep * st[i][e][x];
+          for (int e = 0; e < 4; ++e) sum[x][e] = fade.by * st[i][e][x] + fade.rest * st[i][e][x];
 #pragma unroll
           for (int j = 2; j >= 0; --j) {
             if (!kBf16 && j < 2) sum[x] = mfma16x16x16(k[kRowParts - 1], w[x][j], sum[x]);
@@ -982,7 +987,11 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(ChunkParams c) {
     to->write[tid] = in ? expf(static_cast<float>(gsum[kChunk - 1] - gsum[tid])) * rk[tid] : 0.f;
     to->norm[tid] = rk[tid];
     to->total[tid] = gsum[tid];
-    if (tid == 0) to->keep = expf(static_cast<float>(gsum[kChunk - 1]));
+    if (tid == 0) {
+      const Fade fade = fade_of(static_cast<float>(gsum[kChunk - 1]));
+      to->fade = fade.by;
+      to->rest = fade.rest;
+    }
   }
 }
 
@@ -1202,7 +1211,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
   struct Ops {
     uint4 rows[kSteps], kt[kRowParts][kHeld][2];             // Q, the keys transposed
     f32x4 scale;                                             // e^G rq
-    float keep;                                              // e^G of the chunk
+    Fade fade;                                               // by e^G of the chunk
   };
   const auto load = [&](int i, Ops& o) {
     const int64_t at = static_cast<int64_t>(w.base + i) * p.Hv + w.head;
@@ -1212,7 +1221,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
     for (int m = 0; m < kSteps; ++m) o.rows[m] = *reinterpret_cast<const uint4*>(rows + m * 512);
     const ChunkScalars* f = c.scalars + at;
     o.scale = *reinterpret_cast<const f32x4*>(f->query + 16 * block + 4 * quarter);
-    o.keep = f->keep;
+    o.fade = Fade{f->fade, f->rest};
     const uint16_t* kt = c.kt + shared * (kRowParts * kDim * kChunk) + block * (kHeld * 1024) + lane * 8;
 #pragma unroll
     for (int i3 = 0; i3 < kRowParts; ++i3)
@@ -1230,8 +1239,8 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 #pragma unroll
     for (int i3 = 0; i3 < 3; ++i3) mat[i3][0] = *reinterpret_cast<const uint4*>(from + i3 * kTriangle * 512);
   };
-  // keep S + K^T (the writes in LDS)
-  const auto update = [&](const Ops& o, float keep, f32x4 (&sum)[kHeld][kTiles]) {
+  // S faded + K^T (the writes in LDS)
+  const auto update = [&](const Ops& o, const Fade& fade, f32x4 (&sum)[kHeld][kTiles]) {
 #pragma unroll
     for (int x = 0; x < kTiles; ++x) {
       uint4 u[2][3];
@@ -1240,7 +1249,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 #pragma unroll
         for (int i = 0; i < 3; ++i) u[m][i] = lds.write[x][i][m * 64 + lane];
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h) sum[h][x] = keep * st[h][x];
+      for (int h = 0; h < kHeld; ++h) sum[h][x] = fade.by * st[h][x] + fade.rest * st[h][x];
 #pragma unroll
       for (int i = 2; i >= 0; --i)
 #pragma unroll
@@ -1315,14 +1324,14 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
     for (int x = 0; x < kTiles; ++x) seen[x] = o.scale * rows[x];
     lds_barrier();  // U is there
     f32x4 after[kHeld][kTiles];
-    update(o, o.keep, after);
+    update(o, o.fade, after);
     const int part = s.count - i * kChunk;
     if (part > 0 && part < n) {
       const double end = c.scalars[static_cast<int64_t>(w.base + i) * p.Hv + w.head].total[part - 1];
       lds_barrier();
       lds_barrier();
       f32x4 kept[kHeld][kTiles];
-      update(o, expf(static_cast<float>(end)), kept);
+      update(o, fade_of(static_cast<float>(end)), kept);
       keep_state(kept);
     }
 #pragma unroll

@@ -448,7 +448,7 @@ struct ChunkScalars {
   float key[kRuleChunk], query[kRuleChunk];  // e^G / |k|, e^G scale / |q|
   float write[kRuleChunk], norm[kRuleChunk]; // e^{G_end - G} / |k|, 1 / |k|
   double total[kRuleChunk];                  // G, the log decay summed up to the token
-  float keep, unused[3];                     // e^G of the whole chunk
+  float fade, rest, unused[2];               // the whole chunk's decay: S <- fade S + rest S
 };
 struct ChunkParams {
   RuleParams rule;

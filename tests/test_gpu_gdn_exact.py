@@ -1,4 +1,4 @@
-"""GPU: the delta rule's products where terms cancel, against 64 bits."""
+"""GPU: the delta rule's products where terms cancel, and states that are kept over thousands of tokens, against 64 bits."""
 import pytest
 import torch
 
@@ -79,3 +79,81 @@ def test_outputs_of_tokens_that_cancel(pkg, device, dim, dtype, longest):
     over = (got[1::2] - want).abs() - (66 * EPS * old.abs() + UNIT[dtype] * want.abs() + TINY[dtype])
     assert float(over.max()) <= 0, float((over / old.abs()).max()) / EPS
     assert not bool(got[0::2].any())      # a query of zeros
+
+
+GATES = torch.tensor([-1 / 4000, -1 / 3000, -1e-4, -1 / 2500, -1 / 7000, -2e-4])
+
+
+def kept(layer, calls):
+    """The norm of what the states are off by, over theirs, after their decays alone; and what roundings that act independently leave:
+    each of `calls` steps rounds an element at most three times, by at most EPS."""
+    return (16 + 3 * calls ** 0.5) * EPS
+
+
+@pytest.mark.parametrize("spans,count", [([4, 1, 16], 1), ([7, 3, 2], 2), ([16, 5, 9], 3)])
+@pytest.mark.parametrize("dim,dtype", SHAPES)
+def test_states_after_thousands_of_commits(pkg, device, dim, dtype, spans, count):
+    """A speculative run's commits of a token or a few at a time: a decay that is rounded near 1 would add up over what a head remembers.
+    The decays' own part alone has a closed form: nothing is written (beta 0), and S is e^(sum of g) of what it was."""
+    calls = 6000
+    layer = Layer(pkg, device, spans, value_heads=6, dim=dim, dtype=dtype, raw_gates=False, seed=7, counts=[count] * len(spans))
+    put(layer, "beta", 0.0)
+    put(layer, "decay", GATES.expand(layer.total, 6))
+    for _ in range(calls):
+        layer.advance()
+    got = layer.d["recurrent"].double().cpu()
+    for b, n in enumerate(spans):
+        tokens, was = calls * min(count, n), layer.recurrent[int(layer.slots[b])].double()
+        want = was * (GATES.float().double() * tokens).exp()[:, None, None]
+        off = (got[int(layer.slots[b])] - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+        assert float(off.max()) <= kept(layer, calls), (b, off / kept(layer, calls))
+
+
+@pytest.mark.parametrize("longest,spans", [(1, [1, 1]), (16, [5, 16]), (16, [1, 9]), (16, [17, 4]), (200, [64, 70]), (200, [33, 130])])
+@pytest.mark.parametrize("dim,dtype", SHAPES)
+def test_states_after_thousands_of_blocks(pkg, device, dim, dtype, longest, spans):
+    """The same through the rule, which advances by its blocks: token after token, 16 and 64 at a time."""
+    steps = {1: 1, 16: 16, 200: 64}[longest]
+    calls = 4000 if longest < 200 else 1500
+    layer = Layer(pkg, device, spans, value_heads=6, dim=dim, dtype=dtype, raw_gates=False, seed=8)
+    gates = GATES * (1.0 if longest == 1 else 0.2 if longest == 16 else 0.02)
+    put(layer, "beta", 0.0)
+    put(layer, "decay", gates.expand(layer.total, 6))
+    for _ in range(calls):
+        layer.rule(longest=longest)
+    got = layer.d["recurrent"].double().cpu()
+    for b, n in enumerate(spans):
+        was = layer.recurrent[int(layer.slots[b])].double()
+        want = was * (gates.float().double() * (calls * n)).exp()[:, None, None]
+        off = (got[int(layer.slots[b])] - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+        limit = kept(layer, calls * -(-n // steps))
+        assert float(off.max()) <= limit, (b, off / limit)
+
+
+@pytest.mark.parametrize("dim,dtype", SHAPES)
+def test_a_run_of_commits(pkg, device, dim, dtype):
+    """Commits of one token each with keys, values and writes: the state against the 64-bit recurrence."""
+    calls = 4000
+    layer = Layer(pkg, device, [4], key_heads=3, value_heads=6, dim=dim, dtype=dtype, raw_gates=False, seed=9, counts=[1])
+    ops, d = pkg.ops, layer.d
+    gen = torch.Generator().manual_seed(10)
+    rows = torch.randn((calls + 3, layer.channels), generator=gen).to(dtype)
+    key, value = rows[:, :3 * dim].unflatten(-1, (3, dim)), rows[:, 6 * dim:].unflatten(-1, (6, dim))
+    beta, decay = torch.rand((calls + 3, 6), generator=gen) * 0.1, GATES.expand(calls + 3, 6).contiguous()
+    dev = [t.to(device) for t in (rows, rows, beta, decay)]
+    dkey, dvalue = dev[0][:, :3 * dim].unflatten(-1, (3, dim)), dev[0][:, 6 * dim:].unflatten(-1, (6, dim))
+    for i in range(calls):
+        part = slice(i, i + 4)
+        ops.gdn_advance(layer.pool, dev[0][part], dkey[part], dvalue[part], dev[3][part], dev[2][part], d["starts"], d["counts"])
+    s = layer.recurrent[int(layer.slots[0])].double()
+    k = key.double()
+    k = (k / (k.square().sum(-1, keepdim=True) + 1e-6).sqrt()).repeat_interleave(2, 1)
+    fade = GATES.double().exp()[:, None, None]
+    for i in range(calls):
+        s = fade * s
+        u = beta[i].double()[:, None] * (value[i].double() - (s * k[i][..., None]).sum(1))
+        s = s + k[i][..., None] * u[:, None, :]
+    got = d["recurrent"][int(layer.slots[0])].double().cpu()
+    off = (got - s).flatten(1).norm(dim=1) / s.flatten(1).norm(dim=1)
+    memory = float((1 - (GATES.double() * calls).exp()).div(-GATES.double()).max())
+    assert float(off.max()) <= (16 + 3 * memory ** 0.5) * EPS, off / EPS
