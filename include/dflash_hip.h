@@ -402,7 +402,8 @@ int dflash_paged_attention(const dflash_paged_kv* cache, const dflash_paged_kv* 
  * A NaN or an infinity in a token's rows or gates may reach every output of its sequence's block (of its head, in the rule) and
  * the state it leaves, earlier tokens' among them; other sequences, heads and slots keep theirs.
  * Constraints: dtype BF16 or F16; channels % 8 == 0, <= 2^16; head_dim 64 or 128; history_stride % 8 == 0, recurrent_stride
- * % 4 == 0; sequences * value_heads <= 2^19, tokens <= 2^20, tokens * value_heads <= 2^28.  An output lies apart from the rows.
+ * % 4 == 0; sequences * value_heads <= 2^19, tokens <= 2^20, tokens * value_heads <= 2^28.  An output lies apart from all that
+ * the call reads: rows, gates, weights, the pool's slots, starts and their like (refused otherwise).
  */
 typedef struct dflash_state_pool {
   void* history;

@@ -1365,6 +1365,32 @@ bool rows_meet(const dflash_rows& r, int64_t tokens, int64_t heads, int64_t size
   return from < to + 2 * static_cast<wide>(out_size) && to < end;
 }
 
+// Whether anything else that a call reads lies in its output, whose values workgroups write while others still read.
+struct Output {
+  typedef unsigned __int128 wide;
+  wide from, to;
+  Output(const void* out, int64_t size) : from(reinterpret_cast<uintptr_t>(out)), to(from + 2 * static_cast<wide>(size)) {}
+  bool meets(const void* data, wide bytes) const {
+    const wide at = reinterpret_cast<uintptr_t>(data);
+    return data && at < to && from < at + bytes;
+  }
+  // [tokens][heads] gates, rows `stride` values apart
+  bool meets_gates(const void* data, int64_t tokens, int64_t heads, int64_t stride, int64_t size) const {
+    return meets(data, static_cast<wide>(size) * (static_cast<wide>(tokens - 1) * stride + heads));
+  }
+  // Slots of a pool, not what lies between them: the last that begins before the output's end.
+  bool meets_slots(const void* data, int64_t slots, wide stride, wide slot) const {
+    const wide at = reinterpret_cast<uintptr_t>(data);
+    if (!slots || to <= at) return false;
+    const wide last = stride ? std::min(static_cast<wide>(slots - 1), (to - at - 1) / stride) : 0;
+    return from < at + last * stride + slot;
+  }
+  bool meets_block(const dflash_state_pool* pool, const int32_t* starts, const int32_t* counts, const uint8_t* fresh) const {
+    return meets(pool->slots, 4 * pool->sequences) || meets(starts, 4 * (pool->sequences + 1)) || meets(counts, 4 * pool->sequences) ||
+           meets(fresh, pool->sequences);
+  }
+};
+
 dflash::RuleParams rule_params(const dflash_rule* r, const dflash_state_pool* c, const dflash::PoolParams& pool) {
   dflash::RuleParams p{};
   p.pool = pool;
@@ -1444,6 +1470,11 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
       return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: weight or out is NULL or not 16-byte aligned");
     if (rows_meet(*x, tokens, 1, pool->channels, out, tokens * pool->channels))
       return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: out cannot be x or overlap it, whose rows are read after a row is written");
+    const Output output(out, tokens * pool->channels);
+    if (output.meets(weight, 8 * pool->channels) ||
+        output.meets_slots(pool->history, pool->pool_slots, 2 * static_cast<Output::wide>(pool->history_stride), 6 * pool->channels) ||
+        output.meets_block(pool, starts, counts, fresh))
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn conv: out cannot overlap the weight, the histories, or the slots, starts, counts and fresh");
     p.weight = static_cast<const uint16_t*>(weight);
     p.out = static_cast<uint16_t*>(out);
     dflash::launch_gdn_conv(pool->dtype == DFLASH_DTYPE_BF16, p, static_cast<hipStream_t>(stream));
@@ -1525,9 +1556,18 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
     dflash::RuleParams p = rule_params(rule, pool, pool_params(pool, starts, counts, fresh, tokens));
     p.out = static_cast<uint16_t*>(out);
     const RuleLayout L = rule_layout(tokens, rule->key_heads, pool->value_heads, pool->head_dim, pool->sequences, longest);
+    if (L.chunks && (!workspace || !aligned16(workspace) || workspace_bytes < L.total))
+      return fail(DFLASH_ERR_WORKSPACE, "gdn rule workspace needs " + std::to_string(L.total) + " bytes");
+    const Output output(out, outputs);
+    const int64_t heads = pool->value_heads, gate = rule->gates_dtype == DFLASH_DTYPE_F32 ? 4 : 2;
+    if (output.meets_gates(rule->decay, tokens, heads, rule->decay_stride, gate) ||
+        output.meets_gates(rule->beta, tokens, heads, rule->beta_stride, gate) || output.meets(rule->a_log, 4 * heads) ||
+        output.meets(rule->dt_bias, 4 * heads) ||
+        output.meets_slots(pool->recurrent, pool->pool_slots, 4 * static_cast<Output::wide>(pool->recurrent_stride),
+                           4 * heads * pool->head_dim * pool->head_dim) ||
+        output.meets_block(pool, starts, counts, fresh))
+      return fail(DFLASH_ERR_INVALID_ARGUMENT, "gdn rule: out cannot overlap the gates, the states, or the slots, starts, counts and fresh");
     if (L.chunks) {
-      if (!workspace || !aligned16(workspace) || workspace_bytes < L.total)
-        return fail(DFLASH_ERR_WORKSPACE, "gdn rule workspace needs " + std::to_string(L.total) + " bytes");
       dflash::ChunkParams c{};
       c.rule = p;
       c.least = static_cast<int>(L.least);

@@ -657,7 +657,7 @@ def gdn_conv(x: torch.Tensor, weight: torch.Tensor, pool: StatePool, starts: tor
     ``pool.history`` holds (zeros where ``fresh[b]``); ``weight`` ``[channels, 1, 4]``, its last tap the token's own.  The slot
     then holds the last rows after ``counts[b]`` of the tokens (int32 ``[B]``; None: all of them; 0: it stays as it is).  fp32 inside, one
     rounding.  ``x`` may be a view of a projection's rows.  Tokens in no sequence are not written (``out``: a tensor to write into,
-    which shares no memory with ``x``).
+    which shares no memory with anything that the call reads).
     """
     if _plain(x) and (host := _lib.host()):
         done = host.gdn_conv(x, weight, pool, starts, fresh, counts, out)
@@ -699,7 +699,7 @@ def gdn_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, decay:
     dt_bias)``, ``beta = sigmoid(beta)``.  The slot then holds the state after ``counts[b]`` tokens (int32 ``[B]``; None: all of them;
     0: it stays as it is, as a verify block's does until :func:`gdn_advance`).  ``longest``: tokens of the longest block, if the caller
     knows it, for the choice of the kernels (else as if none were twice the average).  fp32 inside.  Rows may be views; tokens in no sequence are not written (``out``: a
-    tensor to write into, which shares no memory with the rows).  A NaN or infinity in a token may reach all outputs of its block and head.
+    tensor to write into, which shares no memory with anything that the call reads).  A NaN or infinity in a token may reach all outputs of its block and head.
     """
     if _plain(value) and query is not None and (host := _lib.host()):
         done = host.gdn_rule(query, key, value, decay, beta, pool, starts, a_log, dt_bias, normalise, scale, fresh, counts, longest, out,
