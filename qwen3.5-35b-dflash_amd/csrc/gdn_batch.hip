@@ -188,8 +188,8 @@ __global__ __launch_bounds__(256) void gdn_conv_kernel(ConvParams p) {
       for (int j = 0; j < kTaps - 1; ++j)
         unpack8<kBf16>(*reinterpret_cast<const uint4*>(p.x + (lo - (kTaps - 1) + j) * p.x_stride + channel), past[j]);
     }
-    // a block that starts at the tile's last row brings two rows of the next
-    constexpr int kMost = kRows + kTaps - 2;
+    // a whole tile, or a block's first three rows where it starts at the tile's last ones
+    constexpr int kMost = kRows > kTaps - 1 ? kRows : kTaps - 1;
     uint4 x[kMost];
 #pragma unroll
     for (int i = 0; i < kMost; ++i) x[i] = *reinterpret_cast<const uint4*>(p.x + min(lo + i, hi - 1) * p.x_stride + channel);
