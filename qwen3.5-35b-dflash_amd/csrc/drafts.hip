@@ -153,20 +153,22 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   double sum = 0.0;
   int at = kNowhere;
   const float c = t > 0.0f ? static_cast<float>(scale_of(t)) : 0.0f, ahead = t > 0.0f ? 16.0f / c : 0.0f;
-  const auto take = [&](int o, const float (&f)[8]) {
-    float m = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-    if (t == 0.0f) {
-      if (m >= top) {
-        int place = kNowhere;
+  const auto most = [](const float (&f)[8]) {
+    return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  };
+  const auto find = [&](int o, const float (&f)[8]) {
+    const float m = most(f);
+    if (m < top) return;
+    int place = kNowhere;
 #pragma unroll
-        for (int i = 7; i >= 0; --i)
-          if (f[i] == m) place = data.first(o) + i;
-        // by places, not by the order of visits: a row's first eight, where it is not whole, is seen last
-        if (m > top || place < at) at = place;
-        top = m;
-      }
-      return;
-    }
+    for (int i = 7; i >= 0; --i)
+      if (f[i] == m) place = data.first(o) + i;
+    // by places, not by the order of visits: a row's first eight, where it is not whole, is seen last
+    if (m > top || place < at) at = place;
+    top = m;
+  };
+  const auto add = [&](int, const float (&f)[8]) {
+    const float m = most(f);
     top = fmaxf(top, m);
     if (m > base + ahead) {
       sum *= static_cast<double>(exp2f((base - m) * c));
@@ -179,40 +181,44 @@ __global__ __launch_bounds__(256) void draft_stats_kernel(DraftParams p) {
   };
   // the eights inside the row, four loads in flight; its ends
   const int inner0 = max(first, data.ahead ? 1 : 0), inner1 = min(last, (p.V + data.ahead) / 8);
-  int o = inner0 + tid;
-  for (; o + 768 < inner1; o += 1024) {
-    typename Row<kType>::Raw r[4];
+  const auto walk = [&](auto take) {
+    int o = inner0 + tid;
+    for (; o + 768 < inner1; o += 1024) {
+      typename Row<kType>::Raw r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = data.raw(data.first(o + 256 * i));
+      for (int i = 0; i < 4; ++i) r[i] = data.raw(data.first(o + 256 * i));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[8];
-      Row<kType>::unpack(r[i], f);
-      take(o + 256 * i, f);
-    }
-  }
-  {
-    typename Row<kType>::Raw r[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (o + 256 * i < inner1) r[i] = data.raw(data.first(o + 256 * i));
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (o + 256 * i < inner1) {
+      for (int i = 0; i < 4; ++i) {
         float f[8];
         Row<kType>::unpack(r[i], f);
         take(o + 256 * i, f);
       }
-  }
-  for (int e = 0; e < 2; ++e) {
-    const int end = e ? data.eights() - 1 : 0;
-    const bool partial = end < inner0 || end >= inner1;  // not taken above
-    if (tid == 64 * e && end >= first && end < last && partial && (e == 0 || end > 0)) {
-      float f[8];
-      data.eight(data.first(end), f);
-      take(end, f);
     }
-  }
+    {
+      typename Row<kType>::Raw r[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (o + 256 * i < inner1) r[i] = data.raw(data.first(o + 256 * i));
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (o + 256 * i < inner1) {
+          float f[8];
+          Row<kType>::unpack(r[i], f);
+          take(o + 256 * i, f);
+        }
+    }
+    for (int e = 0; e < 2; ++e) {
+      const int end = e ? data.eights() - 1 : 0;
+      const bool partial = end < inner0 || end >= inner1;  // not taken above
+      if (tid == 64 * e && end >= first && end < last && partial && (e == 0 || end > 0)) {
+        float f[8];
+        data.eight(data.first(end), f);
+        take(end, f);
+      }
+    }
+  };
+  if (t == 0.0f) walk(find);
+  else walk(add);
   // join the threads
   Best best = wave_best(Best{top, at});
   if ((tid & 63) == 0) bests[tid >> 6] = best;
