@@ -456,6 +456,7 @@ int dflash_gdn_rule(const dflash_state_pool* pool, const dflash_rule* rule, cons
 /*
  * Conv histories and recurrent states after the first counts[b] (required) tokens of blocks that dflash_gdn_conv (rows x) and
  * dflash_gdn_rule took with counts of 0: what commits the accepted part of every block.  rule->query is not used.
+ * Any counts are right; they are walked 16 tokens at a time, which is meant for verify blocks (dflash_gdn_rule is faster for prompts).
  */
 int dflash_gdn_advance(const dflash_state_pool* pool, const dflash_rows* x, const dflash_rule* rule, const int32_t* starts,
                        const int32_t* counts, const uint8_t* fresh, int64_t tokens, void* stream);

@@ -1428,7 +1428,7 @@ int conv_params(const dflash_state_pool* pool, const dflash_rows* x, const char*
 }
 
 // Parts that the rows of logits are cut into.  In the first pass a workgroup each, about kDraftGroups of them, of 4096 tokens at
-// least (one block of 16 rows 35 us, with 2048 39, with 8192 35; one row 21 each way).  Of the rows that tokens are drawn from a wave each, at most kDraftParts, which one workgroup joins, a thread a part.
+// least (one block of 16 rows 37 us; when it was chosen 35, with 2048 39, with 8192 35; one row 21 each way).  Of the rows that tokens are drawn from a wave each, at most kDraftParts, which one workgroup joins, a thread a part.
 constexpr int64_t kDraftGroups = 4096, kDraftParts = 256;
 struct DraftLayout {
   int64_t splits, split_octets, parts, part_octets;
@@ -1485,10 +1485,10 @@ int dflash_gdn_conv(const dflash_state_pool* pool, const dflash_rows* x, const v
 }
 
 namespace {
-// Whether blocks go 64 tokens at a time.  Sixteen at a time a workgroup walks its sequence in 5.7 us a step, and all of them together
+// Whether blocks go 64 tokens at a time.  Sixteen at a time a workgroup walks its sequence in about 5.7 us a step, and all of them together
 // take 0.83 ns a token and head of 128; 64 at a time a step is 1.7 us and the whole 1.1 ns, 9 us dearer to start (head dim 64: half a
-// token).  Measured us, 16 and 64 at a time: 1 block of 24 tokens 19 and 19, of 64 30 and 19; 8 of 64 37 and 40, of 128 60 and 54; 16 of
-// 256 130 and 148; 64 of 256 433 and 582; at head dim 64 8 of 64 23 and 17, 32 of 64 31 and 34.
+// token); all of them some 8 % more since outputs take three parts.  us a call, 16 and 64 at a time: 1 block of 24 tokens 19.5 and 18.8, of
+// 64 32 and 19; 8 of 64 39 and 44, of 128 64 and 59; 16 of 256 138 and 163; 64 of 256 452 and 626; 16 heads of 64, 8 of 64 24 and 18, 32 of 64 32 and 37.
 bool chunks_pay(int64_t longest, int64_t T, int64_t Hv, int64_t D) {
   if (longest <= 16) return false;
   const double l = static_cast<double>(longest), all = static_cast<double>(T) * static_cast<double>(Hv) * static_cast<double>(D) / 128;
@@ -1513,8 +1513,8 @@ RuleLayout rule_layout(int64_t T, int64_t Hk, int64_t Hv, int64_t D, int64_t B, 
   L.longest = std::min(longest, T);
   if (!chunks_pay(L.longest, T, Hv, D)) return L;
   // Short blocks beside long ones go their own way, in a launch of their own: a workgroup of the scan takes as long for a token as for 64.
-  // us with that launch and without, heads of 128: 1024 tokens and 63 blocks of one 115 and 247, three of one 55 and 58, one 57 and 56; four
-  // prompts 94 and 92; 16 heads of 64, 1024 tokens and 15 of one 52 and 43.
+  // us a call with that launch and without, 32 heads of 128: 1024 tokens and 255 blocks of one 339 and 1450, 63 of one 115 and 336, three of one
+  // 60 and 65, 31 of 16 113 and 173; four prompts 102 both ways; 16 heads of 64, 1024 tokens and 15 of one 52 and 43 (the smallest batches go without).
   L.least = B * Hv * D * D <= 3 << 19 ? 1 : kShortBlock + 1;
   L.sequences = std::min(T / L.least, B);
   if (L.sequences == 0 || L.longest < L.least) return L;

@@ -422,9 +422,9 @@ __global__ __launch_bounds__(256, 3) void gdn_token_kernel(RuleParams p) {
   if (s.tokens > 0) rule_tokens<kBf16, kDim>(p, s, blockIdx.x % p.Hv);
 }
 
-// Blocks of up to so many tokens go token after token.  us, that way and 16 at a time: 64 sequences of one token 45 and 66, of two 49 and
-// 66, of three 57 and 70, of four both 66; 32 of four 41 and 42; one of one 6.7 and 7.5, of four 12.0 and 12.6; head dim 64, 32 of two 7.9 and
-// 11.0, of four 11.9 and 11.0.
+// Blocks of up to so many tokens go token after token.  us a call, that way and 16 at a time: 64 sequences of one token 45 and 68, of two 51
+// and 69, of three 60 and 68, of four 71 and 69; 32 of four both 42; one of one 5.4 and 12.5, of four 12.0 and 12.6; 16 heads of 64, 32
+// sequences of two 8.1 and 11.2, of three 10.0 and 11.2, of four 12.3 and 11.3.
 constexpr int kTokenSteps = 3;
 
 // ------------------------------------------------------------------ the rule, 16 tokens at a time
@@ -433,8 +433,8 @@ constexpr int kTokenSteps = 3;
 // every other one, so that a lane loads two neighbours) and, when the sum over rows is taken in that order, of a B operand.  So
 // the state takes part in products without leaving its registers.  Sub-blocks of up to 16 tokens with the formulas of a chunk (below):
 //   X = V - diag(e^G r) K S,  U = T X,  O = diag(e^G rq) Q S + P U,  S <- e^G S + K^T diag(e^{G_end - G} r) U.
-// 32 sequences of up to 16 tokens 34 us with the state left alone (74 MB: memory takes 14; the rest is the sub-block's chain of
-// K K^T, the substitution, two products and the output, 5.7 us behind the load of the state, in 1.3 rounds of three workgroups a CU),
+// 32 sequences of up to 16 tokens 35 us with the state left alone (74 MB: memory takes 14; the rest is the sub-block's chain of
+// K K^T, the substitution, two products and the output, some 6 us behind the load of the state, in 1.3 rounds of three workgroups a CU),
 // 40 us as gdn_advance, which writes it (139 MB).
 template <bool kBf16, int kDim>
 struct BlockShared {
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(2 * kDim, 3) void gdn_advance_kernel(RuleParams p, 
 // two bf16 parts, since states need bf16's range), norms and gates stand beside them as fp32 factors.  What meets them (S, X, U,
 // T, P) is cut into three bf16 parts, 24 bits, and of their products those above 2^-24 of the whole are taken.  So states and outputs
 // come out as from fp32 products, at 1/3 to 1/6 of the 16-bit rate instead of 1/16 of it.  (Two parts for what only an output sees
-// would be exact enough for the output's own rounding, but not where its terms cancel: a prompt of 4096 tokens took 147 us so, 158 now.)
+// would be exact enough for the output's own rounding, but not where its terms cancel: a prompt of 4096 tokens took 147 us so, 160 now.)
 constexpr int kChunk = 64, kPitch = 68;     // tokens of a chunk; floats of an LDS row
 constexpr int kTriangle = 6;                // 16 x 32 fragments of a lower triangle of 64 x 64
 __device__ __forceinline__ int triangle(int block, int step) { return block < 2 ? block : 2 * block - 2 + step; }
@@ -778,8 +778,8 @@ __device__ __forceinline__ int2 sequence_place(const PoolParams& p, int least, i
   return make_int2(p.B, 0);
 }
 
-// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices: 2048 of them 48 us for 4096 tokens of one
-// sequence, a chain of seven steps with barriers between, two workgroups a CU.  Rows come in whole (256 bytes a
+// One workgroup per (chunk, value head), wave w rows 16 w .. 16 w + 15 of the chunk's matrices: 2048 of them 49 us for 4096 tokens of one
+// sequence, a chain of seven steps with barriers between, three workgroups a CU (LDS).  Rows come in whole (256 bytes a
 // load of 16 lanes) and pass through LDS: what the scan reads eight times over, once a slice, it finds in the order of
 // its operands, 1 KB a load (rows read straight into operands cost a cache line a lane).
 template <bool kBf16, int kDim>
@@ -1355,7 +1355,7 @@ __device__ __forceinline__ void scan_output(const ChunkParams& c, const Span& s,
 }
 
 // One workgroup per (sequence, value head, 16 kTiles columns of the state), the sequence's chunks in turn.  Three barriers a chunk:
-// S, then X, then U are there.  Bound by that chain: 1.75 us a chunk, 112 us for 4096 tokens of one sequence.
+// S, then X, then U are there.  Bound by that chain: 2.0 us a chunk, 127 us for 4096 tokens of one sequence.
 template <bool kBf16, int kDim, int kTiles>
 __global__ __launch_bounds__(512) void gdn_scan_kernel(ChunkParams c) {
   const RuleParams& p = c.rule;
@@ -1401,9 +1401,10 @@ void launch_chunks(const ChunkParams& c, hipStream_t stream) {
   const RuleParams& p = c.rule;
   hipLaunchKernelGGL((gdn_chunk_kernel<kBf16, kDim>), dim3(c.chunks * p.Hv), dim3(256), 0, stream, c);
   const int units = (c.sequences * p.Hv + 7) / 8 * 8, typical = c.typical * p.Hv;
-  // A CU runs a workgroup about as fast as several would share it.  With 32 columns one reads half as much a column and takes 1.5 to 1.7 times as long as with 16: it
-  // pays where that saves rounds of the card.  us, 16 and 32 columns, by sequences of 1024 tokens: one 50 and 60, two 90 and 75, four 160 and
-  // 135; head dim 64, 16 heads, of 512 tokens: six 36 and 35, twelve 58 and 63.
+  // Registers let a CU hold one workgroup at head dim 128 (168 a lane at least, 512 threads; two would have to do with 128), so workgroups
+  // are counted in rounds of the card.  With 32 columns one reads half as much a column and takes longer: it pays where that saves rounds.
+  // us a call, 16 and 32 columns, by sequences of 1024 tokens: one 53 and 62, two 97 and 81, four 172 and 144; 16 heads of 64, of 512 tokens:
+  // six both 39, twelve 66 and 69.
   const auto rounds = [&](int columns) { return (typical * (kDim / columns) + c.cus - 1) / c.cus; };
   if (5 * rounds(32) <= 3 * rounds(16))
     hipLaunchKernelGGL((gdn_scan_kernel<kBf16, kDim, 2>), dim3(units * (kDim / 32)), dim3(512), 0, stream, c);

@@ -738,7 +738,8 @@ def gdn_advance(pool: StatePool, x: torch.Tensor, key: torch.Tensor, value: torc
                 starts: torch.Tensor, counts: torch.Tensor, *, a_log: Optional[torch.Tensor] = None,
                 dt_bias: Optional[torch.Tensor] = None, normalise: bool = True, fresh: Optional[torch.Tensor] = None) -> None:
     """Histories and states after the first ``counts[b]`` tokens of blocks that :func:`gdn_conv` (its ``x``) and :func:`gdn_rule` took
-    without advancing them (``counts`` of 0): commits the accepted part of every sequence's block in one launch."""
+    without advancing them (``counts`` of 0): commits the accepted part of every sequence's block in one launch.  Meant for verify
+    blocks: it walks 16 tokens at a time, where :func:`gdn_rule` takes prompts 64 at a time."""
     if _plain(value) and (host := _lib.host()):
         if host.gdn_advance(pool, x, key, value, decay, beta, starts, counts, a_log, dt_bias, normalise, fresh) is not None:
             return
