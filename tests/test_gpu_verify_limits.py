@@ -45,6 +45,25 @@ def test_acceptance_at_its_limit(pkg, device, vocab, dtype, one):
         check(pkg, device, rows_of(c, b), f"sequence {b}")
 
 
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("stop", [None, 0, 15, 16, 20, 33])
+def test_long_blocks_at_their_limits(pkg, device, stop, one):
+    """Blocks of more rows than are looked at together: every row's number is the last below its limit, or in row `stop` the first that is
+    not, so that each test has to be made in 64 bits."""
+    c = make([40, 17, 35], 5003, BF16, 7, noise=0.3, one=one)
+    for b in range(3):
+        lo, hi = int(c["starts"][b]), int(c["starts"][b + 1])
+        for r in range(lo, hi - 1):
+            x = int(c["drafted"][r])
+            limit = float(chances(c["target"][r], 1.0)[x]) / (1.0 if one else float(chances(c["draft"][r], 1.0)[x]))
+            near = torch.tensor(limit, dtype=torch.float32)
+            under, above = ((near, torch.nextafter(near, torch.tensor(math.inf))) if float(near) < limit else
+                            (torch.nextafter(near, torch.tensor(0.0)), near))
+            c["uniforms"][r] = above if r - lo == stop else under
+    want = [min(hi - 1 if stop is None else stop, hi - 1) for hi in (40, 17, 35)]
+    assert check(pkg, device, c).accepted.tolist() == want
+
+
 @pytest.mark.parametrize("order", [1, -1])
 def test_acceptance_of_sorted_rows(pkg, device, order):
     """Logits that rise or fall all along: a running maximum that moves with every token, or never."""
